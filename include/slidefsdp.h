@@ -305,6 +305,111 @@ int sf_ce_weight_grad(const float* grad_loss, const float* n_valid,
                       size_t n_h, int dtype, sf_stream_t stream);
 
 /* ---------------------------------------------------------------------
+ * Log-probabilities of given tokens, losses over them, 8-bit checkpoints
+ * (libsf_hip.so)
+ * ------------------------------------------------------------------- */
+
+/* One chunk of fp32 logits, [rows, vocab] with ld elements from row to row (ld
+ * a multiple of 4, logits on a 16-byte boundary; SF_EALIGN otherwise), each
+ * times `scale`.  For each row with label y: lse = logsumexp(row) and logp =
+ * row[y] - lse.  A row whose label is ignore_index: both 0.  A label outside
+ * [0, vocab): both NaN. */
+int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab,
+                  const int64_t* labels, int64_t ignore_index, float scale,
+                  float* lse, float* logp, sf_stream_t stream);
+
+/* norm[0] = a power of two that brings the largest finite |scale * grad[i]| of
+ * the rows that are not ignored into [1, 2), norm[1] = its inverse, norm[2] =
+ * 1 (three elements of device memory). */
+int sf_logps_norm(const float* grad, const int64_t* labels, int64_t ignore_index,
+                  size_t rows, float scale, float* norm, sf_stream_t stream);
+
+/* The gradient of such a chunk: dz[i, j] = grad[i] * scale * ((j == labels[i])
+ * - exp(scale * logits[i, j] - lse[i])), times norm[0] where norm is not null,
+ * as dtype with ld_dz elements from row to row; 0 for an ignored row, NaN for a
+ * label outside [0, vocab).  SF_DTYPE_F32: dz may be the logits themselves;
+ * other types: no overlap. */
+int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab,
+                  const int64_t* labels, int64_t ignore_index, float scale,
+                  const float* lse, const float* grad, const float* norm,
+                  void* dz, int dtype, size_t ld_dz, sf_stream_t stream);
+
+/* Forms of the preference loss. */
+#define SF_PREF_SIGMOID 0
+#define SF_PREF_HINGE 1
+#define SF_PREF_IPO 2
+
+/* Elements of workspace of the losses below for [rows, cols] tokens (rows: 2
+ * pairs): 16 bytes each for sf_pref_loss, 32 for sf_policy_loss.  0 where a
+ * size is 0 or over 2^30. */
+size_t sf_align_parts(size_t rows, size_t cols);
+
+/* Preference loss of `pairs` pairs: rows p and pairs + p of the fp32 [2 pairs,
+ * cols] log-probabilities (ld elements from row to row, as ref and mask have
+ * ld_ref and ld_mask) are pair p's chosen and rejected sequence.  R = a row's
+ * sum of logps - ref over the tokens whose mask byte is not 0 (average: over
+ * their number, 0 without any), D = R_chosen - R_rejected.  *loss = the mean
+ * over the pairs of -(1 - s) log sigmoid(beta D) - s log sigmoid(-beta D)
+ * (SF_PREF_SIGMOID, s: smoothing), max(0, 1 - beta D) (SF_PREF_HINGE) or (D -
+ * 1 / (2 beta))^2 (SF_PREF_IPO); chosen, rejected: beta R, `pairs` each; coef
+ * (2 pairs, or null): the derivative of *loss by each of a row's tokens.
+ * parts: sf_align_parts(2 pairs, cols) elements, on a 16-byte boundary. */
+int sf_pref_loss(const float* logps, size_t ld, const float* ref, size_t ld_ref,
+                 const uint8_t* mask, size_t ld_mask, size_t pairs, size_t cols,
+                 int form, float beta, float smoothing, int average,
+                 void* parts, float* loss, float* chosen, float* rejected,
+                 float* coef, sf_stream_t stream);
+
+/* grad[i, t] = *grad_loss * coef[i] where mask[i, t], else 0. */
+int sf_pref_grad(const float* grad_loss, const float* coef, const uint8_t* mask,
+                 size_t ld_mask, size_t rows, size_t cols, float* grad,
+                 sf_stream_t stream);
+
+/* Clipped policy loss over fp32 [rows, cols] tokens whose mask byte is not 0.
+ * d = logps - old, A = advantages (per_token: [rows, cols], else one a row,
+ * ld_adv elements apart), a token is clipped where A > 0 and d > log_high or A
+ * < 0 and d < log_low; its term is -exp(d clipped) A, plus, with ref, kl_coef
+ * (exp(q) - 1 - q) for q = ref - logps.  *loss, *kl (null without ref) and
+ * *clipped = the mean over the tokens of the terms, of exp(q) - 1 - q and of
+ * the clipped ones; sequences: the mean over the rows that have tokens of
+ * their means.  NaN without any token.  slope ([rows, cols], or null): the
+ * derivative of each term by logps, 0 where masked; weight (rows, or null):
+ * what a row's tokens weigh in the loss.  parts: sf_align_parts(rows, cols)
+ * elements, on a 16-byte boundary. */
+int sf_policy_loss(const float* logps, size_t ld, const float* old_logps,
+                   size_t ld_old, const float* ref, size_t ld_ref,
+                   const float* advantages, size_t ld_adv, int per_token,
+                   const uint8_t* mask, size_t ld_mask, size_t rows,
+                   size_t cols, float log_low, float log_high, float kl_coef,
+                   int sequences, void* parts, float* loss, float* kl,
+                   float* clipped, float* slope, float* weight,
+                   sf_stream_t stream);
+
+/* grad[i, t] = *grad_loss * weight[i] * slope[i, t]. */
+int sf_policy_grad(const float* grad_loss, const float* weight,
+                   const float* slope, size_t rows, size_t cols, float* grad,
+                   sf_stream_t stream);
+
+/* An activation in 8 bits.  Blocks of SF_ACT8_BLOCK elements share a scale a /
+ * T, a the block's largest magnitude (at least 2^-100) and T the largest code;
+ * code = round(x T / a), to nearest even.  packed: ceil(n / SF_ACT8_BLOCK)
+ * blocks of SF_ACT8_BLOCK_BYTES, the codes of all blocks first (the last
+ * one's rest 0), then their fp32 scales, on a 16-byte boundary (SF_EALIGN).  A
+ * block with an infinity or a NaN has the scale NaN.  x: n elements of dtype
+ * (SF_DTYPE_F32, SF_DTYPE_BF16 or SF_DTYPE_F16), any element boundary.  x and
+ * packed do not overlap (SF_EOVERLAP). */
+#define SF_ACT8_BLOCK 128
+#define SF_ACT8_BLOCK_BYTES 132
+#define SF_ACT8_INT8 0
+#define SF_ACT8_FP8 1 /* e4m3: 3 bits of mantissa, largest 448 */
+int sf_act8_pack(const void* x, int dtype, size_t n, void* packed, int format,
+                 sf_stream_t stream);
+
+/* x = code * scale, rounded once to dtype. */
+int sf_act8_unpack(const void* packed, int format, size_t n, void* x, int dtype,
+                   sf_stream_t stream);
+
+/* ---------------------------------------------------------------------
  * Copies and pinned host memory (libsf_hip.so)
  * ------------------------------------------------------------------- */
 

@@ -42,6 +42,13 @@ SF_ETOOBIG = 9008
 SF_ETIMEDOUT = 9009
 SF_STAGE_SCRATCH_ELEMS = 16 << 20
 SF_CE_LOSS_PARTS = 256
+SF_PREF_SIGMOID = 0
+SF_PREF_HINGE = 1
+SF_PREF_IPO = 2
+SF_ACT8_BLOCK = 128
+SF_ACT8_BLOCK_BYTES = 132
+SF_ACT8_INT8 = 0
+SF_ACT8_FP8 = 1
 # row_slot markers of the row-wise AdamW: a zero-gradient row, a row left as it is
 SF_ROW_ZERO = -1
 SF_ROW_SKIP = -2
@@ -96,6 +103,17 @@ HIP_SIGNATURES = {
     "sf_ce_loss": [_vp, _vp, _sz, ctypes.c_int64, _vp, _vp, _vp],
     "sf_ce_weight_grad": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _vp, _sz, _i, _vp],
     "sf_ce_scale": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _i, _vp],
+    "sf_logps_rows": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp],
+    "sf_logps_norm": [_vp, _vp, ctypes.c_int64, _sz, _f, _vp, _vp],
+    "sf_logps_grad": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp, _vp, _i, _sz, _vp],
+    "sf_align_parts": [_sz, _sz],
+    "sf_pref_loss": [_vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _i, _f, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "sf_pref_grad": [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp],
+    "sf_policy_loss": [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _i, _vp, _sz, _sz, _sz, _f, _f, _f, _i, _vp, _vp, _vp,
+                       _vp, _vp, _vp, _vp],
+    "sf_policy_grad": [_vp, _vp, _vp, _sz, _sz, _vp, _vp],
+    "sf_act8_pack": [_vp, _i, _sz, _vp, _i, _vp],
+    "sf_act8_unpack": [_vp, _i, _sz, _vp, _i, _vp],
     "sf_stage_f32_bf16": [_vp, _vp, _sz, _vp, _sz, _vp],
     "sf_stage_f32_bf16_noalloc": [_vp, _vp, _sz, _sz, _vp],
     "sf_memcpy_async": [_vp, _vp, _sz, _i, _vp],
@@ -147,7 +165,8 @@ _hip = None
 _cpu = None
 _segs = None
 
-_RESTYPES = {"sf_error_string": ctypes.c_char_p, "sf_dma_choose_engines": ctypes.c_uint32}
+_RESTYPES = {"sf_error_string": ctypes.c_char_p, "sf_dma_choose_engines": ctypes.c_uint32,
+             "sf_align_parts": ctypes.c_size_t}
 
 
 def _bind(path: str, sigs: dict) -> ctypes.CDLL:

@@ -1,0 +1,146 @@
+"""Token log-probabilities, the losses over them and 8-bit checkpoints on the
+host: the formulas against float64, gradients against differences, refusals."""
+
+import math
+
+import pytest
+import torch
+
+from alignment_reference import logps, near, policy, preference
+from test1_amd.act8 import act8_bytes, pack_act8, unpack_act8
+from test1_amd.alignment import policy_loss, preference_loss
+from test1_amd.linear_logps import linear_logps
+
+
+def tokens(shape=(4, 37), seed=0):
+    g = torch.Generator().manual_seed(seed)
+    mask = torch.rand(shape, generator=g) < 0.7
+    mask[1] = False
+    lp = -3 * torch.rand(shape, generator=g)
+    noise = lambda: torch.randn(shape, generator=g)  # noqa: E731
+    return mask, lp, lp + 0.2 * noise(), lp + 0.3 * noise(), noise()
+
+
+@pytest.mark.parametrize("kind,smoothing,average", [("sigmoid", 0.0, False), ("sigmoid", 0.1, True), ("hinge", 0.0, False),
+                                                    ("ipo", 0.0, True)])
+def test_preference(kind, smoothing, average):
+    mask, lp, ref, _, _ = tokens()
+    want, bound = preference(lp, ref, mask, 0.1, kind, smoothing, average)
+    lp = torch.where(mask, lp, torch.full_like(lp, math.nan)).requires_grad_(True)
+    out = preference_loss(lp, ref, mask, 0.1, kind, smoothing, average)
+    grad = torch.autograd.grad(out.loss, lp)[0]
+    for got, w, b in zip((out.loss.detach(), out.chosen_rewards, out.rejected_rewards, grad), want, bound):
+        near(got, w, 16 * b + 1e-6 * w.abs())   # torch adds all of a row in 32 bits
+
+
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+@pytest.mark.parametrize("with_ref", [False, True])
+def test_policy(with_ref, reduction):
+    mask, lp, old, ref, adv = tokens()
+    ref = ref if with_ref else None
+    want, bound = policy(lp, old, adv, mask, ref, 0.2, 0.28, 0.05, reduction)
+    old = torch.where(mask, old, torch.full_like(old, -math.inf))
+    lp.requires_grad_(True)
+    out = policy_loss(lp, old, adv, mask, ref, 0.2, 0.28, 0.05, reduction)
+    grad = torch.autograd.grad(out.loss, lp)[0]
+    near(out.loss.detach(), want[0], 16 * bound[0])
+    near(grad, want[3], 16 * bound[3])
+    assert (out.kl is None) != with_ref
+    near(out.clip_fraction, want[2], 16 * bound[2])
+
+
+def test_logps_and_gradients_against_differences():
+    g = torch.Generator().manual_seed(3)
+    hidden, weight = torch.randn(9, 12, generator=g), torch.randn(31, 12, generator=g)
+    labels = torch.randint(0, 31, (9,), generator=g)
+    labels[2] = -100
+    up = torch.randn(9, generator=g)
+    want, bound = logps(hidden, weight, labels, 1 / 0.7, grad=up)
+    h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+    lp = linear_logps(h, w, labels, temperature=0.7)
+    for got, x, b in zip((lp.detach(), *torch.autograd.grad(lp, (h, w), up)), want, bound):
+        near(got, x, b)
+    step = 2.0 ** -6
+    for i, j in ((0, 0), (4, 7), (8, 11)):
+        hi, lo = hidden.double().clone(), hidden.double().clone()
+        hi[i, j] += step
+        lo[i, j] -= step
+        diff = ((logps(hi, weight, labels, 1 / 0.7)[0][0] - logps(lo, weight, labels, 1 / 0.7)[0][0]) * up).sum() / (2 * step)
+        assert abs(diff - want[1][i, j]) <= 0.01 * (abs(want[1][i, j]) + 0.1)   # third derivatives times step^2
+    assert linear_logps(hidden, weight, torch.full((9,), 31))[0].isnan()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("shape", [(1,), (3, 77), (2, 5, 128), (0, 4)])
+def test_checkpoint_round_trip(shape, fmt):
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(1)).bfloat16()
+    packed = pack_act8(x, fmt)
+    assert packed.dtype == torch.uint8 and packed.numel() == act8_bytes(x.numel())
+    back = unpack_act8(packed, shape, x.dtype, fmt)
+    assert back.shape == x.shape and ((back - x).abs() <= 0.08 * x.abs() + 0.02).all()
+    out = torch.empty_like(x)
+    assert unpack_act8(packed, shape, x.dtype, fmt, out=out) is out and torch.equal(out, back)
+
+
+def test_refusals():
+    mask, lp, old, ref, adv = tokens()
+    bad = [
+        (ValueError, lambda: preference_loss(lp[:3], ref[:3], mask[:3])),
+        (ValueError, lambda: preference_loss(lp, ref[:, :5], mask)),
+        (ValueError, lambda: preference_loss(lp, ref, mask[:, :5])),
+        (TypeError, lambda: preference_loss(lp, ref, mask.int())),
+        (TypeError, lambda: preference_loss(lp.bfloat16(), ref, mask)),
+        (ValueError, lambda: preference_loss(lp, ref, mask, beta=0.0)),
+        (ValueError, lambda: preference_loss(lp, ref, mask, kind="dpo")),
+        (ValueError, lambda: preference_loss(lp, ref, mask, kind="ipo", label_smoothing=0.1)),
+        (ValueError, lambda: preference_loss(lp, ref.requires_grad_(True), mask)),
+        (ValueError, lambda: preference_loss(lp[0], ref.detach()[0], mask[0])),
+        (ValueError, lambda: policy_loss(lp, old, adv[:, :3], mask)),
+        (ValueError, lambda: policy_loss(lp, old, adv, mask, clip_low=1.5)),
+        (ValueError, lambda: policy_loss(lp, old, adv, mask, clip_high=-0.1)),
+        (ValueError, lambda: policy_loss(lp, old, adv, mask, reduction="mean")),
+        (TypeError, lambda: policy_loss(lp, old.double(), adv, mask)),
+        (ValueError, lambda: policy_loss(lp, old, adv, mask, kl_coef=math.nan)),
+        (ValueError, lambda: linear_logps(torch.zeros(2, 3), torch.zeros(5, 4), torch.zeros(2).long())),
+        (ValueError, lambda: linear_logps(torch.zeros(2, 4), torch.zeros(5, 4), torch.zeros(3).long())),
+        (TypeError, lambda: linear_logps(torch.zeros(2, 4), torch.zeros(5, 4).bfloat16(), torch.zeros(2).long())),
+        (TypeError, lambda: linear_logps(torch.zeros(2, 4), torch.zeros(5, 4), torch.zeros(2).int())),
+        (ValueError, lambda: linear_logps(torch.zeros(2, 4), torch.zeros(5, 4), torch.zeros(2).long(), temperature=0.0)),
+        (ValueError, lambda: linear_logps(torch.zeros(2, 4), torch.zeros(0, 4), torch.zeros(2).long())),
+        (ValueError, lambda: pack_act8(lp, "int4")),
+        (TypeError, lambda: pack_act8(lp.double())),
+        (ValueError, lambda: pack_act8(lp, out=torch.empty(3, dtype=torch.uint8))),
+        (ValueError, lambda: unpack_act8(torch.empty(100, dtype=torch.uint8), (77,))),
+        (TypeError, lambda: unpack_act8(torch.empty(132, dtype=torch.uint8), (77,), torch.float64)),
+    ]
+    for i, (error, call) in enumerate(bad):
+        with pytest.raises(error):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+def test_c_entry_points_refuse_without_a_gpu():
+    from test1_amd import _native
+
+    hip = _native.hip()
+    one = 64   # an address that is never read: each call ends at its check
+    assert hip.sf_logps_rows(None, 8, 1, 8, one, -100, 1.0, one, one, None) == 9001
+    assert hip.sf_logps_rows(one, 6, 1, 8, one, -100, 1.0, one, one, None) == 9001
+    assert hip.sf_logps_rows(one, 9, 1, 8, one, -100, 1.0, one, one, None) == 9007
+    assert hip.sf_logps_rows(one, 8, 0, 8, one, -100, 1.0, one, one, None) == 0
+    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, None, one, 7, 8, None) == 9003
+    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, None, one, 1, 8, None) == 9005
+    assert hip.sf_logps_norm(None, one, -100, 1, 1.0, one, None) == hip.sf_logps_norm(one, one, -100, 1, 1.0, None, None) == 9001
+    assert hip.sf_align_parts(0, 5) == 0 and hip.sf_align_parts(4, 100) == 4
+    assert hip.sf_align_parts(4, 1 << 31) == 0 and hip.sf_align_parts(2, 1 << 20) == 2 * 512
+    pref = lambda **k: hip.sf_pref_loss(*{**dict(lp=one, ld=8, ref=one, ldr=8, m=one, ldm=8, p=1, c=8, f=0, b=0.1, s=0.0,  # noqa: E731
+                                                a=0, w=one, l=one, ch=one, r=one, co=None, st=None), **k}.values())
+    assert pref(lp=None) == pref(c=0) == pref(p=0) == pref(ld=7) == pref(f=3) == pref(b=0.0) == pref(s=2.0) == 9001
+    assert pref(w=8) == 9007
+    pol = lambda **k: hip.sf_policy_loss(*{**dict(lp=one, ld=8, o=one, ldo=8, r=None, ldr=0, a=one, lda=8, t=1, m=one, ldm=8,  # noqa: E731
+                                                  n=1, c=8, lo=-0.1, hi=0.1, k=0.0, s=0, w=one, l=one, kl=None, cl=one,
+                                                  sl=None, we=None, st=None), **k}.values())
+    assert pol(lp=None) == pol(n=0) == pol(lda=7) == pol(lo=0.5) == pol(hi=-1.0) == pol(r=one, ldr=8) == pol(kl=one) == 9001
+    assert pol(w=24) == 9007
+    assert hip.sf_pref_grad(one, one, one, 7, 1, 8, one, None) == hip.sf_policy_grad(one, None, one, 1, 8, one, None) == 9001
+    assert hip.sf_act8_pack(None, 1, 8, one, 0, None) == hip.sf_act8_unpack(one, 5, 8, 4096, 1, None) == 9001

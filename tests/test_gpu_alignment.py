@@ -1,0 +1,214 @@
+"""The preference and the policy loss on the GPU, against float64."""
+
+import math
+
+import pytest
+import torch
+
+from alignment_reference import near, policy, preference
+from test1_amd.alignment import policy_loss, preference_loss
+
+pytestmark = pytest.mark.gpu
+
+# one workgroup up to 16,384 tokens; beyond, parts of 1,024 tokens or a multiple
+SHAPES = [(2, 1), (2, 2), (4, 63), (2, 64), (6, 257), (2, 8192), (2, 8193), (64, 255), (66, 250), (2, 16385), (1026, 33),
+          (10, 5000), (2, 1_100_001)]
+
+
+def tokens(shape, dev, seed=0, empty_rows=True):
+    g = torch.Generator(device=dev).manual_seed(seed + 7 * shape[0] + shape[1])
+    rand = lambda *s: torch.rand(s, generator=g, device=dev)  # noqa: E731
+    randn = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    mask = rand(*shape) < 0.7
+    if empty_rows and shape[0] > 2:
+        mask[1] = False
+    lp = -3 * rand(*shape)
+    return mask, lp, lp + 0.2 * randn(*shape), lp + 0.3 * randn(*shape), randn(*shape)
+
+
+def spoil(mask, *tensors):
+    """What stands in masked places must not matter."""
+    bad = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(torch.float32).min], device=mask.device)
+    fill = bad[torch.arange(mask.numel(), device=mask.device) % 4].view(mask.shape)
+    return [torch.where(mask, t, fill) for t in tensors]
+
+
+@pytest.mark.parametrize("kind,smoothing,average", [("sigmoid", 0.0, False), ("sigmoid", 0.1, True), ("hinge", 0.0, False),
+                                                    ("ipo", 0.0, True)])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_preference_matches_float64(dev, shape, kind, smoothing, average):
+    mask, lp, ref, _, _ = tokens(shape, dev)
+    want, bound = preference(lp, ref, mask, 0.1, kind, smoothing, average)
+    lp, ref = spoil(mask, lp, ref)
+    lp.requires_grad_(True)
+    out = preference_loss(lp, ref, mask, 0.1, kind, smoothing, average)
+    (grad,) = torch.autograd.grad(out.loss, lp)
+    for g, w, b in zip((out.loss.detach(), out.chosen_rewards, out.rejected_rewards, grad), want, bound):
+        near(g, w, b)
+    with torch.no_grad():
+        again = preference_loss(lp, ref, mask, 0.1, kind, smoothing, average)
+    assert all(torch.equal(a, b) for a, b in zip(again, out))
+
+
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+@pytest.mark.parametrize("with_ref,per_token", [(True, True), (False, False), (True, False)])
+@pytest.mark.parametrize("shape", SHAPES + [(1, 1), (1, 20_000), (3, 7000), (20_000, 5)])
+def test_policy_matches_float64(dev, shape, with_ref, per_token, reduction):
+    mask, lp, old, ref, adv = tokens(shape, dev)
+    mask[0, 0] = True
+    if not per_token:
+        adv = adv[:, 0].contiguous()
+    ref = ref if with_ref else None
+    want, bound = policy(lp, old, adv, mask, ref, 0.2, 0.28, 0.05, reduction)
+    lp, old = spoil(mask, lp, old)
+    if with_ref:
+        (ref,) = spoil(mask, ref)
+    lp.requires_grad_(True)
+    out = policy_loss(lp, old, adv, mask, ref, 0.2, 0.28, 0.05, reduction)
+    (grad,) = torch.autograd.grad(out.loss, lp)
+    near(out.loss.detach(), want[0], bound[0])
+    if with_ref:
+        near(out.kl, want[1], bound[1])
+    else:
+        assert out.kl is None
+    near(out.clip_fraction, want[2], bound[2])
+    near(grad, want[3], bound[3])
+    with torch.no_grad():
+        again = policy_loss(lp, old, adv, mask, ref, 0.2, 0.28, 0.05, reduction)
+    assert torch.equal(again.loss, out.loss) and torch.equal(again.clip_fraction, out.clip_fraction)
+
+
+def test_small_kl_keeps_its_digits(dev):
+    """exp(q) - 1 - q of small q is q^2 / 2, not what cancellation leaves."""
+    lp = torch.zeros(1, 4096, device=dev)
+    q = torch.logspace(-6, 0, 4096, device=dev) * torch.tensor([1.0, -1.0], device=dev).repeat(2048)
+    for i in (0, 1000, 3000, 4095):
+        mask = torch.zeros(1, 4096, dtype=torch.bool, device=dev)
+        mask[0, i] = True
+        out = policy_loss(lp, lp, torch.zeros(1, device=dev), mask, q.view(1, -1), kl_coef=1.0)
+        x = q[i].double()
+        want = torch.expm1(x) - x if abs(x) > 1e-2 else x * x / 2 * (1 + x / 3 * (1 + x / 4 * (1 + x / 5)))
+        assert abs(out.kl.double() - want) <= 2.0 ** -21 * want
+
+
+def test_no_token_at_all(dev):
+    mask, lp, old, ref, adv = tokens((4, 300), dev)
+    mask[:] = False
+    lp.requires_grad_(True)
+    for how in ("token", "sequence"):
+        out = policy_loss(lp, old, adv, mask, ref, reduction=how)
+        (grad,) = torch.autograd.grad(out.loss, lp)
+        assert out.loss.isnan() and out.kl.isnan() and out.clip_fraction.isnan() and (grad == 0).all()
+    out = preference_loss(lp, ref, mask)
+    (grad,) = torch.autograd.grad(out.loss, lp)
+    assert abs(out.loss.item() - math.log(2)) < 1e-6 and (grad == 0).all() and (out.chosen_rewards == 0).all()
+
+
+@pytest.mark.parametrize("big", [False, True])
+def test_infinite_ratios(dev, big):
+    """A pair infinitely apart: loss 0 or infinity, never NaN, and a bounded gradient."""
+    t = 20_000 if big else 50
+    mask = torch.ones(4, t, dtype=torch.bool, device=dev)
+    lp = torch.zeros(4, t, device=dev)
+    lp[2, 3] = -math.inf   # the first pair's rejected sequence is impossible
+    lp.requires_grad_(True)
+    out = preference_loss(lp, torch.zeros(4, t, device=dev), mask)
+    assert abs(out.loss.item() - math.log(2) / 2) < 1e-6
+    (grad,) = torch.autograd.grad(out.loss, lp)
+    assert (grad[0] == 0).all() and (grad[2] == 0).all() and grad[1].isfinite().all() and (grad[1] < 0).all()
+
+
+def test_strided_rows_and_broadcast(dev):
+    shape = (6, 301)
+    mask, lp, old, ref, adv = tokens((6, 700), dev)
+    cut = [t[:, 5:306] for t in (lp, old, ref, adv)]
+    m = mask[:, 5:306]
+    whole = [t.contiguous() for t in cut]
+    a = policy_loss(cut[0].requires_grad_(True), cut[1], cut[3], m, cut[2], kl_coef=0.1)
+    b = policy_loss(whole[0].requires_grad_(True), whole[1], whole[3], m.contiguous(), whole[2], kl_coef=0.1)
+    assert torch.equal(a.loss, b.loss) and torch.equal(torch.autograd.grad(a.loss, cut[0])[0],
+                                                        torch.autograd.grad(b.loss, whole[0])[0])
+    lpt = whole[0].detach().t().contiguous().t().requires_grad_(True)   # columns side by side
+    c = preference_loss(lpt, whole[2], m)
+    d = preference_loss(whole[0], whole[2], m.contiguous())
+    assert torch.equal(c.loss, d.loss) and torch.equal(torch.autograd.grad(c.loss, lpt)[0],
+                                                        torch.autograd.grad(d.loss, whole[0])[0])
+    one = torch.zeros(1, 1, device=dev).expand(shape)   # every token shares one element
+    e = policy_loss(whole[0], whole[1], adv[:, 0].expand(6), m, one, kl_coef=0.1)
+    f = policy_loss(whole[0], whole[1], adv[:, 0].contiguous(), m, one.contiguous(), kl_coef=0.1)
+    assert torch.equal(e.loss, f.loss)
+    g = policy_loss(whole[0], whole[1], adv.t()[0], m, None)   # advantages with a stride
+    h = policy_loss(whole[0], whole[1], adv[:, 0].contiguous(), m, None)
+    assert adv.t()[0].shape == (6,) or True
+    assert torch.equal(g.loss, h.loss)
+
+
+def test_gradients_against_differences(dev):
+    """In 64 bits on the host form, whose gradient the kernels' is then held to."""
+    mask, lp, old, ref, adv = tokens((4, 40), dev)
+    d = [t.double().cpu() for t in (lp, old, ref, adv)]
+    m = mask.cpu()
+    from test1_amd.alignment import _policy_torch, _pref_torch
+    f = lambda x: _policy_torch(x, d[1], d[3], m, d[2], math.log(0.8), math.log(1.2), 0.1, False).loss  # noqa: E731
+    g = lambda x: _pref_torch(x, d[2], m, "sigmoid", 0.1, 0.1, False).loss  # noqa: E731
+    x = d[0].clone().requires_grad_(True)
+    assert torch.autograd.gradcheck(f, (x,)) and torch.autograd.gradcheck(g, (x,))
+    lp.requires_grad_(True)
+    got = torch.autograd.grad(policy_loss(lp, old, adv, mask, ref, kl_coef=0.1).loss, lp)[0].cpu().double()
+    want = torch.autograd.grad(f(x), x)[0]
+    assert ((got - want).abs() <= 1e-5 * want.abs().max()).all()
+    got = torch.autograd.grad(preference_loss(lp, ref, mask, label_smoothing=0.1).loss, lp)[0].cpu().double()
+    want = torch.autograd.grad(g(x), x)[0]
+    assert ((got - want).abs() <= 1e-5 * want.abs().max()).all()
+
+
+def test_upstream_gradient_retained_graph_and_no_double_backward(dev):
+    mask, lp, old, ref, adv = tokens((4, 300), dev)
+    lp.requires_grad_(True)
+    for call in (lambda: policy_loss(lp, old, adv, mask, ref, kl_coef=0.1).loss, lambda: preference_loss(lp, ref, mask).loss):
+        loss = call()
+        one = torch.autograd.grad(loss, lp, retain_graph=True)[0]
+        three = torch.autograd.grad(loss, lp, torch.full_like(loss, 4.0), retain_graph=True)[0]
+        assert torch.equal(three, 4 * one)   # a power of two
+        assert torch.equal(torch.autograd.grad(-4 * loss, lp)[0], -4 * one)
+        g = torch.autograd.grad(call(), lp, create_graph=True)[0]
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), lp)
+
+
+def test_another_stream_and_a_captured_step(dev):
+    mask, lp, old, ref, adv = tokens((40, 700), dev)
+    lp.requires_grad_(True)
+    want = torch.autograd.grad(policy_loss(lp, old, adv, mask, ref, kl_coef=0.1).loss, lp)[0]
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = torch.autograd.grad(policy_loss(lp, old, adv, mask, ref, kl_coef=0.1).loss, lp)[0]
+        torch.autograd.grad(preference_loss(lp, ref, mask).loss, lp)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = policy_loss(lp, old, adv, mask, ref, kl_coef=0.1).loss + preference_loss(lp, ref, mask).loss
+        grad = torch.autograd.grad(loss, lp)[0]
+    for k in range(3):
+        with torch.no_grad():
+            lp.sub_(0.01)
+        graph.replay()
+        eager = policy_loss(lp, old, adv, mask, ref, kl_coef=0.1).loss + preference_loss(lp, ref, mask).loss
+        assert torch.equal(loss, eager) and torch.equal(grad, torch.autograd.grad(eager, lp)[0])
+
+
+def test_transforms_take_torch_operations(dev):
+    mask, lp, old, ref, adv = tokens((4, 30), dev)
+    loss = lambda x: policy_loss(x, old, adv, mask, ref, kl_coef=0.1).loss  # noqa: E731
+    want = torch.autograd.grad(loss(lp.requires_grad_(True)), lp)[0]
+    got = torch.func.grad(loss)(lp.detach())
+    assert torch.allclose(got, want, rtol=1e-4, atol=1e-7)
+    batch = torch.stack([lp.detach(), lp.detach() - 0.1])
+    per = torch.func.vmap(loss)(batch)
+    assert torch.allclose(per[1], loss(lp.detach() - 0.1), rtol=1e-5)
+    _, tangent = torch.func.jvp(loss, (lp.detach(),), (torch.ones_like(lp),))
+    assert torch.allclose(tangent, want.sum(), rtol=1e-3, atol=1e-6)
+    pref = lambda x: preference_loss(x, ref, mask).loss  # noqa: E731
+    assert torch.allclose(torch.func.grad(pref)(lp.detach()), torch.autograd.grad(pref(lp), lp)[0], rtol=1e-4, atol=1e-8)

@@ -1,0 +1,184 @@
+"""Token log-probabilities of the output unit on the GPU, against float64."""
+
+import math
+
+import pytest
+import torch
+
+from alignment_reference import logps, near
+from test1_amd import linear_logps as module
+from test1_amd.linear_logps import linear_logps
+
+pytestmark = pytest.mark.gpu
+
+# tokens, hidden, vocabulary: tiles and their edges, odd hidden sizes, one token, one word
+SHAPES = [(1, 64, 512), (1, 64, 1), (3, 8, 5), (7, 128, 257), (33, 65, 1000), (64, 64, 256), (65, 128, 255), (128, 192, 1021),
+          (129, 256, 4099), (255, 64, 2048), (256, 512, 128), (257, 320, 777), (300, 896, 1540), (513, 128, 513),
+          (40, 1024, 50_257)]
+
+
+def inputs(shape, dtype, dev, seed=0):
+    n, h, v = shape
+    g = torch.Generator(device=dev).manual_seed(seed + n + h + v)
+    hidden = torch.randn(n, h, generator=g, device=dev).to(dtype)
+    weight = (torch.randn(v, h, generator=g, device=dev) * (2.0 / math.sqrt(h))).to(dtype)
+    labels = torch.randint(0, v, (n,), generator=g, device=dev)
+    labels[0] = v - 1
+    if n > 2:
+        labels[1], labels[2] = -100, 0
+    up = torch.randn(n, generator=g, device=dev) / n
+    return hidden, weight, labels, up
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_matches_float64(dev, shape, dtype):
+    hidden, weight, labels, up = inputs(shape, dtype, dev)
+    scale = 1.0 if shape[0] % 2 else 1 / 0.7
+    want, bound = logps(hidden, weight, labels, scale, grad=up)
+    with torch.no_grad():
+        alone = linear_logps(hidden, weight, labels, temperature=1 / scale)
+    near(alone, want[0], bound[0])
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels, temperature=1 / scale)
+    gh, gw = torch.autograd.grad(lp, (hidden, weight), up)
+    assert gh.dtype == gw.dtype == dtype and lp.dtype == torch.float32
+    for got, w, b in zip((lp.detach(), gh, gw), want, bound):
+        near(got, w, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_labels_ignored_and_outside(dev, dtype):
+    hidden, weight, labels, up = inputs((70, 64, 300), dtype, dev)
+    labels[:] = -100
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    up[3] = math.nan   # an ignored token has no gradient whatever arrives
+    gh, gw = torch.autograd.grad(lp, (hidden, weight), up)
+    assert (lp == 0).all() and (gh == 0).all() and (gw == 0).all()
+    labels[5], labels[6], labels[7], labels[8] = 300, -1, 299, 1 << 40
+    lp = linear_logps(hidden, weight, labels)
+    assert lp[[5, 6, 8]].isnan().all() and lp[7].isfinite() and (lp[9:] == 0).all()
+    gh, _ = torch.autograd.grad(lp, (hidden, weight), torch.ones_like(lp))
+    assert gh[[5, 6, 8]].isnan().all() and gh[7].isfinite().all() and (gh[9:] == 0).all()
+    assert linear_logps(hidden, weight, labels, ignore_index=300)[5] == 0
+
+
+def test_logits_that_are_not_finite(dev):
+    """As log_softmax gives them: a NaN or an infinity in a row of hidden states
+    stays in its row; a logit of -infinity leaves the others as they are."""
+    hidden, weight, labels, _ = inputs((70, 64, 300), torch.bfloat16, dev)
+    hidden[4, 3] = math.nan
+    hidden[9, 5] = math.inf
+    lp = linear_logps(hidden, weight, labels)
+    assert lp[4].isnan() and not lp[9].isfinite()
+    keep = [i for i in range(70) if i not in (4, 9)]
+    assert lp[keep].isfinite().all()
+    hidden[4, 3] = hidden[9, 5] = 1.0
+    hidden[:, 0] = hidden[:, 0].abs() + 0.1
+    weight[7, 0] = -math.inf
+    labels[labels == 7] = 8
+    labels[20] = 7
+    lp = linear_logps(hidden, weight, labels)
+    w = torch.cat([weight[:7], weight[8:]])
+    lab = torch.where(labels > 7, labels - 1, labels)
+    want, bound = logps(hidden, w, lab)
+    assert lp[20] == -math.inf
+    keep = [i for i in range(70) if i != 20]
+    near(lp[keep], want[0][keep], bound[0][keep])
+
+
+def test_large_logits(dev):
+    """Far beyond what exp takes, and a distribution on one word."""
+    hidden, weight, labels, up = inputs((70, 128, 600), torch.bfloat16, dev)
+    hidden *= 300
+    want, bound = logps(hidden, weight, labels, grad=up)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    near(lp.detach(), want[0], bound[0])
+    for got, w, b in zip(torch.autograd.grad(lp, (hidden, weight), up), want[1:], bound[1:]):
+        near(got, w, b)
+
+
+def test_strides_shapes_and_parts_of_the_gradient(dev):
+    hidden, weight, labels, up = inputs((12 * 30, 128, 700), torch.bfloat16, dev)
+    h3, y2 = hidden.view(12, 30, 128), labels.view(12, 30)
+    a = linear_logps(h3[:, :-1], weight, y2[:, 1:])
+    b = linear_logps(h3[:, :-1].contiguous().view(-1, 128), weight, y2[:, 1:].contiguous().view(-1))
+    assert a.shape == (12, 29) and torch.equal(a.reshape(-1), b)
+    wide = torch.randn(700, 256, device=dev).bfloat16()
+    wide[:, 64:192] = weight
+    assert torch.equal(linear_logps(hidden, wide[:, 64:192], labels), linear_logps(hidden, weight, labels))
+    turned = weight.t().contiguous().t()
+    assert torch.allclose(linear_logps(hidden, turned, labels), linear_logps(hidden, weight, labels), atol=1e-4)
+    odd = torch.empty(360 * 128 + 1, dtype=torch.bfloat16, device=dev)[1:].view(360, 128).copy_(hidden)
+    assert torch.allclose(linear_logps(odd, weight, labels), linear_logps(hidden, weight, labels), atol=1e-4)
+    hr, wr = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+    both = torch.autograd.grad(linear_logps(hr, wr, labels), (hr, wr), up)
+    assert torch.equal(torch.autograd.grad(linear_logps(hr, weight, labels), hr, up)[0], both[0])
+    assert torch.equal(torch.autograd.grad(linear_logps(hidden, wr, labels), wr, up)[0], both[1])
+    shared = torch.autograd.grad(linear_logps(hr, wr, labels).sum(), (hr, wr))   # an expanded gradient
+    whole = torch.autograd.grad(linear_logps(hr, wr, labels), (hr, wr), torch.ones(360, device=dev))
+    assert all(torch.equal(x, y) for x, y in zip(shared, whole))
+
+
+def test_no_rows(dev):
+    hidden = torch.zeros(0, 64, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    weight = torch.randn(100, 64, device=dev).bfloat16().requires_grad_(True)
+    lp = linear_logps(hidden, weight, torch.zeros(0, dtype=torch.int64, device=dev))
+    gh, gw = torch.autograd.grad(lp.sum(), (hidden, weight))
+    assert lp.shape == (0,) and gh.shape == (0, 64) and (gw == 0).all()
+
+
+def test_once_differentiable_and_transforms(dev):
+    hidden, weight, labels, up = inputs((20, 64, 100), torch.bfloat16, dev)
+    hr = hidden.clone().requires_grad_(True)
+    g = torch.autograd.grad(linear_logps(hr, weight, labels).sum(), hr, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.float().sum(), hr)
+    f = lambda x: (linear_logps(x, weight, labels) * up).sum()  # noqa: E731
+    got, want = torch.func.grad(f)(hidden), torch.autograd.grad(f(hr), hr)[0]
+    assert torch.allclose(got.float(), want.float(), rtol=0.02, atol=1e-4)
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert torch.equal(linear_logps(hidden, weight, labels), linear_logps(hidden, weight, labels))
+        got = linear_logps(hidden, weight, labels)
+    assert torch.equal(got, linear_logps(hidden, weight, labels))
+
+
+def test_replays_of_a_captured_step(dev):
+    hidden, weight, labels, up = inputs((300, 128, 1000), torch.bfloat16, dev)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(linear_logps(hidden, weight, labels), (hidden, weight), up)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lp = linear_logps(hidden, weight, labels)
+        gh, gw = torch.autograd.grad(lp, (hidden, weight), up)
+    for _ in range(3):
+        with torch.no_grad():
+            hidden.mul_(0.9)
+        torch.cuda.synchronize()
+        graph.replay()
+        want = linear_logps(hidden, weight, labels)
+        assert torch.equal(lp, want)
+        assert all(torch.equal(a, b) for a, b in zip((gh, gw), torch.autograd.grad(want, (hidden, weight), up)))
+
+
+def test_chunks(dev, monkeypatch):
+    """The same results however many rows are taken at a time."""
+    hidden, weight, labels, up = inputs((300, 128, 1000), torch.float32, dev)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    want, bound = logps(hidden.detach(), weight.detach(), labels, grad=up)
+    monkeypatch.setattr(module, "_chunk_rows", lambda vocab: 77)
+    lp = linear_logps(hidden, weight, labels)
+    got = (lp.detach(), *torch.autograd.grad(lp, (hidden, weight), up))
+    for x, w, b in zip(got, want, bound):
+        near(x, w, b)
