@@ -318,21 +318,63 @@ int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab,
                   const int64_t* labels, int64_t ignore_index, float scale,
                   float* lse, float* logp, sf_stream_t stream);
 
-/* norm[0] = a power of two that brings the largest finite |scale * grad[i]| of
- * the rows that are not ignored into [1, 2), norm[1] = its inverse, norm[2] =
- * 1 (three elements of device memory). */
-int sf_logps_norm(const float* grad, const int64_t* labels, int64_t ignore_index,
-                  size_t rows, float scale, float* norm, sf_stream_t stream);
+/* The same for 16-bit operands, the product included: logits = scale * hidden
+ * weight^T of the [rows, hidden_size] hidden rows (ldh elements apart) and the
+ * [vocab, hidden_size] weight (ldw), of dtype SF_DTYPE_BF16 or SF_DTYPE_F16.
+ * lse2 = the row's logsumexp in base 2, logp as above.  parts: workspace of
+ * ceil(vocab / SF_LOGPS_SPAN) * rows * 2 floats, for each span of words its
+ * largest scaled logit m in base 2 and the sum of 2^(logit - m); target: of rows
+ * floats.  keep (or null): [rows, ld_keep] of dtype, every 2^(logit - m), 0
+ * behind the vocabulary up to the next whole span, for sf_logps_keep_grad.
+ * hidden_size is a multiple of 64, ldw and ldh (at most 2^22) and ld_keep of 8,
+ * weight, hidden and keep start on 16-byte boundaries (SF_EALIGN). */
+#define SF_LOGPS_SPAN 256
+int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab,
+                   const void* hidden, size_t ldh, size_t rows,
+                   size_t hidden_size, const int64_t* labels,
+                   int64_t ignore_index, float scale, int dtype, void* parts,
+                   float* target, void* keep, size_t ld_keep, float* lse2,
+                   float* logp, sf_stream_t stream);
 
-/* The gradient of such a chunk: dz[i, j] = grad[i] * scale * ((j == labels[i])
- * - exp(scale * logits[i, j] - lse[i])), times norm[0] where norm is not null,
- * as dtype with ld_dz elements from row to row; 0 for an ignored row, NaN for a
- * label outside [0, vocab).  SF_DTYPE_F32: dz may be the logits themselves;
- * other types: no overlap. */
+/* The gradient of such logits is row_weight[i] * D[i, j], D = ((j == label) -
+ * p) / (1 - p_label): 1 at the label.  row_weight = grad * scale * (1 -
+ * p_label); 0 for an ignored row, NaN for a label outside [0, vocab).  norm (or
+ * null: 1): two floats; the weights are then divided by the power of two
+ * norm[0] that leaves the largest in [1, 2), and norm[1] = 1. */
+int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
+                    int64_t ignore_index, size_t rows, size_t vocab,
+                    float scale, float* row_weight, float* norm,
+                    sf_stream_t stream);
+
+/* D in place of what sf_logps_tiles kept, with its parts, lse2 and logp; rows
+ * without a label that counts become 0 (NaN for a label outside [0, vocab)),
+ * and so do the rows from `rows` up to `padded`.  ld is a multiple of
+ * SF_LOGPS_SPAN (SF_EALIGN). */
+int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
+                       size_t vocab, const void* parts, const int64_t* labels,
+                       int64_t ignore_index, const float* lse2,
+                       const float* logp, int dtype, sf_stream_t stream);
+
+/* D of fp32 logits (as sf_logps_rows takes them, with its lse and logp), as
+ * dtype with ld_dz elements from row to row.  SF_DTYPE_F32: dz may be the
+ * logits themselves; other types: no overlap. */
 int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab,
                   const int64_t* labels, int64_t ignore_index, float scale,
-                  const float* lse, const float* grad, const float* norm,
-                  void* dz, int dtype, size_t ld_dz, sf_stream_t stream);
+                  const float* lse, const float* logp, void* dz, int dtype,
+                  size_t ld_dz, sf_stream_t stream);
+
+/* hidden_t[j, i] = row_weight[i] * hidden[i, j], rounded once; otherwise as
+ * sf_ce_hidden, without a tail. */
+int sf_logps_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols,
+                    const float* row_weight, int dtype, void* hidden_t,
+                    size_t ldt, sf_stream_t stream);
+
+/* As sf_ce_sum, also of one part, each row times row_weight[i], and times
+ * norm[0] where norm is not null. */
+int sf_logps_sum(const float* parts, int nparts, size_t rows, size_t cols,
+                 void* out, int dtype, const void* d_tail, size_t ld,
+                 const void* w_tail, size_t tail, const float* row_weight,
+                 const float* norm, sf_stream_t stream);
 
 /* Forms of the preference loss. */
 #define SF_PREF_SIGMOID 0

@@ -42,6 +42,7 @@ SF_ETOOBIG = 9008
 SF_ETIMEDOUT = 9009
 SF_STAGE_SCRATCH_ELEMS = 16 << 20
 SF_CE_LOSS_PARTS = 256
+SF_LOGPS_SPAN = 256
 SF_PREF_SIGMOID = 0
 SF_PREF_HINGE = 1
 SF_PREF_IPO = 2
@@ -104,8 +105,12 @@ HIP_SIGNATURES = {
     "sf_ce_weight_grad": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _vp, _sz, _i, _vp],
     "sf_ce_scale": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _i, _vp],
     "sf_logps_rows": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp],
-    "sf_logps_norm": [_vp, _vp, ctypes.c_int64, _sz, _f, _vp, _vp],
-    "sf_logps_grad": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp, _vp, _i, _sz, _vp],
+    "sf_logps_tiles": [_vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _i, _vp, _vp, _vp, _sz, _vp, _vp, _vp],
+    "sf_logps_weight": [_vp, _vp, _vp, ctypes.c_int64, _sz, _sz, _f, _vp, _vp, _vp],
+    "sf_logps_keep_grad": [_vp, _sz, _sz, _sz, _sz, _vp, _vp, ctypes.c_int64, _vp, _vp, _i, _vp],
+    "sf_logps_grad": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp, _i, _sz, _vp],
+    "sf_logps_hidden": [_vp, _sz, _sz, _sz, _vp, _i, _vp, _sz, _vp],
+    "sf_logps_sum": [_vp, _i, _sz, _sz, _vp, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp],
     "sf_align_parts": [_sz, _sz],
     "sf_pref_loss": [_vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _i, _f, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     "sf_pref_grad": [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp],

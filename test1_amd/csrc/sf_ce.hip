@@ -23,6 +23,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/slidefsdp.h"
 #include "sf_common.h"
 
@@ -370,11 +372,12 @@ __global__ __launch_bounds__(kScaleThreads) void ce_scale32_kernel(
 constexpr int kTr = 64;
 constexpr int kTrThreads = 256;
 constexpr int kTrLd = kTr + 2;
-template <bool kVec>   // rows on 16-byte boundaries, hidden a multiple of 8
+// With Fmt each row is multiplied by its element of `by`, rounded once.
+template <bool kVec, typename Fmt = void>   // kVec: rows on 16-byte boundaries, hidden a multiple of 8
 __global__ __launch_bounds__(kTrThreads) void ce_hidden_kernel(const uint16_t* __restrict__ hidden, uint64_t ldh,
                                                                uint64_t rows, uint64_t cols, uint16_t* __restrict__ out,
                                                                uint64_t ldt, uint32_t tiles, u32x4* __restrict__ tail,
-                                                               uint64_t tail_groups) {
+                                                               uint64_t tail_groups, const float* __restrict__ by) {
     __shared__ __attribute__((aligned(16))) uint16_t tile[kTr * kTrLd];
     if (blockIdx.x >= tiles) {
         const uint64_t stride = uint64_t(gridDim.x - tiles) * kTrThreads;
@@ -396,6 +399,11 @@ __global__ __launch_bounds__(kTrThreads) void ce_hidden_kernel(const uint16_t* _
 #pragma unroll
                 for (int j = 0; j < kGroup; ++j)
                     if (col0 + c + j < cols) v[j / 2] |= uint32_t(p[j]) << (j % 2 * 16);
+            }
+            if constexpr (!std::is_void<Fmt>::value) {
+                const float f = by[row0 + r];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = Fmt::pack(Fmt::lo(v[j]) * f, Fmt::hi(v[j]) * f);
             }
         }
         uint32_t* t = reinterpret_cast<uint32_t*>(tile + r * kTrLd + c);
@@ -425,11 +433,14 @@ __global__ __launch_bounds__(kTrThreads) void ce_hidden_kernel(const uint16_t* _
 // 1024 x 32000 371 | 285.  Bound by the parts' reads, at most 134 MB, which the
 // last-level cache still holds in part.
 constexpr int kSumThreads = 128;
-template <typename Fmt, int kParts>
+// kWeighted: each row times its element of `by`, and times *norm if there is one.
+template <typename Fmt, int kParts, bool kWeighted = false>
 __global__ __launch_bounds__(kSumThreads) void ce_sum_kernel(const float* __restrict__ parts, uint32_t count,
                                                              uint32_t cols, uint16_t* __restrict__ out,
                                                              const uint16_t* __restrict__ g, uint64_t ld,
-                                                             const uint16_t* __restrict__ w, uint32_t tail) {
+                                                             const uint16_t* __restrict__ w, uint32_t tail,
+                                                             const float* __restrict__ by,
+                                                             const float* __restrict__ norm) {
     const uint32_t i = (blockIdx.x * kSumThreads + threadIdx.x) * kGroup;
     if (i >= count) return;
     f32x4 a[kParts], b[kParts];
@@ -464,6 +475,11 @@ __global__ __launch_bounds__(kSumThreads) void ce_sum_kernel(const float* __rest
         }
         a[0] += ta;
         b[0] += tb;
+    }
+    if constexpr (kWeighted) {
+        const float f = by[i / cols], n = norm != nullptr ? *norm : 1.0f;
+        a[0] = a[0] * f * n;
+        b[0] = b[0] * f * n;
     }
     *reinterpret_cast<u32x4*>(out + i) = pack8<Fmt>(a[0], b[0]);
 }
@@ -598,16 +614,18 @@ int launch_scale(Kernel kernel, const float* grad_loss, const float* n_valid, co
     return SF_OK;
 }
 
-template <typename Fmt>
+template <typename Fmt, bool kWeighted = false>
 int launch_sum(int nparts, const float* parts, uint32_t count, uint32_t cols, void* out, const void* g, size_t ld,
-               const void* w, uint32_t tail, hipStream_t st) {
-    const auto kernel = nparts == 2   ? ce_sum_kernel<Fmt, 2>
-                        : nparts == 4 ? ce_sum_kernel<Fmt, 4>
-                        : nparts == 8 ? ce_sum_kernel<Fmt, 8>
-                                      : ce_sum_kernel<Fmt, 16>;
+               const void* w, uint32_t tail, hipStream_t st, const float* by = nullptr, const float* norm = nullptr) {
+    auto kernel = nparts == 2   ? ce_sum_kernel<Fmt, 2, kWeighted>
+                  : nparts == 4 ? ce_sum_kernel<Fmt, 4, kWeighted>
+                  : nparts == 8 ? ce_sum_kernel<Fmt, 8, kWeighted>
+                                : ce_sum_kernel<Fmt, 16, kWeighted>;
+    if constexpr (kWeighted)
+        if (nparts == 1) kernel = ce_sum_kernel<Fmt, 1, true>;
     hipLaunchKernelGGL(kernel, dim3((count / kGroup + kSumThreads - 1) / kSumThreads), dim3(kSumThreads), 0, st, parts,
                        count, cols, static_cast<uint16_t*>(out), static_cast<const uint16_t*>(g), uint64_t(ld),
-                       static_cast<const uint16_t*>(w), tail);
+                       static_cast<const uint16_t*>(w), tail, by, norm);
     return status();
 }
 
@@ -713,7 +731,27 @@ int sf_ce_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols, void*
     hipLaunchKernelGGL((vec ? ce_hidden_kernel<true> : ce_hidden_kernel<false>), dim3(uint32_t(tiles + clear)),
                        dim3(kTrThreads), 0, reinterpret_cast<hipStream_t>(stream), static_cast<const uint16_t*>(hidden),
                        uint64_t(ldh), uint64_t(rows), uint64_t(cols), static_cast<uint16_t*>(hidden_t), uint64_t(ldt),
-                       uint32_t(tiles), static_cast<u32x4*>(tail), groups);
+                       uint32_t(tiles), static_cast<u32x4*>(tail), groups, static_cast<const float*>(nullptr));
+    return status();
+}
+
+int sf_logps_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols, const float* row_weight, int dtype,
+                    void* hidden_t, size_t ldt, sf_stream_t stream) {
+    if (rows == 0 || cols == 0) return SF_OK;
+    if (hidden == nullptr || row_weight == nullptr || hidden_t == nullptr || ldh < cols || ldt % kTr != 0 ||
+        ldt < rows || ldt - rows >= kTr || misaligned(hidden, 2))
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (misaligned(hidden_t, 16)) return SF_EALIGN;
+    const uint64_t tiles = uint64_t(ldt / kTr) * ((cols + kTr - 1) / kTr);
+    if (tiles > kMaxLanes / kTrThreads) return SF_EINVAL;
+    const bool vec = !misaligned(hidden, 16) && ldh % kGroup == 0 && cols % kGroup == 0;
+    const auto kernel = dtype == SF_DTYPE_BF16 ? (vec ? ce_hidden_kernel<true, Bf16> : ce_hidden_kernel<false, Bf16>)
+                                               : (vec ? ce_hidden_kernel<true, F16> : ce_hidden_kernel<false, F16>);
+    hipLaunchKernelGGL(kernel, dim3(uint32_t(tiles)), dim3(kTrThreads), 0, reinterpret_cast<hipStream_t>(stream),
+                       static_cast<const uint16_t*>(hidden), uint64_t(ldh), uint64_t(rows), uint64_t(cols),
+                       static_cast<uint16_t*>(hidden_t), uint64_t(ldt), uint32_t(tiles), static_cast<u32x4*>(nullptr),
+                       uint64_t(0), row_weight);
     return status();
 }
 
@@ -734,6 +772,30 @@ int sf_ce_sum(const float* parts, int nparts, size_t rows, size_t cols, void* ou
         return launch_sum<Bf16>(nparts, parts, count, uint32_t(cols), out, g_tail, ld, w_tail, uint32_t(tail), st);
     if (dtype == SF_DTYPE_F16)
         return launch_sum<F16>(nparts, parts, count, uint32_t(cols), out, g_tail, ld, w_tail, uint32_t(tail), st);
+    return SF_EDTYPE;
+}
+
+int sf_logps_sum(const float* parts, int nparts, size_t rows, size_t cols, void* out, int dtype, const void* d_tail,
+                 size_t ld, const void* w_tail, size_t tail, const float* row_weight, const float* norm,
+                 sf_stream_t stream) {
+    if (rows == 0 || cols == 0) return SF_OK;
+    if (parts == nullptr || out == nullptr || row_weight == nullptr ||
+        (nparts != 1 && nparts != 2 && nparts != 4 && nparts != 8 && nparts != 16))
+        return SF_EINVAL;
+    if (tail >= size_t(kGroup) * size_t(nparts) || (tail > 0 && (d_tail == nullptr || w_tail == nullptr || ld < tail)))
+        return SF_EINVAL;
+    if (cols > (size_t(1) << 31) || rows > (size_t(1) << 31) / cols) return SF_EINVAL;
+    if (cols % kGroup != 0 || misaligned(parts, 16) || misaligned(out, 16) || (tail > 0 && misaligned(w_tail, 16)) ||
+        (tail > 0 && misaligned(d_tail, 2)))
+        return SF_EALIGN;
+    const uint32_t count = uint32_t(rows * cols);
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (dtype == SF_DTYPE_BF16)
+        return launch_sum<Bf16, true>(nparts, parts, count, uint32_t(cols), out, d_tail, ld, w_tail, uint32_t(tail), st,
+                                      row_weight, norm);
+    if (dtype == SF_DTYPE_F16)
+        return launch_sum<F16, true>(nparts, parts, count, uint32_t(cols), out, d_tail, ld, w_tail, uint32_t(tail), st,
+                                     row_weight, norm);
     return SF_EDTYPE;
 }
 

@@ -1,18 +1,308 @@
-// Log-probabilities of given tokens under the output unit, and their
-// gradient, for MI355X (gfx950).
+// Log-probabilities of given tokens under the output unit, and the gradient
+// of its logits, for MI355X (gfx950).
+//
+// With logits z = scale * hidden weight^T, a token's log-probability is z_y -
+// log sum_j exp z_j.  16-bit operands go through logps_tiles_kernel, the
+// product and the softmax's sums in one: a 256-word tile of a token's logits
+// never leaves the registers, only its maximum and its sum of exponentials do
+// (8 bytes for 256 logits), and the joined sums give the result.  Where a
+// gradient will be wanted the exponentials themselves are kept, relative to
+// their tile's maximum, 2 bytes a logit: from those a probability is off by a
+// rounding of itself, from logits in 16 bits by up to 2^-9 of the logit.
+// Others (fp32, hidden sizes that are no multiple of 64, unaligned rows) have
+// their logits made by a library product in chunks of fp32 and read once.
+//
+// The gradient by the logits of token i is g_i (onehot - p).  Its operand of the
+// two products is D = (onehot - p) / (1 - p_y), 1 at the label, and g_i (1 -
+// p_y) multiplies a row of the hidden gradient afterwards, a hidden row before
+// the weight gradient's product.  The label's element is the largest one: in D
+// it is exact, where rounding g (onehot - p) to 16 bits cost as much as the
+// results' own rounding (relative error of both gradients 2.4e-3 before,
+// 1.7e-3 being the rounding alone).
 //
 // C ABI: include/slidefsdp.h.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/slidefsdp.h"
 #include "sf_common.h"
 
 namespace {
 
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLeastRest = 0x1p-24f;   // of 1 - p_y, so that it can be divided by
+
+// 1 - p of a log-probability.
+__device__ __forceinline__ float rest_of(float logp) { return fmaxf(-expm1f(logp), kLeastRest); }
+
+// ---------------------------------------------------------------------
+// The product with the softmax's sums.  A workgroup has a tile of 256 words
+// by kBT tokens, a wave kFV x kFT products of 16 x 16 (words are the rows of
+// the product: a lane then holds 4 kFV words of each of its kFT tokens, and a
+// token's sums take two exchanges between lanes).
+//
+// The operands go from memory to LDS without passing registers, 64 terms of
+// the sum at a time in two buffers, 16-byte chunk c of row r at c ^ (r % 8) so
+// that a wave's reads of a column of chunks touch every bank.  The products of
+// one half (32 terms) run while the operands of the next are read from LDS;
+// one barrier for each 64 terms, at which the next buffer has arrived (it had
+// the time of 64 terms) and this one is free.
+//
+// Workgroups that run side by side on an XCD take neighbouring tiles, up to 8
+// of tokens by 4 of words: what they read is in its L2 once.
+// ---------------------------------------------------------------------
+constexpr int kSpan = SF_LOGPS_SPAN;   // words of a tile
+constexpr int kTerms = 64;             // of a buffer
+constexpr int kRowBytes = kTerms * 2;
+constexpr int kGroupT = 8;             // tiles of tokens that run side by side
+
+struct Tiles {
+    const uint16_t* weight;   // [vocab, 64 steps], ldw
+    const uint16_t* hidden;   // [tokens, 64 steps], ldh
+    uint32_t ldw, ldh, vocab, tokens, steps;
+    const int64_t* labels;
+    float scale2;             // scale * log2(e)
+    float2* parts;            // [tiles of words, tokens] maximum in base 2 and sum
+    float* target;            // [tokens] the label's product, unscaled
+    uint16_t* keep;           // [tokens, ld_keep] or null
+    uint64_t ld_keep;
+};
+
+// Interleaves what a half's products run beside: kLoads copies into LDS, then
+// kReads reads of it, two products each; all else after.
+template <int kReads, int kMul, int kLoads>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);   // memory
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // product
+    }
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kMul, 0);
+}
+
+template <typename Fmt, int kWV, int kWT, int kFV, int kFT, bool kKeep>
+__global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Tiles a) {
+    constexpr int kWaves = kWV * kWT, kBV = kWV * kFV * 16, kBT = kWT * kFT * 16;
+    static_assert(kBV == kSpan, "a tile is one span of words");
+    constexpr int kBuffer = (kBV + kBT) * kRowBytes;
+    constexpr int kLV = kBV / 8 / kWaves, kLT = kBT / 8 / kWaves;   // a wave copies 8 rows at once
+    static_assert(kLV * 8 * kWaves == kBV && kLT * 8 * kWaves == kBT, "rows divide among the waves");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer];
+
+    // a contiguous run of tiles for each XCD (workgroups go to them in turn)
+    const uint32_t tiles_v = (a.vocab + kBV - 1) / kBV, tiles_t = (a.tokens + kBT - 1) / kBT;
+    const uint32_t xcd = blockIdx.x % 8, each = gridDim.x / 8, more = gridDim.x % 8;
+    const uint32_t id = xcd * each + min(xcd, more) + blockIdx.x / 8;
+    const uint32_t first_t = id / (kGroupT * tiles_v) * kGroupT, group_t = min(uint32_t(kGroupT), tiles_t - first_t);
+    const uint32_t in = id - first_t * tiles_v;
+    const uint32_t tile_v = in / group_t, v0 = tile_v * kBV, t0 = (first_t + in % group_t) * kBT;
+
+    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint8_t* gv = reinterpret_cast<const uint8_t*>(a.weight + uint64_t(v0) * a.ldw);
+    const uint8_t* gt = reinterpret_cast<const uint8_t*>(a.hidden + uint64_t(t0) * a.ldh);
+    // Rows past the last are the last one again: their results are dropped below.
+    uint32_t off[kLV + kLT];
+    const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+#pragma unroll
+    for (int j = 0; j < kLV; ++j)
+        off[j] = min((j * kWaves + wave) * 8 + (lane >> 3), a.vocab - 1 - v0) * (a.ldw * 2) + chunk;
+#pragma unroll
+    for (int j = 0; j < kLT; ++j)
+        off[kLV + j] = min((j * kWaves + wave) * 8 + (lane >> 3), a.tokens - 1 - t0) * (a.ldh * 2) + chunk;
+    typedef __attribute__((address_space(3))) uint8_t Lds;
+    typedef const __attribute__((address_space(1))) uint8_t Global;
+    const auto copy = [&](uint32_t step, uint32_t buf) {
+        uint8_t* to = lds + buf * kBuffer + wave * 1024;
+#pragma unroll
+        for (int j = 0; j < kLV; ++j)
+            __builtin_amdgcn_global_load_lds((Global*)(gv + step * kRowBytes + off[j]),
+                                             (Lds*)(to + j * kWaves * 1024), 16, 0, 0);
+#pragma unroll
+        for (int j = 0; j < kLT; ++j)
+            __builtin_amdgcn_global_load_lds((Global*)(gt + step * kRowBytes + off[kLV + j]),
+                                             (Lds*)(to + kBV * kRowBytes + j * kWaves * 1024), 16, 0, 0);
+    };
+
+    const uint32_t wv = wave / kWT, wt = wave % kWT;
+    const uint32_t at = (quad ^ (l16 & 7)) * 16;
+    const uint32_t at_v = (wv * kFV * 16 + l16) * kRowBytes, at_t = (kBV + wt * kFT * 16 + l16) * kRowBytes;
+    u32x4 x[2][kFV], y[2][kFT];
+    const auto read = [&](uint32_t buf, int half) {
+        const uint8_t* from = lds + buf * kBuffer + (at ^ (half * 64));
+#pragma unroll
+        for (int i = 0; i < kFV; ++i) x[half][i] = *reinterpret_cast<const u32x4*>(from + at_v + i * 16 * kRowBytes);
+#pragma unroll
+        for (int j = 0; j < kFT; ++j) y[half][j] = *reinterpret_cast<const u32x4*>(from + at_t + j * 16 * kRowBytes);
+    };
+    f32x4 acc[kFV][kFT];
+#pragma unroll
+    for (int i = 0; i < kFV; ++i)
+#pragma unroll
+        for (int j = 0; j < kFT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto multiply = [&](int half) {
+#pragma unroll
+        for (int i = 0; i < kFV; ++i)
+#pragma unroll
+            for (int j = 0; j < kFT; ++j) acc[i][j] = mfma(Fmt{}, x[half][i], y[half][j], acc[i][j]);
+    };
+    // All copies and LDS reads of every wave are done, and none moves across.
+    const auto meet = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // kMore: there is a buffer after the next to copy; kNext: there is a next one
+    const auto step = [&](uint32_t s, auto kMore, auto kNext) {
+        read(s & 1, 1);
+        multiply(0);
+        interleave<kFV + kFT, kFV * kFT, 0>();
+        meet();
+        if constexpr (decltype(kMore)::value) copy(s + 2, s & 1);
+        if constexpr (decltype(kNext)::value) read((s + 1) & 1, 0);
+        multiply(1);
+        if constexpr (decltype(kNext)::value) interleave<kFV + kFT, kFV * kFT, decltype(kMore)::value ? kLV + kLT : 0>();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    copy(0, 0);
+    if (a.steps > 1) copy(1, 1);
+    meet();
+    read(0, 0);
+    uint32_t s = 0;
+    for (; s + 2 < a.steps; ++s) step(s, std::true_type{}, std::true_type{});
+    if (s + 1 < a.steps) step(s++, std::false_type{}, std::true_type{});
+    step(s, std::false_type{}, std::false_type{});
+
+    // Every wave is past its last read of LDS at the barrier in its last step.
+    float* top = reinterpret_cast<float*>(lds);          // [kWV][kBT]
+    float* sums = top + kWV * kBT;                       // [kWV][kBT]
+    const uint32_t wv0 = wv * kFV * 16, wt0 = wt * kFT * 16;
+    if (v0 + kBV > a.vocab) {
+#pragma unroll
+        for (int i = 0; i < kFV; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (v0 + wv0 + i * 16 + quad * 4 + r >= a.vocab)
+#pragma unroll
+                    for (int j = 0; j < kFT; ++j) acc[i][j][r] = -__builtin_inff();
+    }
+#pragma unroll
+    for (int j = 0; j < kFT; ++j) {
+        float m = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < kFV; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        if (quad == 0) top[wv * kBT + wt0 + j * 16 + l16] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kFT; ++j) {
+        const uint32_t t = wt0 + j * 16 + l16, token = t0 + t;
+        float m = top[t];
+#pragma unroll
+        for (int w = 1; w < kWV; ++w) m = fmaxf(m, top[w * kBT + t]);
+        m *= a.scale2;
+        // exp2(scale2 x - base(m)): the product is not rounded before the difference
+        const float c = base(m);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFV; ++i) {
+            f32x4 e;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                e[r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], a.scale2, -c));
+                sum += e[r];
+            }
+            if (kKeep && token < a.tokens) {
+                u32x2 p = {Fmt::pack(e[0], e[1]), Fmt::pack(e[2], e[3])};
+                *reinterpret_cast<u32x2*>(a.keep + token * a.ld_keep + v0 + wv0 + i * 16 + quad * 4) = p;
+            }
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (quad == 0) sums[wv * kBT + t] = sum;
+        // the label's product, by the one lane that has it
+        const int64_t label = token < a.tokens ? a.labels[token] : -1;
+        const int64_t from = int64_t(v0) + wv0 + quad * 4;
+        if (label >= from && label < from + kFV * 16 && label < int64_t(a.vocab)) {
+            const uint32_t o = uint32_t(label - from);
+            float z = 0.0f;
+            bool mine = false;
+#pragma unroll
+            for (int i = 0; i < kFV; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (o == uint32_t(i * 16 + r)) z = acc[i][j][r], mine = true;
+            if (mine) a.target[token] = z;
+        }
+    }
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < uint32_t(kBT) && t0 + t < a.tokens; t += kWaves * 64) {
+        float m = top[t], sum = sums[t];
+#pragma unroll
+        for (int w = 1; w < kWV; ++w) {
+            m = fmaxf(m, top[w * kBT + t]);
+            sum += sums[w * kBT + t];
+        }
+        a.parts[uint64_t(tile_v) * a.tokens + t0 + t] = float2{m * a.scale2, sum};
+    }
+}
+
+// The tiles' parts of each token joined.  A workgroup takes 4 tokens, 64 lanes
+// each, so that a wave reads 32 neighbouring bytes of each tile.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinTokens = 4;
+__global__ __launch_bounds__(kJoinThreads) void logps_join_kernel(const float2* __restrict__ parts, uint32_t spans,
+                                                                  uint32_t tokens, const float* __restrict__ target,
+                                                                  const int64_t* __restrict__ labels,
+                                                                  int64_t ignore_index, uint32_t vocab, float scale2,
+                                                                  float* __restrict__ lse2, float* __restrict__ logp) {
+    __shared__ Lse waves[kJoinThreads / 64][kJoinTokens];
+    const uint32_t t = threadIdx.x % kJoinTokens, token = blockIdx.x * kJoinTokens + t;
+    Lse p = {-__builtin_inff(), 0.0f};
+    if (token < tokens)
+        for (uint32_t k = threadIdx.x / kJoinTokens; k < spans; k += kJoinThreads / kJoinTokens) {
+            const float2 v = parts[uint64_t(k) * tokens + token];
+            const float m = fmaxf(p.m, v.x), c = base(m);
+            // an empty part stays empty whatever the bases are; a NaN sum stays NaN
+            p.s = (p.s == 0.0f ? 0.0f : p.s * exp2f(base(p.m) - c)) + (v.y == 0.0f ? 0.0f : v.y * exp2f(base(v.x) - c));
+            p.m = m;
+        }
+    const auto merge = [](Lse p, Lse q) {
+        const float m = fmaxf(p.m, q.m), c = base(m);
+        return Lse{m, (p.s == 0.0f ? 0.0f : p.s * exp2f(base(p.m) - c)) + (q.s == 0.0f ? 0.0f : q.s * exp2f(base(q.m) - c))};
+    };
+#pragma unroll
+    for (int d = 32; d >= kJoinTokens; d >>= 1) p = merge(p, Lse{__shfl_xor(p.m, d), __shfl_xor(p.s, d)});
+    if ((threadIdx.x & 63) < kJoinTokens) waves[threadIdx.x >> 6][t] = p;
+    __syncthreads();
+    if (threadIdx.x >= kJoinTokens || token >= tokens) return;
+#pragma unroll
+    for (int w = 1; w < kJoinThreads / 64; ++w) p = merge(p, waves[w][t]);
+    const RowKind kind = row_kind(labels[token], ignore_index, vocab);
+    const float c = base(p.m), l = log2f(p.s);
+    lse2[token] = kind == kValid ? c + l : kind == kIgnored ? 0.0f : __builtin_nanf("");
+    logp[token] = kind == kValid ? (fmaf(target[token], scale2, -c) - l) * kLn2 : kind == kIgnored ? 0.0f : __builtin_nanf("");
+}
+
+// ---------------------------------------------------------------------
 // fp32 logits that a library product has left: kT lanes per row, one pass, each
 // lane with its own running maximum and sum.
+// ---------------------------------------------------------------------
 template <int kT>
 __global__ __launch_bounds__(kT * kRowsOf<kT>) void logps_rows_kernel(const float* __restrict__ logits, uint64_t ld,
                                                                       uint64_t rows, uint32_t vocab,
@@ -66,39 +356,91 @@ __global__ __launch_bounds__(kT * kRowsOf<kT>) void logps_rows_kernel(const floa
     }
 }
 
-// What an fp16 gradient of the logits is multiplied by: a power of two that
-// brings the largest element of the gradient of the log-probabilities into [1,
-// 2), since per-token gradients are of the order 1 / tokens and a probability
-// times that is below fp16's range.  norm: the factor, its inverse, 1.
-constexpr int kNormThreads = 1024;
-__global__ __launch_bounds__(kNormThreads) void logps_norm_kernel(const float* __restrict__ grad,
-                                                                  const int64_t* __restrict__ labels,
-                                                                  int64_t ignore_index, uint64_t n, float scale,
-                                                                  float* __restrict__ norm) {
-    __shared__ float waves[kNormThreads / 64];
+// ---------------------------------------------------------------------
+// Gradients.  What multiplies each row: grad * scale * (1 - p_y), and, of fp16
+// operands, a power of two that brings the largest of them into [1, 2) (a mean
+// over many tokens leaves them near fp16's least numbers).  One workgroup.
+// ---------------------------------------------------------------------
+constexpr int kWeightThreads = 1024;
+__global__ __launch_bounds__(kWeightThreads) void logps_weight_kernel(const float* __restrict__ grad,
+                                                                      const float* __restrict__ logp,
+                                                                      const int64_t* __restrict__ labels,
+                                                                      int64_t ignore_index, uint64_t n, uint32_t vocab,
+                                                                      float scale, float* __restrict__ weight,
+                                                                      float* __restrict__ norm) {
+    __shared__ float waves[kWeightThreads / 64];
+    const auto of = [&](uint64_t i) {
+        const RowKind kind = row_kind(labels[i], ignore_index, vocab);
+        return kind == kValid ? grad[i] * scale * rest_of(logp[i]) : kind == kIgnored ? 0.0f : __builtin_nanf("");
+    };
+    if (norm == nullptr) {
+        for (uint64_t i = uint64_t(blockIdx.x) * kWeightThreads + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kWeightThreads)
+            weight[i] = of(i);
+        return;
+    }
     float m = 0.0f;
-    for (uint64_t i = threadIdx.x; i < n; i += kNormThreads) {
-        const float g = fabsf(grad[i] * scale);
-        if (labels[i] != ignore_index && __builtin_isfinite(g)) m = fmaxf(m, g);
+    for (uint64_t i = threadIdx.x; i < n; i += kWeightThreads) {
+        const float w = fabsf(of(i));
+        if (__builtin_isfinite(w)) m = fmaxf(m, w);
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kNormThreads / 64; ++w) m = fmaxf(m, waves[w]);
-        // within what both the factor and its inverse can be
-        const int e = m > 0.0f ? min(max(ilogbf(m), -100), 100) : 0;
-        norm[0] = ldexpf(1.0f, -e);
-        norm[1] = ldexpf(1.0f, e);
-        norm[2] = 1.0f;
+    m = waves[0];
+    for (int w = 1; w < kWeightThreads / 64; ++w) m = fmaxf(m, waves[w]);
+    // within what both the factor and its inverse can be
+    const int e = m > 0.0f ? min(max(ilogbf(m), -100), 100) : 0;
+    const float by = ldexpf(1.0f, -e);
+    for (uint64_t i = threadIdx.x; i < n; i += kWeightThreads) weight[i] = of(i) * by;
+    if (threadIdx.x == 0) norm[0] = ldexpf(1.0f, e), norm[1] = 1.0f;
+}
+
+// D from what the product kept, in place.  A workgroup takes 4,096 words of a
+// token, 16 bytes at a time; rows from `tokens` on are cleared (they pad the
+// weight gradient's sum).
+constexpr int kGradThreads = 256;
+constexpr int kKeepColumns = kGradThreads * kGroup * 2;
+template <typename Fmt>
+__global__ __launch_bounds__(kGradThreads) void logps_keep_grad_kernel(uint16_t* __restrict__ keep, uint64_t ld,
+                                                                       uint32_t tokens, uint32_t vocab,
+                                                                       uint32_t col_blocks, uint64_t first,
+                                                                       const float2* __restrict__ parts,
+                                                                       const int64_t* __restrict__ labels,
+                                                                       int64_t ignore_index,
+                                                                       const float* __restrict__ lse2,
+                                                                       const float* __restrict__ logp) {
+    const uint64_t b = first + blockIdx.x, row = b / col_blocks;
+    const uint32_t col = uint32_t(b % col_blocks) * kKeepColumns + threadIdx.x * kGroup;
+    uint16_t* k = keep + row * ld;
+    const int64_t y = row < tokens ? labels[row] : ignore_index;
+    const RowKind kind = row_kind(y, ignore_index, vocab);
+    if (row >= tokens || kind != kValid) {
+        const uint32_t w = row < tokens && kind == kBadLabel ? Fmt::kNan2 : 0u;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (col + j * kGradThreads * kGroup < ld) *reinterpret_cast<u32x4*>(k + col + j * kGradThreads * kGroup) = u32x4{w, w, w, w};
+        return;
+    }
+    const float l = lse2[row], by = -1.0f / rest_of(logp[row]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t c = col + j * kGradThreads * kGroup;
+        if (c >= ld) break;
+        u32x4* p = reinterpret_cast<u32x4*>(k + c);
+        const u32x4 v = *p;
+        const float f = exp2f(base(parts[uint64_t(c / kSpan) * tokens + row].x) - l) * by;
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = Fmt::pack(Fmt::lo(v[i]) * f, Fmt::hi(v[i]) * f);
+        *p = o;
+        // over what this lane has just stored
+        if (uint64_t(y) - c < uint64_t(kGroup)) k[y] = uint16_t(Fmt::pack(1.0f, 0.0f));
     }
 }
 
-// Its gradient, element by element; a workgroup takes 1,024 columns of a row.
-constexpr int kGradThreads = 256;
+// D from fp32 logits; a workgroup takes 1,024 words of a row.
 constexpr int kGradColumns = 1024;
-
 struct Out32 {
     using S = float;
     __device__ static void store(S* p, float f) { *p = f; }
@@ -108,15 +450,13 @@ struct Out16 {
     using S = uint16_t;
     __device__ static void store(S* p, float f) { *p = uint16_t(Fmt::pack(f, 0.0f)); }
 };
-
 template <typename Out>
 __global__ __launch_bounds__(kGradThreads) void logps_grad_kernel(const float* logits, uint64_t ld, uint32_t vocab,
                                                                   uint32_t col_blocks, uint64_t first,
                                                                   const int64_t* __restrict__ labels,
                                                                   int64_t ignore_index, float scale,
                                                                   const float* __restrict__ lse,
-                                                                  const float* __restrict__ grad,
-                                                                  const float* __restrict__ norm,
+                                                                  const float* __restrict__ logp,
                                                                   typename Out::S* dz, uint64_t ld_dz) {
     const uint64_t b = first + blockIdx.x, row = b / col_blocks;
     const uint32_t col = uint32_t(b % col_blocks) * kGradColumns + threadIdx.x;
@@ -124,17 +464,36 @@ __global__ __launch_bounds__(kGradThreads) void logps_grad_kernel(const float* l
     const RowKind kind = row_kind(y, ignore_index, vocab);
     const float* x = logits + row * ld;
     typename Out::S* o = dz + row * ld_dz;
-    const float l = lse[row], by = norm != nullptr ? *norm : 1.0f;
-    const float g = kind == kIgnored ? 0.0f : grad[row] * scale * by;
+    const float l = lse[row], by = -1.0f / rest_of(logp[row]);
 #pragma unroll
     for (int k = 0; k < kGradColumns / kGradThreads; ++k) {
         const uint32_t j = col + k * kGradThreads;
         if (j >= vocab) break;
-        float f = 0.0f;
-        if (kind == kBadLabel) f = __builtin_nanf("");
-        if (kind == kValid) f = g * ((int64_t(j) == y ? 1.0f : 0.0f) - expf(x[j] * scale - l));
+        float f = kind == kIgnored ? 0.0f : __builtin_nanf("");
+        if (kind == kValid) f = int64_t(j) == y ? 1.0f : expf(x[j] * scale - l) * by;
         Out::store(o + j, f);
     }
+}
+
+// ---------------------------------------------------------------------
+template <typename Fmt, int kWV, int kWT, int kFV, int kFT>
+int launch_tiles(const Tiles& a, hipStream_t st) {
+    constexpr uint32_t kBT = kWT * kFT * 16;
+    const uint64_t tiles = uint64_t((a.vocab + kSpan - 1) / kSpan) * ((a.tokens + kBT - 1) / kBT);
+    if (tiles > kMaxLanes / (kWV * kWT * 64)) return SF_EINVAL;
+    const auto kernel = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, true>
+                                          : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, false>;
+    hipLaunchKernelGGL(kernel, dim3(uint32_t(tiles)), dim3(kWV * kWT * 64), 0, st, a);
+    return status();
+}
+
+template <typename Fmt>
+int dispatch_tiles(const Tiles& a, hipStream_t st) {
+    const uint64_t big = uint64_t((a.vocab + kSpan - 1) / kSpan) * ((a.tokens + 255) / 256);
+    if (a.tokens <= 32) return launch_tiles<Fmt, 4, 1, 4, 2>(a, st);
+    if (a.tokens <= 64 || big < 128) return launch_tiles<Fmt, 4, 1, 4, 4>(a, st);
+    if (a.tokens <= 128) return launch_tiles<Fmt, 4, 2, 4, 4>(a, st);
+    return launch_tiles<Fmt, 2, 4, 8, 4>(a, st);
 }
 
 template <int kT>
@@ -152,21 +511,26 @@ int launch_rows(const float* x, uint64_t ld, uint64_t rows, uint32_t vocab, cons
     return SF_OK;
 }
 
-template <typename Out>
-int launch_grad(const float* x, uint64_t ld, uint64_t rows, uint32_t vocab, const int64_t* labels, int64_t ignore,
-                float scale, const float* lse, const float* grad, const float* norm, void* dz, uint64_t ld_dz,
-                hipStream_t st) {
+// kernel(first, blocks) in as many launches as `blocks` workgroups need.
+template <typename Launch>
+int in_launches(uint64_t blocks, Launch launch) {
     constexpr uint64_t kMax = kMaxLanes / kGradThreads;
-    const uint32_t col_blocks = (vocab + kGradColumns - 1) / kGradColumns;
-    const uint64_t blocks = rows * col_blocks;
     for (uint64_t first = 0; first < blocks; first += kMax) {
-        hipLaunchKernelGGL(logps_grad_kernel<Out>, dim3(uint32_t(blocks - first < kMax ? blocks - first : kMax)),
-                           dim3(kGradThreads), 0, st, x, ld, vocab, col_blocks, first, labels, ignore, scale, lse, grad,
-                           norm, static_cast<typename Out::S*>(dz), ld_dz);
+        launch(first, uint32_t(blocks - first < kMax ? blocks - first : kMax));
         const int e = status();
         if (e != SF_OK) return e;
     }
     return SF_OK;
+}
+
+template <typename Out>
+int launch_grad(const float* x, uint64_t ld, uint64_t rows, uint32_t vocab, const int64_t* labels, int64_t ignore,
+                float scale, const float* lse, const float* logp, void* dz, uint64_t ld_dz, hipStream_t st) {
+    const uint32_t col_blocks = (vocab + kGradColumns - 1) / kGradColumns;
+    return in_launches(rows * col_blocks, [&](uint64_t first, uint32_t blocks) {
+        hipLaunchKernelGGL(logps_grad_kernel<Out>, dim3(blocks), dim3(kGradThreads), 0, st, x, ld, vocab, col_blocks,
+                           first, labels, ignore, scale, lse, logp, static_cast<typename Out::S*>(dz), ld_dz);
+    });
 }
 
 bool sizes_bad(size_t rows, size_t vocab) {
@@ -176,6 +540,52 @@ bool sizes_bad(size_t rows, size_t vocab) {
 }  // namespace
 
 extern "C" {
+
+int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab, const void* hidden, size_t ldh, size_t rows,
+                   size_t hidden_size, const int64_t* labels, int64_t ignore_index, float scale, int dtype, void* parts,
+                   float* target, void* keep, size_t ld_keep, float* lse2, float* logp, sf_stream_t stream) {
+    if (rows == 0) return SF_OK;
+    if (weight == nullptr || hidden == nullptr || labels == nullptr || parts == nullptr || target == nullptr ||
+        lse2 == nullptr || logp == nullptr || sizes_bad(rows, vocab))
+        return SF_EINVAL;
+    // 32-bit byte offsets inside a tile of 256 rows
+    constexpr size_t kMostLd = size_t(1) << 22;
+    if (hidden_size == 0 || ldw < hidden_size || ldh < hidden_size || ldw > kMostLd || ldh > kMostLd || !(scale > 0.0f))
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    const size_t spans = (vocab + kSpan - 1) / kSpan;
+    if (keep != nullptr && ld_keep < spans * kSpan) return SF_EINVAL;
+    if (hidden_size % kTerms != 0 || ldw % kGroup != 0 || ldh % kGroup != 0 || misaligned(weight, 16) ||
+        misaligned(hidden, 16) || misaligned(parts, 8) || misaligned(keep, 16) || ld_keep % kGroup != 0)
+        return SF_EALIGN;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const Tiles a = {static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(hidden), uint32_t(ldw),
+                     uint32_t(ldh), uint32_t(vocab), uint32_t(rows), uint32_t(hidden_size / kTerms), labels,
+                     scale * kLog2e, static_cast<float2*>(parts), target, static_cast<uint16_t*>(keep), ld_keep};
+    const int e = dtype == SF_DTYPE_BF16 ? dispatch_tiles<Bf16>(a, st) : dispatch_tiles<F16>(a, st);
+    if (e != SF_OK) return e;
+    hipLaunchKernelGGL(logps_join_kernel, dim3((a.tokens + kJoinTokens - 1) / kJoinTokens), dim3(kJoinThreads), 0, st,
+                       a.parts, uint32_t(spans), a.tokens, target, labels, ignore_index, a.vocab, a.scale2, lse2, logp);
+    return status();
+}
+
+int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded, size_t vocab, const void* parts,
+                       const int64_t* labels, int64_t ignore_index, const float* lse2, const float* logp, int dtype,
+                       sf_stream_t stream) {
+    if (padded == 0) return SF_OK;
+    if (keep == nullptr || parts == nullptr || labels == nullptr || lse2 == nullptr || logp == nullptr ||
+        sizes_bad(padded, vocab) || padded < rows || ld < (vocab + kSpan - 1) / kSpan * kSpan || ld > (size_t(1) << 31))
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (misaligned(keep, 16) || misaligned(parts, 8) || ld % kSpan != 0) return SF_EALIGN;
+    const uint32_t col_blocks = uint32_t((ld + kKeepColumns - 1) / kKeepColumns);
+    const auto kernel = dtype == SF_DTYPE_BF16 ? logps_keep_grad_kernel<Bf16> : logps_keep_grad_kernel<F16>;
+    return in_launches(uint64_t(padded) * col_blocks, [&](uint64_t first, uint32_t blocks) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kGradThreads), 0, reinterpret_cast<hipStream_t>(stream),
+                           static_cast<uint16_t*>(keep), uint64_t(ld), uint32_t(rows), uint32_t(vocab), col_blocks, first,
+                           static_cast<const float2*>(parts), labels, ignore_index, lse2, logp);
+    });
+}
 
 int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab, const int64_t* labels,
                   int64_t ignore_index, float scale, float* lse, float* logp, sf_stream_t stream) {
@@ -191,19 +601,23 @@ int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab, con
     return launch_rows<1024>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
 }
 
-int sf_logps_norm(const float* grad, const int64_t* labels, int64_t ignore_index, size_t rows, float scale, float* norm,
-                  sf_stream_t stream) {
-    if (norm == nullptr || (rows > 0 && (grad == nullptr || labels == nullptr))) return SF_EINVAL;
-    hipLaunchKernelGGL(logps_norm_kernel, dim3(1), dim3(kNormThreads), 0, reinterpret_cast<hipStream_t>(stream), grad,
-                       labels, ignore_index, uint64_t(rows), scale, norm);
+int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels, int64_t ignore_index, size_t rows,
+                    size_t vocab, float scale, float* weight, float* norm, sf_stream_t stream) {
+    if (rows == 0 && norm == nullptr) return SF_OK;
+    if (sizes_bad(rows, vocab) || (rows > 0 && (grad == nullptr || logp == nullptr || labels == nullptr || weight == nullptr)))
+        return SF_EINVAL;
+    const uint64_t want = (rows + kWeightThreads - 1) / kWeightThreads;
+    const uint32_t blocks = norm != nullptr ? 1 : uint32_t(want < 1024 ? want : 1024);
+    hipLaunchKernelGGL(logps_weight_kernel, dim3(blocks), dim3(kWeightThreads), 0, reinterpret_cast<hipStream_t>(stream),
+                       grad, logp, labels, ignore_index, uint64_t(rows), uint32_t(vocab), scale, weight, norm);
     return status();
 }
 
 int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab, const int64_t* labels,
-                  int64_t ignore_index, float scale, const float* lse, const float* grad, const float* norm, void* dz,
-                  int dtype, size_t ld_dz, sf_stream_t stream) {
+                  int64_t ignore_index, float scale, const float* lse, const float* logp, void* dz, int dtype,
+                  size_t ld_dz, sf_stream_t stream) {
     if (rows == 0) return SF_OK;
-    if (logits == nullptr || labels == nullptr || lse == nullptr || grad == nullptr || dz == nullptr) return SF_EINVAL;
+    if (logits == nullptr || labels == nullptr || lse == nullptr || logp == nullptr || dz == nullptr) return SF_EINVAL;
     if (sizes_bad(rows, vocab) || ld < vocab || ld_dz < vocab) return SF_EINVAL;
     if (dtype != SF_DTYPE_F32 && dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
     const size_t item = dtype == SF_DTYPE_F32 ? 4 : 2;
@@ -215,10 +629,10 @@ int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab, con
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const uint32_t v = uint32_t(vocab);
     if (dtype == SF_DTYPE_BF16)
-        return launch_grad<Out16<Bf16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, grad, norm, dz, ld_dz, st);
+        return launch_grad<Out16<Bf16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, dz, ld_dz, st);
     if (dtype == SF_DTYPE_F16)
-        return launch_grad<Out16<F16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, grad, norm, dz, ld_dz, st);
-    return launch_grad<Out32>(logits, ld, rows, v, labels, ignore_index, scale, lse, grad, norm, dz, ld_dz, st);
+        return launch_grad<Out16<F16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, dz, ld_dz, st);
+    return launch_grad<Out32>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, dz, ld_dz, st);
 }
 
 }  // extern "C"

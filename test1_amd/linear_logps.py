@@ -8,21 +8,34 @@ log-probabilities themselves, of the policy with gradients and of a reference
 or an old policy without.
 
 Numerics: the logits stay fp32 (they are not rounded to 16 bits in between),
-maximum and sum of the softmax are fp32, and the gradient of the logits is
-rounded to the inputs' type once, for its two products.
+maximum and sum of the softmax are fp32.  The gradient's products take 16-bit
+operands, fp32 of fp32 ones: the exponentials, kept to 16 bits relative to their
+span of the vocabulary, and their share of 1 - p, rounded again; the label's
+element is exact, and the rows' own factors stay fp32 up to the hidden rows of
+the weight gradient's product.
 """
 
 from __future__ import annotations
 
 import math
+from typing import Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
 from .alignment import _on_device, _stream
-from .fused_ce import _DTYPES, _PLAIN, _memory_is_value, _traced
+from .fused_ce import _DTYPES, _PLAIN, _memory_is_value, _saved_plain, _traced, _vocabulary_parts
 from .kernels import _CE_DTYPES
+
+
+_SPAN = _native.SF_LOGPS_SPAN
+# What the forward keeps for the backward at most, 2 bytes a logit, and what a
+# backward that makes it again takes at a time.  Keeping it saves one of four
+# products; 8 GiB is a thirty-sixth of the device's memory, where 30,000 tokens
+# of a vocabulary of 128256 fit.
+_KEEP_BYTES = 8 << 30
+_AGAIN_BYTES = 2 << 30
 
 
 def _f32_out(dtype: torch.dtype) -> dict:
@@ -38,12 +51,35 @@ def _logits_buffer(rows: int, vocab: int, device) -> torch.Tensor:
     return torch.empty((rows, -(-vocab // 64) * 64), dtype=torch.float32, device=device)
 
 
-def _forward_kernels(hidden, weight, labels, ignore_index, scale):
+def _padded(n: int, unit: int) -> int:
+    return -(-n // unit) * unit
+
+
+def _in_tiles(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
+    """Whether ``logps_tiles_kernel`` takes the call: 16-bit operands whose rows
+    start on 16-byte boundaries, a sum of whole 64 terms."""
+    return (hidden.element_size() == 2 and hidden.shape[1] % 64 == 0
+            and all(t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= 1 << 22 and t.stride(0) % 8 == 0
+                    and t.data_ptr() % 16 == 0 for t in (hidden, weight)))
+
+
+def _tiles(hidden, weight, labels, ignore_index, scale, keep, lse2, logp):
+    """Results into ``lse2`` and ``logp``; returns the spans' parts."""
+    n, v = hidden.shape[0], weight.shape[0]
+    parts = torch.empty((2 * -(-v // _SPAN) + 1) * n, dtype=torch.float32, device=hidden.device)
+    at = parts.data_ptr()
+    _native.check(_native.hip().sf_logps_tiles(
+        weight.data_ptr(), weight.stride(0), v, hidden.data_ptr(), hidden.stride(0), n, hidden.shape[1],
+        labels.data_ptr(), ignore_index, scale, _CE_DTYPES[hidden.dtype], at, at + 4 * (parts.numel() - n),
+        None if keep is None else keep.data_ptr(), 0 if keep is None else keep.stride(0), lse2.data_ptr(),
+        logp.data_ptr(), _stream()), "sf_logps_tiles")
+    return parts
+
+
+def _rows_product(hidden, weight, labels, ignore_index, scale, lse, logp):
     n, v = hidden.shape[0], weight.shape[0]
     step = min(n, _chunk_rows(v))
     buf = _logits_buffer(step, v, hidden.device)
-    lse = torch.empty(n, dtype=torch.float32, device=hidden.device)
-    logp = torch.empty(n, dtype=torch.float32, device=hidden.device)
     wt = weight.t()
     for s in range(0, n, step):
         e = min(n, s + step)
@@ -51,66 +87,151 @@ def _forward_kernels(hidden, weight, labels, ignore_index, scale):
         _native.check(_native.hip().sf_logps_rows(
             buf.data_ptr(), buf.stride(0), e - s, v, labels.data_ptr() + 8 * s, ignore_index, scale,
             lse.data_ptr() + 4 * s, logp.data_ptr() + 4 * s, _stream()), "sf_logps_rows")
-    return logp, lse
 
 
-def _rescale(out: torch.Tensor, grad: torch.Tensor, norm: torch.Tensor) -> torch.Tensor:
-    """``out`` = the fp32 ``grad`` over ``norm[0]``, rounded once."""
-    _native.check(_native.hip().sf_ce_scale(norm.data_ptr() + 4, norm.data_ptr() + 8, None, None, 0, grad.data_ptr(),
-                                            out.data_ptr(), out.numel(), _CE_DTYPES[out.dtype], _stream()),
-                  "sf_ce_scale")
+def _forward_kernels(hidden, weight, labels, ignore_index, scale, need_grad):
+    """(logp, lse, what the backward finds kept or None)"""
+    n, v = hidden.shape[0], weight.shape[0]
+    dev = hidden.device
+    lse = torch.empty(n, dtype=torch.float32, device=dev)
+    logp = torch.empty(n, dtype=torch.float32, device=dev)
+    if not _in_tiles(hidden, weight):
+        _rows_product(hidden, weight, labels, ignore_index, scale, lse, logp)
+        return logp, lse, None
+    keep = None
+    if need_grad and 2 * _padded(n, 64) * _padded(v, _SPAN) <= _KEEP_BYTES:
+        keep = torch.empty((_padded(n, 64), _padded(v, _SPAN)), dtype=hidden.dtype, device=dev)
+    parts = _tiles(hidden, weight, labels, ignore_index, scale, keep, lse, logp)
+    return logp, lse, None if keep is None else (keep, parts)
+
+
+def _row_weight(grad, logp, labels, vocab, ignore_index, scale, dtype):
+    """What multiplies the rows of D, and fp16's factor (``sf_logps_weight``)."""
+    n = labels.shape[0]
+    weight = torch.empty(n, dtype=torch.float32, device=grad.device)
+    norm = torch.empty(2, dtype=torch.float32, device=grad.device) if dtype == torch.float16 else None
+    _native.check(_native.hip().sf_logps_weight(grad.data_ptr(), logp.data_ptr(), labels.data_ptr(), ignore_index, n,
+                                                vocab, scale, weight.data_ptr(),
+                                                None if norm is None else norm.data_ptr(), _stream()),
+                  "sf_logps_weight")
+    return weight, norm
+
+
+def _add_product(total, a, b, first):
+    """``total`` (+)= a @ b in fp32 or, of the only one, in the operands' type."""
+    f32 = _f32_out(a.dtype) if total.dtype == torch.float32 else {}
+    if first:
+        torch.mm(a, b, **f32, out=total)
+    else:
+        torch.addmm(total, a, b, **f32, out=total)
+
+
+def _rescaled(grad: Optional[torch.Tensor], dtype, norm) -> Optional[torch.Tensor]:
+    """The weight gradient in ``dtype``, fp16's factor taken out before the rounding."""
+    if grad is None or grad.dtype == dtype and norm is None:
+        return grad
+    if norm is None:
+        return grad.to(dtype)
+    out = torch.empty(grad.shape, dtype=dtype, device=grad.device)
+    _native.check(_native.hip().sf_ce_scale(norm.data_ptr(), norm.data_ptr() + 4, None, None, 0, grad.data_ptr(),
+                                            out.data_ptr(), out.numel(), _CE_DTYPES[dtype], _stream()), "sf_ce_scale")
     return out
 
 
-def _backward_kernels(grad, hidden, weight, labels, lse, ignore_index, scale, need_hidden, need_weight):
+def _hidden_product(d, ld, weight, row_weight_at, norm, out):
+    """``out`` = row_weight * (d @ weight), rounded once; the sum over the
+    vocabulary in parts where that fills the chip (``_vocabulary_parts``)."""
+    n, v = d.shape
+    h = weight.shape[1]
+    nparts = _vocabulary_parts(n, weight)
+    part = v if nparts == 1 else v // nparts // 8 * 8
+    parts = torch.empty((nparts, n, h), dtype=torch.float32, device=d.device)
+    if nparts == 1:
+        torch.mm(d, weight, out_dtype=torch.float32, out=parts[0])
+    else:
+        torch.bmm(d.as_strided((nparts, n, part), (part, ld, 1)), weight[:nparts * part].view(nparts, part, h),
+                  out_dtype=torch.float32, out=parts)
+    done = nparts * part
+    _native.check(_native.hip().sf_logps_sum(
+        parts.data_ptr(), nparts, n, h, out.data_ptr(), _CE_DTYPES[out.dtype], d.data_ptr() + 2 * done, ld,
+        weight.data_ptr() + 2 * done * h, v - done, row_weight_at, None if norm is None else norm.data_ptr(),
+        _stream()), "sf_logps_sum")
+
+
+def _backward_tiles(grad, hidden, weight, labels, logp, lse2, kept, ignore_index, scale, need_hidden, need_weight):
     n, h = hidden.shape
     v = weight.shape[0]
     dev, dtype = hidden.device, hidden.dtype
-    f32 = _f32_out(dtype)
+    row_weight, norm = _row_weight(grad, logp, labels, v, ignore_index, scale, dtype)
+    ld = _padded(v, _SPAN)
+    step = n if kept is not None else min(n, max(64, _AGAIN_BYTES // (2 * ld) // 64 * 64))
+    one = step == n
+    gh = torch.empty((n, h), dtype=dtype, device=dev) if need_hidden else None
+    gw = None
+    if need_weight:
+        gw = torch.empty((v, h), dtype=dtype if one and norm is None else torch.float32, device=dev)
+    keep, parts = kept if kept is not None else (torch.empty((_padded(step, 64), ld), dtype=dtype, device=dev), None)
+    again = torch.empty((2, step), dtype=torch.float32, device=dev) if kept is None else None
+    for s in range(0, n, step):
+        m = min(n, s + step) - s
+        hc, pad = hidden[s:s + m], _padded(m, 64)
+        if kept is None:
+            parts = _tiles(hc, weight, labels[s:s + m], ignore_index, scale, keep, again[0], again[1])
+        _native.check(_native.hip().sf_logps_keep_grad(
+            keep.data_ptr(), ld, m, pad, v, parts.data_ptr(), labels.data_ptr() + 8 * s, ignore_index,
+            lse2.data_ptr() + 4 * s, logp.data_ptr() + 4 * s, _CE_DTYPES[dtype], _stream()), "sf_logps_keep_grad")
+        if need_hidden:
+            _hidden_product(keep[:m, :v], ld, weight, row_weight.data_ptr() + 4 * s, norm, gh[s:s + m])
+        if need_weight:
+            ht = torch.empty((h, pad), dtype=dtype, device=dev)
+            _native.check(_native.hip().sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h,
+                                                        row_weight.data_ptr() + 4 * s, _CE_DTYPES[dtype],
+                                                        ht.data_ptr(), pad, _stream()), "sf_logps_hidden")
+            _add_product(gw, keep[:pad, :v].t(), ht.t(), s == 0)
+    return gh, _rescaled(gw, dtype, norm)
+
+
+def _backward_rows(grad, hidden, weight, labels, logp, lse, ignore_index, scale, need_hidden, need_weight):
+    n, h = hidden.shape
+    v = weight.shape[0]
+    dev, dtype = hidden.device, hidden.dtype
+    row_weight, norm = _row_weight(grad, logp, labels, v, ignore_index, scale, dtype)
+    row_weight = row_weight.unsqueeze(1)
     step = min(n, _chunk_rows(v))
+    one = step == n
     buf = _logits_buffer(step, v, dev)
-    dz_buf = buf if dtype == torch.float32 else torch.empty(buf.shape, dtype=dtype, device=dev)
-    norm = None
-    if dtype == torch.float16:
-        norm = torch.empty(3, dtype=torch.float32, device=dev)
-        _native.check(_native.hip().sf_logps_norm(grad.data_ptr(), labels.data_ptr(), ignore_index, n, scale,
-                                                  norm.data_ptr(), _stream()), "sf_logps_norm")
-    wide = norm is not None   # products into fp32, for the factor to leave before the rounding
-    gh = torch.empty((n, h), dtype=torch.float32 if wide else dtype, device=dev) if need_hidden else None
-    one = step == n and not wide
-    gw = torch.empty((v, h), dtype=dtype if one else torch.float32, device=dev) if need_weight else None
+    d_buf = buf if dtype == torch.float32 else torch.empty(buf.shape, dtype=dtype, device=dev)
+    gh = torch.empty((n, h), dtype=torch.float32, device=dev) if need_hidden else None
+    gw = None
+    if need_weight:
+        gw = torch.empty((v, h), dtype=dtype if one and norm is None else torch.float32, device=dev)
+        weighted = (hidden * row_weight).to(dtype)
     wt = weight.t()
     for s in range(0, n, step):
         e = min(n, s + step)
-        torch.mm(hidden[s:e], wt, **f32, out=buf[:e - s, :v])
-        dz = dz_buf[:e - s, :v]
+        torch.mm(hidden[s:e], wt, **_f32_out(dtype), out=buf[:e - s, :v])
+        d = d_buf[:e - s, :v]
         _native.check(_native.hip().sf_logps_grad(
             buf.data_ptr(), buf.stride(0), e - s, v, labels.data_ptr() + 8 * s, ignore_index, scale,
-            lse.data_ptr() + 4 * s, grad.data_ptr() + 4 * s, norm.data_ptr() if wide else None, dz_buf.data_ptr(),
-            _CE_DTYPES[dtype], dz_buf.stride(0), _stream()), "sf_logps_grad")
+            lse.data_ptr() + 4 * s, logp.data_ptr() + 4 * s, d_buf.data_ptr(), _CE_DTYPES[dtype], d_buf.stride(0),
+            _stream()), "sf_logps_grad")
         if need_hidden:
-            torch.mm(dz, weight, **(f32 if wide else {}), out=gh[s:e])
-        if not need_weight:
-            continue
-        if one:
-            torch.mm(dz.t(), hidden, out=gw)
-        elif s == 0:
-            torch.mm(dz.t(), hidden[s:e], **f32, out=gw)
-        else:
-            torch.addmm(gw, dz.t(), hidden[s:e], **f32, out=gw)
-    if wide:
-        gh = None if gh is None else _rescale(torch.empty((n, h), dtype=dtype, device=dev), gh, norm)
-        gw = None if gw is None else _rescale(torch.empty((v, h), dtype=dtype, device=dev), gw, norm)
-    return gh, None if gw is None else gw.to(dtype)
+            torch.mm(d, weight, **_f32_out(dtype), out=gh[s:e])
+        if need_weight:
+            _add_product(gw, d.t(), weighted[s:e], s == 0)
+    if need_hidden:
+        gh.mul_(row_weight)
+        gh = (gh if norm is None else gh.mul_(norm[0])).to(dtype)
+    return gh, _rescaled(gw, dtype, norm)
 
 
 class _LinearLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, scale):
         ctx.set_materialize_grads(False)
-        logp, lse = _forward_kernels(hidden, weight, labels, ignore_index, scale)
-        ctx.save_for_backward(hidden, weight, labels, lse)
-        ctx.ignore_index, ctx.scale = ignore_index, scale
+        logp, lse, ctx.kept = _forward_kernels(hidden, weight, labels, ignore_index, scale, True)
+        ctx.save_for_backward(hidden, weight, labels, lse, logp)
+        ctx.ignore_index, ctx.scale, ctx.tiles = ignore_index, scale, _in_tiles(hidden, weight)   # lse in base 2
         return logp
 
     @staticmethod
@@ -118,13 +239,22 @@ class _LinearLogps(torch.autograd.Function):
     def backward(ctx, grad):
         if grad is None:
             return None, None, None, None, None
-        hidden, weight, labels, lse = ctx.saved_tensors
+        hidden, weight, labels, lse, logp = ctx.saved_tensors
         need = ctx.needs_input_grad[:2]
-        if (type(grad) is torch.Tensor and _memory_is_value(grad) and _kernels_take(hidden, weight, labels)
-                and lse.dtype == torch.float32 and lse.is_contiguous() and labels.is_contiguous()):
+        if (type(grad) is torch.Tensor and grad.is_cuda and _memory_is_value(grad) and _kernels_take(hidden, weight, labels)
+                and _saved_plain(lse, torch.float32, hidden.device) and _saved_plain(logp, torch.float32, hidden.device)
+                and labels.is_contiguous()):
+            # What was kept turns into the gradient in place: a second backward
+            # of a retained graph makes it again.
+            kept, ctx.kept = ctx.kept, None
+            args = (grad.to(torch.float32).contiguous(), hidden, weight, labels, logp, lse)
             with _on_device(hidden):
-                return (*_backward_kernels(grad.to(torch.float32).contiguous(), hidden, weight, labels, lse,
-                                           ctx.ignore_index, ctx.scale, *need), None, None, None)
+                if ctx.tiles and _in_tiles(hidden, weight):
+                    return (*_backward_tiles(*args, kept, ctx.ignore_index, ctx.scale, *need), None, None, None)
+                if not ctx.tiles:
+                    return (*_backward_rows(*args, ctx.ignore_index, ctx.scale, *need), None, None, None)
+        if ctx.tiles:
+            lse = lse * math.log(2)
         with torch.autocast(hidden.device.type, enabled=False):
             valid, at, bad = _label_kinds(labels, weight.shape[0], ctx.ignore_index)
             p = torch.exp(hidden.float() @ weight.float().t() * ctx.scale - lse.float().unsqueeze(1))
@@ -193,5 +323,5 @@ def linear_logps(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tenso
         if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
             logp = _LinearLogps.apply(rows, weight, flat, ignore_index, scale)
         else:
-            logp = _forward_kernels(rows, weight, flat, ignore_index, scale)[0]
+            logp = _forward_kernels(rows, weight, flat, ignore_index, scale, False)[0]
     return logp if labels.dim() == 1 else logp.view(labels.shape)

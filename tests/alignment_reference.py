@@ -95,7 +95,8 @@ def logps(hidden, weight, labels, scale=1.0, ignore_index=-100, grad=None):
     evaluation with fp32 logits: each logit is a sum of K products, wrong by at
     most 2 K U of the sum of magnitudes in any order, scaled once; the softmax
     adds up to 512 terms in a row and takes a few roundings of its argument.
-    The gradient of the logits is rounded to the inputs' type once."""
+    An element of the logits' gradient is rounded to the inputs' type twice, a
+    weighted hidden row once more, a result once."""
     h, w = hidden.double(), weight.double()
     z = h @ w.t() * scale
     ez = (h.abs() @ w.abs().t()).amax(1) * (2 * h.shape[1] + 2) * U * scale
@@ -116,14 +117,18 @@ def logps(hidden, weight, labels, scale=1.0, ignore_index=-100, grad=None):
     dz[rows, ys] += 1
     g = torch.where(ignored, torch.zeros_like(lp), grad.double()) * scale
     dz = dz * g[:, None]
-    # of a gradient's elements: the rounding to the type, and the probability's own error
-    edz = dz.abs() * (half + 4 * U) + (p * (2 * ez + (512 + 8 * big) * U)[:, None]) * g.abs()[:, None]
-    edz = edz + tiny * (g.abs().max() if hidden.dtype == torch.float16 else 1.0) * 2
+    # of a gradient's elements: both roundings, and the probability's own error
+    edz = dz.abs() * (2 * half + 8 * U) + (p * (2 * ez + (512 + 8 * big) * U)[:, None]) * g.abs()[:, None]
+    # fp16: relative to the largest row weight, half its least subnormal each time
+    least = tiny * (2 * g.abs().nan_to_num().max() if hidden.dtype == torch.float16 else 1.0)
+    edz = edz + 2 * least
     dz[bad] = math.nan
     gh, gw = dz @ w, dz.t() @ h
     # the products' own sums in fp32, and one rounding of the result
     egh = edz @ w.abs() + (dz.abs() @ w.abs()) * (2 * w.shape[0] * U) + half * gh.abs() + tiny
-    egw = edz.t() @ h.abs() + (dz.abs().t() @ h.abs()) * (2 * len(labels) * U) + half * gw.abs() + tiny
+    egw = edz.t() @ h.abs() + (dz.abs().t() @ h.abs()) * (half + 2 * len(labels) * U) + half * gw.abs() + tiny
+    if hidden.dtype == torch.float16:   # of the weighted hidden rows; no element of D is over 1
+        egw = egw + len(labels) * least
     return (lp, gh, gw), (e, egh * 1.01, egw * 1.01)
 
 

@@ -128,9 +128,18 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert hip.sf_logps_rows(one, 6, 1, 8, one, -100, 1.0, one, one, None) == 9001
     assert hip.sf_logps_rows(one, 9, 1, 8, one, -100, 1.0, one, one, None) == 9007
     assert hip.sf_logps_rows(one, 8, 0, 8, one, -100, 1.0, one, one, None) == 0
-    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, None, one, 7, 8, None) == 9003
-    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, None, one, 1, 8, None) == 9005
-    assert hip.sf_logps_norm(None, one, -100, 1, 1.0, one, None) == hip.sf_logps_norm(one, one, -100, 1, 1.0, None, None) == 9001
+    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, one, 7, 8, None) == 9003
+    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, one, 1, 8, None) == 9005
+    assert hip.sf_logps_weight(None, one, one, -100, 1, 8, 1.0, one, None, None) == 9001
+    tiles = lambda **k: hip.sf_logps_tiles(*{**dict(w=one, ldw=64, v=8, h=one, ldh=64, n=1, k=64, y=one, ig=-100, s=1.0, t=1,  # noqa: E731
+                                                    p=one, tg=one, kp=None, ldk=0, l=one, lp=one, st=None), **k}.values())
+    assert tiles(w=None) == tiles(v=0) == tiles(ldw=32) == tiles(s=0.0) == tiles(kp=one, ldk=64) == tiles(ldh=1 << 23) == 9001
+    assert tiles(k=32) == tiles(w=72) == tiles(ldh=68) == tiles(kp=72, ldk=256) == 9007
+    assert tiles(t=0) == 9003 and tiles(n=0) == 0
+    assert hip.sf_logps_keep_grad(one, 256, 2, 1, 8, one, one, -100, one, one, 1, None) == 9001
+    assert hip.sf_logps_keep_grad(one, 264, 1, 1, 8, one, one, -100, one, one, 1, None) == 9007
+    assert hip.sf_logps_hidden(one, 8, 1, 8, None, 1, one, 64, None) == hip.sf_logps_hidden(one, 8, 1, 8, one, 1, one, 32, None) == 9001
+    assert hip.sf_logps_sum(one, 3, 1, 8, one, 1, None, 0, None, 0, one, None, None) == 9001
     assert hip.sf_align_parts(0, 5) == 0 and hip.sf_align_parts(4, 100) == 4
     assert hip.sf_align_parts(4, 1 << 31) == 0 and hip.sf_align_parts(2, 1 << 20) == 2 * 512
     pref = lambda **k: hip.sf_pref_loss(*{**dict(lp=one, ld=8, ref=one, ldr=8, m=one, ldm=8, p=1, c=8, f=0, b=0.1, s=0.0,  # noqa: E731

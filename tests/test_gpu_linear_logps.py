@@ -182,3 +182,47 @@ def test_chunks(dev, monkeypatch):
     got = (lp.detach(), *torch.autograd.grad(lp, (hidden, weight), up))
     for x, w, b in zip(got, want, bound):
         near(x, w, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [64, 192, 1 << 20])
+def test_backward_without_what_was_kept(dev, monkeypatch, rows, dtype):
+    """Made again, in chunks of any whole 64 rows, as from what was kept."""
+    hidden, weight, labels, up = inputs((300, 128, 1000), dtype, dev)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    want, bound = logps(hidden.detach(), weight.detach(), labels, grad=up)
+    kept = torch.autograd.grad(linear_logps(hidden, weight, labels), (hidden, weight), up)
+    monkeypatch.setattr(module, "_KEEP_BYTES", 0)
+    monkeypatch.setattr(module, "_AGAIN_BYTES", 2 * 1024 * rows)
+    lp = linear_logps(hidden, weight, labels)
+    again = torch.autograd.grad(lp, (hidden, weight), up)
+    for x, w, b in zip((lp.detach(), *again), want, bound):
+        near(x, w, b)
+    if rows >= 300:
+        assert all(torch.equal(x, y) for x, y in zip(kept, again))
+
+
+def test_a_retained_graph_gives_the_same_gradients_again(dev):
+    hidden, weight, labels, up = inputs((300, 128, 1000), torch.bfloat16, dev)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    one = torch.autograd.grad(lp, (hidden, weight), up, retain_graph=True)
+    two = torch.autograd.grad(lp, (hidden, weight), up, retain_graph=True)
+    three = torch.autograd.grad(lp, (hidden, weight), 2 * up)
+    assert all(torch.equal(x, y) and torch.equal(z, 2 * x) for x, y, z in zip(one, two, three))
+
+
+def test_saved_on_the_host(dev):
+    """Hooks that bring the saved tensors back from host memory, or in another type."""
+    hidden, weight, labels, up = inputs((70, 64, 300), torch.bfloat16, dev)
+    hr, wr = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+    want = torch.autograd.grad(linear_logps(hr, wr, labels), (hr, wr), up)
+    with torch.autograd.graph.save_on_cpu():
+        lp = linear_logps(hr, wr, labels)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(lp, (hr, wr), up), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.float() if t.is_floating_point() else t):
+        lp = linear_logps(hr, wr, labels)
+    got = torch.autograd.grad(lp, (hr, wr), up)
+    assert all(torch.allclose(a.float(), b.float(), rtol=0.03, atol=1e-4) for a, b in zip(got, want))
