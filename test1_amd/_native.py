@@ -24,6 +24,7 @@ LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib")
 HIP_LIB = os.path.join(LIB_DIR, "libsf_hip.so")
 CPU_LIB = os.path.join(LIB_DIR, "libsf_cpu.so")
 SEGS_LIB = os.path.join(LIB_DIR, "_sf_segs.so")
+OPS_LIB = os.path.join(LIB_DIR, "_sf_ops.so")
 
 SF_COPY_H2D = 1
 SF_COPY_D2H = 2
@@ -169,6 +170,7 @@ _lock = threading.Lock()
 _hip = None
 _cpu = None
 _segs = None
+_ops = None
 
 _RESTYPES = {"sf_error_string": ctypes.c_char_p, "sf_dma_choose_engines": ctypes.c_uint32,
              "sf_align_parts": ctypes.c_size_t}
@@ -230,6 +232,30 @@ def _load_segs():
         warnings.warn(f"{SEGS_LIB}: {e}; segment tables are made in Python, some 0.5 us a tensor slower "
                       f"(`python -m test1_amd.build` builds it)", RuntimeWarning)
         return None
+
+
+def ops():
+    """The module with the calls and autograd nodes of the losses, the token
+    log-probabilities and the 8-bit checkpoints.  They have no other form on a
+    GPU: it raises where the module is missing or built against another torch."""
+    global _ops
+    if _ops is None:
+        with _lock:
+            if _ops is None:
+                _ops = _load_ops()
+    return _ops
+
+
+def _load_ops():
+    try:
+        spec = importlib.util.spec_from_file_location("_sf_ops", OPS_LIB)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        if module.TORCH_VERSION != torch.__version__:
+            raise ImportError(f"built against torch {module.TORCH_VERSION}, this is {torch.__version__}")
+        return module
+    except ImportError as e:
+        raise RuntimeError(f"native module not loaded: {OPS_LIB}: {e}. Build it with `python -m test1_amd.build`.") from e
 
 
 class NativeError(RuntimeError):

@@ -60,6 +60,10 @@ def pack_act8(x: torch.Tensor, fmt: str = "int8", out: Optional[torch.Tensor] = 
     if out is not None and (out.dtype != torch.uint8 or out.numel() != nbytes or not out.is_contiguous()
                             or out.device != x.device):
         raise ValueError(f"pack_act8: out must be {nbytes} contiguous uint8 on {x.device}")
+    if out is None and stream is None and n > 0 and x.is_cuda and not _traced():
+        packed = _native.ops().act8_pack(x, _CE_DTYPES[x.dtype], code, nbytes)
+        if packed is not None:
+            return packed
     x = x.detach()
     if not _reads_memory(x) or (out is not None and not _reads_memory(out)):
         packed = _pack_torch(x, fmt)
@@ -94,6 +98,10 @@ def unpack_act8(packed: torch.Tensor, shape: Sequence[int], dtype: torch.dtype =
     if out is not None and (out.dtype != dtype or out.shape != shape or not out.is_contiguous()
                             or out.device != packed.device):
         raise ValueError(f"unpack_act8: out must be a contiguous {dtype} tensor of {tuple(shape)} on {packed.device}")
+    if stream is None and n > 0 and packed.is_cuda and not _traced():
+        to = torch.empty(shape, dtype=dtype, device=packed.device) if out is None else out
+        if _native.ops().act8_unpack(packed, to, _CE_DTYPES[dtype], code):
+            return to
     if not _reads_memory(packed) or (out is not None and not _reads_memory(out)):
         x = _unpack_torch(packed, n, dtype, fmt).view(shape)
         return x if out is None else out.copy_(x)

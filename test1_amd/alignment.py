@@ -15,15 +15,13 @@ differentiated again.  Masked tokens count for nothing, whatever stands there.
 
 from __future__ import annotations
 
-import functools
 import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
-from .fused_ce import _PLAIN, _memory_is_value, _saved_plain, _traced
+from .fused_ce import _traced
 
 _FORMS = {"sigmoid": _native.SF_PREF_SIGMOID, "hinge": _native.SF_PREF_HINGE, "ipo": _native.SF_PREF_IPO}
 _REDUCTIONS = ("token", "sequence")
@@ -59,103 +57,6 @@ def _check_tokens(what: str, logps: torch.Tensor, mask: torch.Tensor, **others: 
             raise ValueError(f"{what}: {name} has to be on {logps.device}")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what}: {name} takes no gradient; detach it")
-
-
-def _kernels_take(logps: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
-    if not logps.is_cuda or logps.numel() == 0 or _traced():
-        return False
-    return all(t is None or (type(t) in _PLAIN and _memory_is_value(t)) for t in (logps, *others))
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the kernels read it: the elements of a row side by side, rows
-    any whole number of elements apart that holds one."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        return t.contiguous()
-    return t
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
-
-
-@functools.lru_cache(maxsize=256)
-def _parts(rows: int, cols: int) -> int:
-    return _native.hip().sf_align_parts(rows, cols)
-
-
-def _stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
-
-
-class _on_device:
-    """The tensors' device as the current one, without cost where it is."""
-
-    def __new__(cls, t: torch.Tensor):
-        return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-class _Nothing:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Nothing()
-
-
-# ---------------------------------------------------------------------------
-def _pref_kernels(logps, ref, mask, form, beta, smoothing, average, need_grad):
-    rows, cols = logps.shape
-    pairs = rows // 2
-    logps, ref = _rows(logps), _rows(ref)
-    dev = logps.device
-    parts = torch.empty(2 * _parts(rows, cols), dtype=torch.float64, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    chosen = torch.empty(pairs, dtype=torch.float32, device=dev)
-    rejected = torch.empty(pairs, dtype=torch.float32, device=dev)
-    coef = torch.empty(rows, dtype=torch.float32, device=dev) if need_grad else None
-    _native.check(_native.hip().sf_pref_loss(
-        logps.data_ptr(), _ld(logps), ref.data_ptr(), _ld(ref), mask.data_ptr(), _ld(mask), pairs, cols, form, beta,
-        smoothing, average, parts.data_ptr(), loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(),
-        coef.data_ptr() if need_grad else None, _stream()), "sf_pref_loss")
-    return loss, chosen, rejected, coef
-
-
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logps, ref, mask, form, beta, smoothing, average):
-        ctx.set_materialize_grads(False)
-        loss, chosen, rejected, coef = _pref_kernels(logps, ref, mask, form, beta, smoothing, average, True)
-        ctx.save_for_backward(coef, mask)
-        ctx.mark_non_differentiable(chosen, rejected)
-        return loss, chosen, rejected
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss, *_):
-        if grad_loss is None:
-            return (None,) * 7
-        coef, mask = ctx.saved_tensors
-        if (not _traced() and _saved_plain(coef, torch.float32, grad_loss.device) and type(mask) is torch.Tensor
-                and mask.dtype == torch.bool and mask.device == coef.device and _rows(mask) is mask
-                and _plain_grad(grad_loss)):
-            with _on_device(coef):
-                rows, cols = mask.shape
-                grad = torch.empty((rows, cols), dtype=torch.float32, device=coef.device)
-                _native.check(_native.hip().sf_pref_grad(grad_loss.data_ptr(), coef.data_ptr(), mask.data_ptr(),
-                                                         _ld(mask), rows, cols, grad.data_ptr(), _stream()),
-                              "sf_pref_grad")
-        else:
-            coef = coef.to(torch.float32) * grad_loss
-            grad = torch.where(mask.to(torch.bool), coef.unsqueeze(1), torch.zeros((), device=coef.device))
-        return grad, None, None, None, None, None, None
-
-
-def _plain_grad(g: torch.Tensor) -> bool:
-    return type(g) is torch.Tensor and g.is_cuda and g.dtype == torch.float32 and g.numel() == 1 and _memory_is_value(g)
 
 
 def _log_sigmoid(x: torch.Tensor) -> torch.Tensor:
@@ -209,69 +110,14 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor, mask: torch.Te
         raise ValueError("preference_loss: beta must be above 0")
     if not 0 <= label_smoothing <= 1 or (label_smoothing and kind != "sigmoid"):
         raise ValueError("preference_loss: label_smoothing is in [0, 1], for kind 'sigmoid'")
-    if not _kernels_take(logps, ref_logps, mask):
-        return _pref_torch(logps, ref_logps, mask, kind, beta, label_smoothing, average)
-    args = (_FORMS[kind], float(beta), float(label_smoothing), bool(average))
-    with _on_device(logps):
-        mask = _rows(mask)
-        if torch.is_grad_enabled() and logps.requires_grad:
-            return PreferenceLoss(*_Preference.apply(logps, ref_logps, mask, *args))
-        return PreferenceLoss(*_pref_kernels(logps, ref_logps, mask, *args, False)[:3])
+    if logps.is_cuda and logps.numel() > 0 and not _traced():
+        out = _native.ops().pref_loss(logps, ref_logps, mask, _FORMS[kind], beta, label_smoothing, average)
+        if out is not None:
+            return PreferenceLoss(*out)
+    return _pref_torch(logps, ref_logps, mask, kind, beta, label_smoothing, average)
 
 
 # ---------------------------------------------------------------------------
-def _policy_kernels(logps, old, adv, mask, ref, log_low, log_high, kl_coef, sequences, need_grad):
-    rows, cols = logps.shape
-    logps, old, mask = _rows(logps), _rows(old), _rows(mask)
-    per_token = adv.dim() == 2
-    if per_token:
-        adv = _rows(adv)
-    if ref is not None:
-        ref = _rows(ref)
-    dev = logps.device
-    parts = torch.empty(4 * _parts(rows, cols), dtype=torch.float64, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    kl = torch.empty((), dtype=torch.float32, device=dev) if ref is not None else None
-    clipped = torch.empty((), dtype=torch.float32, device=dev)
-    slope = torch.empty((rows, cols), dtype=torch.float32, device=dev) if need_grad else None
-    weight = torch.empty(rows, dtype=torch.float32, device=dev) if need_grad else None
-    _native.check(_native.hip().sf_policy_loss(
-        logps.data_ptr(), _ld(logps), old.data_ptr(), _ld(old), None if ref is None else ref.data_ptr(),
-        0 if ref is None else _ld(ref), adv.data_ptr(), _ld(adv) if per_token else adv.stride(0), per_token,
-        mask.data_ptr(), _ld(mask), rows, cols, log_low, log_high, kl_coef, sequences, parts.data_ptr(),
-        loss.data_ptr(), None if kl is None else kl.data_ptr(), clipped.data_ptr(),
-        slope.data_ptr() if need_grad else None, weight.data_ptr() if need_grad else None, _stream()), "sf_policy_loss")
-    return loss, kl, clipped, slope, weight
-
-
-class _Policy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logps, *args):
-        ctx.set_materialize_grads(False)
-        loss, kl, clipped, slope, weight = _policy_kernels(logps, *args, True)
-        ctx.save_for_backward(slope, weight)
-        ctx.mark_non_differentiable(*(t for t in (kl, clipped) if t is not None))
-        return loss, kl, clipped
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss, *_):
-        if grad_loss is None:
-            return (None,) * 9
-        slope, weight = ctx.saved_tensors
-        dev = grad_loss.device
-        if (not _traced() and _saved_plain(slope, torch.float32, dev) and _saved_plain(weight, torch.float32, dev)
-                and _plain_grad(grad_loss)):
-            with _on_device(slope):
-                rows, cols = slope.shape
-                grad = torch.empty_like(slope)
-                _native.check(_native.hip().sf_policy_grad(grad_loss.data_ptr(), weight.data_ptr(), slope.data_ptr(),
-                                                           rows, cols, grad.data_ptr(), _stream()), "sf_policy_grad")
-        else:
-            grad = slope.to(torch.float32) * (weight.to(torch.float32) * grad_loss).unsqueeze(-1)
-        return (grad,) + (None,) * 8
-
-
 def _mean_torch(x, mask, sequences):
     x = torch.where(mask, x, torch.zeros_like(x))
     if not sequences:
@@ -332,9 +178,8 @@ def policy_loss(logps: torch.Tensor, old_logps: torch.Tensor, advantages: torch.
     log_low = math.log1p(-clip_low) if clip_low < 1 else -math.inf
     args = (old_logps, advantages, mask, ref_logps, log_low, math.log1p(clip_high), float(kl_coef),
             reduction == "sequence")
-    if not _kernels_take(logps, old_logps, advantages, mask, ref_logps):
-        return _policy_torch(logps, *args)
-    with _on_device(logps):
-        if torch.is_grad_enabled() and logps.requires_grad:
-            return PolicyLoss(*_Policy.apply(logps, *args))
-        return PolicyLoss(*_policy_kernels(logps, *args, False)[:3])
+    if logps.is_cuda and logps.numel() > 0 and not _traced():
+        out = _native.ops().policy_loss(logps, *args)
+        if out is not None:
+            return PolicyLoss(*out)
+    return _policy_torch(logps, *args)

@@ -10,6 +10,8 @@ and -ffp-contract=off keeps every scalar operation a single rounding.  The
 storage offload engine (worker threads, pread/pwrite) is in the same library.
 _sf_segs.so: g++ against torch's headers, a CPython module that reads segment
 tables from lists of tensors.
+_sf_ops.so: g++ against torch's headers and libsf_hip.so, a CPython module with
+the calls and autograd nodes of the losses, log-probabilities and checkpoints.
 """
 
 from __future__ import annotations
@@ -84,10 +86,31 @@ def build_segs(verbose: bool = False) -> str:
     return out
 
 
+def build_ops(verbose: bool = False) -> str:
+    """After ``build_hip``: it links against libsf_hip.so, beside which it lies."""
+    import torch
+
+    out = os.path.join(LIB, "_sf_ops.so")
+    tmp = _atomic_out(out)
+    base = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(HIPCC)))
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__",
+          "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          f'-DSF_TORCH_VERSION="{torch.__version__}"', "-I", INCLUDE, "-I", sysconfig.get_paths()["include"],
+          "-isystem", os.path.join(base, "include"),
+          "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+          "-isystem", os.path.join(rocm, "include"), "-o", tmp, os.path.join(CSRC, "sf_ops.cpp"),
+          "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10",
+          "-L", LIB, "-l:libsf_hip.so", "-Wl,-rpath,$ORIGIN"], verbose)
+    os.replace(tmp, out)
+    return out
+
+
 def build_all(verbose: bool = False) -> None:
     build_hip(verbose)
     build_cpu(verbose)
     build_segs(verbose)
+    build_ops(verbose)
 
 
 if __name__ == "__main__":

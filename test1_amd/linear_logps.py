@@ -17,14 +17,14 @@ the weight gradient's product.
 
 from __future__ import annotations
 
+import contextlib
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .alignment import _on_device, _stream
 from .fused_ce import _DTYPES, _PLAIN, _memory_is_value, _saved_plain, _traced, _vocabulary_parts
 from .kernels import _CE_DTYPES
 
@@ -38,8 +38,28 @@ _KEEP_BYTES = 8 << 30
 _AGAIN_BYTES = 2 << 30
 
 
+def _backward_rows(n: int, vocab: int) -> Tuple[int, bool]:
+    """Rows that the backward takes at a time, and whether the forward keeps
+    their exponentials for it (then all)."""
+    row = 2 * (-(-vocab // _SPAN) * _SPAN)
+    step = max(64, _AGAIN_BYTES // row // 64 * 64)
+    return (n, True) if (n + 63) * row <= _KEEP_BYTES else (min(n, step), False)
+
+
 def _f32_out(dtype: torch.dtype) -> dict:
     return {} if dtype == torch.float32 else dict(out_dtype=torch.float32)
+
+
+def _stream() -> int:
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def _on_device(t: torch.Tensor):
+    """The tensors' device as the current one, without cost where it is."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _chunk_rows(vocab: int) -> int:
@@ -51,33 +71,10 @@ def _logits_buffer(rows: int, vocab: int, device) -> torch.Tensor:
     return torch.empty((rows, -(-vocab // 64) * 64), dtype=torch.float32, device=device)
 
 
-def _padded(n: int, unit: int) -> int:
-    return -(-n // unit) * unit
-
-
-def _in_tiles(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
-    """Whether ``logps_tiles_kernel`` takes the call: 16-bit operands whose rows
-    start on 16-byte boundaries, a sum of whole 64 terms."""
-    return (hidden.element_size() == 2 and hidden.shape[1] % 64 == 0
-            and all(t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= 1 << 22 and t.stride(0) % 8 == 0
-                    and t.data_ptr() % 16 == 0 for t in (hidden, weight)))
-
-
-def _tiles(hidden, weight, labels, ignore_index, scale, keep, lse2, logp):
-    """Results into ``lse2`` and ``logp``; returns the spans' parts."""
+def _forward_kernels(hidden, weight, labels, ignore_index, scale):
     n, v = hidden.shape[0], weight.shape[0]
-    parts = torch.empty((2 * -(-v // _SPAN) + 1) * n, dtype=torch.float32, device=hidden.device)
-    at = parts.data_ptr()
-    _native.check(_native.hip().sf_logps_tiles(
-        weight.data_ptr(), weight.stride(0), v, hidden.data_ptr(), hidden.stride(0), n, hidden.shape[1],
-        labels.data_ptr(), ignore_index, scale, _CE_DTYPES[hidden.dtype], at, at + 4 * (parts.numel() - n),
-        None if keep is None else keep.data_ptr(), 0 if keep is None else keep.stride(0), lse2.data_ptr(),
-        logp.data_ptr(), _stream()), "sf_logps_tiles")
-    return parts
-
-
-def _rows_product(hidden, weight, labels, ignore_index, scale, lse, logp):
-    n, v = hidden.shape[0], weight.shape[0]
+    lse = torch.empty(n, dtype=torch.float32, device=hidden.device)
+    logp = torch.empty(n, dtype=torch.float32, device=hidden.device)
     step = min(n, _chunk_rows(v))
     buf = _logits_buffer(step, v, hidden.device)
     wt = weight.t()
@@ -87,22 +84,7 @@ def _rows_product(hidden, weight, labels, ignore_index, scale, lse, logp):
         _native.check(_native.hip().sf_logps_rows(
             buf.data_ptr(), buf.stride(0), e - s, v, labels.data_ptr() + 8 * s, ignore_index, scale,
             lse.data_ptr() + 4 * s, logp.data_ptr() + 4 * s, _stream()), "sf_logps_rows")
-
-
-def _forward_kernels(hidden, weight, labels, ignore_index, scale, need_grad):
-    """(logp, lse, what the backward finds kept or None)"""
-    n, v = hidden.shape[0], weight.shape[0]
-    dev = hidden.device
-    lse = torch.empty(n, dtype=torch.float32, device=dev)
-    logp = torch.empty(n, dtype=torch.float32, device=dev)
-    if not _in_tiles(hidden, weight):
-        _rows_product(hidden, weight, labels, ignore_index, scale, lse, logp)
-        return logp, lse, None
-    keep = None
-    if need_grad and 2 * _padded(n, 64) * _padded(v, _SPAN) <= _KEEP_BYTES:
-        keep = torch.empty((_padded(n, 64), _padded(v, _SPAN)), dtype=hidden.dtype, device=dev)
-    parts = _tiles(hidden, weight, labels, ignore_index, scale, keep, lse, logp)
-    return logp, lse, None if keep is None else (keep, parts)
+    return logp, lse
 
 
 def _row_weight(grad, logp, labels, vocab, ignore_index, scale, dtype):
@@ -138,60 +120,7 @@ def _rescaled(grad: Optional[torch.Tensor], dtype, norm) -> Optional[torch.Tenso
     return out
 
 
-def _hidden_product(d, ld, weight, row_weight_at, norm, out):
-    """``out`` = row_weight * (d @ weight), rounded once; the sum over the
-    vocabulary in parts where that fills the chip (``_vocabulary_parts``)."""
-    n, v = d.shape
-    h = weight.shape[1]
-    nparts = _vocabulary_parts(n, weight)
-    part = v if nparts == 1 else v // nparts // 8 * 8
-    parts = torch.empty((nparts, n, h), dtype=torch.float32, device=d.device)
-    if nparts == 1:
-        torch.mm(d, weight, out_dtype=torch.float32, out=parts[0])
-    else:
-        torch.bmm(d.as_strided((nparts, n, part), (part, ld, 1)), weight[:nparts * part].view(nparts, part, h),
-                  out_dtype=torch.float32, out=parts)
-    done = nparts * part
-    _native.check(_native.hip().sf_logps_sum(
-        parts.data_ptr(), nparts, n, h, out.data_ptr(), _CE_DTYPES[out.dtype], d.data_ptr() + 2 * done, ld,
-        weight.data_ptr() + 2 * done * h, v - done, row_weight_at, None if norm is None else norm.data_ptr(),
-        _stream()), "sf_logps_sum")
-
-
-def _backward_tiles(grad, hidden, weight, labels, logp, lse2, kept, ignore_index, scale, need_hidden, need_weight):
-    n, h = hidden.shape
-    v = weight.shape[0]
-    dev, dtype = hidden.device, hidden.dtype
-    row_weight, norm = _row_weight(grad, logp, labels, v, ignore_index, scale, dtype)
-    ld = _padded(v, _SPAN)
-    step = n if kept is not None else min(n, max(64, _AGAIN_BYTES // (2 * ld) // 64 * 64))
-    one = step == n
-    gh = torch.empty((n, h), dtype=dtype, device=dev) if need_hidden else None
-    gw = None
-    if need_weight:
-        gw = torch.empty((v, h), dtype=dtype if one and norm is None else torch.float32, device=dev)
-    keep, parts = kept if kept is not None else (torch.empty((_padded(step, 64), ld), dtype=dtype, device=dev), None)
-    again = torch.empty((2, step), dtype=torch.float32, device=dev) if kept is None else None
-    for s in range(0, n, step):
-        m = min(n, s + step) - s
-        hc, pad = hidden[s:s + m], _padded(m, 64)
-        if kept is None:
-            parts = _tiles(hc, weight, labels[s:s + m], ignore_index, scale, keep, again[0], again[1])
-        _native.check(_native.hip().sf_logps_keep_grad(
-            keep.data_ptr(), ld, m, pad, v, parts.data_ptr(), labels.data_ptr() + 8 * s, ignore_index,
-            lse2.data_ptr() + 4 * s, logp.data_ptr() + 4 * s, _CE_DTYPES[dtype], _stream()), "sf_logps_keep_grad")
-        if need_hidden:
-            _hidden_product(keep[:m, :v], ld, weight, row_weight.data_ptr() + 4 * s, norm, gh[s:s + m])
-        if need_weight:
-            ht = torch.empty((h, pad), dtype=dtype, device=dev)
-            _native.check(_native.hip().sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h,
-                                                        row_weight.data_ptr() + 4 * s, _CE_DTYPES[dtype],
-                                                        ht.data_ptr(), pad, _stream()), "sf_logps_hidden")
-            _add_product(gw, keep[:pad, :v].t(), ht.t(), s == 0)
-    return gh, _rescaled(gw, dtype, norm)
-
-
-def _backward_rows(grad, hidden, weight, labels, logp, lse, ignore_index, scale, need_hidden, need_weight):
+def _backward_kernels(grad, hidden, weight, labels, logp, lse, ignore_index, scale, need_hidden, need_weight):
     n, h = hidden.shape
     v = weight.shape[0]
     dev, dtype = hidden.device, hidden.dtype
@@ -229,9 +158,9 @@ class _LinearLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, scale):
         ctx.set_materialize_grads(False)
-        logp, lse, ctx.kept = _forward_kernels(hidden, weight, labels, ignore_index, scale, True)
+        logp, lse = _forward_kernels(hidden, weight, labels, ignore_index, scale)
         ctx.save_for_backward(hidden, weight, labels, lse, logp)
-        ctx.ignore_index, ctx.scale, ctx.tiles = ignore_index, scale, _in_tiles(hidden, weight)   # lse in base 2
+        ctx.ignore_index, ctx.scale = ignore_index, scale
         return logp
 
     @staticmethod
@@ -244,17 +173,9 @@ class _LinearLogps(torch.autograd.Function):
         if (type(grad) is torch.Tensor and grad.is_cuda and _memory_is_value(grad) and _kernels_take(hidden, weight, labels)
                 and _saved_plain(lse, torch.float32, hidden.device) and _saved_plain(logp, torch.float32, hidden.device)
                 and labels.is_contiguous()):
-            # What was kept turns into the gradient in place: a second backward
-            # of a retained graph makes it again.
-            kept, ctx.kept = ctx.kept, None
-            args = (grad.to(torch.float32).contiguous(), hidden, weight, labels, logp, lse)
             with _on_device(hidden):
-                if ctx.tiles and _in_tiles(hidden, weight):
-                    return (*_backward_tiles(*args, kept, ctx.ignore_index, ctx.scale, *need), None, None, None)
-                if not ctx.tiles:
-                    return (*_backward_rows(*args, ctx.ignore_index, ctx.scale, *need), None, None, None)
-        if ctx.tiles:
-            lse = lse * math.log(2)
+                return (*_backward_kernels(grad.to(torch.float32).contiguous(), hidden, weight, labels, logp, lse,
+                                           ctx.ignore_index, ctx.scale, *need), None, None, None)
         with torch.autocast(hidden.device.type, enabled=False):
             valid, at, bad = _label_kinds(labels, weight.shape[0], ctx.ignore_index)
             p = torch.exp(hidden.float() @ weight.float().t() * ctx.scale - lse.float().unsqueeze(1))
@@ -319,9 +240,16 @@ def linear_logps(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tenso
         return _torch_logps(hidden, weight, labels, ignore_index, scale)
     rows = hidden.reshape(-1, hidden.shape[-1]) if hidden.dim() != 2 else hidden
     flat = labels.reshape(-1).contiguous()
-    with _on_device(hidden):
-        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-            logp = _LinearLogps.apply(rows, weight, flat, ignore_index, scale)
-        else:
-            logp = _forward_kernels(rows, weight, flat, ignore_index, scale, False)[0]
+    need_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+    step, keep, nparts = rows.shape[0], False, 1
+    if need_grad:
+        step, keep = _backward_rows(step, weight.shape[0])
+        nparts = _vocabulary_parts(step, weight)
+    logp = _native.ops().linear_logps(rows, weight, flat, ignore_index, scale, nparts, step, keep)
+    if logp is None:
+        with _on_device(hidden):
+            if need_grad:
+                logp = _LinearLogps.apply(rows, weight, flat, ignore_index, scale)
+            else:
+                logp = _forward_kernels(rows, weight, flat, ignore_index, scale)[0]
     return logp if labels.dim() == 1 else logp.view(labels.shape)
