@@ -3,6 +3,9 @@
 Public API, matching the reference's:
     SlideFSDPConfig, SlideFSDP, LayerAdam, SlidingCheckpoint,
     LayerBufferPool, LayerRuntimeState
+and beside it the operators of preference and policy fine-tuning:
+    preference_loss, policy_loss, pack_act8, unpack_act8 and
+    ``linear_logps.linear_logps``
 The device work runs in hand-written HIP kernels for gfx950 behind the C ABI
 declared in include/slidefsdp.h (``test1_amd/lib/libsf_hip.so``); the host
 AdamW runs in ``test1_amd/lib/libsf_cpu.so``.
@@ -23,6 +26,12 @@ def __getattr__(name):
     if name in ("SlidingCheckpoint", "ActivationRing", "StorageSpill", "save_on_cpu"):
         from . import sliding_checkpoint
         return getattr(sliding_checkpoint, name)
+    if name in ("preference_loss", "policy_loss", "PreferenceLoss", "PolicyLoss"):
+        from . import alignment
+        return getattr(alignment, name)
+    if name in ("pack_act8", "unpack_act8", "act8_bytes"):
+        from . import act8
+        return getattr(act8, name)
     if name == "LayerAdam":
         from .optimizer import LayerAdam
         return LayerAdam

@@ -49,7 +49,8 @@ from __future__ import annotations
 
 import os
 import warnings
-from typing import List, Optional
+from dataclasses import dataclass
+from typing import Any, Callable, List, Optional
 
 import torch
 import torch.nn as nn
@@ -57,9 +58,11 @@ from torch.utils.checkpoint import checkpoint
 from transformers.modeling_outputs import CausalLMOutputWithPast
 
 from . import _native, kernels
+from .act8 import _check_format, act8_bytes
 from .config import SlideFSDPConfig
 from .distributed_sync import create_distributed_sync
 from .fused_ce import chunked_linear_cross_entropy
+from .linear_logps import linear_logps
 from .layer_state import GradSlotRing, LayerRuntimeState, StreamingRuntime
 from .optimizer import LayerAdam
 from .sliding_checkpoint import ActivationRing, KeptOnDevice, SlidingCheckpoint, StorageSpill, pin_or_keep
@@ -69,6 +72,15 @@ try:  # transformers >= 5: masks are built by a module-level function
     from transformers.masking_utils import create_causal_mask as _hf_create_causal_mask
 except ImportError:  # older versions keep the decoder's _update_causal_mask
     _hf_create_causal_mask = None
+
+@dataclass
+class ObjectiveOutput(CausalLMOutputWithPast):
+    """What a step on an ``objective`` returns: the loss, the log-probabilities
+    it was computed from, [B, S - 1], and what the objective returned."""
+
+    logps: Optional[torch.Tensor] = None
+    result: Any = None
+
 
 class OutputLayer(nn.Module):
     """Final norm + lm_head + shifted cross-entropy as one unit (reference
@@ -88,6 +100,12 @@ class OutputLayer(nn.Module):
         self.chunk_rows = chunk_rows
         self.lce = chunked_linear_cross_entropy if fused else None
         self.loss_fn = nn.CrossEntropyLoss()
+
+    def token_logps(self, hidden_states: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
+        """Log-probabilities of the shifted labels, [B, S - 1] fp32, 0 where
+        they are ignored; no logits are kept."""
+        return linear_logps(self.norm(hidden_states)[..., :-1, :], self.lm_head.weight, labels[..., 1:],
+                            self.loss_fn.ignore_index, temperature)
 
     def forward(self, hidden_states: torch.Tensor, labels: Optional[torch.Tensor] = None):
         hidden_states = self.norm(hidden_states)
@@ -257,6 +275,14 @@ class SlideFSDP(nn.Module):
                          parameter of pinned host memory for those units,
                          pinned after the gradient slots; units the host
                          cannot pin reload fp32.
+      checkpoint_format  None (default): checkpoints keep the model's type;
+                         "int8" or "fp8": the decoders' inputs are packed into
+                         8 bits with a scale for each 128 elements (``act8``)
+                         for the host link, their pinned slots or files, and
+                         restored for the recompute: 1.03 bytes an element
+                         instead of 2.  Gradients then carry the format's
+                         error; the loss does not, and the last decoder's
+                         checkpoint, which stays on the GPU, is exact.
     """
 
     def __init__(self, model, config: SlideFSDPConfig, *, stage_chunk_elems: Optional[int] = None,
@@ -267,8 +293,14 @@ class SlideFSDP(nn.Module):
                  fused_cross_entropy: bool = False, stage_after_update: bool = True,
                  update_piece_elems: int = 0, cast_at_use: bool = True, early_embedding_update: bool = True,
                  bf16_reload: Optional[bool] = None, checkpoint_d2h: Optional[str] = None,
-                 h2d_issue_limit: int = 3):
+                 h2d_issue_limit: int = 3, checkpoint_format: Optional[str] = None):
         super().__init__()
+        if checkpoint_format is not None:
+            _check_format(checkpoint_format)
+            if not config.enable_activation_checkpoint or config.ac_offload_mode == "none":
+                raise ValueError("checkpoint_format needs checkpoints that are offloaded (enable_activation_checkpoint "
+                                 "and ac_offload_mode 'cpu' or 'nvme')")
+        self._checkpoint_format = checkpoint_format
         if config.param_transfer_mode != "full":
             raise NotImplementedError("SlideFSDP runs on one GPU: only param_transfer_mode='full' is supported")
         self.config = config
@@ -647,22 +679,85 @@ class SlideFSDP(nn.Module):
         that layer's checkpoint in device memory; the reference raises there."""
         if self.config.ac_offload_mode == "none":
             return
-        self.layer_tensors = [
-            [pin_or_keep((batch_size, seq_length, hidden_size), self.dtype)]
-            for _ in range(self.num_decoder_layers)
-        ]
+        shape, dtype = self._checkpoint_slot(batch_size, seq_length, hidden_size)
+        self.layer_tensors = [[pin_or_keep(shape, dtype)] for _ in range(self.num_decoder_layers)]
         kept = sum(isinstance(t[0], KeptOnDevice) for t in self.layer_tensors)
         if kept:
             warnings.warn(f"{kept} of {self.num_decoder_layers} checkpoint slots could not be pinned; "
                           "those layers keep their checkpoints in device memory")
+
+    def _checkpoint_slot(self, batch_size: int, seq_length: int, hidden_size: int):
+        """Shape and type of a decoder's checkpoint as it lies on the host (of
+        packed ones the 16-bit words)."""
+        shape = (batch_size, seq_length, hidden_size)
+        if self._checkpoint_format is None:
+            return shape, self.dtype
+        return (act8_bytes(batch_size * seq_length * hidden_size) // 2,), torch.int16
 
     @staticmethod
     def _first(out):
         return out[0] if isinstance(out, (tuple, list)) else out
 
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
-                labels: Optional[torch.Tensor] = None, **kwargs) -> CausalLMOutputWithPast:
-        """One training step (reference slide_fsdp.py:507-640)."""
+                labels: Optional[torch.Tensor] = None, objective: Optional[Callable] = None,
+                temperature: float = 1.0, **kwargs) -> CausalLMOutputWithPast:
+        """One training step (reference slide_fsdp.py:507-640).
+
+        ``objective``: in place of the cross entropy, a callable of the
+        labels' log-probabilities under the model, [B, S - 1] fp32 at
+        ``temperature`` and shifted by one, and of the bool mask of those that
+        count (labels that are not -100); it returns the loss, or something
+        with the loss in its ``loss`` (``alignment.preference_loss`` and
+        ``policy_loss`` do).  The step's backward starts from that loss, and
+        the output is an ``ObjectiveOutput``."""
+        if objective is not None and labels is None:
+            raise ValueError("SlideFSDP: an objective needs labels")
+        hidden_states = self._run_decoders(input_ids, attention_mask)
+        output_state = self.layer_states[-1]
+        hidden_states = self._PreLayerFunction.apply(hidden_states, output_state, None)
+        if objective is None:
+            loss, logits = self.output_layer(hidden_states, labels)
+        else:
+            labels = labels.to(hidden_states.device)
+            logps = self.output_layer.token_logps(hidden_states, labels, temperature)
+            logits, result = None, objective(logps, labels[..., 1:] != self.output_layer.loss_fn.ignore_index)
+            loss = result if isinstance(result, torch.Tensor) else result.loss
+        if loss is not None:
+            loss = self._PostLayerFunction.apply(loss, output_state, True)
+            if self._early_embedding_update and torch.is_grad_enabled() and loss.requires_grad:
+                # the backward below reaches the lookup: the embedding's
+                # gradient-free rows can be updated while it starts
+                self.layer_states[0].start_early_update()
+            try:
+                loss.backward()
+            except BaseException:
+                self._after_failed_backward()
+                raise
+            if isinstance(self.runtime.grad_ring, GradSlotRing) and not self._ring_grown:
+                self._ring_grow_pending = True
+        if objective is not None:
+            return ObjectiveOutput(loss=loss, logps=logps.detach(), result=result)
+        return CausalLMOutputWithPast(loss=loss, logits=logits)
+
+    @torch.no_grad()
+    def token_logps(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
+                    labels: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
+        """Log-probabilities of ``labels`` (default: the input) under the model
+        as it is, [B, S - 1] fp32, shifted by one, 0 where the label is -100:
+        what a preference or policy objective takes of its reference policy or
+        of the policy that sampled.  Nothing is kept for a backward."""
+        labels = (input_ids if labels is None else labels).to(self.device)
+        hidden_states = self._run_decoders(input_ids, attention_mask)
+        hidden_states = self._PreLayerFunction.apply(hidden_states, self.layer_states[-1], None)
+        logps = self.output_layer.token_logps(hidden_states, labels, temperature)
+        # No backward follows, for which the last two units stay loaded: what
+        # they hold of the pool goes back to it, or the next forward waits for it.
+        for state in self.layer_states[-2:]:
+            state.to_offload_async(is_backward=False)
+        return logps
+
+    def _run_decoders(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor]) -> torch.Tensor:
+        """The lookup and every decoder: the last hidden states."""
         batch_size, seq_length = input_ids.shape
         self._prepare_host_buffers(batch_size, seq_length)
         self._act_ring.reset()
@@ -735,31 +830,15 @@ class SlideFSDP(nn.Module):
                                        on_prefetch_ready=self._reopen_compute,
                                        before_pin=self._drain,
                                        served=self.runtime.capture_served,
-                                       pack_engine=self._checkpoint_d2h):
+                                       pack_engine=self._checkpoint_d2h,
+                                       checkpoint_format=self._checkpoint_format):
                     hidden_states = checkpoint(_layer_forward, hidden_states, causal_mask, self.position_embeddings,
                                                layer_state.layer, **ckpt_kw)
             else:
                 hidden_states = checkpoint(_layer_forward, hidden_states, causal_mask, self.position_embeddings,
                                            layer_state.layer, **ckpt_kw)
             hidden_states = self._PostLayerFunction.apply(hidden_states, layer_state, is_last_decoder)
-
-        output_state = self.layer_states[-1]
-        hidden_states = self._PreLayerFunction.apply(hidden_states, output_state, None)
-        loss, logits = self.output_layer(hidden_states, labels)
-        if loss is not None:
-            loss = self._PostLayerFunction.apply(loss, output_state, True)
-            if self._early_embedding_update and torch.is_grad_enabled() and loss.requires_grad:
-                # the backward below reaches the lookup: the embedding's
-                # gradient-free rows can be updated while it starts
-                self.layer_states[0].start_early_update()
-            try:
-                loss.backward()
-            except BaseException:
-                self._after_failed_backward()
-                raise
-            if isinstance(self.runtime.grad_ring, GradSlotRing) and not self._ring_grown:
-                self._ring_grow_pending = True
-        return CausalLMOutputWithPast(loss=loss, logits=logits)
+        return hidden_states
 
     def _prepare_host_buffers(self, batch_size: int, seq_length: int) -> None:
         """Before a step's first copy: widen the gradient slot ring once (after
@@ -775,8 +854,8 @@ class SlideFSDP(nn.Module):
             self._drain()
             self._grow_grad_ring()
         act_alloc = (self.config.ac_offload_mode == "cpu" and self.config.enable_activation_checkpoint
-                     and (self.layer_tensors is None
-                          or self.layer_tensors[0][0].shape != (batch_size, seq_length, hidden_size)))
+                     and (self.layer_tensors is None or self.layer_tensors[0][0].shape
+                          != self._checkpoint_slot(batch_size, seq_length, hidden_size)[0]))
         embed_rows = (self.layer_states[0].row_sparse
                       and not self.layer_states[0].host_buffers_fit(batch_size * seq_length))
         if act_alloc or embed_rows:

@@ -29,7 +29,14 @@ What is different, and why:
     engine, started by a worker thread once the tensor is produced (a kernel
     writing into host memory slows the kernels beside it); otherwise 16-bit
     tensors are packed into their slot by a kernel with a capped grid instead
-    of the runtime's full-device copy kernel.
+    of the runtime's full-device copy kernel;
+  * with ``checkpoint_format="int8"`` or ``"fp8"`` a layer's first 16-bit
+    tensor, its hidden states, is packed into 8 bits on the producing stream
+    (``act8``) and crosses the link, lies in its slot or file and comes back so,
+    half the bytes, to be restored on the consuming stream when it is served.
+    The recompute then reads what was restored: gradients differ by the
+    format's error.  The last layer's checkpoint, which stays on the GPU, and
+    masks are as they were.
 
 Storage mode (``gds_offload=True``, reference sliding_checkpoint.py:133-202):
 the reference writes each checkpoint input from device memory straight to
@@ -60,6 +67,7 @@ from torch.autograd.graph import saved_tensors_hooks
 from torch.autograd.graph import save_on_cpu  # noqa: F401
 
 from . import _native, kernels, storage
+from .act8 import _check_format, pack_act8, unpack_act8
 from .pinned import pinned_empty
 
 _offload_streams = {}
@@ -238,6 +246,16 @@ class _OnStorage:
 
     def __init__(self, path: str, shape, dtype):
         self.path, self.shape, self.dtype = path, shape, dtype
+
+
+class _In8Bits:
+    """What pack returns for a tensor packed into 8 bits: what it would return
+    for the packed one, and what that restores to."""
+
+    __slots__ = ("held", "shape", "dtype")
+
+    def __init__(self, held: Any, shape, dtype):
+        self.held, self.shape, self.dtype = held, tuple(shape), dtype
 
 
 class _Unless:
@@ -463,7 +481,12 @@ class SlidingCheckpoint(saved_tensors_hooks):
         before_pin=None,
         served=None,
         pack_engine: str = "kernel",
+        checkpoint_format: Optional[str] = None,
     ):
+        if checkpoint_format is not None:
+            _check_format(checkpoint_format)
+            if not pin_memory:
+                raise ValueError("SlidingCheckpoint: checkpoint_format needs pin_memory")
         if pack_engine not in ("kernel", "sdma"):
             raise ValueError("SlidingCheckpoint: pack_engine must be 'kernel' or 'sdma'")
         if gds_offload:
@@ -520,8 +543,31 @@ class SlidingCheckpoint(saved_tensors_hooks):
         # write_after_dma``; needs ``prefetch_ring`` and a contiguous tensor,
         # else the kernel is used).
         self.pack_engine = pack_engine
+        # None: checkpoints keep their type; "int8" or "fp8": see the module's
+        # docstring.
+        self.checkpoint_format = checkpoint_format
 
         def pack_hook(tensor: torch.Tensor) -> Tuple[torch.device, Any]:
+            if (self.checkpoint_format is None or self.is_last_layer or self.pack_counter > 0
+                    or tensor.dtype not in (torch.bfloat16, torch.float16) or tensor.numel() == 0):
+                return pack(tensor)
+            # 16-bit words from here on, which every way to the host takes
+            packed = pack_act8(tensor, self.checkpoint_format).view(torch.int16)
+            device, held = pack(packed)
+            return (device, _In8Bits(held, tensor.shape, tensor.dtype))
+
+        def unpack_hook(packed: Tuple[torch.device, Any]) -> torch.Tensor:
+            device, where = packed
+            if not isinstance(where, _In8Bits):
+                return unpack(packed)
+            at = (self.layer_idx, self.unpack_counter)
+            got = unpack((device, where.held)).view(torch.uint8)
+            tensor = unpack_act8(got, where.shape, where.dtype, self.checkpoint_format)
+            if self.served is not None:
+                self.served[at] = tensor.detach().clone()
+            return tensor
+
+        def pack(tensor: torch.Tensor) -> Tuple[torch.device, Any]:
             if tensor.size() == torch.Size([0]):
                 # The checkpoint's empty placeholder: nothing to copy.  The
                 # reference's `.cpu()` (sliding_checkpoint.py:54-55) is a
@@ -608,7 +654,7 @@ class SlidingCheckpoint(saved_tensors_hooks):
                 return (tensor.device, self._on_storage(path, tensor))
             return (tensor.device, slot)
 
-        def unpack_hook(packed: Tuple[torch.device, Any]) -> torch.Tensor:
+        def unpack(packed: Tuple[torch.device, Any]) -> torch.Tensor:
             device, tensor = packed
             if isinstance(tensor, torch.Tensor) and tensor.size() == torch.Size([0]):
                 return torch.empty(tensor.shape, dtype=tensor.dtype, device=device)
