@@ -285,6 +285,8 @@ class SlideFSDP(nn.Module):
                          checkpoint, which stays on the GPU, is exact.
     """
 
+    _checkpoint_format: Optional[str] = None
+
     def __init__(self, model, config: SlideFSDPConfig, *, stage_chunk_elems: Optional[int] = None,
                  stage_depth: int = 3, grad_ring_depth: Optional[int] = None,
                  wait_timeout: Optional[float] = DEFAULT_WAIT_TIMEOUT,
