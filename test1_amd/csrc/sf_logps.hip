@@ -88,6 +88,7 @@ __device__ __forceinline__ void interleave() {
     __builtin_amdgcn_sched_group_barrier(0x008, kMul, 0);
 }
 
+// kWV x kWT waves of words and of tokens.
 template <typename Fmt, int kWV, int kWT, int kFV, int kFT, bool kKeep>
 __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Tiles a) {
     constexpr int kWaves = kWV * kWT, kBV = kWV * kFV * 16, kBT = kWT * kFT * 16;
@@ -95,18 +96,24 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
     constexpr int kBuffer = (kBV + kBT) * kRowBytes;
     constexpr int kLV = kBV / 8 / kWaves, kLT = kBT / 8 / kWaves;   // a wave copies 8 rows at once
     static_assert(kLV * 8 * kWaves == kBV && kLT * 8 * kWaves == kBT, "rows divide among the waves");
+    // The end exchanges maxima and sums between the waves and turns each wave's 16
+    // tokens of kept words around, over the buffers.
+    constexpr int kTurnRow = kFV * 32;   // bytes of a token's words of a wave
+    static_assert(kWaves * 16 * kTurnRow <= 2 * kBuffer && kWV * kBT * 4 <= 2 * kBuffer, "the buffers hold it");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer];
 
-    // a contiguous run of tiles for each XCD (workgroups go to them in turn)
+    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wv = wave / kWT, wt = wave % kWT, wv0 = wv * kFV * 16, wt0 = wt * kFT * 16;
+
+    // Workgroups go to the XCDs in turn: each XCD has a contiguous run of tiles.
     const uint32_t tiles_v = (a.vocab + kBV - 1) / kBV, tiles_t = (a.tokens + kBT - 1) / kBT;
     const uint32_t xcd = blockIdx.x % 8, each = gridDim.x / 8, more = gridDim.x % 8;
     const uint32_t id = xcd * each + min(xcd, more) + blockIdx.x / 8;
     const uint32_t first_t = id / (kGroupT * tiles_v) * kGroupT, group_t = min(uint32_t(kGroupT), tiles_t - first_t);
     const uint32_t in = id - first_t * tiles_v;
-    const uint32_t tile_v = in / group_t, v0 = tile_v * kBV, t0 = (first_t + in % group_t) * kBT;
+    const uint32_t v0 = in / group_t * kBV, t0 = (first_t + in % group_t) * kBT;
 
-    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint8_t* gv = reinterpret_cast<const uint8_t*>(a.weight + uint64_t(v0) * a.ldw);
     const uint8_t* gt = reinterpret_cast<const uint8_t*>(a.hidden + uint64_t(t0) * a.ldh);
     // Rows past the last are the last one again: their results are dropped below.
@@ -131,8 +138,6 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
             __builtin_amdgcn_global_load_lds((Global*)(gt + step * kRowBytes + off[kLV + j]),
                                              (Lds*)(to + kBV * kRowBytes + j * kWaves * 1024), 16, 0, 0);
     };
-
-    const uint32_t wv = wave / kWT, wt = wave % kWT;
     const uint32_t at = (quad ^ (l16 & 7)) * 16;
     const uint32_t at_v = (wv * kFV * 16 + l16) * kRowBytes, at_t = (kBV + wt * kFT * 16 + l16) * kRowBytes;
     u32x4 x[2][kFV], y[2][kFT];
@@ -144,10 +149,6 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
         for (int j = 0; j < kFT; ++j) y[half][j] = *reinterpret_cast<const u32x4*>(from + at_t + j * 16 * kRowBytes);
     };
     f32x4 acc[kFV][kFT];
-#pragma unroll
-    for (int i = 0; i < kFV; ++i)
-#pragma unroll
-        for (int j = 0; j < kFT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const auto multiply = [&](int half) {
 #pragma unroll
         for (int i = 0; i < kFV; ++i)
@@ -163,31 +164,43 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // kMore: there is a buffer after the next to copy; kNext: there is a next one
-    const auto step = [&](uint32_t s, auto kMore, auto kNext) {
+    // kMore: there is a buffer after the next to copy
+    const auto step = [&](uint32_t s, auto kMore) {
         read(s & 1, 1);
         multiply(0);
         interleave<kFV + kFT, kFV * kFT, 0>();
         meet();
         if constexpr (decltype(kMore)::value) copy(s + 2, s & 1);
-        if constexpr (decltype(kNext)::value) read((s + 1) & 1, 0);
+        read((s + 1) & 1, 0);
         multiply(1);
-        if constexpr (decltype(kNext)::value) interleave<kFV + kFT, kFV * kFT, decltype(kMore)::value ? kLV + kLT : 0>();
+        interleave<kFV + kFT, kFV * kFT, decltype(kMore)::value ? kLV + kLT : 0>();
         __builtin_amdgcn_sched_barrier(0);
     };
+#pragma unroll
+    for (int i = 0; i < kFV; ++i)
+#pragma unroll
+        for (int j = 0; j < kFT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     copy(0, 0);
     if (a.steps > 1) copy(1, 1);
     meet();
     read(0, 0);
     uint32_t s = 0;
-    for (; s + 2 < a.steps; ++s) step(s, std::true_type{}, std::true_type{});
-    if (s + 1 < a.steps) step(s++, std::false_type{}, std::true_type{});
-    step(s, std::false_type{}, std::false_type{});
+    for (; s + 2 < a.steps; ++s) step(s, std::true_type{});
+    if (s + 1 < a.steps) step(s++, std::false_type{});
+    read(s & 1, 1);
+    multiply(0);
+    interleave<kFV + kFT, kFV * kFT, 0>();
+    meet();   // the buffers are not read again
+    int32_t label[kFT];   // as an index from this lane's first word
+#pragma unroll
+    for (int j = 0; j < kFT; ++j) {
+        const uint32_t token = t0 + wt0 + j * 16 + l16;
+        const int64_t y64 = a.labels[min(token, a.tokens - 1)];
+        const bool inside = token < a.tokens && y64 >= 0 && y64 < int64_t(a.vocab);
+        label[j] = inside ? int32_t(y64) - int32_t(v0 + wv0 + quad * 4) : -1;
+    }
+    multiply(1);
 
-    // Every wave is past its last read of LDS at the barrier in its last step.
-    float* top = reinterpret_cast<float*>(lds);          // [kWV][kBT]
-    float* sums = top + kWV * kBT;                       // [kWV][kBT]
-    const uint32_t wv0 = wv * kFV * 16, wt0 = wt * kFT * 16;
     if (v0 + kBV > a.vocab) {
 #pragma unroll
         for (int i = 0; i < kFV; ++i)
@@ -197,6 +210,8 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
 #pragma unroll
                     for (int j = 0; j < kFT; ++j) acc[i][j][r] = -__builtin_inff();
     }
+    float* const shared = reinterpret_cast<float*>(lds);   // [kWV][kBT]
+    float top[kFT], sum[kFT];
 #pragma unroll
     for (int j = 0; j < kFT; ++j) {
         float m = -__builtin_inff();
@@ -206,60 +221,78 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
             for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        if (quad == 0) top[wv * kBT + wt0 + j * 16 + l16] = m;
+        if (quad == 0) shared[wv * kBT + wt0 + j * 16 + l16] = m;
+        // the label's product, by the one lane that has it
+        if (uint32_t(label[j]) < uint32_t(kFV * 16) && (label[j] & 15) < 4) {
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFV; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (label[j] == i * 16 + r) z = acc[i][j][r];
+            a.target[t0 + wt0 + j * 16 + l16] = z;
+        }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kFT; ++j) {
-        const uint32_t t = wt0 + j * 16 + l16, token = t0 + t;
-        float m = top[t];
+        const uint32_t t = wt0 + j * 16 + l16;
+        float m = shared[t];
 #pragma unroll
-        for (int w = 1; w < kWV; ++w) m = fmaxf(m, top[w * kBT + t]);
-        m *= a.scale2;
-        // exp2(scale2 x - base(m)): the product is not rounded before the difference
-        const float c = base(m);
-        float sum = 0.0f;
+        for (int w = 1; w < kWV; ++w) m = fmaxf(m, shared[w * kBT + t]);
+        top[j] = m * a.scale2;
+    }
+    __syncthreads();   // read by all before it is overwritten
+    uint8_t* const turn = lds + wave * 16 * kTurnRow;
+#pragma unroll
+    for (int j = 0; j < kFT; ++j) {
+        // exp2(scale2 x - base(top)): the product is not rounded before the difference
+        const float c = base(top[j]);
+        sum[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kFV; ++i) {
             f32x4 e;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 e[r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], a.scale2, -c));
-                sum += e[r];
+                sum[j] += e[r];
             }
-            if (kKeep && token < a.tokens) {
-                u32x2 p = {Fmt::pack(e[0], e[1]), Fmt::pack(e[2], e[3])};
-                *reinterpret_cast<u32x2*>(a.keep + token * a.ld_keep + v0 + wv0 + i * 16 + quad * 4) = p;
+            if constexpr (kKeep) {
+                const uint32_t to = ((i * 2 + (quad >> 1)) ^ (l16 & (kFV * 2 - 1))) * 16 + (quad & 1) * 8;
+                *reinterpret_cast<u32x2*>(turn + l16 * kTurnRow + to) =
+                    u32x2{Fmt::pack(e[0], e[1]), Fmt::pack(e[2], e[3])};
             }
         }
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        if (quad == 0) sums[wv * kBT + t] = sum;
-        // the label's product, by the one lane that has it
-        const int64_t label = token < a.tokens ? a.labels[token] : -1;
-        const int64_t from = int64_t(v0) + wv0 + quad * 4;
-        if (label >= from && label < from + kFV * 16 && label < int64_t(a.vocab)) {
-            const uint32_t o = uint32_t(label - from);
-            float z = 0.0f;
-            bool mine = false;
+        sum[j] += __shfl_xor(sum[j], 16);
+        sum[j] += __shfl_xor(sum[j], 32);
+        if constexpr (kKeep) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            constexpr int kAcross = kTurnRow / 16, kRows = 64 / kAcross;   // lanes of a row, rows at once
 #pragma unroll
-            for (int i = 0; i < kFV; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (o == uint32_t(i * 16 + r)) z = acc[i][j][r], mine = true;
-            if (mine) a.target[token] = z;
+            for (int k = 0; k < 16 / kRows; ++k) {
+                const uint32_t r = k * kRows + lane / kAcross, c16 = lane % kAcross;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(turn + r * kTurnRow + (c16 ^ (r & (kFV * 2 - 1))) * 16);
+                const uint32_t token = t0 + wt0 + j * 16 + r;
+                if (token < a.tokens)
+                    *reinterpret_cast<u32x4*>(a.keep + token * a.ld_keep + v0 + wv0 + c16 * 8) = v;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
+    if constexpr (kKeep) __syncthreads();
+    if (wv > 0 && quad == 0)
+#pragma unroll
+        for (int j = 0; j < kFT; ++j) shared[wv * kBT + wt0 + j * 16 + l16] = sum[j];
     __syncthreads();
-    for (uint32_t t = threadIdx.x; t < uint32_t(kBT) && t0 + t < a.tokens; t += kWaves * 64) {
-        float m = top[t], sum = sums[t];
+    if (wv == 0 && quad == 0)
 #pragma unroll
-        for (int w = 1; w < kWV; ++w) {
-            m = fmaxf(m, top[w * kBT + t]);
-            sum += sums[w * kBT + t];
+        for (int j = 0; j < kFT; ++j) {
+            const uint32_t t = wt0 + j * 16 + l16;
+#pragma unroll
+            for (int w = 1; w < kWV; ++w) sum[j] += shared[w * kBT + t];
+            if (t0 + t < a.tokens)
+                a.parts[uint64_t(v0 / kSpan) * a.tokens + t0 + t] = float2{top[j], sum[j]};
         }
-        a.parts[uint64_t(tile_v) * a.tokens + t0 + t] = float2{m * a.scale2, sum};
-    }
 }
 
 // The tiles' parts of each token joined.  A workgroup takes 4 tokens, 64 lanes
@@ -487,13 +520,45 @@ int launch_tiles(const Tiles& a, hipStream_t st) {
     return status();
 }
 
+// The tile for a call: tokens of a tile, and the time of a round of them over
+// the chip (256 tiles of 256 or 128 tokens, 512 of the smaller ones, of which a
+// compute unit holds two; `half`: where there is at most one for each unit), in
+// that of a round of the largest.  Small sums (`brief`, under 2048 terms) spend
+// more of it at the ends of their tiles.  Measured, us, 256 | 128 | 64 | 32
+// tokens a tile: 128256 words x 4092 terms and 64 tokens 212 | 200 | 170 | 201,
+// 128 tokens 218 | 204 | 217 | 331, 256 tokens 230 | 349 | 356 | 586, 1023
+// tokens 799 | 1207 | 1166 | 2028; 777 tokens x 1024, 50257 words 109 | 101 |
+// 98 | 168, 32000 words 58 | 68 | 65 | 113; 300 x 2560 x 8192 52 | 37 | 35 | 40,
+// 126 x 2048 x 16384 43 | 31 | 28 | 26, 8000 x 1024 x 1000 27 | 20 | 22 | 30.
+struct TileKind {
+    uint32_t tokens, slots;
+    float round, half, brief, brief_half;
+};
+constexpr TileKind kTileKinds[] = {
+    {256, 256, 1.00f, 1.00f, 1.00f, 1.00f},
+    {128, 256, 0.75f, 0.75f, 0.60f, 0.60f},
+    {64, 512, 0.76f, 0.66f, 0.60f, 0.57f},
+    {32, 512, 0.78f, 0.60f, 0.60f, 0.50f},
+};
+
 template <typename Fmt>
 int dispatch_tiles(const Tiles& a, hipStream_t st) {
-    const uint64_t big = uint64_t((a.vocab + kSpan - 1) / kSpan) * ((a.tokens + 255) / 256);
-    if (a.tokens <= 32) return launch_tiles<Fmt, 4, 1, 4, 2>(a, st);
-    if (a.tokens <= 64 || big < 128) return launch_tiles<Fmt, 4, 1, 4, 4>(a, st);
-    if (a.tokens <= 128) return launch_tiles<Fmt, 4, 2, 4, 4>(a, st);
-    return launch_tiles<Fmt, 2, 4, 8, 4>(a, st);
+    const uint64_t spans = (a.vocab + kSpan - 1) / kSpan;
+    const bool brief = a.steps * kTerms < 2048;
+    uint32_t best = 0;
+    float least = 0.0f;
+    for (const TileKind& k : kTileKinds) {
+        const uint64_t tiles = spans * ((a.tokens + k.tokens - 1) / k.tokens);
+        const float one = tiles <= 256 ? (brief ? k.brief_half : k.half) : brief ? k.brief : k.round;
+        const float time = one * float((tiles + k.slots - 1) / k.slots);
+        if (best == 0 || time < least) best = k.tokens, least = time;
+    }
+    switch (best) {
+        case 32: return launch_tiles<Fmt, 4, 1, 4, 2>(a, st);
+        case 64: return launch_tiles<Fmt, 4, 1, 4, 4>(a, st);
+        case 128: return launch_tiles<Fmt, 4, 2, 4, 4>(a, st);
+        default: return launch_tiles<Fmt, 2, 4, 8, 4>(a, st);
+    }
 }
 
 template <int kT>

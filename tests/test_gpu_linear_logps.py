@@ -226,3 +226,12 @@ def test_saved_on_the_host(dev):
         lp = linear_logps(hr, wr, labels)
     got = torch.autograd.grad(lp, (hr, wr), up)
     assert all(torch.allclose(a.float(), b.float(), rtol=0.03, atol=1e-4) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1000, 128, 16_300), (300, 128, 33_000), (250, 64, 16_384), (31, 128, 16_500),
+                                   (520, 2048, 33_000), (130, 2048, 16_400), (64, 2048, 70_000), (9, 2048, 3000)])
+def test_every_tile(dev, shape, dtype):
+    """Tiles of 256, 128, 64 and 32 tokens, of brief and of long sums, with and
+    without what they keep."""
+    test_matches_float64(dev, shape, dtype)
