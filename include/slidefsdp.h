@@ -349,11 +349,16 @@ int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
 /* D in place of what sf_logps_tiles kept, with its parts, lse2 and logp; rows
  * without a label that counts become 0 (NaN for a label outside [0, vocab)),
  * and so do the rows from `rows` up to `padded`.  ld is a multiple of
- * SF_LOGPS_SPAN (SF_EALIGN). */
+ * SF_LOGPS_SPAN (SF_EALIGN).  grad (or null): in the same launch the row
+ * weights of all_rows rows, of which these are the first, as sf_logps_weight
+ * makes them; with `normalise` as with its norm, without it norm (or null) is
+ * set to 1, 1. */
 int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
                        size_t vocab, const void* parts, const int64_t* labels,
                        int64_t ignore_index, const float* lse2,
-                       const float* logp, int dtype, sf_stream_t stream);
+                       const float* logp, int dtype, const float* grad,
+                       size_t all_rows, float scale, float* row_weight,
+                       float* norm, int normalise, sf_stream_t stream);
 
 /* D of fp32 logits (as sf_logps_rows takes them, with its lse and logp), as
  * dtype with ld_dz elements from row to row.  SF_DTYPE_F32: dz may be the

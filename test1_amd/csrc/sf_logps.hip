@@ -394,44 +394,56 @@ __global__ __launch_bounds__(kT * kRowsOf<kT>) void logps_rows_kernel(const floa
 // operands, a power of two that brings the largest of them into [1, 2) (a mean
 // over many tokens leaves them near fp16's least numbers).  One workgroup.
 // ---------------------------------------------------------------------
-constexpr int kWeightThreads = 1024;
-__global__ __launch_bounds__(kWeightThreads) void logps_weight_kernel(const float* __restrict__ grad,
-                                                                      const float* __restrict__ logp,
-                                                                      const int64_t* __restrict__ labels,
-                                                                      int64_t ignore_index, uint64_t n, uint32_t vocab,
-                                                                      float scale, float* __restrict__ weight,
-                                                                      float* __restrict__ norm) {
-    __shared__ float waves[kWeightThreads / 64];
+struct Weights {
+    const float *grad, *logp;
+    const int64_t* labels;
+    int64_t ignore_index;
+    uint64_t n;
+    uint32_t vocab;
+    float scale;
+    float* weight;
+    float* norm;   // or null
+    bool normalise;
+};
+
+// The share of workgroup `block` of `blocks`; one alone where they are normalised.
+template <int kT>
+__device__ __forceinline__ void row_weights(const Weights& a, uint64_t block, uint64_t blocks) {
     const auto of = [&](uint64_t i) {
-        const RowKind kind = row_kind(labels[i], ignore_index, vocab);
-        return kind == kValid ? grad[i] * scale * rest_of(logp[i]) : kind == kIgnored ? 0.0f : __builtin_nanf("");
+        const RowKind kind = row_kind(a.labels[i], a.ignore_index, a.vocab);
+        return kind == kValid ? a.grad[i] * a.scale * rest_of(a.logp[i]) : kind == kIgnored ? 0.0f : __builtin_nanf("");
     };
-    if (norm == nullptr) {
-        for (uint64_t i = uint64_t(blockIdx.x) * kWeightThreads + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kWeightThreads)
-            weight[i] = of(i);
-        return;
-    }
-    float m = 0.0f;
-    for (uint64_t i = threadIdx.x; i < n; i += kWeightThreads) {
-        const float w = fabsf(of(i));
-        if (__builtin_isfinite(w)) m = fmaxf(m, w);
-    }
+    float by = 1.0f, back = 1.0f;
+    if (a.normalise) {
+        __shared__ float waves[kT / 64];
+        float m = 0.0f;
+        for (uint64_t i = threadIdx.x; i < a.n; i += kT) {
+            const float w = fabsf(of(i));
+            if (__builtin_isfinite(w)) m = fmaxf(m, w);
+        }
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = waves[0];
-    for (int w = 1; w < kWeightThreads / 64; ++w) m = fmaxf(m, waves[w]);
-    // within what both the factor and its inverse can be
-    const int e = m > 0.0f ? min(max(ilogbf(m), -100), 100) : 0;
-    const float by = ldexpf(1.0f, -e);
-    for (uint64_t i = threadIdx.x; i < n; i += kWeightThreads) weight[i] = of(i) * by;
-    if (threadIdx.x == 0) norm[0] = ldexpf(1.0f, e), norm[1] = 1.0f;
+        for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = waves[0];
+        for (int w = 1; w < kT / 64; ++w) m = fmaxf(m, waves[w]);
+        // within what both the factor and its inverse can be
+        const int e = m > 0.0f ? min(max(ilogbf(m), -100), 100) : 0;
+        by = ldexpf(1.0f, -e), back = ldexpf(1.0f, e);
+    }
+    for (uint64_t i = block * kT + threadIdx.x; i < a.n; i += blocks * kT) a.weight[i] = of(i) * by;
+    if (a.norm != nullptr && block == 0 && threadIdx.x == 0) a.norm[0] = back, a.norm[1] = 1.0f;
+}
+
+constexpr int kWeightThreads = 1024;
+__global__ __launch_bounds__(kWeightThreads) void logps_weight_kernel(const Weights a) {
+    row_weights<kWeightThreads>(a, blockIdx.x, gridDim.x);
 }
 
 // D from what the product kept, in place.  A workgroup takes 4,096 words of a
 // token, 16 bytes at a time; rows from `tokens` on are cleared (they pad the
-// weight gradient's sum).
+// weight gradient's sum).  The launch's first `others` workgroups make the rows'
+// weights, which nothing here needs.
 constexpr int kGradThreads = 256;
 constexpr int kKeepColumns = kGradThreads * kGroup * 2;
 template <typename Fmt>
@@ -442,8 +454,10 @@ __global__ __launch_bounds__(kGradThreads) void logps_keep_grad_kernel(uint16_t*
                                                                        const int64_t* __restrict__ labels,
                                                                        int64_t ignore_index,
                                                                        const float* __restrict__ lse2,
-                                                                       const float* __restrict__ logp) {
-    const uint64_t b = first + blockIdx.x, row = b / col_blocks;
+                                                                       const float* __restrict__ logp,
+                                                                       const Weights weights, uint32_t others) {
+    if (blockIdx.x < others) return row_weights<kGradThreads>(weights, blockIdx.x, others);
+    const uint64_t b = first + blockIdx.x - others, row = b / col_blocks;
     const uint32_t col = uint32_t(b % col_blocks) * kKeepColumns + threadIdx.x * kGroup;
     uint16_t* k = keep + row * ld;
     const int64_t y = row < tokens ? labels[row] : ignore_index;
@@ -636,8 +650,12 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab, const void* hid
 
 int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded, size_t vocab, const void* parts,
                        const int64_t* labels, int64_t ignore_index, const float* lse2, const float* logp, int dtype,
+                       const float* grad, size_t all_rows, float scale, float* row_weight, float* norm, int normalise,
                        sf_stream_t stream) {
     if (padded == 0) return SF_OK;
+    if (grad != nullptr && (row_weight == nullptr || all_rows < rows || sizes_bad(all_rows, vocab) ||
+                            (normalise && norm == nullptr)))
+        return SF_EINVAL;
     if (keep == nullptr || parts == nullptr || labels == nullptr || lse2 == nullptr || logp == nullptr ||
         sizes_bad(padded, vocab) || padded < rows || ld < (vocab + kSpan - 1) / kSpan * kSpan || ld > (size_t(1) << 31))
         return SF_EINVAL;
@@ -645,10 +663,15 @@ int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded, size_t
     if (misaligned(keep, 16) || misaligned(parts, 8) || ld % kSpan != 0) return SF_EALIGN;
     const uint32_t col_blocks = uint32_t((ld + kKeepColumns - 1) / kKeepColumns);
     const auto kernel = dtype == SF_DTYPE_BF16 ? logps_keep_grad_kernel<Bf16> : logps_keep_grad_kernel<F16>;
+    const Weights weights = {grad, logp, labels, ignore_index, all_rows, uint32_t(vocab), scale, row_weight, norm,
+                             normalise != 0};
+    const uint64_t want = (all_rows + 4 * kGradThreads - 1) / (4 * kGradThreads);
+    const uint32_t share = grad == nullptr ? 0 : normalise ? 1 : uint32_t(want < 1024 ? want : 1024);
     return in_launches(uint64_t(padded) * col_blocks, [&](uint64_t first, uint32_t blocks) {
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kGradThreads), 0, reinterpret_cast<hipStream_t>(stream),
+        const uint32_t others = first == 0 ? share : 0;
+        hipLaunchKernelGGL(kernel, dim3(blocks + others), dim3(kGradThreads), 0, reinterpret_cast<hipStream_t>(stream),
                            static_cast<uint16_t*>(keep), uint64_t(ld), uint32_t(rows), uint32_t(vocab), col_blocks, first,
-                           static_cast<const float2*>(parts), labels, ignore_index, lse2, logp);
+                           static_cast<const float2*>(parts), labels, ignore_index, lse2, logp, weights, others);
     });
 }
 
@@ -673,8 +696,8 @@ int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
         return SF_EINVAL;
     const uint64_t want = (rows + kWeightThreads - 1) / kWeightThreads;
     const uint32_t blocks = norm != nullptr ? 1 : uint32_t(want < 1024 ? want : 1024);
-    hipLaunchKernelGGL(logps_weight_kernel, dim3(blocks), dim3(kWeightThreads), 0, reinterpret_cast<hipStream_t>(stream),
-                       grad, logp, labels, ignore_index, uint64_t(rows), uint32_t(vocab), scale, weight, norm);
+    const Weights a = {grad, logp, labels, ignore_index, rows, uint32_t(vocab), scale, weight, norm, norm != nullptr};
+    hipLaunchKernelGGL(logps_weight_kernel, dim3(blocks), dim3(kWeightThreads), 0, reinterpret_cast<hipStream_t>(stream), a);
     return status();
 }
 

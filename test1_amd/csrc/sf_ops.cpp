@@ -296,6 +296,17 @@ void hidden_product(const Tensor& keep, int64_t n, const Tensor& weight, int64_t
           "sf_logps_sum");
 }
 
+// Whether the weight gradient of a call in one piece is formed by
+// sf_ce_weight_grad instead of a library's product.  bf16: where the product is
+// shorter than the host's time for it (whole calls with both gradients, us,
+// product | kernel, tokens x hidden x vocabulary: 126 x 512 x 4096 123 | 107, 128
+// x 2048 x 16384 122 | 118, 200 x 1024 x 32000 164 | 192, 64 x 4096 x 128256 798 |
+// 866).  fp16: up to the 256 tokens that it takes, since the product is into
+// fp32 and rescaled (200 x 1024 x 32000 301 | 192).
+bool own_weight_grad(int64_t n, int64_t h, int64_t v, bool fp16) {
+    return n <= 256 && (fp16 || n * h * v <= int64_t(1) << 32);
+}
+
 // Both gradients (undefined where not needed).  What was kept turns into the
 // gradient of the logits in place; without it, it is made again, `step` rows at
 // a time.
@@ -311,13 +322,11 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
     const int type = type_of(hidden);
     const int64_t* y = at_ptr<int64_t>(labels);
     const float *lp = at_ptr<float>(logp), *l2 = at_ptr<float>(lse2);
-    const Tensor by = like(hidden, {n}), norm = fp16 ? like(hidden, {2}) : Tensor();
-    check(sf_logps_weight(at_ptr<float>(grad), lp, y, a.ignore_index, n, v, float(a.scale), at_ptr<float>(by),
-                          at_ptr<float>(norm), st),
-          "sf_logps_weight");
+    const Tensor by = like(hidden, {n}), norm = like(hidden, {2});
+    const bool few = one && own_weight_grad(n, h, v, fp16);
     Tensor gh, gw, again;
     if (need_hidden) gh = at::empty({n, h}, hidden.options());
-    if (need_weight) gw = at::empty({v, h}, one && !fp16 ? weight.options() : weight.options().dtype(at::kFloat));
+    if (need_weight) gw = at::empty({v, h}, few || (one && !fp16) ? weight.options() : weight.options().dtype(at::kFloat));
     if (!kept) {
         keep = at::empty({up(step, 64), row}, hidden.options());
         again = like(hidden, {2, step});
@@ -330,15 +339,23 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
             parts = tiles(hc, weight, y + s, a, keep, results, results + step);
         }
         check(sf_logps_keep_grad(keep.data_ptr(), row, m, pad, v, parts.data_ptr(), y + s, a.ignore_index, l2 + s, lp + s,
-                                 type, st),
+                                 type, s == 0 ? at_ptr<float>(grad) : nullptr, n, float(a.scale), at_ptr<float>(by),
+                                 at_ptr<float>(norm), fp16, st),
               "sf_logps_keep_grad");
         if (need_hidden)
-            hidden_product(keep, m, weight, a.nparts, at_ptr<float>(by) + s, norm, one ? gh : gh.narrow(0, s, m));
+            hidden_product(keep, m, weight, a.nparts, at_ptr<float>(by) + s, fp16 ? norm : Tensor(),
+                           one ? gh : gh.narrow(0, s, m));
         if (!need_weight) continue;
         // transposed: a library's product with an operand laid out along the sum is faster
         const Tensor ht = at::empty({h, pad}, hidden.options());
         check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, ht.data_ptr(), pad, st),
               "sf_logps_hidden");
+        if (few) {
+            check(sf_ce_weight_grad(at_ptr<float>(norm), at_ptr<float>(norm) + 1, keep.data_ptr(), row, v, ht.data_ptr(), pad,
+                                    h, gw.data_ptr(), nullptr, nullptr, 0, type, st),
+                  "sf_ce_weight_grad");
+            break;
+        }
         const Tensor dt = keep.as_strided({v, pad}, {1, row}), hp = ht.t();
         if (one && !fp16) at::mm_out(gw, dt, hp);
         else if (s == 0) at::mm_out(gw, dt, hp, at::kFloat);

@@ -136,8 +136,11 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert tiles(w=None) == tiles(v=0) == tiles(ldw=32) == tiles(s=0.0) == tiles(kp=one, ldk=64) == tiles(ldh=1 << 23) == 9001
     assert tiles(k=32) == tiles(w=72) == tiles(ldh=68) == tiles(kp=72, ldk=256) == 9007
     assert tiles(t=0) == 9003 and tiles(n=0) == 0
-    assert hip.sf_logps_keep_grad(one, 256, 2, 1, 8, one, one, -100, one, one, 1, None) == 9001
-    assert hip.sf_logps_keep_grad(one, 264, 1, 1, 8, one, one, -100, one, one, 1, None) == 9007
+    none = (None, 0, 1.0, None, None, 0, None)
+    assert hip.sf_logps_keep_grad(one, 256, 2, 1, 8, one, one, -100, one, one, 1, *none) == 9001
+    assert hip.sf_logps_keep_grad(one, 264, 1, 1, 8, one, one, -100, one, one, 1, *none) == 9007
+    assert hip.sf_logps_keep_grad(one, 256, 2, 2, 8, one, one, -100, one, one, 1, one, 1, 1.0, one, None, 0, None) == 9001
+    assert hip.sf_logps_keep_grad(one, 256, 1, 1, 8, one, one, -100, one, one, 1, one, 1, 1.0, one, None, 1, None) == 9001
     assert hip.sf_logps_hidden(one, 8, 1, 8, None, 1, one, 64, None) == hip.sf_logps_hidden(one, 8, 1, 8, one, 1, one, 32, None) == 9001
     assert hip.sf_logps_sum(one, 3, 1, 8, one, 1, None, 0, None, 0, one, None, None) == 9001
     assert hip.sf_align_parts(0, 5) == 0 and hip.sf_align_parts(4, 100) == 4
