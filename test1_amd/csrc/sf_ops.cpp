@@ -346,7 +346,17 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
             hidden_product(keep, m, weight, a.nparts, at_ptr<float>(by) + s, fp16 ? norm : Tensor(),
                            one ? gh : gh.narrow(0, s, m));
         if (!need_weight) continue;
-        // transposed: a library's product with an operand laid out along the sum is faster
+        if (fp16 && !few) {
+            // into fp32, of rows as they lie: 4096 x 4096 x 128256 4.2 ms, of transposed ones 28.8
+            Tensor weighted = at::empty({m, h}, hidden.options());
+            at::mul_out(weighted, hc, by.narrow(0, s, m).unsqueeze(1));
+            const Tensor dt = keep.as_strided({v, m}, {1, row});
+            if (s == 0) at::mm_out(gw, dt, weighted, at::kFloat);
+            else at::addmm_out(gw, gw, dt, weighted, at::kFloat);
+            continue;
+        }
+        // transposed: of bf16 the product with an operand laid out along the sum is
+        // faster, 3.3 ms there instead of 4.0
         const Tensor ht = at::empty({h, pad}, hidden.options());
         check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, ht.data_ptr(), pad, st),
               "sf_logps_hidden");
@@ -357,7 +367,7 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
             break;
         }
         const Tensor dt = keep.as_strided({v, pad}, {1, row}), hp = ht.t();
-        if (one && !fp16) at::mm_out(gw, dt, hp);
+        if (one) at::mm_out(gw, dt, hp);
         else if (s == 0) at::mm_out(gw, dt, hp, at::kFloat);
         else at::addmm_out(gw, gw, dt, hp, at::kFloat);
     }
