@@ -338,7 +338,8 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab,
 
 /* The gradient of such logits is row_weight[i] * D[i, j], D = ((j == label) -
  * p) / (1 - p_label): 1 at the label.  row_weight = grad * scale * (1 -
- * p_label); 0 for an ignored row, NaN for a label outside [0, vocab).  norm (or
+ * p_label); 0 for an ignored row or a grad of 0, NaN for a label outside [0,
+ * vocab).  norm (or
  * null: 1): two floats; the weights are then divided by the power of two
  * norm[0] that leaves the largest in [1, 2), and norm[1] = 1. */
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
@@ -347,12 +348,12 @@ int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
                     sf_stream_t stream);
 
 /* D in place of what sf_logps_tiles kept, with its parts, lse2 and logp; rows
- * without a label that counts become 0 (NaN for a label outside [0, vocab)),
- * and so do the rows from `rows` up to `padded`.  ld is a multiple of
- * SF_LOGPS_SPAN (SF_EALIGN).  grad (or null): in the same launch the row
- * weights of all_rows rows, of which these are the first, as sf_logps_weight
- * makes them; with `normalise` as with its norm, without it norm (or null) is
- * set to 1, 1. */
+ * without a label that counts or whose grad is 0 become 0, whatever they held
+ * (NaN for a label outside [0, vocab)), and so do the rows from `rows` up to
+ * `padded`.  ld is a multiple of SF_LOGPS_SPAN (SF_EALIGN).  all_rows (or 0): in
+ * the same launch the row weights of that many rows, of which these are the
+ * first, as sf_logps_weight makes them; with `normalise` as with its norm,
+ * without it norm (or null) is set to 1, 1. */
 int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
                        size_t vocab, const void* parts, const int64_t* labels,
                        int64_t ignore_index, const float* lse2,
@@ -360,22 +361,22 @@ int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
                        size_t all_rows, float scale, float* row_weight,
                        float* norm, int normalise, sf_stream_t stream);
 
-/* D of fp32 logits (as sf_logps_rows takes them, with its lse and logp), as
- * dtype with ld_dz elements from row to row.  SF_DTYPE_F32: dz may be the
+/* D of fp32 logits (as sf_logps_rows takes them, with its lse and logp; 0 in
+ * rows whose grad is 0), as dtype with ld_dz elements from row to row.  SF_DTYPE_F32: dz may be the
  * logits themselves; other types: no overlap. */
 int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab,
                   const int64_t* labels, int64_t ignore_index, float scale,
-                  const float* lse, const float* logp, void* dz, int dtype,
-                  size_t ld_dz, sf_stream_t stream);
+                  const float* lse, const float* logp, const float* grad,
+                  void* dz, int dtype, size_t ld_dz, sf_stream_t stream);
 
-/* hidden_t[j, i] = row_weight[i] * hidden[i, j], rounded once; otherwise as
- * sf_ce_hidden, without a tail. */
+/* hidden_t[j, i] = row_weight[i] * hidden[i, j], rounded once, 0 where the
+ * weight is; otherwise as sf_ce_hidden, without a tail. */
 int sf_logps_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols,
                     const float* row_weight, int dtype, void* hidden_t,
                     size_t ldt, sf_stream_t stream);
 
-/* As sf_ce_sum, also of one part, each row times row_weight[i], and times
- * norm[0] where norm is not null. */
+/* As sf_ce_sum, also of one part, each row times row_weight[i], 0 where that
+ * is, and times norm[0] where norm is not null. */
 int sf_logps_sum(const float* parts, int nparts, size_t rows, size_t cols,
                  void* out, int dtype, const void* d_tail, size_t ld,
                  const void* w_tail, size_t tail, const float* row_weight,

@@ -372,7 +372,8 @@ __global__ __launch_bounds__(kScaleThreads) void ce_scale32_kernel(
 constexpr int kTr = 64;
 constexpr int kTrThreads = 256;
 constexpr int kTrLd = kTr + 2;
-// With Fmt each row is multiplied by its element of `by`, rounded once.
+// With Fmt each row is multiplied by its element of `by`, rounded once; one of
+// weight 0 becomes 0, whatever it holds.
 template <bool kVec, typename Fmt = void>   // kVec: rows on 16-byte boundaries, hidden a multiple of 8
 __global__ __launch_bounds__(kTrThreads) void ce_hidden_kernel(const uint16_t* __restrict__ hidden, uint64_t ldh,
                                                                uint64_t rows, uint64_t cols, uint16_t* __restrict__ out,
@@ -403,7 +404,7 @@ __global__ __launch_bounds__(kTrThreads) void ce_hidden_kernel(const uint16_t* _
             if constexpr (!std::is_void<Fmt>::value) {
                 const float f = by[row0 + r];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = Fmt::pack(Fmt::lo(v[j]) * f, Fmt::hi(v[j]) * f);
+                for (int j = 0; j < 4; ++j) v[j] = f == 0.0f ? 0u : Fmt::pack(Fmt::lo(v[j]) * f, Fmt::hi(v[j]) * f);
             }
         }
         uint32_t* t = reinterpret_cast<uint32_t*>(tile + r * kTrLd + c);
@@ -433,7 +434,8 @@ __global__ __launch_bounds__(kTrThreads) void ce_hidden_kernel(const uint16_t* _
 // 1024 x 32000 371 | 285.  Bound by the parts' reads, at most 134 MB, which the
 // last-level cache still holds in part.
 constexpr int kSumThreads = 128;
-// kWeighted: each row times its element of `by`, and times *norm if there is one.
+// kWeighted: each row times its element of `by`, 0 where that is 0, and times
+// *norm if there is one.
 template <typename Fmt, int kParts, bool kWeighted = false>
 __global__ __launch_bounds__(kSumThreads) void ce_sum_kernel(const float* __restrict__ parts, uint32_t count,
                                                              uint32_t cols, uint16_t* __restrict__ out,
@@ -478,8 +480,8 @@ __global__ __launch_bounds__(kSumThreads) void ce_sum_kernel(const float* __rest
     }
     if constexpr (kWeighted) {
         const float f = by[i / cols], n = norm != nullptr ? *norm : 1.0f;
-        a[0] = a[0] * f * n;
-        b[0] = b[0] * f * n;
+        a[0] = f == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : a[0] * f * n;
+        b[0] = f == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : b[0] * f * n;
     }
     *reinterpret_cast<u32x4*>(out + i) = pack8<Fmt>(a[0], b[0]);
 }

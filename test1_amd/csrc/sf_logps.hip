@@ -410,8 +410,10 @@ struct Weights {
 template <int kT>
 __device__ __forceinline__ void row_weights(const Weights& a, uint64_t block, uint64_t blocks) {
     const auto of = [&](uint64_t i) {
+        const float g = a.grad[i];
         const RowKind kind = row_kind(a.labels[i], a.ignore_index, a.vocab);
-        return kind == kValid ? a.grad[i] * a.scale * rest_of(a.logp[i]) : kind == kIgnored ? 0.0f : __builtin_nanf("");
+        if (kind == kIgnored || g == 0.0f) return 0.0f;
+        return kind == kValid ? g * a.scale * rest_of(a.logp[i]) : __builtin_nanf("");
     };
     float by = 1.0f, back = 1.0f;
     if (a.normalise) {
@@ -441,7 +443,8 @@ __global__ __launch_bounds__(kWeightThreads) void logps_weight_kernel(const Weig
 }
 
 // D from what the product kept, in place.  A workgroup takes 4,096 words of a
-// token, 16 bytes at a time; rows from `tokens` on are cleared (they pad the
+// token, 16 bytes at a time.  A token without a gradient of its own, masked ones
+// above all, has D = 0 whatever its hidden states hold, and is not read; rows from `tokens` on are cleared (they pad the
 // weight gradient's sum).  The launch's first `others` workgroups make the rows'
 // weights, which nothing here needs.
 constexpr int kGradThreads = 256;
@@ -455,13 +458,14 @@ __global__ __launch_bounds__(kGradThreads) void logps_keep_grad_kernel(uint16_t*
                                                                        int64_t ignore_index,
                                                                        const float* __restrict__ lse2,
                                                                        const float* __restrict__ logp,
+                                                                       const float* __restrict__ grad,
                                                                        const Weights weights, uint32_t others) {
     if (blockIdx.x < others) return row_weights<kGradThreads>(weights, blockIdx.x, others);
     const uint64_t b = first + blockIdx.x - others, row = b / col_blocks;
     const uint32_t col = uint32_t(b % col_blocks) * kKeepColumns + threadIdx.x * kGroup;
     uint16_t* k = keep + row * ld;
     const int64_t y = row < tokens ? labels[row] : ignore_index;
-    const RowKind kind = row_kind(y, ignore_index, vocab);
+    const RowKind kind = row < tokens && grad[row] == 0.0f ? kIgnored : row_kind(y, ignore_index, vocab);
     if (row >= tokens || kind != kValid) {
         const uint32_t w = row < tokens && kind == kBadLabel ? Fmt::kNan2 : 0u;
 #pragma unroll
@@ -504,11 +508,12 @@ __global__ __launch_bounds__(kGradThreads) void logps_grad_kernel(const float* l
                                                                   int64_t ignore_index, float scale,
                                                                   const float* __restrict__ lse,
                                                                   const float* __restrict__ logp,
+                                                                  const float* __restrict__ grad,
                                                                   typename Out::S* dz, uint64_t ld_dz) {
     const uint64_t b = first + blockIdx.x, row = b / col_blocks;
     const uint32_t col = uint32_t(b % col_blocks) * kGradColumns + threadIdx.x;
     const int64_t y = labels[row];
-    const RowKind kind = row_kind(y, ignore_index, vocab);
+    const RowKind kind = grad[row] == 0.0f ? kIgnored : row_kind(y, ignore_index, vocab);
     const float* x = logits + row * ld;
     typename Out::S* o = dz + row * ld_dz;
     const float l = lse[row], by = -1.0f / rest_of(logp[row]);
@@ -604,11 +609,12 @@ int in_launches(uint64_t blocks, Launch launch) {
 
 template <typename Out>
 int launch_grad(const float* x, uint64_t ld, uint64_t rows, uint32_t vocab, const int64_t* labels, int64_t ignore,
-                float scale, const float* lse, const float* logp, void* dz, uint64_t ld_dz, hipStream_t st) {
+                float scale, const float* lse, const float* logp, const float* grad, void* dz, uint64_t ld_dz,
+                hipStream_t st) {
     const uint32_t col_blocks = (vocab + kGradColumns - 1) / kGradColumns;
     return in_launches(rows * col_blocks, [&](uint64_t first, uint32_t blocks) {
         hipLaunchKernelGGL(logps_grad_kernel<Out>, dim3(blocks), dim3(kGradThreads), 0, st, x, ld, vocab, col_blocks,
-                           first, labels, ignore, scale, lse, logp, static_cast<typename Out::S*>(dz), ld_dz);
+                           first, labels, ignore, scale, lse, logp, grad, static_cast<typename Out::S*>(dz), ld_dz);
     });
 }
 
@@ -653,7 +659,8 @@ int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded, size_t
                        const float* grad, size_t all_rows, float scale, float* row_weight, float* norm, int normalise,
                        sf_stream_t stream) {
     if (padded == 0) return SF_OK;
-    if (grad != nullptr && (row_weight == nullptr || all_rows < rows || sizes_bad(all_rows, vocab) ||
+    if (rows > 0 && grad == nullptr) return SF_EINVAL;
+    if (all_rows > 0 && (row_weight == nullptr || all_rows < rows || sizes_bad(all_rows, vocab) ||
                             (normalise && norm == nullptr)))
         return SF_EINVAL;
     if (keep == nullptr || parts == nullptr || labels == nullptr || lse2 == nullptr || logp == nullptr ||
@@ -666,12 +673,12 @@ int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded, size_t
     const Weights weights = {grad, logp, labels, ignore_index, all_rows, uint32_t(vocab), scale, row_weight, norm,
                              normalise != 0};
     const uint64_t want = (all_rows + 4 * kGradThreads - 1) / (4 * kGradThreads);
-    const uint32_t share = grad == nullptr ? 0 : normalise ? 1 : uint32_t(want < 1024 ? want : 1024);
+    const uint32_t share = all_rows == 0 ? 0 : normalise ? 1 : uint32_t(want < 1024 ? want : 1024);
     return in_launches(uint64_t(padded) * col_blocks, [&](uint64_t first, uint32_t blocks) {
         const uint32_t others = first == 0 ? share : 0;
         hipLaunchKernelGGL(kernel, dim3(blocks + others), dim3(kGradThreads), 0, reinterpret_cast<hipStream_t>(stream),
                            static_cast<uint16_t*>(keep), uint64_t(ld), uint32_t(rows), uint32_t(vocab), col_blocks, first,
-                           static_cast<const float2*>(parts), labels, ignore_index, lse2, logp, weights, others);
+                           static_cast<const float2*>(parts), labels, ignore_index, lse2, logp, grad, weights, others);
     });
 }
 
@@ -702,10 +709,11 @@ int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
 }
 
 int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab, const int64_t* labels,
-                  int64_t ignore_index, float scale, const float* lse, const float* logp, void* dz, int dtype,
-                  size_t ld_dz, sf_stream_t stream) {
+                  int64_t ignore_index, float scale, const float* lse, const float* logp, const float* grad, void* dz,
+                  int dtype, size_t ld_dz, sf_stream_t stream) {
     if (rows == 0) return SF_OK;
-    if (logits == nullptr || labels == nullptr || lse == nullptr || logp == nullptr || dz == nullptr) return SF_EINVAL;
+    if (logits == nullptr || labels == nullptr || lse == nullptr || logp == nullptr || grad == nullptr || dz == nullptr)
+        return SF_EINVAL;
     if (sizes_bad(rows, vocab) || ld < vocab || ld_dz < vocab) return SF_EINVAL;
     if (dtype != SF_DTYPE_F32 && dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
     const size_t item = dtype == SF_DTYPE_F32 ? 4 : 2;
@@ -717,10 +725,10 @@ int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab, con
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const uint32_t v = uint32_t(vocab);
     if (dtype == SF_DTYPE_BF16)
-        return launch_grad<Out16<Bf16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, dz, ld_dz, st);
+        return launch_grad<Out16<Bf16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, grad, dz, ld_dz, st);
     if (dtype == SF_DTYPE_F16)
-        return launch_grad<Out16<F16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, dz, ld_dz, st);
-    return launch_grad<Out32>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, dz, ld_dz, st);
+        return launch_grad<Out16<F16>>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, grad, dz, ld_dz, st);
+    return launch_grad<Out32>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, grad, dz, ld_dz, st);
 }
 
 }  // extern "C"

@@ -23,7 +23,10 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <math.h>
 #include <stdint.h>
+
+#include <cmath>
 
 #include "../../include/slidefsdp.h"
 
@@ -339,7 +342,7 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
             parts = tiles(hc, weight, y + s, a, keep, results, results + step);
         }
         check(sf_logps_keep_grad(keep.data_ptr(), row, m, pad, v, parts.data_ptr(), y + s, a.ignore_index, l2 + s, lp + s,
-                                 type, s == 0 ? at_ptr<float>(grad) : nullptr, n, float(a.scale), at_ptr<float>(by),
+                                 type, at_ptr<float>(grad) + s, s == 0 ? n : 0, float(a.scale), at_ptr<float>(by),
                                  at_ptr<float>(norm), fp16, st),
               "sf_logps_keep_grad");
         if (need_hidden)
@@ -349,7 +352,8 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
         if (fp16 && !few) {
             // into fp32, of rows as they lie: 4096 x 4096 x 128256 4.2 ms, of transposed ones 28.8
             Tensor weighted = at::empty({m, h}, hidden.options());
-            at::mul_out(weighted, hc, by.narrow(0, s, m).unsqueeze(1));
+            const Tensor f = by.narrow(0, s, m).unsqueeze(1);
+            at::mul_out(weighted, hc.masked_fill(f == 0, 0), f);
             const Tensor dt = keep.as_strided({v, m}, {1, row});
             if (s == 0) at::mm_out(gw, dt, weighted, at::kFloat);
             else at::addmm_out(gw, gw, dt, weighted, at::kFloat);
@@ -361,8 +365,8 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
         check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, ht.data_ptr(), pad, st),
               "sf_logps_hidden");
         if (few) {
-            check(sf_ce_weight_grad(at_ptr<float>(norm), at_ptr<float>(norm) + 1, keep.data_ptr(), row, v, ht.data_ptr(), pad,
-                                    h, gw.data_ptr(), nullptr, nullptr, 0, type, st),
+            check(sf_ce_weight_grad(at_ptr<float>(norm), at_ptr<float>(norm) + 1, keep.data_ptr(), row, v, ht.data_ptr(),
+                                    pad, h, gw.data_ptr(), nullptr, nullptr, 0, type, st),
                   "sf_ce_weight_grad");
             break;
         }
@@ -433,13 +437,15 @@ struct LinearLogps : torch::autograd::Function<LinearLogps> {
                 std::tie(gh, gw) = logps_backward(g.to(at::kFloat).contiguous(), hidden, weight, labels, logp, lse2, keep,
                                                   parts, a, need_hidden, need_weight);
             } else {
-                const Tensor h = hidden.to(at::kFloat), w = weight.to(at::kFloat);
+                const Tensor w = weight.to(at::kFloat), lse = lse2.to(at::kFloat) * std::log(2.0);
                 const Tensor valid = labels != a.ignore_index, inside = labels.ge(0).logical_and(labels < w.size(0));
-                const Tensor at_label = at::where(valid.logical_and(inside), labels, at::zeros_like(labels));
-                const Tensor p = at::exp(at::matmul(h, w.t()) * a.scale - (lse2.to(at::kFloat) * 0.69314718055994530942).unsqueeze(1));
-                Tensor dz = (at::one_hot(at_label, w.size(0)) - p) * (g.to(at::kFloat) * a.scale).unsqueeze(-1);
-                dz = at::where(valid.unsqueeze(1), dz, at::zeros_like(dz));
-                dz = at::where(valid.logical_and(inside.logical_not()).unsqueeze(1), at::full_like(dz, NAN), dz);
+                const Tensor index = at::where(valid.logical_and(inside), labels, at::zeros_like(labels));
+                const Tensor counts = valid.logical_and(g != 0).unsqueeze(-1);
+                const Tensor h = at::where(counts, hidden.to(at::kFloat), at::zeros({}, w.options()));
+                const Tensor p = at::exp(at::matmul(h, w.t()) * a.scale - lse.unsqueeze(1));
+                Tensor dz = (at::one_hot(index, w.size(0)) - p) * (g.to(at::kFloat) * a.scale).unsqueeze(-1);
+                dz = at::where(counts, dz, at::zeros_like(dz));
+                dz = at::where(counts.logical_and(inside.logical_not().unsqueeze(-1)), at::full_like(dz, NAN), dz);
                 if (need_hidden) gh = at::matmul(dz, w).to(hidden.scalar_type());
                 if (need_weight) gw = at::matmul(dz.transpose(-1, -2), h).to(weight.scalar_type());
             }
@@ -473,8 +479,8 @@ PyObject* pref_loss(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
-// policy_loss(logps, old, advantages, mask, ref or None, log_low, log_high, kl_coef, sequences): (loss, kl or None, clipped),
-// or None
+// policy_loss(logps, old, advantages, mask, ref or None, log_low, log_high, kl_coef, sequences):
+// (loss, kl or None, clipped), or None
 PyObject* policy_loss(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
     PyObject *l, *o_, *ad, *m, *r;
@@ -489,7 +495,8 @@ PyObject* policy_loss(PyObject*, PyObject* args) {
     const PolicyArgs a = {low, high, kl, sequences != 0};
     Tensor loss, kl_mean, clipped;
     if (at::GradMode::is_enabled() && logps.requires_grad()) {
-        const variable_list o = PolicyNode::apply(logps, old, adv, mask, ref.defined() ? c10::optional<Tensor>(ref) : c10::nullopt, a);
+        const c10::optional<Tensor> given = ref.defined() ? c10::optional<Tensor>(ref) : c10::nullopt;
+        const variable_list o = PolicyNode::apply(logps, old, adv, mask, given, a);
         loss = o[0], clipped = o[1];
         if (o.size() > 2) kl_mean = o[2];
     } else {

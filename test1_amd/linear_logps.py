@@ -134,7 +134,7 @@ def _backward_kernels(grad, hidden, weight, labels, logp, lse, ignore_index, sca
     gw = None
     if need_weight:
         gw = torch.empty((v, h), dtype=dtype if one and norm is None else torch.float32, device=dev)
-        weighted = (hidden * row_weight).to(dtype)
+        weighted = (hidden.masked_fill(row_weight == 0, 0) * row_weight).to(dtype)
     wt = weight.t()
     for s in range(0, n, step):
         e = min(n, s + step)
@@ -142,14 +142,14 @@ def _backward_kernels(grad, hidden, weight, labels, logp, lse, ignore_index, sca
         d = d_buf[:e - s, :v]
         _native.check(_native.hip().sf_logps_grad(
             buf.data_ptr(), buf.stride(0), e - s, v, labels.data_ptr() + 8 * s, ignore_index, scale,
-            lse.data_ptr() + 4 * s, logp.data_ptr() + 4 * s, d_buf.data_ptr(), _CE_DTYPES[dtype], d_buf.stride(0),
-            _stream()), "sf_logps_grad")
+            lse.data_ptr() + 4 * s, logp.data_ptr() + 4 * s, grad.data_ptr() + 4 * s, d_buf.data_ptr(),
+            _CE_DTYPES[dtype], d_buf.stride(0), _stream()), "sf_logps_grad")
         if need_hidden:
             torch.mm(d, weight, **_f32_out(dtype), out=gh[s:e])
         if need_weight:
             _add_product(gw, d.t(), weighted[s:e], s == 0)
     if need_hidden:
-        gh.mul_(row_weight)
+        gh.masked_fill_(row_weight == 0, 0).mul_(row_weight)
         gh = (gh if norm is None else gh.mul_(norm[0])).to(dtype)
     return gh, _rescaled(gw, dtype, norm)
 
@@ -178,13 +178,15 @@ class _LinearLogps(torch.autograd.Function):
                                            ctx.ignore_index, ctx.scale, *need), None, None, None)
         with torch.autocast(hidden.device.type, enabled=False):
             valid, at, bad = _label_kinds(labels, weight.shape[0], ctx.ignore_index)
-            p = torch.exp(hidden.float() @ weight.float().t() * ctx.scale - lse.float().unsqueeze(1))
+            counts = (valid & (grad != 0)).unsqueeze(-1)
+            hidden32 = torch.where(counts, hidden.float(), torch.zeros((), device=hidden.device))
+            p = torch.exp(hidden32 @ weight.float().t() * ctx.scale - lse.float().unsqueeze(1))
             onehot = torch.nn.functional.one_hot(at, weight.shape[0]).to(p.dtype)
             dz = (onehot - p) * (grad.to(torch.float32) * ctx.scale).unsqueeze(-1)
-            dz = torch.where(valid.unsqueeze(1), dz, torch.zeros_like(dz))
-            dz = torch.where(bad.unsqueeze(1), torch.full_like(dz, math.nan), dz)
+            dz = torch.where(counts, dz, torch.zeros_like(dz))
+            dz = torch.where(counts & bad.unsqueeze(-1), torch.full_like(dz, math.nan), dz)
             gh = (dz @ weight.float()).to(hidden.dtype) if need[0] else None
-            gw = (dz.transpose(-1, -2) @ hidden.float()).to(weight.dtype) if need[1] else None
+            gw = (dz.transpose(-1, -2) @ hidden32).to(weight.dtype) if need[1] else None
         return gh, gw, None, None, None
 
 
@@ -197,6 +199,8 @@ def _label_kinds(labels, vocab, ignore_index):
 def _torch_logps(hidden, weight, labels, ignore_index, scale):
     with torch.autocast(hidden.device.type, enabled=False):
         valid, at, bad = _label_kinds(labels, weight.shape[0], ignore_index)
+        # what ignored tokens hold does not reach the weight's gradient
+        hidden = torch.where(valid.unsqueeze(-1), hidden, torch.zeros_like(hidden))
         logp = torch.log_softmax(hidden.float() @ weight.float().t() * scale, dim=-1)
         logp = logp.gather(-1, at.unsqueeze(-1)).squeeze(-1)
         logp = logp * torch.where(bad, math.nan, 1.0)
@@ -214,7 +218,8 @@ def _kernels_take(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tens
 def linear_logps(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
                  temperature: float = 1.0) -> torch.Tensor:
     """``log_softmax(hidden @ weight.T / temperature)`` at ``labels``, float32,
-    of the labels' shape.
+    of the labels' shape.  On a GPU, tokens that are ignored or whose upstream
+    gradient is 0 leave the gradients alone, whatever their hidden states hold.
 
     ``hidden`` [..., H] and ``weight`` [V, H] of one float type (bfloat16,
     float16 or float32), ``labels`` [...] int64.  0, without gradient, where

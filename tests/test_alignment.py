@@ -128,15 +128,15 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert hip.sf_logps_rows(one, 6, 1, 8, one, -100, 1.0, one, one, None) == 9001
     assert hip.sf_logps_rows(one, 9, 1, 8, one, -100, 1.0, one, one, None) == 9007
     assert hip.sf_logps_rows(one, 8, 0, 8, one, -100, 1.0, one, one, None) == 0
-    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, one, 7, 8, None) == 9003
-    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, one, 1, 8, None) == 9005
+    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, one, one, 7, 8, None) == 9003
+    assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, one, one, 1, 8, None) == 9005
     assert hip.sf_logps_weight(None, one, one, -100, 1, 8, 1.0, one, None, None) == 9001
     tiles = lambda **k: hip.sf_logps_tiles(*{**dict(w=one, ldw=64, v=8, h=one, ldh=64, n=1, k=64, y=one, ig=-100, s=1.0, t=1,  # noqa: E731
                                                     p=one, tg=one, kp=None, ldk=0, l=one, lp=one, st=None), **k}.values())
     assert tiles(w=None) == tiles(v=0) == tiles(ldw=32) == tiles(s=0.0) == tiles(kp=one, ldk=64) == tiles(ldh=1 << 23) == 9001
     assert tiles(k=32) == tiles(w=72) == tiles(ldh=68) == tiles(kp=72, ldk=256) == 9007
     assert tiles(t=0) == 9003 and tiles(n=0) == 0
-    none = (None, 0, 1.0, None, None, 0, None)
+    none = (one, 0, 1.0, None, None, 0, None)
     assert hip.sf_logps_keep_grad(one, 256, 2, 1, 8, one, one, -100, one, one, 1, *none) == 9001
     assert hip.sf_logps_keep_grad(one, 264, 1, 1, 8, one, one, -100, one, one, 1, *none) == 9007
     assert hip.sf_logps_keep_grad(one, 256, 2, 2, 8, one, one, -100, one, one, 1, one, 1, 1.0, one, None, 0, None) == 9001
@@ -156,3 +156,18 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert pol(w=24) == 9007
     assert hip.sf_pref_grad(one, one, one, 7, 1, 8, one, None) == hip.sf_policy_grad(one, None, one, 1, 8, one, None) == 9001
     assert hip.sf_act8_pack(None, 1, 8, one, 0, None) == hip.sf_act8_unpack(one, 5, 8, 4096, 1, None) == 9001
+
+
+def test_ignored_tokens_may_hold_anything():
+    g = torch.Generator().manual_seed(8)
+    hidden, weight = torch.randn(6, 8, generator=g), torch.randn(20, 8, generator=g)
+    labels = torch.tensor([1, -100, 3, -100, 5, 6])
+    results = []
+    for fill in (0.0, math.nan):
+        h = hidden.clone()
+        h[labels == -100] = fill
+        h.requires_grad_(True)
+        w = weight.clone().requires_grad_(True)
+        lp = linear_logps(h, w, labels)
+        results.append((lp.detach(), *torch.autograd.grad(lp.sum(), (h, w))))
+    assert all(a.isfinite().all() and torch.equal(a, b) for a, b in zip(*results))

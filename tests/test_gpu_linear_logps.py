@@ -235,3 +235,74 @@ def test_every_tile(dev, shape, dtype):
     """Tiles of 256, 128, 64 and 32 tokens, of brief and of long sums, with and
     without what they keep."""
     test_matches_float64(dev, shape, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(70, 64, 300), (300, 128, 40_000)])
+def test_tokens_without_a_gradient_may_hold_anything(dev, shape, dtype):
+    """Ignored tokens and those whose upstream gradient is 0, with NaN and
+    infinities for hidden states: the others' results are as without them."""
+    hidden, weight, labels, up = inputs(shape, dtype, dev)
+    out = torch.rand(shape[0], generator=torch.Generator(device=dev).manual_seed(3), device=dev) < 0.4
+    labels = torch.where(out & (torch.arange(shape[0], device=dev) % 2 == 0), torch.full_like(labels, -100), labels)
+    up = torch.where(out, torch.zeros_like(up), up)
+    bad = torch.tensor([math.nan, math.inf, -math.inf], device=dev).to(dtype)[torch.arange(shape[0], device=dev) % 3]
+    results = []
+    for spoiled in (False, True):
+        h = torch.where(out[:, None], bad[:, None], hidden) if spoiled else hidden.clone()
+        h.requires_grad_(True)
+        w = weight.clone().requires_grad_(True)
+        lp = linear_logps(h, w, labels)
+        results.append((lp.detach()[~out], *torch.autograd.grad(lp, (h, w), up)))
+    for a, b in zip(*results):
+        assert a.isfinite().all() and torch.equal(a, b)
+    assert (results[1][1][out] == 0).all()
+
+
+def test_more_than_2_31_kept_elements(dev):
+    """Offsets past 32 bits in what the forward keeps; chunk by chunk against 64 bits."""
+    n, h, v = 17_000, 64, 130_000
+    hidden, weight, labels, up = inputs((n, h, v), torch.bfloat16, dev)
+    assert n * v > 1 << 31
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    gh, gw = torch.autograd.grad(lp, (hidden, weight), up)
+    want_w = torch.zeros(v, h, dtype=torch.float64, device=dev)
+    bound_w = torch.zeros_like(want_w)
+    for s in range(0, n, 2000):
+        part = slice(s, min(n, s + 2000))
+        want, bound = logps(hidden.detach()[part], weight.detach(), labels[part], grad=up[part])
+        near(lp.detach()[part], want[0], bound[0])
+        near(gh[part], want[1], bound[1])
+        want_w += want[2]
+        bound_w += bound[2]
+    near(gw, want_w, bound_w)
+
+
+def test_recorded_calls_are_torch_operations(dev):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    hidden, weight, labels, _ = inputs((20, 64, 100), torch.bfloat16, dev)
+    graph = make_fx(lambda x: linear_logps(x, weight, labels))(hidden)
+    other = hidden * 0.5
+    want = linear_logps(other, weight, labels)
+    assert torch.allclose(graph(other), want, atol=1e-4) and len(list(graph.graph.nodes)) > 5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_batched_backward_takes_torch_operations(dev, dtype):
+    """A backward over a batch of upstream gradients: each as by itself."""
+    hidden, weight, labels, up = inputs((20, 64, 100), dtype, dev)
+    labels[4] = 100
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    ups = torch.stack([up, 2 * up, torch.zeros_like(up)])
+    ups[:, 4] = 0.0
+    got = torch.autograd.grad(lp, (hidden, weight), ups, is_grads_batched=True, retain_graph=True)
+    for k in range(3):
+        want = torch.autograd.grad(lp, (hidden, weight), ups[k], retain_graph=True)
+        for a, b in zip(got, want):
+            assert torch.allclose(a[k].float(), b.float(), rtol=0.02, atol=2e-4)
+    assert (got[0][2] == 0).all() and (got[1][2] == 0).all()
