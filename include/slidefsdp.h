@@ -324,8 +324,11 @@ int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab,
  * lse2 = the row's logsumexp in base 2, logp as above.  parts: workspace of
  * ceil(vocab / SF_LOGPS_SPAN) * rows * 2 floats, for each span of words its
  * largest scaled logit m in base 2 and the sum of 2^(logit - m); target: of rows
- * floats.  keep (or null): [rows, ld_keep] of dtype, every 2^(logit - m), 0
- * behind the vocabulary up to the next whole span, for sf_logps_keep_grad.
+ * floats; order (or null): of rows + 1 integers, with which rows without a label
+ * inside the vocabulary take no part in the product, where the hidden rows
+ * span less than 4 GiB (SF_ETOOBIG).  keep (or null): [rows,
+ * ld_keep] of dtype, every 2^(logit - m) of the rows that do, 0 behind the
+ * vocabulary up to the next whole span, for sf_logps_keep_grad.
  * hidden_size is a multiple of 64, ldw and ldh (at most 2^22) and ld_keep of 8,
  * weight, hidden and keep start on 16-byte boundaries (SF_EALIGN). */
 #define SF_LOGPS_SPAN 256
@@ -333,8 +336,8 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab,
                    const void* hidden, size_t ldh, size_t rows,
                    size_t hidden_size, const int64_t* labels,
                    int64_t ignore_index, float scale, int dtype, void* parts,
-                   float* target, void* keep, size_t ld_keep, float* lse2,
-                   float* logp, sf_stream_t stream);
+                   float* target, int32_t* order, void* keep, size_t ld_keep,
+                   float* lse2, float* logp, sf_stream_t stream);
 
 /* The gradient of such logits is row_weight[i] * D[i, j], D = ((j == label) -
  * p) / (1 - p_label): 1 at the label.  row_weight = grad * scale * (1 -

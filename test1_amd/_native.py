@@ -106,7 +106,8 @@ HIP_SIGNATURES = {
     "sf_ce_weight_grad": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _vp, _sz, _i, _vp],
     "sf_ce_scale": [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _i, _vp],
     "sf_logps_rows": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp],
-    "sf_logps_tiles": [_vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _i, _vp, _vp, _vp, _sz, _vp, _vp, _vp],
+    "sf_logps_tiles": [_vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _i, _vp, _vp, _vp, _vp, _sz, _vp, _vp,
+                       _vp],
     "sf_logps_weight": [_vp, _vp, _vp, ctypes.c_int64, _sz, _sz, _f, _vp, _vp, _vp],
     "sf_logps_keep_grad": [_vp, _sz, _sz, _sz, _sz, _vp, _vp, ctypes.c_int64, _vp, _vp, _i, _vp, _sz, _f, _vp, _vp, _i, _vp],
     "sf_logps_grad": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp, _vp, _i, _sz, _vp],

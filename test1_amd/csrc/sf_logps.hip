@@ -64,12 +64,41 @@ struct Tiles {
     const uint16_t* hidden;   // [tokens, 64 steps], ldh
     uint32_t ldw, ldh, vocab, tokens, steps;
     const int64_t* labels;
+    const int32_t* order;     // [tokens + 1] the rows with a label and their number, or null: all rows
     float scale2;             // scale * log2(e)
     float2* parts;            // [tiles of words, tokens] maximum in base 2 and sum
     float* target;            // [tokens] the label's product, unscaled
     uint16_t* keep;           // [tokens, ld_keep] or null
     uint64_t ld_keep;
 };
+
+// The rows whose label is inside the vocabulary, in their order, and behind
+// `rows` of them their number.  The product skips the others, prompts above all:
+// their share of its time for one launch, 5 us at 8190 rows.  One workgroup,
+// each lane a run of rows.
+constexpr int kOrderThreads = 1024;
+__global__ __launch_bounds__(kOrderThreads) void logps_order_kernel(const int64_t* __restrict__ labels,
+                                                                    int64_t ignore_index, uint32_t vocab,
+                                                                    uint32_t rows, int32_t* __restrict__ order) {
+    __shared__ uint32_t waves[kOrderThreads / 64];
+    const uint32_t each = (rows + kOrderThreads - 1) / kOrderThreads;
+    const uint32_t from = min(threadIdx.x * each, rows), to = min(from + each, rows);
+    uint32_t mine = 0;
+    for (uint32_t i = from; i < to; ++i) mine += row_kind(labels[i], ignore_index, vocab) == kValid;
+    uint32_t before = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t below = __shfl_up(before, d);
+        if ((threadIdx.x & 63) >= uint32_t(d)) before += below;
+    }
+    if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = before;
+    before -= mine;
+    __syncthreads();
+    for (uint32_t w = 0; w < (threadIdx.x >> 6); ++w) before += waves[w];
+    for (uint32_t i = from; i < to; ++i)
+        if (row_kind(labels[i], ignore_index, vocab) == kValid) order[before++] = int32_t(i);
+    if (threadIdx.x == kOrderThreads - 1) order[rows] = int32_t(before);
+}
 
 // Interleaves what a half's products run beside: kLoads copies into LDS, then
 // kReads reads of it, two products each; all else after.
@@ -88,8 +117,9 @@ __device__ __forceinline__ void interleave() {
     __builtin_amdgcn_sched_group_barrier(0x008, kMul, 0);
 }
 
-// kWV x kWT waves of words and of tokens.
-template <typename Fmt, int kWV, int kWT, int kFV, int kFT, bool kKeep>
+// kWV x kWT waves of words and of tokens.  kOrder: tokens in the order of
+// a.order, otherwise all of them.
+template <typename Fmt, int kWV, int kWT, int kFV, int kFT, bool kKeep, bool kOrder>
 __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Tiles a) {
     constexpr int kWaves = kWV * kWT, kBV = kWV * kFV * 16, kBT = kWT * kFT * 16;
     static_assert(kBV == kSpan, "a tile is one span of words");
@@ -100,22 +130,39 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
     // tokens of kept words around, over the buffers.
     constexpr int kTurnRow = kFV * 32;   // bytes of a token's words of a wave
     static_assert(kWaves * 16 * kTurnRow <= 2 * kBuffer && kWV * kBT * 4 <= 2 * kBuffer, "the buffers hold it");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer];
+    // Where one workgroup fills a compute unit: each token's row and label (-1: none
+    // inside the vocabulary), which the end would otherwise wait for.
+    constexpr bool kNoted = 4 * kBuffer > 160 * 1024;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer + (kNoted ? kBT * 8 : 0)];
+    int32_t* const noted_row = reinterpret_cast<int32_t*>(lds + 2 * kBuffer);
+    int32_t* const noted_label = noted_row + kBT;
 
     const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wv = wave / kWT, wt = wave % kWT, wv0 = wv * kFV * 16, wt0 = wt * kFT * 16;
 
-    // Workgroups go to the XCDs in turn: each XCD has a contiguous run of tiles.
-    const uint32_t tiles_v = (a.vocab + kBV - 1) / kBV, tiles_t = (a.tokens + kBT - 1) / kBT;
-    const uint32_t xcd = blockIdx.x % 8, each = gridDim.x / 8, more = gridDim.x % 8;
+    // Workgroups go to the XCDs in turn: each XCD has a contiguous run of tiles;
+    // those that no token needs end here.
+    const uint32_t count = kOrder ? uint32_t(a.order[a.tokens]) : a.tokens;
+    const uint32_t tiles_v = (a.vocab + kBV - 1) / kBV, tiles_t = (count + kBT - 1) / kBT, tiles = tiles_v * tiles_t;
+    const uint32_t xcd = blockIdx.x % 8, each = tiles / 8, more = tiles % 8;
+    if (blockIdx.x / 8 >= each + (xcd < more)) return;
     const uint32_t id = xcd * each + min(xcd, more) + blockIdx.x / 8;
+    const auto row_of = [&](uint32_t token) {   // past the last one: the last one's
+        token = min(token, count - 1);
+        return kOrder ? uint32_t(a.order[token]) : token;
+    };
+    const auto label_of = [&](uint32_t token, uint32_t row) {
+        const int64_t y = a.labels[row];
+        return token < count && y >= 0 && y < int64_t(a.vocab) ? int32_t(y) : -1;
+    };
     const uint32_t first_t = id / (kGroupT * tiles_v) * kGroupT, group_t = min(uint32_t(kGroupT), tiles_t - first_t);
     const uint32_t in = id - first_t * tiles_v;
     const uint32_t v0 = in / group_t * kBV, t0 = (first_t + in % group_t) * kBT;
 
     const uint8_t* gv = reinterpret_cast<const uint8_t*>(a.weight + uint64_t(v0) * a.ldw);
-    const uint8_t* gt = reinterpret_cast<const uint8_t*>(a.hidden + uint64_t(t0) * a.ldh);
+    const uint32_t t_base = kOrder ? 0 : t0;
+    const uint8_t* gt = reinterpret_cast<const uint8_t*>(a.hidden + uint64_t(t_base) * a.ldh);
     // Rows past the last are the last one again: their results are dropped below.
     uint32_t off[kLV + kLT];
     const uint32_t chunk = ((lane & 7) ^ (lane >> 3)) * 16;
@@ -124,7 +171,7 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
         off[j] = min((j * kWaves + wave) * 8 + (lane >> 3), a.vocab - 1 - v0) * (a.ldw * 2) + chunk;
 #pragma unroll
     for (int j = 0; j < kLT; ++j)
-        off[kLV + j] = min((j * kWaves + wave) * 8 + (lane >> 3), a.tokens - 1 - t0) * (a.ldh * 2) + chunk;
+        off[kLV + j] = (row_of(t0 + (j * kWaves + wave) * 8 + (lane >> 3)) - t_base) * (a.ldh * 2) + chunk;
     typedef __attribute__((address_space(3))) uint8_t Lds;
     typedef const __attribute__((address_space(1))) uint8_t Global;
     const auto copy = [&](uint32_t step, uint32_t buf) {
@@ -182,6 +229,11 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
         for (int j = 0; j < kFT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     copy(0, 0);
     if (a.steps > 1) copy(1, 1);
+    if (kNoted && threadIdx.x < kBT) {
+        const uint32_t token = t0 + threadIdx.x, row = row_of(token);
+        noted_row[threadIdx.x] = int32_t(row);
+        noted_label[threadIdx.x] = label_of(token, row);
+    }
     meet();
     read(0, 0);
     uint32_t s = 0;
@@ -191,15 +243,16 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
     multiply(0);
     interleave<kFV + kFT, kFV * kFT, 0>();
     meet();   // the buffers are not read again
+    multiply(1);
+    uint32_t row[kFT];
     int32_t label[kFT];   // as an index from this lane's first word
 #pragma unroll
     for (int j = 0; j < kFT; ++j) {
-        const uint32_t token = t0 + wt0 + j * 16 + l16;
-        const int64_t y64 = a.labels[min(token, a.tokens - 1)];
-        const bool inside = token < a.tokens && y64 >= 0 && y64 < int64_t(a.vocab);
-        label[j] = inside ? int32_t(y64) - int32_t(v0 + wv0 + quad * 4) : -1;
+        const uint32_t t = wt0 + j * 16 + l16;
+        row[j] = kNoted ? uint32_t(noted_row[t]) : row_of(t0 + t);
+        label[j] = kNoted ? noted_label[t] : label_of(t0 + t, row[j]);
+        if (label[j] >= 0) label[j] -= int32_t(v0 + wv0 + quad * 4);
     }
-    multiply(1);
 
     if (v0 + kBV > a.vocab) {
 #pragma unroll
@@ -230,7 +283,7 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (label[j] == i * 16 + r) z = acc[i][j][r];
-            a.target[t0 + wt0 + j * 16 + l16] = z;
+            a.target[row[j]] = z;
         }
     }
     __syncthreads();
@@ -272,9 +325,9 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
             for (int k = 0; k < 16 / kRows; ++k) {
                 const uint32_t r = k * kRows + lane / kAcross, c16 = lane % kAcross;
                 const u32x4 v = *reinterpret_cast<const u32x4*>(turn + r * kTurnRow + (c16 ^ (r & (kFV * 2 - 1))) * 16);
-                const uint32_t token = t0 + wt0 + j * 16 + r;
-                if (token < a.tokens)
-                    *reinterpret_cast<u32x4*>(a.keep + token * a.ld_keep + v0 + wv0 + c16 * 8) = v;
+                const uint32_t to = __shfl(row[j], r);   // of the lane that has this token
+                if (t0 + wt0 + j * 16 + r < count)
+                    *reinterpret_cast<u32x4*>(a.keep + to * a.ld_keep + v0 + wv0 + c16 * 8) = v;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
@@ -290,8 +343,7 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
             const uint32_t t = wt0 + j * 16 + l16;
 #pragma unroll
             for (int w = 1; w < kWV; ++w) sum[j] += shared[w * kBT + t];
-            if (t0 + t < a.tokens)
-                a.parts[uint64_t(v0 / kSpan) * a.tokens + t0 + t] = float2{top[j], sum[j]};
+            if (t0 + t < count) a.parts[uint64_t(v0 / kSpan) * a.tokens + row[j]] = float2{top[j], sum[j]};
         }
 }
 
@@ -307,7 +359,8 @@ __global__ __launch_bounds__(kJoinThreads) void logps_join_kernel(const float2* 
     __shared__ Lse waves[kJoinThreads / 64][kJoinTokens];
     const uint32_t t = threadIdx.x % kJoinTokens, token = blockIdx.x * kJoinTokens + t;
     Lse p = {-__builtin_inff(), 0.0f};
-    if (token < tokens)
+    const RowKind kind = token < tokens ? row_kind(labels[token], ignore_index, vocab) : kIgnored;
+    if (kind == kValid)   // the others may have no parts
         for (uint32_t k = threadIdx.x / kJoinTokens; k < spans; k += kJoinThreads / kJoinTokens) {
             const float2 v = parts[uint64_t(k) * tokens + token];
             const float m = fmaxf(p.m, v.x), c = base(m);
@@ -326,10 +379,13 @@ __global__ __launch_bounds__(kJoinThreads) void logps_join_kernel(const float2* 
     if (threadIdx.x >= kJoinTokens || token >= tokens) return;
 #pragma unroll
     for (int w = 1; w < kJoinThreads / 64; ++w) p = merge(p, waves[w][t]);
-    const RowKind kind = row_kind(labels[token], ignore_index, vocab);
+    if (kind != kValid) {
+        lse2[token] = logp[token] = kind == kIgnored ? 0.0f : __builtin_nanf("");
+        return;
+    }
     const float c = base(p.m), l = log2f(p.s);
-    lse2[token] = kind == kValid ? c + l : kind == kIgnored ? 0.0f : __builtin_nanf("");
-    logp[token] = kind == kValid ? (fmaf(target[token], scale2, -c) - l) * kLn2 : kind == kIgnored ? 0.0f : __builtin_nanf("");
+    lse2[token] = c + l;
+    logp[token] = (fmaf(target[token], scale2, -c) - l) * kLn2;
 }
 
 // ---------------------------------------------------------------------
@@ -533,8 +589,11 @@ int launch_tiles(const Tiles& a, hipStream_t st) {
     constexpr uint32_t kBT = kWT * kFT * 16;
     const uint64_t tiles = uint64_t((a.vocab + kSpan - 1) / kSpan) * ((a.tokens + kBT - 1) / kBT);
     if (tiles > kMaxLanes / (kWV * kWT * 64)) return SF_EINVAL;
-    const auto kernel = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, true>
-                                          : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, false>;
+    const auto all = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, true, false>
+                                       : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, false, false>;
+    const auto some = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, true, true>
+                                        : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, false, true>;
+    const auto kernel = a.order != nullptr ? some : all;
     hipLaunchKernelGGL(kernel, dim3(uint32_t(tiles)), dim3(kWV * kWT * 64), 0, st, a);
     return status();
 }
@@ -628,7 +687,8 @@ extern "C" {
 
 int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab, const void* hidden, size_t ldh, size_t rows,
                    size_t hidden_size, const int64_t* labels, int64_t ignore_index, float scale, int dtype, void* parts,
-                   float* target, void* keep, size_t ld_keep, float* lse2, float* logp, sf_stream_t stream) {
+                   float* target, int32_t* order, void* keep, size_t ld_keep, float* lse2, float* logp,
+                   sf_stream_t stream) {
     if (rows == 0) return SF_OK;
     if (weight == nullptr || hidden == nullptr || labels == nullptr || parts == nullptr || target == nullptr ||
         lse2 == nullptr || logp == nullptr || sizes_bad(rows, vocab))
@@ -645,9 +705,17 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab, const void* hid
         return SF_EALIGN;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const Tiles a = {static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(hidden), uint32_t(ldw),
-                     uint32_t(ldh), uint32_t(vocab), uint32_t(rows), uint32_t(hidden_size / kTerms), labels,
+                     uint32_t(ldh), uint32_t(vocab), uint32_t(rows), uint32_t(hidden_size / kTerms), labels, order,
                      scale * kLog2e, static_cast<float2*>(parts), target, static_cast<uint16_t*>(keep), ld_keep};
-    const int e = dtype == SF_DTYPE_BF16 ? dispatch_tiles<Bf16>(a, st) : dispatch_tiles<F16>(a, st);
+    int e = SF_OK;
+    if (order != nullptr) {   // 32-bit byte offsets of all rows
+        if (uint64_t(rows) * ldh * 2 > UINT32_MAX) return SF_ETOOBIG;
+        hipLaunchKernelGGL(logps_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, labels, ignore_index, a.vocab, a.tokens,
+                           order);
+        e = status();
+        if (e != SF_OK) return e;
+    }
+    e = dtype == SF_DTYPE_BF16 ? dispatch_tiles<Bf16>(a, st) : dispatch_tiles<F16>(a, st);
     if (e != SF_OK) return e;
     hipLaunchKernelGGL(logps_join_kernel, dim3((a.tokens + kJoinTokens - 1) / kJoinTokens), dim3(kJoinThreads), 0, st,
                        a.parts, uint32_t(spans), a.tokens, target, labels, ignore_index, a.vocab, a.scale2, lse2, logp);

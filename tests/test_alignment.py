@@ -132,7 +132,7 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert hip.sf_logps_grad(one, 8, 1, 8, one, -100, 1.0, one, one, one, one, 1, 8, None) == 9005
     assert hip.sf_logps_weight(None, one, one, -100, 1, 8, 1.0, one, None, None) == 9001
     tiles = lambda **k: hip.sf_logps_tiles(*{**dict(w=one, ldw=64, v=8, h=one, ldh=64, n=1, k=64, y=one, ig=-100, s=1.0, t=1,  # noqa: E731
-                                                    p=one, tg=one, kp=None, ldk=0, l=one, lp=one, st=None), **k}.values())
+                                                    p=one, tg=one, od=None, kp=None, ldk=0, l=one, lp=one, st=None), **k}.values())
     assert tiles(w=None) == tiles(v=0) == tiles(ldw=32) == tiles(s=0.0) == tiles(kp=one, ldk=64) == tiles(ldh=1 << 23) == 9001
     assert tiles(k=32) == tiles(w=72) == tiles(ldh=68) == tiles(kp=72, ldk=256) == 9007
     assert tiles(t=0) == 9003 and tiles(n=0) == 0

@@ -306,3 +306,26 @@ def test_batched_backward_takes_torch_operations(dev, dtype):
         for a, b in zip(got, want):
             assert torch.allclose(a[k].float(), b.float(), rtol=0.02, atol=2e-4)
     assert (got[0][2] == 0).all() and (got[1][2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("live", [600, 420, 256, 3, 1, 0])
+def test_tokens_left_out_of_the_product(dev, live, dtype):
+    """Large products take only the tokens with a label; the others are 0, or
+    NaN where their label is outside the vocabulary."""
+    shape = (600, 2048, 33_000)
+    hidden, weight, labels, up = inputs(shape, dtype, dev)
+    labels = torch.where(labels == -100, torch.zeros_like(labels), labels)
+    out = torch.randperm(600, generator=torch.Generator().manual_seed(live))[: 600 - live].to(dev)
+    labels[out] = -100
+    want, bound = logps(hidden, weight, labels, grad=up)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    for got, w, b in zip((lp.detach(), *torch.autograd.grad(lp, (hidden, weight), up)), want, bound):
+        near(got, w, b)
+    if live and live < 600:
+        labels[out[0]] = 33_000
+        with torch.no_grad():
+            again = linear_logps(hidden, weight, labels)
+        assert again[out[0]].isnan() and torch.equal(again[labels != 33_000], lp.detach()[labels != 33_000])
