@@ -25,7 +25,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .fused_ce import _DTYPES, _PLAIN, _memory_is_value, _saved_plain, _traced, _vocabulary_parts
+from .fused_ce import (_DTYPES, _PARTS_TILES, _PARTS_VOCAB, _PLAIN, _memory_is_value, _saved_plain, _tiles, _traced,
+                       _vocabulary_parts)
 from .kernels import _CE_DTYPES
 
 
@@ -44,6 +45,32 @@ def _backward_rows(n: int, vocab: int) -> Tuple[int, bool]:
     row = 2 * (-(-vocab // _SPAN) * _SPAN)
     step = max(64, _AGAIN_BYTES // row // 64 * 64)
     return (n, True) if (n + 63) * row <= _KEEP_BYTES else (min(n, step), False)
+
+
+def _hidden_parts(rows: int, weight: torch.Tensor) -> int:
+    """Parts in which the hidden gradient's product sums over the vocabulary: up
+    to 64 tiles of 256 x 256 by the rule of the fused output unit, beyond by how
+    well the tiles fill rounds of 256 compute units.  The library's product of
+    640 tiles (two and a half rounds) runs at 0.96 PFLOP/s, in two parts at
+    1.31; us, one product | parts, tokens x hidden x vocabulary: 8190 x 5120 x
+    152064 13264 | 9718 (2), 8190 x 2560 x 50257 2157 | 1715 (4), 3000 x 5120 x
+    32000 1136 | 796 (4), 4000 x 3584 x 152064 4838 | 3349 (8), 6500 x 2048 x
+    128256 4171 | 3181 (8), 5000 x 2048 x 50257 903 | 894 (8); adding the parts up
+    takes 10 to 100.  Whole rounds need none: 4092 x 4096 x 128256 3094 | 3105."""
+    v, h = weight.shape
+    tiles = _tiles(rows, h)
+    if tiles <= _PARTS_TILES:
+        return _vocabulary_parts(rows, weight)
+    if (tiles % 256 == 0 or v < _PARTS_VOCAB or weight.element_size() != 2 or h % 8 != 0 or not weight.is_contiguous()
+            or weight.data_ptr() % 16 != 0 or rows * h >= 1 << 31):
+        return 1
+
+    def filled(parts: int) -> float:
+        return tiles * parts / (-(-tiles * parts // 256) * 256)
+
+    able = [p for p in (2, 4, 8) if v >= 4096 * p]
+    whole = [p for p in able if filled(p) == 1]
+    return whole[0] if whole else max((p for p in able if p > 2), key=filled)
 
 
 def _f32_out(dtype: torch.dtype) -> dict:
@@ -249,7 +276,7 @@ def linear_logps(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tenso
     step, keep, nparts = rows.shape[0], False, 1
     if need_grad:
         step, keep = _backward_rows(step, weight.shape[0])
-        nparts = _vocabulary_parts(step, weight)
+        nparts = _hidden_parts(step, weight)
     logp = _native.ops().linear_logps(rows, weight, flat, ignore_index, scale, nparts, step, keep)
     if logp is None:
         with _on_device(hidden):

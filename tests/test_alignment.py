@@ -171,3 +171,31 @@ def test_ignored_tokens_may_hold_anything():
         lp = linear_logps(h, w, labels)
         results.append((lp.detach(), *torch.autograd.grad(lp.sum(), (h, w))))
     assert all(a.isfinite().all() and torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_parts_of_the_hidden_gradient():
+    """Powers of two that the adding kernel takes, one where the tiles fill whole rounds."""
+    from test1_amd.linear_logps import _hidden_parts
+
+    class Weight:   # a weight without its memory
+        def __init__(self, v, h):
+            self.shape = torch.Size((v, h))
+
+        def element_size(self):
+            return 2
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 4096
+
+    for (n, h, v), want in {(8190, 5120, 152_064): 2, (4092, 4096, 128_256): 1, (8190, 4096, 32_000): 1,
+                            (8190, 2560, 50_257): 4, (3000, 5120, 32_000): 4, (4000, 3584, 152_064): 8,
+                            (8190, 5120, 8192): 1}.items():
+        assert _hidden_parts(n, Weight(v, h)) == want, (n, h, v)
+    for n in range(256, 9000, 300):
+        for h in (512, 896, 2048, 4096, 5120):
+            for v in (5000, 16_384, 32_000, 152_064):
+                p = _hidden_parts(n, Weight(v, h))
+                assert p in (1, 2, 4, 8, 16) and (p == 1 or v // p >= 1024)

@@ -329,3 +329,17 @@ def test_tokens_left_out_of_the_product(dev, live, dtype):
         with torch.no_grad():
             again = linear_logps(hidden, weight, labels)
         assert again[out[0]].isnan() and torch.equal(again[labels != 33_000], lp.detach()[labels != 33_000])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,parts", [((2100, 2048, 16_400), 4), ((2100, 2048, 33_000), 8), ((8190, 1024, 16_387), 2)])
+def test_hidden_gradient_of_many_tiles_in_parts(dev, shape, parts, dtype):
+    """More than 64 tiles that fill no whole round, the last words in no part."""
+    hidden, weight, labels, up = inputs(shape, dtype, dev)
+    assert module._hidden_parts(shape[0], weight) == parts
+    want, bound = logps(hidden, weight, labels, grad=up)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    for got, w, b in zip((lp.detach(), *torch.autograd.grad(lp, (hidden, weight), up)), want, bound):
+        near(got, w, b)
