@@ -117,9 +117,10 @@ __device__ __forceinline__ void interleave() {
     __builtin_amdgcn_sched_group_barrier(0x008, kMul, 0);
 }
 
-// kWV x kWT waves of words and of tokens.  kOrder: tokens in the order of
+// kWV x kWT waves of words and of tokens.  kDeep buffers of 64 terms each: all
+// but one are on their way while one is used.  kOrder: tokens in the order of
 // a.order, otherwise all of them.
-template <typename Fmt, int kWV, int kWT, int kFV, int kFT, bool kKeep, bool kOrder>
+template <typename Fmt, int kWV, int kWT, int kFV, int kFT, int kDeep, bool kKeep, bool kOrder>
 __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Tiles a) {
     constexpr int kWaves = kWV * kWT, kBV = kWV * kFV * 16, kBT = kWT * kFT * 16;
     static_assert(kBV == kSpan, "a tile is one span of words");
@@ -129,12 +130,14 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
     // The end exchanges maxima and sums between the waves and turns each wave's 16
     // tokens of kept words around, over the buffers.
     constexpr int kTurnRow = kFV * 32;   // bytes of a token's words of a wave
-    static_assert(kWaves * 16 * kTurnRow <= 2 * kBuffer && kWV * kBT * 4 <= 2 * kBuffer, "the buffers hold it");
-    // Where one workgroup fills a compute unit: each token's row and label (-1: none
-    // inside the vocabulary), which the end would otherwise wait for.
-    constexpr bool kNoted = 4 * kBuffer > 160 * 1024;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer + (kNoted ? kBT * 8 : 0)];
-    int32_t* const noted_row = reinterpret_cast<int32_t*>(lds + 2 * kBuffer);
+    static_assert(kWaves * 16 * kTurnRow <= kDeep * kBuffer && kWV * kBT * 4 <= kDeep * kBuffer, "the buffers hold it");
+    // Where LDS has room for it and a compute unit only one workgroup: each token's
+    // row and label (-1: none inside the vocabulary), which the end would otherwise
+    // wait for.
+    constexpr int kLds = 160 * 1024;
+    constexpr bool kNoted = 2 * kDeep * kBuffer > kLds && kDeep * kBuffer + kBT * 8 <= kLds;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kDeep * kBuffer + (kNoted ? kBT * 8 : 0)];
+    int32_t* const noted_row = reinterpret_cast<int32_t*>(lds + kDeep * kBuffer);
     int32_t* const noted_label = noted_row + kBT;
 
     const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
@@ -202,23 +205,30 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
 #pragma unroll
             for (int j = 0; j < kFT; ++j) acc[i][j] = mfma(Fmt{}, x[half][i], y[half][j], acc[i][j]);
     };
-    // All copies and LDS reads of every wave are done, and none moves across.
-    const auto meet = [] {
+    // Every wave's LDS reads are done, and its copies but those of the last `ahead`
+    // buffers; nothing moves across.
+    const auto meet = [](auto ahead) {
+        constexpr uint32_t kLeft = decltype(ahead)::value * (kLV + kLT);
+        static_assert(kLeft < 64, "what the counter holds");
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);
+        __builtin_amdgcn_s_waitcnt(0x0070 | (kLeft & 15) | kLeft >> 4 << 14);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // kMore: there is a buffer after the next to copy
+    // kMore: there are buffers left to copy
     const auto step = [&](uint32_t s, auto kMore) {
-        read(s & 1, 1);
+        read(s % kDeep, 1);
         multiply(0);
         interleave<kFV + kFT, kFV * kFT, 0>();
-        meet();
-        if constexpr (decltype(kMore)::value) copy(s + 2, s & 1);
-        read((s + 1) & 1, 0);
+        if constexpr (decltype(kMore)::value) {
+            meet(std::integral_constant<int, kDeep - 2>{});
+            copy(s + kDeep, s % kDeep);
+        } else {
+            meet(std::integral_constant<int, 0>{});
+        }
+        read((s + 1) % kDeep, 0);
         multiply(1);
         interleave<kFV + kFT, kFV * kFT, decltype(kMore)::value ? kLV + kLT : 0>();
         __builtin_amdgcn_sched_barrier(0);
@@ -227,22 +237,25 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
     for (int i = 0; i < kFV; ++i)
 #pragma unroll
         for (int j = 0; j < kFT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    copy(0, 0);
-    if (a.steps > 1) copy(1, 1);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+        if (uint32_t(d) < a.steps) copy(d, d);
     if (kNoted && threadIdx.x < kBT) {
         const uint32_t token = t0 + threadIdx.x, row = row_of(token);
         noted_row[threadIdx.x] = int32_t(row);
         noted_label[threadIdx.x] = label_of(token, row);
     }
-    meet();
+    // The note above waits for its own loads: the counter is at 0 with them, so the
+    // first buffer needs no other rule.
+    meet(std::integral_constant<int, 0>{});
     read(0, 0);
     uint32_t s = 0;
-    for (; s + 2 < a.steps; ++s) step(s, std::true_type{});
-    if (s + 1 < a.steps) step(s++, std::false_type{});
-    read(s & 1, 1);
+    for (; s + kDeep < a.steps; ++s) step(s, std::true_type{});
+    while (s + 1 < a.steps) step(s++, std::false_type{});
+    read(s % kDeep, 1);
     multiply(0);
     interleave<kFV + kFT, kFV * kFT, 0>();
-    meet();   // the buffers are not read again
+    meet(std::integral_constant<int, 0>{});   // the buffers are not read again
     multiply(1);
     uint32_t row[kFT];
     int32_t label[kFT];   // as an index from this lane's first word
@@ -584,15 +597,15 @@ __global__ __launch_bounds__(kGradThreads) void logps_grad_kernel(const float* l
 }
 
 // ---------------------------------------------------------------------
-template <typename Fmt, int kWV, int kWT, int kFV, int kFT>
+template <typename Fmt, int kWV, int kWT, int kFV, int kFT, int kDeep>
 int launch_tiles(const Tiles& a, hipStream_t st) {
     constexpr uint32_t kBT = kWT * kFT * 16;
     const uint64_t tiles = uint64_t((a.vocab + kSpan - 1) / kSpan) * ((a.tokens + kBT - 1) / kBT);
     if (tiles > kMaxLanes / (kWV * kWT * 64)) return SF_EINVAL;
-    const auto all = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, true, false>
-                                       : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, false, false>;
-    const auto some = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, true, true>
-                                        : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, false, true>;
+    const auto all = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, kDeep, true, false>
+                                       : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, kDeep, false, false>;
+    const auto some = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, kDeep, true, true>
+                                        : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, kDeep, false, true>;
     const auto kernel = a.order != nullptr ? some : all;
     hipLaunchKernelGGL(kernel, dim3(uint32_t(tiles)), dim3(kWV * kWT * 64), 0, st, a);
     return status();
@@ -603,20 +616,28 @@ int launch_tiles(const Tiles& a, hipStream_t st) {
 // compute unit holds two; `half`: where there is at most one for each unit), in
 // that of a round of the largest.  Small sums (`brief`, under 2048 terms) spend
 // more of it at the ends of their tiles.  Measured, us, 256 | 128 | 64 | 32
-// tokens a tile: 128256 words x 4092 terms and 64 tokens 212 | 200 | 170 | 201,
+// tokens a tile: 128256 words x 4096 terms and 64 tokens 220 | 178 | 171 | 203,
 // 128 tokens 218 | 204 | 217 | 331, 256 tokens 230 | 349 | 356 | 586, 1023
 // tokens 799 | 1207 | 1166 | 2028; 777 tokens x 1024, 50257 words 109 | 101 |
-// 98 | 168, 32000 words 58 | 68 | 65 | 113; 300 x 2560 x 8192 52 | 37 | 35 | 40,
-// 126 x 2048 x 16384 43 | 31 | 28 | 26, 8000 x 1024 x 1000 27 | 20 | 22 | 30.
+// 98 | 168, 32000 words 58 | 68 | 65 | 113; 300 x 2560 x 8192 51 | 36 | 35 | 41,
+// 126 x 2048 x 16384 42 | 29 | 28 | 22, 8000 x 1024 x 1000 27 | 20 | 22 | 30.
+//
+// Buffers: what fits, but where two workgroups are to share a compute unit's LDS.
+// 128 tokens with 3 against 2: 200 x 4096 x 32000 64 against 76 us, 64 x 4096 x
+// 128256 178 against 200, at the worst (1000 x 1024 x 2000) 17.9 against 17.2.
+// 32 tokens with 4 against 2, at one tile a unit: 64 x 4096 x 32000 47 against 59
+// us, 126 x 2048 x 16384 22 against 26, 126 x 512 x 4096 (a weight that stays in
+// L2) 8.8 against 8.4.  With two tiles a unit, 4 buffers cost what the second
+// tile gives: 200 x 4096 x 32000 138 against 113 us.
 struct TileKind {
     uint32_t tokens, slots;
     float round, half, brief, brief_half;
 };
 constexpr TileKind kTileKinds[] = {
     {256, 256, 1.00f, 1.00f, 1.00f, 1.00f},
-    {128, 256, 0.75f, 0.75f, 0.60f, 0.60f},
+    {128, 256, 0.75f, 0.68f, 0.60f, 0.60f},
     {64, 512, 0.76f, 0.66f, 0.60f, 0.57f},
-    {32, 512, 0.78f, 0.60f, 0.60f, 0.50f},
+    {32, 512, 0.78f, 0.53f, 0.60f, 0.50f},
 };
 
 template <typename Fmt>
@@ -624,18 +645,19 @@ int dispatch_tiles(const Tiles& a, hipStream_t st) {
     const uint64_t spans = (a.vocab + kSpan - 1) / kSpan;
     const bool brief = a.steps * kTerms < 2048;
     uint32_t best = 0;
+    bool alone = false;
     float least = 0.0f;
     for (const TileKind& k : kTileKinds) {
         const uint64_t tiles = spans * ((a.tokens + k.tokens - 1) / k.tokens);
         const float one = tiles <= 256 ? (brief ? k.brief_half : k.half) : brief ? k.brief : k.round;
         const float time = one * float((tiles + k.slots - 1) / k.slots);
-        if (best == 0 || time < least) best = k.tokens, least = time;
+        if (best == 0 || time < least) best = k.tokens, least = time, alone = tiles <= 256;
     }
     switch (best) {
-        case 32: return launch_tiles<Fmt, 4, 1, 4, 2>(a, st);
-        case 64: return launch_tiles<Fmt, 4, 1, 4, 4>(a, st);
-        case 128: return launch_tiles<Fmt, 4, 2, 4, 4>(a, st);
-        default: return launch_tiles<Fmt, 2, 4, 8, 4>(a, st);
+        case 32: return alone ? launch_tiles<Fmt, 4, 1, 4, 2, 4>(a, st) : launch_tiles<Fmt, 4, 1, 4, 2, 2>(a, st);
+        case 64: return launch_tiles<Fmt, 4, 1, 4, 4, 2>(a, st);
+        case 128: return launch_tiles<Fmt, 4, 2, 4, 4, 3>(a, st);
+        default: return launch_tiles<Fmt, 2, 4, 8, 4, 2>(a, st);
     }
 }
 

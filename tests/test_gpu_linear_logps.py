@@ -237,6 +237,13 @@ def test_every_tile(dev, shape, dtype):
     test_matches_float64(dev, shape, dtype)
 
 
+@pytest.mark.parametrize("terms", [2, 3, 4, 5, 6, 9])
+@pytest.mark.parametrize("tokens,words", [(40, 700), (33, 66_000), (100, 4200), (120, 33_000)])
+def test_sums_shorter_and_longer_than_the_buffers(dev, terms, tokens, words):
+    """Every tile with fewer, as many and more 64-term steps than it has buffers."""
+    test_matches_float64(dev, (tokens, 64 * terms, words), torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("shape", [(70, 64, 300), (300, 128, 40_000)])
 def test_tokens_without_a_gradient_may_hold_anything(dev, shape, dtype):
