@@ -3,7 +3,11 @@
 //
 // Both read every token once and write its gradient once.  As separate
 // elementwise and reduction operations, forward and backward, they are some 30
-// to 60 launches.  The sums are taken in fp32 by each lane over its few tokens
+// to 60 launches; here they are two or three, and the host's time for a forward
+// and a backward, 50 to 65 us with autograd's, is what bounds a call.  On the
+// device, parts | join | gradient, us: preference, 128 x 8191 tokens 3.7 | 4.0 |
+// 3.5, 9.4 MB and 5.2 MB; policy, 256 x 8191 with every input 9.6 | 4.1 | 4.8, 44
+// MB, 4.6 TB/s, and 17 MB.  The sums are taken in fp32 by each lane over its few tokens
 // and in fp64 from there on, in an order fixed by the shape alone: no atomics.
 // Masked tokens are selected away before any arithmetic, so NaN and infinities
 // there reach neither a sum nor a gradient.
@@ -115,21 +119,25 @@ __device__ __forceinline__ void ratio_sum(const Pref& a, uint64_t row, uint32_t 
 // log(1 + exp(-x)) for any x: -log sigmoid(x).
 __device__ __forceinline__ double softplus_neg(double x) { return fmax(-x, 0.0) + log1p(exp(-fabs(x))); }
 
-// The pairs' losses from the rows' sums, by one workgroup.  part(row, k): the
-// k-th part's sum and count.
-template <int kT, typename Part>
-__device__ __forceinline__ void pref_join(const Pref& a, const PrefOut& o, Part part, double* waves) {
+// The pairs' losses from the rows' sums, by one workgroup, kN lanes to a pair.
+template <int kN>
+__device__ __forceinline__ void pref_join(const Pref& a, const PrefOut& o, const double2* parts, double* waves) {
     double loss[1] = {0.0};
     const double beta = a.beta, e = a.smooth;
-    for (uint32_t p = threadIdx.x; p < a.pairs; p += kT) {
+    const uint32_t lane = threadIdx.x % kN;
+    for (uint32_t p = threadIdx.x / kN; p < a.pairs; p += kSoloThreads / kN) {
         double r[2], scale[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
+            const double2* row = parts + (p + w * uint64_t(a.pairs)) * a.splits;
             double sum = 0.0, count = 0.0;
-            for (uint32_t k = 0; k < a.splits; ++k) part(p + w * uint64_t(a.pairs), k, sum, count);
+            for (uint32_t k = lane; k < a.splits; k += kN) sum += row[k].x, count += row[k].y;
+            sum = lane_sum<kN>(sum);
+            count = lane_sum<kN>(count);
             scale[w] = a.average ? 1.0 / fmax(count, 1.0) : 1.0;
             r[w] = sum * scale[w];
         }
+        if (lane != 0) continue;
         const double gap = r[0] - r[1], x = beta * gap;
         double term, slope;   // and its derivative by the gap
         if (a.form == SF_PREF_SIGMOID) {
@@ -153,7 +161,7 @@ __device__ __forceinline__ void pref_join(const Pref& a, const PrefOut& o, Part 
             o.coef[uint64_t(a.pairs) + p] = float(-slope * scale[1] / a.pairs);
         }
     }
-    block_sums<1, kT>(loss, waves);
+    block_sums<1, kSoloThreads>(loss, waves);
     if (threadIdx.x == 0) *o.loss = float(loss[0] / a.pairs);
 }
 
@@ -166,10 +174,7 @@ __global__ __launch_bounds__(kSoloThreads) void pref_solo_kernel(Pref a, PrefOut
         if ((threadIdx.x & 63) == 0) parts[r] = double2{s, n};
     }
     __syncthreads();
-    pref_join<kSoloThreads>(a, o, [&](uint64_t r, uint32_t, double& s, double& n) {
-        s += parts[r].x;
-        n += parts[r].y;
-    }, waves);
+    pref_join<1>(a, o, parts, waves);
 }
 
 // A row's parts by a workgroup each.
@@ -191,13 +196,10 @@ __global__ __launch_bounds__(kThreads) void pref_parts_kernel(Pref a, uint32_t p
     }
 }
 
+template <int kN>
 __global__ __launch_bounds__(kSoloThreads) void pref_join_kernel(Pref a, PrefOut o, const double2* __restrict__ parts) {
     __shared__ double waves[kSoloThreads / 64];
-    pref_join<kSoloThreads>(a, o, [&](uint64_t r, uint32_t k, double& s, double& n) {
-        const double2 v = parts[r * a.splits + k];
-        s += v.x;
-        n += v.y;
-    }, waves);
+    pref_join<kN>(a, o, parts, waves);
 }
 
 // ---------------------------------------------------------------------
@@ -296,15 +298,20 @@ __device__ __forceinline__ Sums policy_sums(const Policy& a, const PolicyOut& o,
     return {{lane_sum<64>(term), lane_sum<64>(kl), lane_sum<64>(double(clipped)), lane_sum<64>(double(tokens))}};
 }
 
-// The loss from the rows' sums, by one workgroup.
-template <int kT>
+// The loss from the rows' sums, by one workgroup, kN lanes to a row.
+template <int kN>
 __device__ __forceinline__ void policy_join(const Policy& a, const PolicyOut& o, const Sums* parts, double* waves) {
     double total[kSums] = {0.0, 0.0, 0.0, 0.0};
-    for (uint32_t r = threadIdx.x; r < a.rows; r += kT) {
+    const uint32_t lane = threadIdx.x % kN;
+    for (uint32_t r = threadIdx.x / kN; r < a.rows; r += kSoloThreads / kN) {
+        const Sums* row = parts + uint64_t(r) * a.splits;
         double x[kSums] = {0.0, 0.0, 0.0, 0.0};
-        for (uint32_t k = 0; k < a.splits; ++k)
+        for (uint32_t k = lane; k < a.splits; k += kN)
 #pragma unroll
-            for (int j = 0; j < kSums; ++j) x[j] += parts[uint64_t(r) * a.splits + k].x[j];
+            for (int j = 0; j < kSums; ++j) x[j] += row[k].x[j];
+#pragma unroll
+        for (int j = 0; j < kSums; ++j) x[j] = lane_sum<kN>(x[j]);
+        if (lane != 0) continue;
         if (a.sequences) {
             const double n = x[3];
             if (n > 0.0) {
@@ -316,7 +323,7 @@ __device__ __forceinline__ void policy_join(const Policy& a, const PolicyOut& o,
 #pragma unroll
         for (int j = 0; j < kSums; ++j) total[j] += x[j];
     }
-    block_sums<kSums, kT>(total, waves);
+    block_sums<kSums, kSoloThreads>(total, waves);
     const double n = total[3];
     if (threadIdx.x == 0) {   // 0 / 0 where there is no token at all
         *o.loss = float(total[0] / n);
@@ -324,14 +331,15 @@ __device__ __forceinline__ void policy_join(const Policy& a, const PolicyOut& o,
         *o.clipped = float(total[2] / n);
     }
     if (o.weight == nullptr) return;
-    for (uint32_t r = threadIdx.x; r < a.rows; r += kT) {
+    for (uint32_t r = threadIdx.x / kN; r < a.rows; r += kSoloThreads / kN) {
         double own = 1.0;
         if (a.sequences) {
             own = 0.0;
-            for (uint32_t k = 0; k < a.splits; ++k) own += parts[uint64_t(r) * a.splits + k].x[3];
+            for (uint32_t k = lane; k < a.splits; k += kN) own += parts[uint64_t(r) * a.splits + k].x[3];
+            own = lane_sum<kN>(own);
         }
         // a row without tokens has slopes of 0 alone
-        o.weight[r] = own > 0.0 && n > 0.0 ? float(1.0 / (own * n)) : 0.0f;
+        if (lane == 0) o.weight[r] = own > 0.0 && n > 0.0 ? float(1.0 / (own * n)) : 0.0f;
     }
 }
 
@@ -342,7 +350,7 @@ __global__ __launch_bounds__(kSoloThreads) void policy_solo_kernel(Policy a, Pol
         if ((threadIdx.x & 63) == 0) parts[r] = s;
     }
     __syncthreads();
-    policy_join<kSoloThreads>(a, o, parts, waves);
+    policy_join<1>(a, o, parts, waves);
 }
 
 __global__ __launch_bounds__(kThreads) void policy_parts_kernel(Policy a, PolicyOut o, uint32_t per, uint64_t first,
@@ -362,9 +370,10 @@ __global__ __launch_bounds__(kThreads) void policy_parts_kernel(Policy a, Policy
     }
 }
 
+template <int kN>
 __global__ __launch_bounds__(kSoloThreads) void policy_join_kernel(Policy a, PolicyOut o, const Sums* __restrict__ parts) {
     __shared__ double waves[kSums * kSoloThreads / 64];
-    policy_join<kSoloThreads>(a, o, parts, waves);
+    policy_join<kN>(a, o, parts, waves);
 }
 
 // ---------------------------------------------------------------------
@@ -401,20 +410,33 @@ __global__ __launch_bounds__(kThreads) void policy_grad_kernel(const float* __re
         if (t + k * kThreads < cols) g[t + k * kThreads] = s[t + k * kThreads] * w;
 }
 
-// Up to here one workgroup takes a whole call, in one launch.
-constexpr uint64_t kSoloTokens = 16384;
+// Parts of a row that one lane of the join adds up; more take a wave.  Parts and
+// join together, preference | policy, us, a lane against a wave for a row: 100
+// rows of 10 parts 8.5 | 10.6, 17.0 | 25.0; 64 of 16 9.5 | 11.5, 13.5 | 19.9; 32
+// of 32 12.1 | 13.5, 10.1 | 14.9; 2 of 512 95 | 69, 10.9 | 11.4.
+constexpr uint32_t kLaneParts = 24;
 
 constexpr uint64_t kMaxBlocks = kMaxLanes / kThreads;
 
 // Tokens of one part: a row is divided so that there are some 1,024 parts, each
-// of 1,024 tokens or more.
+// of 1,024 tokens or more.  us, preference | policy, at this, half and twice as
+// many: 256 rows of 8191 7.9 | 13.9 (2,048 tokens), 9.3 | 15.9, 8.0 | 16.5; 128
+// of 8191 8.0 | 10.6 (1,024 tokens) and, twice as many, 7.1 | 10.7.
 uint32_t part_tokens(uint64_t rows, uint64_t cols) {
     const uint64_t want = (1024 + rows - 1) / rows;
     uint64_t per = (cols + want - 1) / want;
     per = (per + 1023) / 1024 * 1024;
     return uint32_t(per);
 }
-bool solo(uint64_t rows, uint64_t cols) { return rows * cols <= kSoloTokens; }
+
+// Whether one workgroup takes a whole call, in one launch: where each of its waves
+// has 512 tokens or fewer.  us, preference | policy, in one launch and in two,
+// without the host's 3 for the second: 8 x 128 4.0 | 6.6 and 5.6 | 7.4, 8 x 512
+// 4.7 | 8.6 and 5.8 | 8.0, 4 x 2048 7.3 | 17.8 and 6.0 | 8.1.
+bool solo(uint64_t rows, uint64_t cols) {
+    constexpr uint64_t kWaves = kSoloThreads / 64;
+    return (rows + kWaves - 1) / kWaves * ((cols + 255) / 256) <= 2;
+}
 
 bool sizes_bad(size_t rows, size_t cols) {
     return rows == 0 || cols == 0 || rows > (size_t(1) << 30) || cols > (size_t(1) << 30);
@@ -460,7 +482,7 @@ int sf_pref_loss(const float* logps, size_t ld, const float* ref, size_t ld_ref,
         const int e = status();
         if (e != SF_OK) return e;
     }
-    hipLaunchKernelGGL(pref_join_kernel, dim3(1), dim3(kSoloThreads), 0, st, a, o, p);
+    hipLaunchKernelGGL(a.splits > kLaneParts ? pref_join_kernel<64> : pref_join_kernel<1>, dim3(1), dim3(kSoloThreads), 0, st, a, o, p);
     return status();
 }
 
@@ -513,7 +535,7 @@ int sf_policy_loss(const float* logps, size_t ld, const float* old_logps, size_t
         const int e = status();
         if (e != SF_OK) return e;
     }
-    hipLaunchKernelGGL(policy_join_kernel, dim3(1), dim3(kSoloThreads), 0, st, a, o, p);
+    hipLaunchKernelGGL(a.splits > kLaneParts ? policy_join_kernel<64> : policy_join_kernel<1>, dim3(1), dim3(kSoloThreads), 0, st, a, o, p);
     return status();
 }
 

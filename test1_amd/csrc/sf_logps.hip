@@ -403,7 +403,11 @@ __global__ __launch_bounds__(kJoinThreads) void logps_join_kernel(const float2* 
 
 // ---------------------------------------------------------------------
 // fp32 logits that a library product has left: kT lanes per row, one pass, each
-// lane with its own running maximum and sum.
+// lane with its own running maximum and sum.  Bound by the read, 4.9 to 6.5 TB/s
+// (part of it from cache) from 1,000 words on.  us at 16 | 64 | 256 | 1024 lanes,
+// 1 GiB of logits: 512 words 180 | 308 | 967 | 2924, 1024 189 | 174 | 686 | 1498,
+// 4096 193 | 180 | 188 | 617, 8192 206 | 187 | 167 | 317, 16384 192 | 196 | 178 |
+// 174, 32000 236 | 201 | 183 | 164; 64 rows of 16384 45 | 14 | 5.8 | 5.2.
 // ---------------------------------------------------------------------
 template <int kT>
 __global__ __launch_bounds__(kT * kRowsOf<kT>) void logps_rows_kernel(const float* __restrict__ logits, uint64_t ld,
@@ -780,8 +784,8 @@ int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab, con
     if (misaligned(logits, 16) || ld % 4 != 0) return SF_EALIGN;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const uint32_t v = uint32_t(vocab);
-    if (v <= 256) return launch_rows<16>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
-    if (v <= 1024) return launch_rows<64>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
+    if (v <= 512) return launch_rows<16>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
+    if (v <= 4096) return launch_rows<64>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
     if (v <= 16384) return launch_rows<256>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
     return launch_rows<1024>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
 }

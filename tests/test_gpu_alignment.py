@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 # one workgroup up to 16,384 tokens; beyond, parts of 1,024 tokens or a multiple
 SHAPES = [(2, 1), (2, 2), (4, 63), (2, 64), (6, 257), (2, 8192), (2, 8193), (64, 255), (66, 250), (2, 16385), (1026, 33),
-          (10, 5000), (2, 1_100_001)]
+          (10, 5000), (2, 1_100_001), (16, 512), (32, 256), (18, 300), (12, 50_000)]
 
 
 def tokens(shape, dev, seed=0, empty_rows=True):
