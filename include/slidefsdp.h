@@ -342,8 +342,7 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab,
 /* The gradient of such logits is row_weight[i] * D[i, j], D = ((j == label) -
  * p) / (1 - p_label): 1 at the label.  row_weight = grad * scale * (1 -
  * p_label); 0 for an ignored row or a grad of 0, NaN for a label outside [0,
- * vocab).  norm (or
- * null: 1): two floats; the weights are then divided by the power of two
+ * vocab).  norm (or null: 1): two floats; the weights are then divided by the power of two
  * norm[0] that leaves the largest in [1, 2), and norm[1] = 1. */
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
                     int64_t ignore_index, size_t rows, size_t vocab,
@@ -364,9 +363,21 @@ int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
                        size_t all_rows, float scale, float* row_weight,
                        float* norm, int normalise, sf_stream_t stream);
 
+/* out[i, j] = row_weight[i] * sum over words k of d[i, k] * weight[k, j], rounded
+ * once, 0 where the weight is, times norm[0] where norm is not null: the hidden
+ * gradient from D of 16-bit elements, for few rows.  d holds whole 16 rows and
+ * zeros from vocab up to the next multiple of 32 columns; out is contiguous, and
+ * cols, ld and ldw are multiples of 8, d and weight aligned to 16 bytes, out to
+ * 8 (SF_EALIGN). */
+int sf_logps_hidden_grad(const void* d, size_t ld, size_t rows,
+                         const void* weight, size_t ldw, size_t vocab,
+                         size_t cols, const float* row_weight,
+                         const float* norm, int dtype, void* out,
+                         sf_stream_t stream);
+
 /* D of fp32 logits (as sf_logps_rows takes them, with its lse and logp; 0 in
- * rows whose grad is 0), as dtype with ld_dz elements from row to row.  SF_DTYPE_F32: dz may be the
- * logits themselves; other types: no overlap. */
+ * rows whose grad is 0), as dtype with ld_dz elements from row to row.
+ * SF_DTYPE_F32: dz may be the logits themselves; other types: no overlap. */
 int sf_logps_grad(const float* logits, size_t ld, size_t rows, size_t vocab,
                   const int64_t* labels, int64_t ignore_index, float scale,
                   const float* lse, const float* logp, const float* grad,

@@ -517,9 +517,11 @@ __global__ __launch_bounds__(kWeightThreads) void logps_weight_kernel(const Weig
 
 // D from what the product kept, in place.  A workgroup takes 4,096 words of a
 // token, 16 bytes at a time.  A token without a gradient of its own, masked ones
-// above all, has D = 0 whatever its hidden states hold, and is not read; rows from `tokens` on are cleared (they pad the
-// weight gradient's sum).  The launch's first `others` workgroups make the rows'
-// weights, which nothing here needs.
+// above all, has D = 0 whatever its hidden states hold, and is not read; rows
+// from `tokens` on are cleared (they pad the weight gradient's sum).  The launch's
+// first `others` workgroups make the rows' weights, which nothing here needs.
+// Bound by its bytes, 2.1 GB at 4092 tokens of 128256 words: 0.32 ms with all of
+// them, 6.6 TB/s, part of it from the last-level cache.
 constexpr int kGradThreads = 256;
 constexpr int kKeepColumns = kGradThreads * kGroup * 2;
 template <typename Fmt>
@@ -561,6 +563,91 @@ __global__ __launch_bounds__(kGradThreads) void logps_keep_grad_kernel(uint16_t*
         // over what this lane has just stored
         if (uint64_t(y) - c < uint64_t(kGroup)) k[y] = uint16_t(Fmt::pack(1.0f, 0.0f));
     }
+}
+
+// The hidden gradient of a few tokens, row weight * (D W), in one launch.  A
+// workgroup takes 16 tokens and 128 of the hidden dimensions, its waves the words
+// in turns of 32.  The words are the sum's dimension here and W's rows lie along
+// the other: a lane reads 8 neighbouring dimensions of 8 words and turns them
+// around in registers, so that its operand for dimension j of the 8 is one
+// register from each pair of words, and it ends up with 8 neighbours of a token.
+// No LDS but for the waves' sums.
+constexpr int kHgWaves = 8;
+constexpr int kHgTokens = 16;
+constexpr int kHgColumns = 128;
+template <typename Fmt>
+__global__ __launch_bounds__(kHgWaves * 64, 2) void logps_hidden_grad_kernel(
+    const uint16_t* __restrict__ d, uint64_t ld, uint32_t tokens, const uint16_t* __restrict__ weight, uint64_t ldw,
+    uint32_t vocab, uint32_t cols, uint32_t col_blocks, const float* __restrict__ by, const float* __restrict__ norm,
+    uint16_t* __restrict__ out) {
+    constexpr uint32_t kWords = 32;
+    __shared__ float sums[kHgWaves][32][64];
+    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t token0 = blockIdx.x / col_blocks * kHgTokens;
+    const uint32_t col = blockIdx.x % col_blocks * kHgColumns + l16 * 8;
+    const uint32_t from = col < cols ? col : 0;   // columns past the last are not stored
+    const uint16_t* dp = d + uint64_t(token0 + l16) * ld;
+
+    struct Words {
+        u32x4 d, w[8];
+    };
+    const auto load = [&](uint32_t v) {
+        Words x;
+        v += quad * 8;
+        x.d = *reinterpret_cast<const u32x4*>(dp + v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x.w[i] = v + i < vocab ? *reinterpret_cast<const u32x4*>(weight + (v + i) * ldw + from) : u32x4{0, 0, 0, 0};
+        return x;
+    };
+    f32x4 acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto add = [&](const Words& x) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            u32x4 b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                b[i] = __builtin_amdgcn_perm(x.w[2 * i + 1][j / 2], x.w[2 * i][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+            acc[j] = mfma(Fmt{}, x.d, b, acc[j]);
+        }
+    };
+    // the next words are on their way while these are used (four turns on their way:
+    // 250 x 1024 x 16384 42 -> 38 us, twice the registers, and no less for a call)
+    constexpr uint32_t kTurn = kHgWaves * kWords;
+    uint32_t v = wave * kWords;
+    if (v < vocab) {
+        Words x = load(v);
+        for (; v + kTurn < vocab; v += kTurn) {
+            const Words next = load(v + kTurn);
+            add(x);
+            x = next;
+        }
+        add(x);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[wave][j * 4 + i][lane] = acc[j][i];
+    __syncthreads();
+    // a wave takes one of a lane's four tokens and half of its columns
+    static_assert(kHgWaves == 8, "four tokens, two halves");
+    const uint32_t i = wave / 2, j0 = wave % 2 * 4, token = token0 + quad * 4 + i;
+    f32x4 t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float s[kHgWaves];
+#pragma unroll
+        for (int w = 0; w < kHgWaves; ++w) s[w] = sums[w][(j0 + j) * 4 + i][lane];
+        t[j] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    }
+    if (token >= tokens || col >= cols) return;
+    const float f = by[token];
+    t = f == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : t * f * (norm != nullptr ? *norm : 1.0f);
+    uint32_t* o = reinterpret_cast<uint32_t*>(out + uint64_t(token) * cols + col + j0);
+    o[0] = Fmt::pack(t[0], t[1]), o[1] = Fmt::pack(t[2], t[3]);
 }
 
 // D from fp32 logits; a workgroup takes 1,024 words of a row.
@@ -788,6 +875,26 @@ int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab, con
     if (v <= 4096) return launch_rows<64>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
     if (v <= 16384) return launch_rows<256>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
     return launch_rows<1024>(logits, ld, rows, v, labels, ignore_index, scale, lse, logp, st);
+}
+
+int sf_logps_hidden_grad(const void* d, size_t ld, size_t rows, const void* weight, size_t ldw, size_t vocab, size_t cols,
+                         const float* row_weight, const float* norm, int dtype, void* out, sf_stream_t stream) {
+    if (rows == 0) return SF_OK;
+    if (d == nullptr || weight == nullptr || row_weight == nullptr || out == nullptr || sizes_bad(rows, vocab) ||
+        cols == 0 || cols > (size_t(1) << 22) || ld < (vocab + 31) / 32 * 32 || ldw < cols)
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (cols % 8 != 0 || ld % 8 != 0 || ldw % 8 != 0 || misaligned(d, 16) || misaligned(weight, 16) || misaligned(out, 8))
+        return SF_EALIGN;
+    const uint64_t col_blocks = (cols + kHgColumns - 1) / kHgColumns;
+    const uint64_t blocks = (uint64_t(rows) + kHgTokens - 1) / kHgTokens * col_blocks;
+    if (blocks > kMaxLanes / (kHgWaves * 64)) return SF_EINVAL;
+    const auto kernel = dtype == SF_DTYPE_BF16 ? logps_hidden_grad_kernel<Bf16> : logps_hidden_grad_kernel<F16>;
+    hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(kHgWaves * 64), 0, reinterpret_cast<hipStream_t>(stream),
+                       static_cast<const uint16_t*>(d), uint64_t(ld), uint32_t(rows),
+                       static_cast<const uint16_t*>(weight), uint64_t(ldw), uint32_t(vocab), uint32_t(cols),
+                       uint32_t(col_blocks), row_weight, norm, static_cast<uint16_t*>(out));
+    return status();
 }
 
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels, int64_t ignore_index, size_t rows,

@@ -319,6 +319,15 @@ bool own_weight_grad(int64_t n, int64_t h, int64_t v, bool fp16) {
     return n <= 256 && (fp16 || n * h * v <= int64_t(1) << 32);
 }
 
+// Whether the hidden gradient of a call in one piece is formed by
+// sf_logps_hidden_grad instead of a library's product and a scaling: where the
+// host's time for those, 18 to 22 us more, is longer.  Whole calls with this
+// gradient, us, product | kernel: 126 x 512 x 4096 60 | 43, 64 x 1024 x 8192 63 |
+// 49, 250 x 4096 x 4096 95 | 74; not with more to do, 1000 x 2048 x 4096 94 | 95,
+// 2000 x 4096 x 1000 97 | 122, nor with more words for a workgroup, 128 x 2048 x
+// 16384 86 | 85, 32 x 2048 x 32000 61 | 142.
+bool own_hidden_grad(int64_t n, int64_t h, int64_t v) { return v <= 8192 && n * h * v <= int64_t(1) << 32; }
+
 // Both gradients (undefined where not needed).  What was kept turns into the
 // gradient of the logits in place; without it, it is made again, `step` rows at
 // a time.
@@ -354,7 +363,11 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
                                  type, at_ptr<float>(grad) + s, s == 0 ? n : 0, float(a.scale), at_ptr<float>(by),
                                  at_ptr<float>(norm), fp16, st),
               "sf_logps_keep_grad");
-        if (need_hidden)
+        if (need_hidden && one && own_hidden_grad(n, h, v))
+            check(sf_logps_hidden_grad(keep.data_ptr(), row, n, weight.data_ptr(), weight.stride(0), v, h,
+                                       at_ptr<float>(by), fp16 ? at_ptr<float>(norm) : nullptr, type, gh.data_ptr(), st),
+                  "sf_logps_hidden_grad");
+        else if (need_hidden)
             hidden_product(keep, m, weight, a.nparts, at_ptr<float>(by) + s, fp16 ? norm : Tensor(),
                            one ? gh : gh.narrow(0, s, m));
         if (!need_weight) continue;

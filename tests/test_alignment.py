@@ -141,6 +141,12 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert hip.sf_logps_keep_grad(one, 264, 1, 1, 8, one, one, -100, one, one, 1, *none) == 9007
     assert hip.sf_logps_keep_grad(one, 256, 2, 2, 8, one, one, -100, one, one, 1, one, 1, 1.0, one, None, 0, None) == 9001
     assert hip.sf_logps_keep_grad(one, 256, 1, 1, 8, one, one, -100, one, one, 1, one, 1, 1.0, one, None, 1, None) == 9001
+    grad = lambda **k: hip.sf_logps_hidden_grad(*{**dict(d=one, ld=32, n=1, w=one, ldw=8, v=8, h=8, by=one, s=None, t=1,  # noqa: E731
+                                                         o=one, st=None), **k}.values())
+    assert grad(n=0) == 0
+    assert grad(d=None) == grad(w=None) == grad(by=None) == grad(o=None) == grad(v=0) == grad(h=0) == 9001
+    assert grad(ld=31) == grad(ldw=7) == grad(n=1 << 31) == 9001 and grad(t=0) == grad(t=5) == 9003
+    assert grad(ld=36) == grad(ldw=12) == grad(h=4) == 9007
     assert hip.sf_logps_hidden(one, 8, 1, 8, None, 1, one, 64, None) == hip.sf_logps_hidden(one, 8, 1, 8, one, 1, one, 32, None) == 9001
     assert hip.sf_logps_sum(one, 3, 1, 8, one, 1, None, 0, None, 0, one, None, None) == 9001
     assert hip.sf_align_parts(0, 5) == 0 and hip.sf_align_parts(4, 100) == 4
