@@ -389,6 +389,13 @@ int sf_logps_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols,
                     const float* row_weight, int dtype, void* hidden_t,
                     size_t ldt, sf_stream_t stream);
 
+/* out[i, j] = row_weight[i] * hidden[i, j] of 16-bit elements, rounded once, 0
+ * where the weight is; out is contiguous.  cols and ldh are multiples of 8, both
+ * aligned to 16 bytes (SF_EALIGN). */
+int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols,
+                      const float* row_weight, int dtype, void* out,
+                      sf_stream_t stream);
+
 /* As sf_ce_sum, also of one part, each row times row_weight[i], 0 where that
  * is, and times norm[0] where norm is not null. */
 int sf_logps_sum(const float* parts, int nparts, size_t rows, size_t cols,

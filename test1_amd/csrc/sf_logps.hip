@@ -650,6 +650,27 @@ __global__ __launch_bounds__(kHgWaves * 64, 2) void logps_hidden_grad_kernel(
     o[0] = Fmt::pack(t[0], t[1]), o[1] = Fmt::pack(t[2], t[3]);
 }
 
+// Rows times their weights, 0 where that is whatever the row holds.  Bound by its
+// bytes; as separate operations it is three launches.
+template <typename Fmt>
+__global__ __launch_bounds__(kGradThreads) void logps_weighted_kernel(const uint16_t* __restrict__ hidden, uint64_t ldh,
+                                                                      uint32_t groups, uint32_t cols, uint64_t first,
+                                                                      uint64_t count, const float* __restrict__ by,
+                                                                      uint16_t* __restrict__ out) {
+    const uint64_t i = (first + blockIdx.x) * kGradThreads + threadIdx.x;
+    if (i >= count) return;
+    const uint64_t row = i / groups;
+    const uint32_t col = uint32_t(i - row * groups) * kGroup;
+    const float f = by[row];
+    u32x4 o = {0, 0, 0, 0};
+    if (f != 0.0f) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(hidden + row * ldh + col);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = Fmt::pack(Fmt::lo(v[j]) * f, Fmt::hi(v[j]) * f);
+    }
+    *reinterpret_cast<u32x4*>(out + row * cols + col) = o;
+}
+
 // D from fp32 logits; a workgroup takes 1,024 words of a row.
 constexpr int kGradColumns = 1024;
 struct Out32 {
@@ -895,6 +916,22 @@ int sf_logps_hidden_grad(const void* d, size_t ld, size_t rows, const void* weig
                        static_cast<const uint16_t*>(weight), uint64_t(ldw), uint32_t(vocab), uint32_t(cols),
                        uint32_t(col_blocks), row_weight, norm, static_cast<uint16_t*>(out));
     return status();
+}
+
+int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols, const float* row_weight, int dtype, void* out,
+                      sf_stream_t stream) {
+    if (rows == 0) return SF_OK;
+    if (hidden == nullptr || row_weight == nullptr || out == nullptr || sizes_bad(rows, cols) || ldh < cols)
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (cols % kGroup != 0 || ldh % kGroup != 0 || misaligned(hidden, 16) || misaligned(out, 16)) return SF_EALIGN;
+    const auto kernel = dtype == SF_DTYPE_BF16 ? logps_weighted_kernel<Bf16> : logps_weighted_kernel<F16>;
+    const uint64_t count = uint64_t(rows) * (cols / kGroup);
+    return in_launches((count + kGradThreads - 1) / kGradThreads, [&](uint64_t first, uint32_t blocks) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kGradThreads), 0, reinterpret_cast<hipStream_t>(stream),
+                           static_cast<const uint16_t*>(hidden), uint64_t(ldh), uint32_t(cols / kGroup), uint32_t(cols),
+                           first, count, row_weight, static_cast<uint16_t*>(out));
+    });
 }
 
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels, int64_t ignore_index, size_t rows,

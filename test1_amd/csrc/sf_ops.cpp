@@ -373,9 +373,9 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
         if (!need_weight) continue;
         if (fp16 && !few) {
             // into fp32, of rows as they lie: 4096 x 4096 x 128256 4.2 ms, of transposed ones 28.8
-            Tensor weighted = at::empty({m, h}, hidden.options());
-            const Tensor f = by.narrow(0, s, m).unsqueeze(1);
-            at::mul_out(weighted, hc.masked_fill(f == 0, 0), f);
+            const Tensor weighted = at::empty({m, h}, hidden.options());
+            check(sf_logps_weighted(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, weighted.data_ptr(), st),
+                  "sf_logps_weighted");
             const Tensor dt = keep.as_strided({v, m}, {1, row});
             if (s == 0) at::mm_out(gw, dt, weighted, at::kFloat);
             else at::addmm_out(gw, gw, dt, weighted, at::kFloat);

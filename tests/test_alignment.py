@@ -147,6 +147,9 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert grad(d=None) == grad(w=None) == grad(by=None) == grad(o=None) == grad(v=0) == grad(h=0) == 9001
     assert grad(ld=31) == grad(ldw=7) == grad(n=1 << 31) == 9001 and grad(t=0) == grad(t=5) == 9003
     assert grad(ld=36) == grad(ldw=12) == grad(h=4) == 9007
+    rows = lambda h=one, ld=8, n=1, k=8, w=one, t=2, o=one: hip.sf_logps_weighted(h, ld, n, k, w, t, o, None)  # noqa: E731
+    assert rows(n=0) == 0 and rows(h=None) == rows(w=None) == rows(o=None) == rows(k=0) == rows(ld=0) == 9001
+    assert rows(t=0) == 9003 and rows(ld=12) == rows(k=4) == rows(h=72) == 9007
     assert hip.sf_logps_hidden(one, 8, 1, 8, None, 1, one, 64, None) == hip.sf_logps_hidden(one, 8, 1, 8, one, 1, one, 32, None) == 9001
     assert hip.sf_logps_sum(one, 3, 1, 8, one, 1, None, 0, None, 0, one, None, None) == 9001
     assert hip.sf_align_parts(0, 5) == 0 and hip.sf_align_parts(4, 100) == 4
