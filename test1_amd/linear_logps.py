@@ -25,8 +25,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .fused_ce import (_DTYPES, _PARTS_TILES, _PARTS_VOCAB, _PLAIN, _memory_is_value, _saved_plain, _tiles, _traced,
-                       _vocabulary_parts)
+from .fused_ce import _DTYPES, _PARTS_VOCAB, _PLAIN, _memory_is_value, _saved_plain, _tiles, _traced
 from .kernels import _CE_DTYPES
 
 
@@ -52,21 +51,29 @@ def _backward_rows(n: int, vocab: int) -> Tuple[int, bool]:
 
 
 def _hidden_parts(rows: int, weight: torch.Tensor) -> int:
-    """Parts in which the hidden gradient's product sums over the vocabulary: up
-    to 64 tiles of 256 x 256 by the rule of the fused output unit, beyond by how
-    well the tiles fill rounds of 256 compute units.  The library's product of
-    640 tiles (two and a half rounds) runs at 0.96 PFLOP/s, in two parts at
-    1.31; us, one product | parts, tokens x hidden x vocabulary: 8190 x 5120 x
-    152064 13264 | 9718 (2), 8190 x 2560 x 50257 2157 | 1715 (4), 3000 x 5120 x
-    32000 1136 | 796 (4), 4000 x 3584 x 152064 4838 | 3349 (8), 6500 x 2048 x
-    128256 4171 | 3181 (8), 5000 x 2048 x 50257 903 | 894 (8); adding the parts up
-    takes 10 to 100.  Whole rounds need none: 4092 x 4096 x 128256 3094 | 3105."""
+    """Parts in which the hidden gradient's product sums over the vocabulary.
+    The library sums each of its tiles in one workgroup, so up to 128 tiles of
+    256 x 256 as many parts as give every compute unit one, at most 16 and of
+    2000 words or more; us, one product | parts, tokens x hidden x vocabulary: 3
+    x 512 x 59040 107 | 20 (16), 32 x 768 x 50257 120 | 40 (16), 16 x 4096 x
+    128256 421 | 173 (16), 200 x 1024 x 32000 103 | 30 (16), 400 x 1024 x 16000
+    70 | 29 (8), 834 x 896 x 6640 45 | 30 (2), 1000 x 2048 x 32000 279 | 122 (8),
+    500 x 4096 x 128256 849 | 458 (8), 2000 x 2048 x 32000 388 | 212 (4).  Beyond
+    by how well the tiles fill rounds of 256 compute units: the product of 640
+    tiles (two and a half rounds) runs at 0.96 PFLOP/s, in two parts at 1.31;
+    8190 x 5120 x 152064 13264 | 9718 (2), 8190 x 2560 x 50257 2157 | 1715 (4),
+    3000 x 5120 x 32000 1136 | 796 (4), 4000 x 3584 x 152064 4838 | 3349 (8), 6500
+    x 2048 x 128256 4171 | 3181 (8), 5000 x 2048 x 50257 903 | 894 (8).  Adding the
+    parts up takes 5 to 100 in the launch that scales and rounds the sum.  Whole
+    rounds need none: 4092 x 4096 x 128256 3094 | 3105."""
     v, h = weight.shape
     tiles = _tiles(rows, h)
-    if tiles <= _PARTS_TILES:
-        return _vocabulary_parts(rows, weight)
-    if (tiles % 256 == 0 or v < _PARTS_VOCAB or weight.element_size() != 2 or h % 8 != 0 or not weight.is_contiguous()
+    if (tiles % 256 == 0 or v < 4000 or weight.element_size() != 2 or h % 8 != 0 or not weight.is_contiguous()
             or weight.data_ptr() % 16 != 0 or rows * h >= 1 << 31):
+        return 1
+    if tiles <= 128:
+        return max(p for p in (1, 2, 4, 8, 16) if p == 1 or tiles * p <= 256 and v >= 2000 * p)
+    if v < _PARTS_VOCAB:
         return 1
 
     def filled(parts: int) -> float:
