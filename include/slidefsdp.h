@@ -396,6 +396,19 @@ int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols,
                       const float* row_weight, int dtype, void* out,
                       sf_stream_t stream);
 
+/* Tokens that sf_logps_weight_grad takes at most. */
+#define SF_LOGPS_WEIGHT_TOKENS 256
+
+/* out[k, j] = sum over i of d[i, k] * hidden_t[j, i], times norm[0] where norm is
+ * not null, rounded once: the weight gradient of few tokens from D of 16-bit
+ * elements and what sf_logps_hidden leaves.  tokens: whole 64s, of d (ld
+ * elements from row to row) and of the contiguous [cols, tokens] hidden_t.  out
+ * is contiguous; cols is a multiple of 8, ld of 4, d aligned to 8 bytes, the
+ * others to 16 (SF_EALIGN). */
+int sf_logps_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab,
+                         const void* hidden_t, size_t cols, const float* norm,
+                         int dtype, void* out, sf_stream_t stream);
+
 /* As sf_ce_sum, also of one part, each row times row_weight[i], 0 where that
  * is, and times norm[0] where norm is not null. */
 int sf_logps_sum(const float* parts, int nparts, size_t rows, size_t cols,

@@ -650,6 +650,108 @@ __global__ __launch_bounds__(kHgWaves * 64, 2) void logps_hidden_grad_kernel(
     o[0] = Fmt::pack(t[0], t[1]), o[1] = Fmt::pack(t[2], t[3]);
 }
 
+// The weight gradient of up to 256 tokens, D^T times the weighted hidden rows: an
+// outer product with a short sum, which its output's bytes bound: 64 x 4096 x
+// 128256, 1.05 GB, 219 us, 4.8 TB/s (a fill of that size reaches 6.9), a library's
+// product 362; 256 x 4096 x 128256 288 | 464, 128 x 768 x 50257 20 | 31, 200 x 1024
+// x 32000 30 | 32.  A workgroup takes 256 words, each wave 64 with all their
+// tokens as operands in registers, and goes along the hidden dimensions 128 at a
+// time; the hidden rows of those, transposed, come through LDS in the order in
+// which lanes read them, the next ones while these are used.  The words of D lie
+// side by side, so a lane reads 4 of them of 8 tokens and turns them around; word
+// l and dimension l of an operand are 4 l + i and 8 l + j of the wave's 64 and
+// 128, so that a lane ends up with 8 neighbours of a word, 16 lanes with 256
+// bytes.  Over 128 tokens the operands take half of a wave's registers and the
+// dimensions go 64 at a time, which leaves room for a second workgroup: 256 x
+// 4096 x 128256 288 us, alone and 128 at a time 357.
+constexpr int kWgThreads = 256;
+constexpr int kWgTokens = SF_LOGPS_WEIGHT_TOKENS;
+constexpr int kWgWords = 256;
+template <int kSteps>   // tokens / 32, padded
+constexpr int kWgLane = kSteps > 4 ? 4 : 8;   // neighbouring dimensions of a lane
+template <typename Fmt, int kSteps>
+__global__ __launch_bounds__(kWgThreads, 2) void logps_weight_grad_kernel(
+    const uint16_t* __restrict__ d, uint64_t ld, uint32_t vocab, const uint16_t* __restrict__ hidden_t, uint32_t cols,
+    uint32_t runs, uint32_t per, const float* __restrict__ norm, uint16_t* __restrict__ out) {
+    constexpr uint32_t kTokens = kSteps * 32;
+    constexpr int kWaves = kWgThreads / 64, kFW = 4, kFH = kWgLane<kSteps>, kColumns = 16 * kFH;
+    using Piece = std::conditional_t<kFH == 8, u32x4, u32x2>;
+    constexpr int kPieces = kFH * kSteps;   // of 1 KB: an operand of a wave
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][kPieces * 1024];
+    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t word0 = blockIdx.x / runs * kWgWords + wave * 64;
+    const uint32_t first = blockIdx.x % runs * per, last = min(first + per, (cols + kColumns - 1) / kColumns);
+
+    typedef __attribute__((address_space(3))) uint8_t Lds;
+    typedef const __attribute__((address_space(1))) uint8_t Global;
+    // Rows past the last are the last one again and are not stored.
+    const auto copy = [&](uint32_t block, uint32_t buf) {
+#pragma unroll
+        for (int k = 0; k < kPieces / kWaves; ++k) {
+            const uint32_t piece = k * kWaves + wave, j = piece / kSteps, s = piece % kSteps;
+            const uint32_t row = min(block * kColumns + l16 * kFH + j, cols - 1);
+            __builtin_amdgcn_global_load_lds((Global*)(hidden_t + uint64_t(row) * kTokens + s * 32 + quad * 8),
+                                             (Lds*)(&lds[buf][piece * 1024]), 16, 0, 0);
+        }
+    };
+    const auto meet = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    copy(first, 0);
+    u32x4 a[kFW][kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        u32x2 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] = *reinterpret_cast<const u32x2*>(d + (s * 32 + quad * 8 + i) * ld + min(word0 + l16 * 4, uint32_t(ld) - 4));
+#pragma unroll
+        for (int w = 0; w < kFW; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                a[w][s][i] = __builtin_amdgcn_perm(x[2 * i + 1][w / 2], x[2 * i][w / 2], w % 2 ? 0x07060302u : 0x05040100u);
+    }
+    const float scale = norm != nullptr ? *norm : 1.0f;
+    meet();
+    for (uint32_t block = first; block < last; ++block) {
+        const uint32_t buf = (block - first) & 1;
+        if (block + 1 < last) copy(block + 1, buf ^ 1);
+        f32x4 acc[kFW][kFH];
+#pragma unroll
+        for (int w = 0; w < kFW; ++w)
+#pragma unroll
+            for (int j = 0; j < kFH; ++j) acc[w][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kFH; ++j)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const u32x4 b = *reinterpret_cast<const u32x4*>(&lds[buf][(j * kSteps + s) * 1024 + lane * 16]);
+#pragma unroll
+                for (int w = 0; w < kFW; ++w) acc[w][j] = mfma(Fmt{}, a[w][s], b, acc[w][j]);
+            }
+        // the next rows are there, and these are not read again
+        meet();
+        const uint32_t col = block * kColumns + l16 * kFH;
+        if (col >= cols) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < kFW; ++w) {
+                const uint32_t word = word0 + (quad * 4 + i) * 4 + w;
+                Piece o;
+#pragma unroll
+                for (int j = 0; j < kFH / 2; ++j) o[j] = Fmt::pack(acc[w][2 * j][i] * scale, acc[w][2 * j + 1][i] * scale);
+                if (word < vocab) *reinterpret_cast<Piece*>(out + uint64_t(word) * cols + col) = o;
+            }
+    }
+}
+
 // Rows times their weights, 0 where that is whatever the row holds.  Bound by its
 // bytes; as separate operations it is three launches.
 template <typename Fmt>
@@ -786,6 +888,37 @@ int launch_rows(const float* x, uint64_t ld, uint64_t rows, uint32_t vocab, cons
         if (e != SF_OK) return e;
     }
     return SF_OK;
+}
+
+template <typename Fmt, int kSteps>
+int launch_weight_grad(const void* d, size_t ld, size_t vocab, const void* hidden_t, size_t cols, const float* norm,
+                       void* out, hipStream_t st) {
+    // Runs along the hidden dimensions: what fits one round of two workgroups a
+    // compute unit, and with too many words for that 1,024 workgroups.  us at one
+    // round | two, 256 x 768 x 50257 30 | 40, 200 x 2048 x 50257 59 | 72; at about
+    // 500 | 1,000 | 1,500 workgroups, 64 x 4096 x 128256 239 | 262 | 219, 256 x 4096 x
+    // 128256 316 | 331 | 288.
+    constexpr uint32_t kColumns = 16 * kWgLane<kSteps>;
+    const uint32_t groups = uint32_t((vocab + kWgWords - 1) / kWgWords);
+    const uint32_t blocks = uint32_t((cols + kColumns - 1) / kColumns);
+    const uint32_t want = groups <= 256 ? 512 / groups : (1024 + groups - 1) / groups;
+    const uint32_t per = (blocks + want - 1) / want, runs = (blocks + per - 1) / per;
+    hipLaunchKernelGGL((logps_weight_grad_kernel<Fmt, kSteps>), dim3(groups * runs), dim3(kWgThreads), 0, st,
+                       static_cast<const uint16_t*>(d), uint64_t(ld), uint32_t(vocab),
+                       static_cast<const uint16_t*>(hidden_t), uint32_t(cols), runs, per, norm,
+                       static_cast<uint16_t*>(out));
+    return status();
+}
+
+template <typename Fmt>
+int dispatch_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab, const void* hidden_t, size_t cols,
+                         const float* norm, void* out, hipStream_t st) {
+    switch (tokens / 64) {
+        case 1: return launch_weight_grad<Fmt, 2>(d, ld, vocab, hidden_t, cols, norm, out, st);
+        case 2: return launch_weight_grad<Fmt, 4>(d, ld, vocab, hidden_t, cols, norm, out, st);
+        case 3: return launch_weight_grad<Fmt, 6>(d, ld, vocab, hidden_t, cols, norm, out, st);
+        default: return launch_weight_grad<Fmt, 8>(d, ld, vocab, hidden_t, cols, norm, out, st);
+    }
 }
 
 // kernel(first, blocks) in as many launches as `blocks` workgroups need.
@@ -932,6 +1065,19 @@ int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols, 
                            static_cast<const uint16_t*>(hidden), uint64_t(ldh), uint32_t(cols / kGroup), uint32_t(cols),
                            first, count, row_weight, static_cast<uint16_t*>(out));
     });
+}
+
+int sf_logps_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab, const void* hidden_t, size_t cols,
+                         const float* norm, int dtype, void* out, sf_stream_t stream) {
+    if (d == nullptr || hidden_t == nullptr || out == nullptr || sizes_bad(tokens, vocab) || tokens == 0 ||
+        tokens > kWgTokens || cols == 0 || cols > (size_t(1) << 22) || ld < vocab || ld > (size_t(1) << 31))
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (tokens % 64 != 0 || cols % 8 != 0 || ld % 4 != 0 || misaligned(d, 8) || misaligned(hidden_t, 16) || misaligned(out, 16))
+        return SF_EALIGN;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    return dtype == SF_DTYPE_BF16 ? dispatch_weight_grad<Bf16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st)
+                                  : dispatch_weight_grad<F16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st);
 }
 
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels, int64_t ignore_index, size_t rows,

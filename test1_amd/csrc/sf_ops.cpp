@@ -308,17 +308,6 @@ void hidden_product(const Tensor& keep, int64_t n, const Tensor& weight, int64_t
           "sf_logps_sum");
 }
 
-// Whether the weight gradient of a call in one piece is formed by
-// sf_ce_weight_grad instead of a library's product.  bf16: where the product is
-// shorter than the host's time for it (whole calls with both gradients, us,
-// product | kernel, tokens x hidden x vocabulary: 126 x 512 x 4096 123 | 107, 128
-// x 2048 x 16384 122 | 118, 200 x 1024 x 32000 164 | 192, 64 x 4096 x 128256 798 |
-// 866).  fp16: up to the 256 tokens that it takes, since the product is into
-// fp32 and rescaled (200 x 1024 x 32000 301 | 192).
-bool own_weight_grad(int64_t n, int64_t h, int64_t v, bool fp16) {
-    return n <= 256 && (fp16 || n * h * v <= int64_t(1) << 32);
-}
-
 // Whether the hidden gradient of a call in one piece is formed by
 // sf_logps_hidden_grad instead of a library's product and a scaling: where the
 // host's time for those, 18 to 22 us more, is longer.  Whole calls with this
@@ -344,7 +333,9 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
     const int64_t* y = at_ptr<int64_t>(labels);
     const float *lp = at_ptr<float>(logp), *l2 = at_ptr<float>(lse2);
     const Tensor by = like(hidden, {n}), norm = like(hidden, {2});
-    const bool few = one && own_weight_grad(n, h, v, fp16);
+    // the weight gradient by its own kernel: all that it takes, whose cases the
+    // library's product is slower at (sf_logps.hip)
+    const bool few = one && n <= SF_LOGPS_WEIGHT_TOKENS;
     Tensor gh, gw, again;
     if (need_hidden) gh = at::empty({n, h}, hidden.options());
     if (need_weight) gw = at::empty({v, h}, few || (one && !fp16) ? weight.options() : weight.options().dtype(at::kFloat));
@@ -387,9 +378,9 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
         check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, ht.data_ptr(), pad, st),
               "sf_logps_hidden");
         if (few) {
-            check(sf_ce_weight_grad(at_ptr<float>(norm), at_ptr<float>(norm) + 1, keep.data_ptr(), row, v, ht.data_ptr(),
-                                    pad, h, gw.data_ptr(), nullptr, nullptr, 0, type, st),
-                  "sf_ce_weight_grad");
+            check(sf_logps_weight_grad(keep.data_ptr(), row, pad, v, ht.data_ptr(), h, fp16 ? at_ptr<float>(norm) : nullptr,
+                                       type, gw.data_ptr(), st),
+                  "sf_logps_weight_grad");
             break;
         }
         const Tensor dt = keep.as_strided({v, pad}, {1, row}), hp = ht.t();

@@ -52,7 +52,7 @@ def _backward_rows(n: int, vocab: int) -> Tuple[int, bool]:
 
 def _hidden_parts(rows: int, weight: torch.Tensor) -> int:
     """Parts in which the hidden gradient's product sums over the vocabulary.
-    The library sums each of its tiles in one workgroup, so up to 128 tiles of
+    The library sums each of its tiles in one workgroup, so up to 64 tiles of
     256 x 256 as many parts as give every compute unit one, at most 16 and of
     2000 words or more; us, one product | parts, tokens x hidden x vocabulary: 3
     x 512 x 59040 107 | 20 (16), 32 x 768 x 50257 120 | 40 (16), 16 x 4096 x
@@ -71,7 +71,7 @@ def _hidden_parts(rows: int, weight: torch.Tensor) -> int:
     if (tiles % 256 == 0 or v < 4000 or weight.element_size() != 2 or h % 8 != 0 or not weight.is_contiguous()
             or weight.data_ptr() % 16 != 0 or rows * h >= 1 << 31):
         return 1
-    if tiles <= 128:
+    if tiles <= 64:
         return max(p for p in (1, 2, 4, 8, 16) if p == 1 or tiles * p <= 256 and v >= 2000 * p)
     if v < _PARTS_VOCAB:
         return 1

@@ -147,6 +147,11 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert grad(d=None) == grad(w=None) == grad(by=None) == grad(o=None) == grad(v=0) == grad(h=0) == 9001
     assert grad(ld=31) == grad(ldw=7) == grad(n=1 << 31) == 9001 and grad(t=0) == grad(t=5) == 9003
     assert grad(ld=36) == grad(ldw=12) == grad(h=4) == 9007
+    grad = lambda **k: hip.sf_logps_weight_grad(*{**dict(d=one, ld=8, n=64, v=8, h=one, k=8, s=None, t=1, o=one,  # noqa: E731
+                                                         st=None), **k}.values())
+    assert grad(d=None) == grad(h=None) == grad(o=None) == grad(v=0) == grad(k=0) == grad(n=0) == 9001
+    assert grad(n=320) == grad(ld=7) == grad(k=1 << 23) == 9001 and grad(t=0) == 9003
+    assert grad(n=65) == grad(ld=10) == grad(k=4) == grad(d=68) == grad(h=72) == grad(o=72) == 9007
     rows = lambda h=one, ld=8, n=1, k=8, w=one, t=2, o=one: hip.sf_logps_weighted(h, ld, n, k, w, t, o, None)  # noqa: E731
     assert rows(n=0) == 0 and rows(h=None) == rows(w=None) == rows(o=None) == rows(k=0) == rows(ld=0) == 9001
     assert rows(t=0) == 9003 and rows(ld=12) == rows(k=4) == rows(h=72) == 9007

@@ -237,6 +237,15 @@ def test_every_tile(dev, shape, dtype):
     test_matches_float64(dev, shape, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(5, 192, 515), (70, 576, 999), (130, 320, 3001), (250, 192, 70_001), (192, 448, 8193),
+                                   (256, 2048, 1000), (257, 192, 515), (60, 64, 66_000)])
+def test_gradients_of_few_tokens(dev, shape, dtype):
+    """Their own kernels at every padding of the tokens, hidden dimensions that end
+    inside a block, in one run and in several; and one token too many."""
+    test_matches_float64(dev, shape, dtype)
+
+
 @pytest.mark.parametrize("terms", [2, 3, 4, 5, 6, 9])
 @pytest.mark.parametrize("tokens,words", [(40, 700), (33, 66_000), (100, 4200), (120, 33_000)])
 def test_sums_shorter_and_longer_than_the_buffers(dev, terms, tokens, words):
