@@ -396,15 +396,22 @@ int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols,
                       const float* row_weight, int dtype, void* out,
                       sf_stream_t stream);
 
-/* Tokens that sf_logps_weight_grad takes at most. */
-#define SF_LOGPS_WEIGHT_TOKENS 256
+/* parts[s, i, j], contiguous fp32: the sum over the s-th of nparts runs of words,
+ * equal in whole 64s but for the last, of d[i, k] * weight[k, j], for
+ * sf_logps_sum.  d (at most 2^22 elements from row to row) holds zeros from vocab
+ * up to the next multiple of 64 columns; otherwise as sf_logps_hidden_grad.  A
+ * number of parts that leaves one without words is refused (SF_EINVAL). */
+int sf_logps_hidden_product(const void* d, size_t ld, size_t rows,
+                            const void* weight, size_t ldw, size_t vocab,
+                            size_t cols, int nparts, float* parts, int dtype,
+                            sf_stream_t stream);
 
 /* out[k, j] = sum over i of d[i, k] * hidden_t[j, i], times norm[0] where norm is
- * not null, rounded once: the weight gradient of few tokens from D of 16-bit
- * elements and what sf_logps_hidden leaves.  tokens: whole 64s, of d (ld
- * elements from row to row) and of the contiguous [cols, tokens] hidden_t.  out
- * is contiguous; cols is a multiple of 8, ld of 4, d aligned to 8 bytes, the
- * others to 16 (SF_EALIGN). */
+ * not null, rounded once: the weight gradient from D of 16-bit elements and what
+ * sf_logps_hidden leaves.  tokens: whole 64s, of d (ld elements from row to row,
+ * at most 2^22) and of the contiguous [cols, tokens] hidden_t.  out is
+ * contiguous; cols and ld are multiples of 8, all aligned to 16 bytes
+ * (SF_EALIGN). */
 int sf_logps_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab,
                          const void* hidden_t, size_t cols, const float* norm,
                          int dtype, void* out, sf_stream_t stream);

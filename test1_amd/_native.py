@@ -113,6 +113,7 @@ HIP_SIGNATURES = {
     "sf_logps_grad": [_vp, _sz, _sz, _sz, _vp, ctypes.c_int64, _f, _vp, _vp, _vp, _vp, _i, _sz, _vp],
     "sf_logps_hidden_grad": [_vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _i, _vp, _vp],
     "sf_logps_weighted": [_vp, _sz, _sz, _sz, _vp, _i, _vp, _vp],
+    "sf_logps_hidden_product": [_vp, _sz, _sz, _vp, _sz, _sz, _sz, _i, _vp, _i, _vp],
     "sf_logps_weight_grad": [_vp, _sz, _sz, _sz, _vp, _sz, _vp, _i, _vp, _vp],
     "sf_logps_hidden": [_vp, _sz, _sz, _sz, _vp, _i, _vp, _sz, _vp],
     "sf_logps_sum": [_vp, _i, _sz, _sz, _vp, _i, _vp, _sz, _vp, _sz, _vp, _vp, _vp],

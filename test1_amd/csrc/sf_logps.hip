@@ -665,7 +665,7 @@ __global__ __launch_bounds__(kHgWaves * 64, 2) void logps_hidden_grad_kernel(
 // dimensions go 64 at a time, which leaves room for a second workgroup: 256 x
 // 4096 x 128256 288 us, alone and 128 at a time 357.
 constexpr int kWgThreads = 256;
-constexpr int kWgTokens = SF_LOGPS_WEIGHT_TOKENS;
+constexpr size_t kWgTokens = 256;
 constexpr int kWgWords = 256;
 template <int kSteps>   // tokens / 32, padded
 constexpr int kWgLane = kSteps > 4 ? 4 : 8;   // neighbouring dimensions of a lane
@@ -749,6 +749,183 @@ __global__ __launch_bounds__(kWgThreads, 2) void logps_weight_grad_kernel(
                 for (int j = 0; j < kFH / 2; ++j) o[j] = Fmt::pack(acc[w][2 * j][i] * scale, acc[w][2 * j + 1][i] * scale);
                 if (word < vocab) *reinterpret_cast<Piece*>(out + uint64_t(word) * cols + col) = o;
             }
+    }
+}
+
+// The gradients' large products, 256 x 256 outputs a workgroup.  Both have one
+// operand whose rows lie along the sum (X: D's tokens for the hidden gradient, the
+// transposed hidden rows for the weight gradient) and one whose rows lie across it
+// (Y: W, D).  X goes through LDS as the forward's operands do; Y's rows of 256
+// columns go there as they lie and are read four rows at once, transposed, by
+// ds_read_b64_tr_b16.  Its 32-byte granules are swizzled by the row, so that the 16
+// rows of a wave's read take every bank twice, the least there is.  The copies,
+// reads and products go on as in the forward's kernel; LDS, 96 KB read and 32 KB
+// written for every 32 terms, is as busy as the matrix cores.  us, a library's
+// product | this: hidden gradient 8190 x 5120 x 152064 in two parts 9655 | 9473,
+// 4092 x 4096 x 128256 3049 | 3034, 2046 x 2560 x 151936 1806 | 1310, 4000 x 3584 x
+// 152064 3319 | 3484; weight gradient, bf16 and fp16 (there into fp32, still to be
+// scaled), 500 x 4096 x 128256 714, 1045 | 679, 8190 x 2560 x 50257 1732, 2101 |
+// 1597, 4092 x 4096 x 128256 3219 bf16 | 3310.  Four waves of 128 x 128 outputs
+// read a third less from LDS, but one wave a SIMD leaves its waits open: 3900.
+struct Product {
+    const uint16_t* x;   // [rows, 64 steps], ldx
+    const uint16_t* y;   // [sum, cols], ldy, of which wide may be read
+    uint32_t ldx, ldy, rows, cols, wide, sum;
+    uint32_t steps, each;   // 64 terms each: in all and in a part
+    void* out;
+    const float* norm;
+};
+constexpr int kPrTile = 256;
+typedef short Four __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) Four LdsFour;
+// restrict: or the compiler waits for every copy into LDS before this read
+__device__ __forceinline__ u32x2 read_turned(LdsFour* __restrict__ p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+}
+template <typename Fmt, bool kHidden>   // out: fp32 [parts, rows, cols], or 16-bit [cols, rows]
+__global__ __launch_bounds__(512, 2) void logps_product_kernel(const Product a) {
+    constexpr int kWP = 2, kWQ = 4, kFP = 8, kFQ = 4, kWaves = kWP * kWQ;
+    constexpr int kBuffer = 2 * kPrTile * kRowBytes, kLX = kPrTile / 8 / kWaves, kLY = kTerms / 2 / kWaves;
+    constexpr int kTurnRow = kFP * 32;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuffer];
+    const uint32_t lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wp = wave / kWQ, wq = wave % kWQ;
+
+    // as in the forward: each XCD has a contiguous run, 8 tiles of rows beside each other
+    const uint32_t tiles_p = (a.rows + kPrTile - 1) / kPrTile, tiles_q = (a.cols + kPrTile - 1) / kPrTile;
+    const uint32_t tiles = gridDim.x, xcd = blockIdx.x % 8, run = tiles / 8, more = tiles % 8;
+    uint32_t id = xcd * run + min(xcd, more) + blockIdx.x / 8;
+    const uint32_t part = id / (tiles_p * tiles_q);
+    id -= part * tiles_p * tiles_q;
+    const uint32_t first_p = id / (kGroupT * tiles_q) * kGroupT, group = min(uint32_t(kGroupT), tiles_p - first_p);
+    const uint32_t in = id - first_p * tiles_q;
+    const uint32_t q0 = in / group * kPrTile, p0 = (first_p + in % group) * kPrTile;
+    const uint32_t step0 = part * a.each, steps = min(a.steps - step0, a.each);
+
+    const uint8_t* gx = reinterpret_cast<const uint8_t*>(a.x + uint64_t(p0) * a.ldx + uint64_t(step0) * kTerms);
+    const uint8_t* gy = reinterpret_cast<const uint8_t*>(a.y + uint64_t(step0) * kTerms * a.ldy + q0);
+    const uint64_t y_step = uint64_t(a.ldy) * (2 * kTerms);
+    uint32_t off_x[kLX], row_y[kLY], col_y[kLY];
+#pragma unroll
+    for (int j = 0; j < kLX; ++j)
+        off_x[j] = min((j * kWaves + wave) * 8 + (lane >> 3), a.rows - 1 - p0) * (a.ldx * 2) +
+                   ((lane & 7) ^ (lane >> 3)) * 16;
+#pragma unroll
+    for (int j = 0; j < kLY; ++j) {
+        const uint32_t row = (j * kWaves + wave) * 2 + (lane >> 5), chunk = lane & 31;
+        const uint32_t from = ((chunk >> 1 ^ (row & 3) ^ (row >> 3 & 1) << 2) << 1 | (chunk & 1)) * 8;
+        row_y[j] = row;
+        col_y[j] = min(from, a.wide - 8 - q0) * 2;   // columns past the last are not stored
+    }
+    typedef __attribute__((address_space(3))) uint8_t Lds;
+    typedef const __attribute__((address_space(1))) uint8_t Global;
+    const auto copy = [&](uint32_t step, uint32_t buf) {
+        uint8_t* to = lds + buf * kBuffer + wave * 1024;
+#pragma unroll
+        for (int j = 0; j < kLX; ++j)
+            __builtin_amdgcn_global_load_lds((Global*)(gx + step * kRowBytes + off_x[j]), (Lds*)(to + j * kWaves * 1024),
+                                             16, 0, 0);
+        // rows past the sum's end are its last: X has zeros there
+        const uint32_t last = a.sum - 1 - (step0 + step) * kTerms;
+#pragma unroll
+        for (int j = 0; j < kLY; ++j)
+            __builtin_amdgcn_global_load_lds((Global*)(gy + step * y_step + min(row_y[j], last) * (a.ldy * 2) + col_y[j]),
+                                             (Lds*)(to + kPrTile * kRowBytes + j * kWaves * 1024), 16, 0, 0);
+    };
+    const uint32_t at = (quad ^ (l16 & 7)) * 16, at_x = (wp * kFP * 16 + l16) * kRowBytes;
+    const uint32_t turn_y = (l16 >> 2) | (quad & 1) << 2;
+    const uint32_t at_y = kPrTile * kRowBytes + (quad * 8 + (l16 >> 2)) * (kPrTile * 2) + (l16 & 3) * 8;
+    u32x4 x[2][kFP], y[2][kFQ];
+    const auto read = [&](uint32_t buf, int half) {
+        const uint8_t* from = lds + buf * kBuffer;
+#pragma unroll
+        for (int i = 0; i < kFP; ++i)
+            x[half][i] = *reinterpret_cast<const u32x4*>(from + (at ^ (half * 64)) + at_x + i * 16 * kRowBytes);
+#pragma unroll
+        for (int j = 0; j < kFQ; ++j) {
+            const uint8_t* p = from + at_y + half * 32 * (kPrTile * 2) + (((wq * kFQ + j) ^ turn_y) * 32);
+            const u32x2 lo = read_turned((LdsFour*)p), hi = read_turned((LdsFour*)(p + 4 * kPrTile * 2));
+            y[half][j] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        }
+    };
+    f32x4 acc[kFP][kFQ];
+    const auto multiply = [&](int half) {
+#pragma unroll
+        for (int i = 0; i < kFP; ++i)
+#pragma unroll
+            for (int j = 0; j < kFQ; ++j)
+                acc[i][j] = kHidden ? mfma(Fmt{}, y[half][j], x[half][i], acc[i][j])
+                                    : mfma(Fmt{}, x[half][i], y[half][j], acc[i][j]);
+    };
+    const auto meet = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto step = [&](uint32_t s, auto kMore) {
+        read(s & 1, 1);
+        multiply(0);
+        interleave<kFP + 2 * kFQ, kFP * kFQ, 0>();
+        meet();
+        if constexpr (decltype(kMore)::value) copy(s + 2, s & 1);
+        read((s + 1) & 1, 0);
+        multiply(1);
+        interleave<kFP + 2 * kFQ, kFP * kFQ, decltype(kMore)::value ? kLX + kLY : 0>();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int i = 0; i < kFP; ++i)
+#pragma unroll
+        for (int j = 0; j < kFQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    copy(0, 0);
+    if (steps > 1) copy(1, 1);
+    meet();
+    read(0, 0);
+    uint32_t s = 0;
+    for (; s + 2 < steps; ++s) step(s, std::true_type{});
+    if (s + 1 < steps) step(s++, std::false_type{});
+    read(s & 1, 1);
+    multiply(0);
+    meet();   // the buffers are not read again
+    multiply(1);
+    if constexpr (kHidden) {
+        float* out = static_cast<float*>(a.out) + uint64_t(part) * a.rows * a.cols;
+#pragma unroll
+        for (int i = 0; i < kFP; ++i) {
+            const uint32_t row = p0 + wp * kFP * 16 + i * 16 + l16;
+            if (row >= a.rows) continue;
+#pragma unroll
+            for (int j = 0; j < kFQ; ++j) {
+                const uint32_t col = q0 + wq * kFQ * 16 + j * 16 + quad * 4;
+                if (col < a.cols) *reinterpret_cast<f32x4*>(out + uint64_t(row) * a.cols + col) = acc[i][j];
+            }
+        }
+    } else {
+        const float scale = a.norm != nullptr ? *a.norm : 1.0f;
+        uint16_t* out = static_cast<uint16_t*>(a.out);
+        uint8_t* const turn = lds + wave * 16 * kTurnRow;
+#pragma unroll
+        for (int j = 0; j < kFQ; ++j) {
+#pragma unroll
+            for (int i = 0; i < kFP; ++i) {
+                const f32x4 e = acc[i][j] * scale;
+                const uint32_t to = ((i * 2 + (quad >> 1)) ^ l16) * 16 + (quad & 1) * 8;
+                *reinterpret_cast<u32x2*>(turn + l16 * kTurnRow + to) = u32x2{Fmt::pack(e[0], e[1]), Fmt::pack(e[2], e[3])};
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at_row = k * 4 + quad;
+                const u32x4 o = *reinterpret_cast<const u32x4*>(turn + at_row * kTurnRow + (l16 ^ at_row) * 16);
+                const uint32_t col = q0 + wq * kFQ * 16 + j * 16 + at_row, row = p0 + wp * kFP * 16 + l16 * 8;
+                if (col < a.cols && row < a.rows) *reinterpret_cast<u32x4*>(out + uint64_t(col) * a.rows + row) = o;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
     }
 }
 
@@ -921,6 +1098,15 @@ int dispatch_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab, 
     }
 }
 
+template <bool kHidden>
+int launch_product(const Product& a, uint32_t parts, int dtype, hipStream_t st) {
+    const uint64_t tiles = uint64_t((a.rows + kPrTile - 1) / kPrTile) * ((a.cols + kPrTile - 1) / kPrTile) * parts;
+    if (tiles > kMaxLanes / 512) return SF_EINVAL;
+    const auto kernel = dtype == SF_DTYPE_BF16 ? logps_product_kernel<Bf16, kHidden> : logps_product_kernel<F16, kHidden>;
+    hipLaunchKernelGGL(kernel, dim3(uint32_t(tiles)), dim3(512), 0, st, a);
+    return status();
+}
+
 // kernel(first, blocks) in as many launches as `blocks` workgroups need.
 template <typename Launch>
 int in_launches(uint64_t blocks, Launch launch) {
@@ -1067,15 +1253,41 @@ int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols, 
     });
 }
 
+int sf_logps_hidden_product(const void* d, size_t ld, size_t rows, const void* weight, size_t ldw, size_t vocab,
+                            size_t cols, int nparts, float* parts, int dtype, sf_stream_t stream) {
+    if (rows == 0) return SF_OK;
+    if (d == nullptr || weight == nullptr || parts == nullptr || sizes_bad(rows, vocab) || cols == 0 ||
+        cols > (size_t(1) << 22) || ld < (vocab + kTerms - 1) / kTerms * kTerms || ld > (size_t(1) << 22) || ldw < cols ||
+        ldw > (size_t(1) << 22) || nparts < 1 || size_t(nparts) > (vocab + kTerms - 1) / kTerms)
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (cols % 8 != 0 || ld % 8 != 0 || ldw % 8 != 0 || misaligned(d, 16) || misaligned(weight, 16) || misaligned(parts, 16))
+        return SF_EALIGN;
+    Product a = {static_cast<const uint16_t*>(d), static_cast<const uint16_t*>(weight), uint32_t(ld), uint32_t(ldw),
+                 uint32_t(rows), uint32_t(cols), uint32_t(cols), uint32_t(vocab),
+                 uint32_t((vocab + kTerms - 1) / kTerms), 0, parts, nullptr};
+    a.each = (a.steps + nparts - 1) / nparts;
+    if ((a.steps + a.each - 1) / a.each != uint32_t(nparts)) return SF_EINVAL;
+    return launch_product<true>(a, nparts, dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
 int sf_logps_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab, const void* hidden_t, size_t cols,
                          const float* norm, int dtype, void* out, sf_stream_t stream) {
     if (d == nullptr || hidden_t == nullptr || out == nullptr || sizes_bad(tokens, vocab) || tokens == 0 ||
-        tokens > kWgTokens || cols == 0 || cols > (size_t(1) << 22) || ld < vocab || ld > (size_t(1) << 31))
+        tokens > (size_t(1) << 22) || cols == 0 || cols > (size_t(1) << 22) || ld < vocab || ld > (size_t(1) << 22))
         return SF_EINVAL;
     if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
-    if (tokens % 64 != 0 || cols % 8 != 0 || ld % 4 != 0 || misaligned(d, 8) || misaligned(hidden_t, 16) || misaligned(out, 16))
+    if (tokens % 64 != 0 || cols % 8 != 0 || ld % 8 != 0 || misaligned(d, 16) || misaligned(hidden_t, 16) ||
+        misaligned(out, 16))
         return SF_EALIGN;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (tokens > kWgTokens) {
+        const uint32_t steps = uint32_t(tokens / kTerms);
+        const Product a = {static_cast<const uint16_t*>(hidden_t), static_cast<const uint16_t*>(d), uint32_t(tokens),
+                           uint32_t(ld), uint32_t(cols), uint32_t(vocab), uint32_t(ld), uint32_t(tokens), steps, steps,
+                           out, norm};
+        return launch_product<false>(a, 1, dtype, st);
+    }
     return dtype == SF_DTYPE_BF16 ? dispatch_weight_grad<Bf16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st)
                                   : dispatch_weight_grad<F16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st);
 }

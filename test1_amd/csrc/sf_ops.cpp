@@ -289,13 +289,28 @@ LogpsOut logps_forward(const Tensor& hidden, const Tensor& weight, const Tensor&
     return o;
 }
 
+int64_t tiles_of(int64_t rows, int64_t cols) { return ((rows + 255) / 256) * ((cols + 255) / 256); }
+
+// Whether the hidden gradient's product in `nparts` parts is
+// sf_logps_hidden_product: over 64 tiles of 256 x 256, whose parts fill rounds of
+// the chip.  With fewer tiles a library's smaller ones win: 300 x 4096 x 32000 (32)
+// 99 | 118 us, 200 x 1024 x 32000 (4) 34 | 48.
+bool own_hidden_product(int64_t n, int64_t h, int64_t row) {
+    return tiles_of(n, h) > 64 && row <= int64_t(1) << 22;
+}
+
 // out = row weight * (d @ weight), rounded once.
 void hidden_product(const Tensor& keep, int64_t n, const Tensor& weight, int64_t nparts, const float* row_weight,
                     const Tensor& norm, const Tensor& out) {
     const int64_t v = weight.size(0), h = weight.size(1), row = keep.stride(0);
-    const int64_t part = nparts == 1 ? v : v / nparts / 8 * 8, done = nparts * part;
+    const bool own = own_hidden_product(n, h, row);
+    const int64_t part = own || nparts == 1 ? v : v / nparts / 8 * 8, done = own ? v : nparts * part;
     Tensor parts = like(keep, {nparts, n, h});
-    if (nparts == 1) {
+    if (own) {
+        check(sf_logps_hidden_product(keep.data_ptr(), row, n, weight.data_ptr(), weight.stride(0), v, h, int(nparts),
+                                      at_ptr<float>(parts), type_of(keep), stream_of(keep)),
+              "sf_logps_hidden_product");
+    } else if (nparts == 1) {
         Tensor whole = parts.select(0, 0);
         at::mm_out(whole, keep.as_strided({n, v}, {row, 1}), weight, at::kFloat);
     } else {
@@ -306,6 +321,18 @@ void hidden_product(const Tensor& keep, int64_t n, const Tensor& weight, int64_t
     check(sf_logps_sum(at_ptr<float>(parts), int(nparts), n, h, out.data_ptr(), type_of(keep), d + 2 * done, row,
                        w + 2 * done * h, v - done, row_weight, at_ptr<float>(norm), stream_of(keep)),
           "sf_logps_sum");
+}
+
+// Whether the weight gradient of a call in one piece is formed by
+// sf_logps_weight_grad: up to 256 tokens always.  Beyond, a library's product wins
+// with few tiles, 2000 x 512 x 4096 (32) 22 | 41 us, 834 x 896 x 6640 (104) 25 | 24,
+// 400 x 1024 x 16000 (252) 25 | 19, and in bf16 by 2 to 4 % with the largest
+// products: 4000 x 3584 x 152064 3318 | 3399, 8190 x 5120 x 152064 9340 | 9706, but
+// 6500 x 2048 x 128256 2700 | 2584, 8190 x 2560 x 50257 1732 | 1597.  Of fp16 it is
+// into fp32 and has to be scaled: 4000 x 3584 x 152064 4297 | 3541.
+bool own_weight_grad(int64_t n, int64_t h, int64_t v, int64_t row, bool fp16) {
+    if (row > int64_t(1) << 22) return false;
+    return n <= 256 || (tiles_of(h, v) >= 96 && (fp16 || double(n) * h * v <= 2e12));
 }
 
 // Whether the hidden gradient of a call in one piece is formed by
@@ -333,12 +360,10 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
     const int64_t* y = at_ptr<int64_t>(labels);
     const float *lp = at_ptr<float>(logp), *l2 = at_ptr<float>(lse2);
     const Tensor by = like(hidden, {n}), norm = like(hidden, {2});
-    // the weight gradient by its own kernel: all that it takes, whose cases the
-    // library's product is slower at (sf_logps.hip)
-    const bool few = one && n <= SF_LOGPS_WEIGHT_TOKENS;
+    const bool own = one && own_weight_grad(n, h, v, row, fp16);
     Tensor gh, gw, again;
     if (need_hidden) gh = at::empty({n, h}, hidden.options());
-    if (need_weight) gw = at::empty({v, h}, few || (one && !fp16) ? weight.options() : weight.options().dtype(at::kFloat));
+    if (need_weight) gw = at::empty({v, h}, own || (one && !fp16) ? weight.options() : weight.options().dtype(at::kFloat));
     if (!kept) {
         keep = at::empty({up(step, 64), row}, hidden.options());
         again = like(hidden, {2, step});
@@ -362,7 +387,7 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
             hidden_product(keep, m, weight, a.nparts, at_ptr<float>(by) + s, fp16 ? norm : Tensor(),
                            one ? gh : gh.narrow(0, s, m));
         if (!need_weight) continue;
-        if (fp16 && !few) {
+        if (fp16 && !own) {
             // into fp32, of rows as they lie: 4096 x 4096 x 128256 4.2 ms, of transposed ones 28.8
             const Tensor weighted = at::empty({m, h}, hidden.options());
             check(sf_logps_weighted(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, weighted.data_ptr(), st),
@@ -377,7 +402,7 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
         const Tensor ht = at::empty({h, pad}, hidden.options());
         check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, ht.data_ptr(), pad, st),
               "sf_logps_hidden");
-        if (few) {
+        if (own) {
             check(sf_logps_weight_grad(keep.data_ptr(), row, pad, v, ht.data_ptr(), h, fp16 ? at_ptr<float>(norm) : nullptr,
                                        type, gw.data_ptr(), st),
                   "sf_logps_weight_grad");

@@ -25,7 +25,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .fused_ce import _DTYPES, _PARTS_VOCAB, _PLAIN, _memory_is_value, _saved_plain, _tiles, _traced
+from .fused_ce import _DTYPES, _PLAIN, _memory_is_value, _saved_plain, _tiles, _traced
 from .kernels import _CE_DTYPES
 
 
@@ -58,30 +58,23 @@ def _hidden_parts(rows: int, weight: torch.Tensor) -> int:
     x 512 x 59040 107 | 20 (16), 32 x 768 x 50257 120 | 40 (16), 16 x 4096 x
     128256 421 | 173 (16), 200 x 1024 x 32000 103 | 30 (16), 400 x 1024 x 16000
     70 | 29 (8), 834 x 896 x 6640 45 | 30 (2), 1000 x 2048 x 32000 279 | 122 (8),
-    500 x 4096 x 128256 849 | 458 (8), 2000 x 2048 x 32000 388 | 212 (4).  Beyond
-    by how well the tiles fill rounds of 256 compute units: the product of 640
-    tiles (two and a half rounds) runs at 0.96 PFLOP/s, in two parts at 1.31;
-    8190 x 5120 x 152064 13264 | 9718 (2), 8190 x 2560 x 50257 2157 | 1715 (4),
-    3000 x 5120 x 32000 1136 | 796 (4), 4000 x 3584 x 152064 4838 | 3349 (8), 6500
-    x 2048 x 128256 4171 | 3181 (8), 5000 x 2048 x 50257 903 | 894 (8).  Adding the
-    parts up takes 5 to 100 in the launch that scales and rounds the sum.  Whole
-    rounds need none: 4092 x 4096 x 128256 3094 | 3105."""
+    500 x 4096 x 128256 849 | 458 (8), 2000 x 2048 x 32000 388 | 212 (4).  Beyond,
+    where the product is the framework's own, by how well the tiles fill rounds
+    of 256 compute units, with what adding the parts up costs (1250 parts / V of
+    the product); us, 2 | 4 | 8 | 16 parts: 8190 x 5120 x 152064 (640 tiles) 9616 |
+    9762 | - | -, in one 10931, 8190 x 2560 x 50257 (320) 1797 | 1674 | 1772 | -,
+    2046 x 2560 x 151936 (80) - | 1749 | 1408 | 1310, 6000 x 1024 x 32000 (96) 394 |
+    411 | 333 | -, 4000 x 3584 x 152064 (224) - | 3725 | 3484 | 3593.  Whole rounds
+    need none: 4092 x 4096 x 128256 3081, in two 3155."""
     v, h = weight.shape
     tiles = _tiles(rows, h)
-    if (tiles % 256 == 0 or v < 4000 or weight.element_size() != 2 or h % 8 != 0 or not weight.is_contiguous()
+    if (v < 4000 or weight.element_size() != 2 or h % 8 != 0 or not weight.is_contiguous()
             or weight.data_ptr() % 16 != 0 or rows * h >= 1 << 31):
         return 1
+    able = [p for p in (1, 2, 4, 8, 16) if p == 1 or v >= 2000 * p]
     if tiles <= 64:
-        return max(p for p in (1, 2, 4, 8, 16) if p == 1 or tiles * p <= 256 and v >= 2000 * p)
-    if v < _PARTS_VOCAB:
-        return 1
-
-    def filled(parts: int) -> float:
-        return tiles * parts / (-(-tiles * parts // 256) * 256)
-
-    able = [p for p in (2, 4, 8) if v >= 4096 * p]
-    whole = [p for p in able if filled(p) == 1]
-    return whole[0] if whole else max((p for p in able if p > 2), key=filled)
+        return max(p for p in able if p == 1 or tiles * p <= 256)
+    return min(able, key=lambda p: -(-tiles * p // 256) * 256 / (tiles * p) + (1250 * p / v if p > 1 else 0))
 
 
 def _f32_out(dtype: torch.dtype) -> dict:

@@ -150,8 +150,14 @@ def test_c_entry_points_refuse_without_a_gpu():
     grad = lambda **k: hip.sf_logps_weight_grad(*{**dict(d=one, ld=8, n=64, v=8, h=one, k=8, s=None, t=1, o=one,  # noqa: E731
                                                          st=None), **k}.values())
     assert grad(d=None) == grad(h=None) == grad(o=None) == grad(v=0) == grad(k=0) == grad(n=0) == 9001
-    assert grad(n=320) == grad(ld=7) == grad(k=1 << 23) == 9001 and grad(t=0) == 9003
+    assert grad(n=1 << 23) == grad(ld=7) == grad(k=1 << 23) == 9001 and grad(t=0) == 9003
     assert grad(n=65) == grad(ld=10) == grad(k=4) == grad(d=68) == grad(h=72) == grad(o=72) == 9007
+    product = lambda **k: hip.sf_logps_hidden_product(*{**dict(d=one, ld=64, n=1, w=one, ldw=8, v=8, k=8, p=1,  # noqa: E731
+                                                               o=one, t=1, st=None), **k}.values())
+    assert product(n=0) == 0 and product(d=None) == product(w=None) == product(o=None) == product(v=0) == 9001
+    assert product(k=0) == product(ld=56) == product(ldw=7) == product(p=0) == product(p=2) == product(n=1 << 31) == 9001
+    assert product(v=512, ld=512, p=5) == 9001 and product(t=0) == 9003   # 8 steps: 2, 2, 2, 2 and none
+    assert product(ld=68) == product(ldw=12) == product(k=4) == product(d=72) == product(o=72) == 9007
     rows = lambda h=one, ld=8, n=1, k=8, w=one, t=2, o=one: hip.sf_logps_weighted(h, ld, n, k, w, t, o, None)  # noqa: E731
     assert rows(n=0) == 0 and rows(h=None) == rows(w=None) == rows(o=None) == rows(k=0) == rows(ld=0) == 9001
     assert rows(t=0) == 9003 and rows(ld=12) == rows(k=4) == rows(h=72) == 9007
@@ -205,7 +211,7 @@ def test_parts_of_the_hidden_gradient():
             return 4096
 
     for (n, h, v), want in {(8190, 5120, 152_064): 2, (4092, 4096, 128_256): 1, (8190, 4096, 32_000): 1,
-                            (8190, 2560, 50_257): 4, (3000, 5120, 32_000): 4, (4000, 3584, 152_064): 8,
+                            (8190, 2560, 50_257): 4, (3000, 5120, 32_000): 1, (4000, 3584, 152_064): 8,
                             (8190, 5120, 8192): 1}.items():
         assert _hidden_parts(n, Weight(v, h)) == want, (n, h, v)
     for n in range(256, 9000, 300):

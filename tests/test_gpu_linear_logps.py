@@ -348,9 +348,10 @@ def test_tokens_left_out_of_the_product(dev, live, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("shape,parts", [((2100, 2048, 16_400), 4), ((2100, 2048, 33_000), 8), ((8190, 1024, 16_387), 2)])
+@pytest.mark.parametrize("shape,parts", [((2100, 2048, 16_400), 2), ((2100, 2048, 33_000), 8), ((8190, 1024, 16_387), 2),
+                                         ((1800, 2560, 5_001), 2), ((16_400, 320, 700), 1)])
 def test_hidden_gradient_of_many_tiles_in_parts(dev, shape, parts, dtype):
-    """More than 64 tiles that fill no whole round, the last words in no part."""
+    """More than 64 tiles, rows, words and dimensions that end inside one."""
     hidden, weight, labels, up = inputs(shape, dtype, dev)
     assert module._hidden_parts(shape[0], weight) == parts
     want, bound = logps(hidden, weight, labels, grad=up)
