@@ -92,16 +92,16 @@ def unpack_act8(packed: torch.Tensor, shape: Sequence[int], dtype: torch.dtype =
     if dtype not in _CE_DTYPES:
         raise TypeError(f"unpack_act8: float32, bfloat16 or float16 expected, got {dtype}")
     shape = torch.Size(shape)
+    if out is None and stream is None and packed.is_cuda and not _traced():
+        x = _native.ops().act8_unpack(packed, shape, _CE_DTYPES[dtype], code)
+        if x is not None:
+            return x
     n = math.prod(shape)
     if packed.dtype != torch.uint8 or packed.numel() != act8_bytes(n) or not packed.is_contiguous():
         raise ValueError(f"unpack_act8: {act8_bytes(n)} contiguous uint8 expected for {tuple(shape)}")
     if out is not None and (out.dtype != dtype or out.shape != shape or not out.is_contiguous()
                             or out.device != packed.device):
         raise ValueError(f"unpack_act8: out must be a contiguous {dtype} tensor of {tuple(shape)} on {packed.device}")
-    if stream is None and n > 0 and packed.is_cuda and not _traced():
-        to = torch.empty(shape, dtype=dtype, device=packed.device) if out is None else out
-        if _native.ops().act8_unpack(packed, to, _CE_DTYPES[dtype], code):
-            return to
     if not _reads_memory(packed) or (out is not None and not _reads_memory(out)):
         x = _unpack_torch(packed, n, dtype, fmt).view(shape)
         return x if out is None else out.copy_(x)

@@ -581,18 +581,34 @@ PyObject* act8_pack(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
-// act8_unpack(packed, out, dtype, format): whether it was taken
+// act8_unpack(packed, shape, dtype, format): the elements, or None.  shape: a
+// tuple of sizes that packed holds.
 PyObject* act8_unpack(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
-    PyObject *p, *o;
+    PyObject *p, *shape;
     int dtype, format;
-    if (!PyArg_ParseTuple(args, "OOii", &p, &o, &dtype, &format)) return nullptr;
-    if (!plain(p) || !plain(o)) Py_RETURN_FALSE;
-    const Tensor &packed = THPVariable_Unpack(p), &out = THPVariable_Unpack(o);
+    if (!PyArg_ParseTuple(args, "OO!ii", &p, &PyTuple_Type, &shape, &dtype, &format)) return nullptr;
+    if (!plain(p)) Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 6> sizes;
+    uint64_t n = 1;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(shape); ++i) {
+        const int64_t k = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+        if (k == -1 && PyErr_Occurred()) return nullptr;
+        if (k <= 0 || n > (uint64_t(1) << 48) / uint64_t(k)) Py_RETURN_NONE;
+        n *= uint64_t(k);
+        sizes.push_back(k);
+    }
+    const Tensor& packed = THPVariable_Unpack(p);
+    if (packed.scalar_type() != at::kByte || !packed.is_contiguous() ||
+        uint64_t(packed.numel()) != (n + SF_ACT8_BLOCK - 1) / SF_ACT8_BLOCK * SF_ACT8_BLOCK_BYTES)
+        Py_RETURN_NONE;
+    at::AutoDispatchBelowADInplaceOrView below;
     const c10::DeviceGuard guard(packed.device());
-    check(sf_act8_unpack(packed.data_ptr(), format, size_t(out.numel()), out.data_ptr(), dtype, stream_of(packed)),
+    const auto type = dtype == SF_DTYPE_F32 ? at::kFloat : dtype == SF_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
+    const Tensor out = at::empty(sizes, packed.options().dtype(type));
+    check(sf_act8_unpack(packed.data_ptr(), format, size_t(n), out.data_ptr(), dtype, stream_of(packed)),
           "sf_act8_unpack");
-    Py_RETURN_TRUE;
+    return wrap(out);
     END_HANDLE_TH_ERRORS
 }
 
@@ -601,7 +617,7 @@ PyMethodDef methods[] = {
     {"policy_loss", policy_loss, METH_VARARGS, "(loss, kl, clipped), or None."},
     {"linear_logps", linear_logps, METH_VARARGS, "Log-probabilities, or None."},
     {"act8_pack", act8_pack, METH_VARARGS, "Packed elements, or None."},
-    {"act8_unpack", act8_unpack, METH_VARARGS, "Whether the call was taken."},
+    {"act8_unpack", act8_unpack, METH_VARARGS, "Restored elements, or None."},
     {nullptr, nullptr, 0, nullptr},
 };
 
