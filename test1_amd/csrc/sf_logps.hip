@@ -545,7 +545,8 @@ __global__ __launch_bounds__(kGradThreads) void logps_keep_grad_kernel(uint16_t*
         const uint32_t w = row < tokens && kind == kBadLabel ? Fmt::kNan2 : 0u;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            if (col + j * kGradThreads * kGroup < ld) *reinterpret_cast<u32x4*>(k + col + j * kGradThreads * kGroup) = u32x4{w, w, w, w};
+            if (col + j * kGradThreads * kGroup < ld)
+                *reinterpret_cast<u32x4*>(k + col + j * kGradThreads * kGroup) = u32x4{w, w, w, w};
         return;
     }
     const float l = lse2[row], by = -1.0f / rest_of(logp[row]);
@@ -571,7 +572,10 @@ __global__ __launch_bounds__(kGradThreads) void logps_keep_grad_kernel(uint16_t*
 // the other: a lane reads 8 neighbouring dimensions of 8 words and turns them
 // around in registers, so that its operand for dimension j of the 8 is one
 // register from each pair of words, and it ends up with 8 neighbours of a token.
-// No LDS but for the waves' sums.
+// No LDS but for the waves' sums.  14 us at 126 x 512 x 4096, 15 at 128 x 2048 x
+// 4096, 32 at 250 x 4096 x 4096: the waits for W's words bind it, some 0.8 us a turn
+// of 256, whatever is on its way; 16 waves or 64 dimensions a workgroup took 14 and
+// 13 there.  A call this small waits longer for the host.
 constexpr int kHgWaves = 8;
 constexpr int kHgTokens = 16;
 constexpr int kHgColumns = 128;
@@ -614,8 +618,8 @@ __global__ __launch_bounds__(kHgWaves * 64, 2) void logps_hidden_grad_kernel(
             acc[j] = mfma(Fmt{}, x.d, b, acc[j]);
         }
     };
-    // the next words are on their way while these are used (four turns on their way:
-    // 250 x 1024 x 16384 42 -> 38 us, twice the registers, and no less for a call)
+    // the next words are on their way while these are used (four turns on their way
+    // took twice the registers and gave 5 % at 16384 words, none at 4096)
     constexpr uint32_t kTurn = kHgWaves * kWords;
     uint32_t v = wave * kWords;
     if (v < vocab) {
@@ -710,7 +714,8 @@ __global__ __launch_bounds__(kWgThreads, 2) void logps_weight_grad_kernel(
         u32x2 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            x[i] = *reinterpret_cast<const u32x2*>(d + (s * 32 + quad * 8 + i) * ld + min(word0 + l16 * 4, uint32_t(ld) - 4));
+            x[i] = *reinterpret_cast<const u32x2*>(d + (s * 32 + quad * 8 + i) * ld +
+                                                   min(word0 + l16 * 4, uint32_t(ld) - 4));
 #pragma unroll
         for (int w = 0; w < kFW; ++w)
 #pragma unroll
@@ -1237,8 +1242,8 @@ int sf_logps_hidden_grad(const void* d, size_t ld, size_t rows, const void* weig
     return status();
 }
 
-int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols, const float* row_weight, int dtype, void* out,
-                      sf_stream_t stream) {
+int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols, const float* row_weight, int dtype,
+                      void* out, sf_stream_t stream) {
     if (rows == 0) return SF_OK;
     if (hidden == nullptr || row_weight == nullptr || out == nullptr || sizes_bad(rows, cols) || ldh < cols)
         return SF_EINVAL;
@@ -1295,7 +1300,8 @@ int sf_logps_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab, 
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels, int64_t ignore_index, size_t rows,
                     size_t vocab, float scale, float* weight, float* norm, sf_stream_t stream) {
     if (rows == 0 && norm == nullptr) return SF_OK;
-    if (sizes_bad(rows, vocab) || (rows > 0 && (grad == nullptr || logp == nullptr || labels == nullptr || weight == nullptr)))
+    if (sizes_bad(rows, vocab) ||
+        (rows > 0 && (grad == nullptr || logp == nullptr || labels == nullptr || weight == nullptr)))
         return SF_EINVAL;
     const uint64_t want = (rows + kWeightThreads - 1) / kWeightThreads;
     const uint32_t blocks = norm != nullptr ? 1 : uint32_t(want < 1024 ? want : 1024);
