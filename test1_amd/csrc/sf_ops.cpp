@@ -331,7 +331,7 @@ void hidden_product(const Tensor& keep, int64_t n, const Tensor& weight, int64_t
 // 6500 x 2048 x 128256 2700 | 2584, 8190 x 2560 x 50257 1732 | 1597.  Of fp16 it is
 // into fp32 and has to be scaled: 4000 x 3584 x 152064 4297 | 3541.
 bool own_weight_grad(int64_t n, int64_t h, int64_t v, int64_t row, bool fp16) {
-    if (row > int64_t(1) << 22) return false;
+    if (row > int64_t(1) << 22 || n > int64_t(1) << 21) return false;   // what its offsets hold
     return n <= 256 || (tiles_of(h, v) >= 96 && (fp16 || double(n) * h * v <= 2e12));
 }
 
