@@ -171,6 +171,51 @@ def test_replays_of_a_captured_step(dev):
         assert all(torch.equal(a, b) for a, b in zip((gh, gw), torch.autograd.grad(want, (hidden, weight), up)))
 
 
+# the gradients' own kernels: of few tokens, and of more than 64 and 96 tiles
+OWN = [(60, 128, 5000), (200, 320, 9000), (1800, 2560, 5001)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", OWN)
+def test_replays_of_captured_gradients(dev, shape, dtype):
+    hidden, weight, labels, up = inputs(shape, dtype, dev)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(linear_logps(hidden, weight, labels), (hidden, weight), up)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(linear_logps(hidden, weight, labels), (hidden, weight), up)
+    for _ in range(3):
+        with torch.no_grad():
+            hidden.mul_(0.9)
+        torch.cuda.synchronize()
+        graph.replay()
+        want = torch.autograd.grad(linear_logps(hidden, weight, labels), (hidden, weight), up)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", OWN)
+def test_gradients_whatever_tokens_without_a_label_hold(dev, shape, dtype):
+    hidden, weight, labels, up = inputs(shape, dtype, dev)
+    labels[3:20] = -100
+    up[21] = 0.0
+    grads = []
+    for there in (0.0, math.nan, math.inf):
+        h = hidden.clone()
+        h[3:20] = there
+        h[21] = there
+        grads.append(torch.autograd.grad(linear_logps(h.requires_grad_(True), weight.requires_grad_(True), labels),
+                                         (h, weight), up))
+    for gh, gw in grads:
+        assert torch.equal(gh, grads[0][0]) and torch.equal(gw, grads[0][1])
+        assert (gh[3:20] == 0).all() and (gh[21] == 0).all() and gw.isfinite().all()
+
+
 def test_chunks(dev, monkeypatch):
     """The same results however many rows are taken at a time."""
     hidden, weight, labels, up = inputs((300, 128, 1000), torch.float32, dev)
