@@ -343,7 +343,7 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab,
  * p) / (1 - p_label): 1 at the label.  row_weight = grad * scale * (1 -
  * p_label); 0 for an ignored row or a grad of 0, NaN for a label outside [0,
  * vocab).  norm (or null: 1): two floats; the weights are then divided by the power of two
- * norm[0] that leaves the largest in [1, 2), and norm[1] = 1. */
+ * norm[0] that leaves the largest in [1/2, 1), and norm[1] = 1. */
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
                     int64_t ignore_index, size_t rows, size_t vocab,
                     float scale, float* row_weight, float* norm,

@@ -464,8 +464,9 @@ __global__ __launch_bounds__(kT * kRowsOf<kT>) void logps_rows_kernel(const floa
 
 // ---------------------------------------------------------------------
 // Gradients.  What multiplies each row: grad * scale * (1 - p_y), and, of fp16
-// operands, a power of two that brings the largest of them into [1, 2) (a mean
-// over many tokens leaves them near fp16's least numbers).  One workgroup.
+// operands, a power of two that brings the largest of them into [1/2, 1): a mean
+// over many tokens leaves them near fp16's least numbers, and a hidden row times
+// a factor below 1 is finite in fp16 whenever the row is.  One workgroup.
 // ---------------------------------------------------------------------
 struct Weights {
     const float *grad, *logp;
@@ -503,7 +504,7 @@ __device__ __forceinline__ void row_weights(const Weights& a, uint64_t block, ui
         m = waves[0];
         for (int w = 1; w < kT / 64; ++w) m = fmaxf(m, waves[w]);
         // within what both the factor and its inverse can be
-        const int e = m > 0.0f ? min(max(ilogbf(m), -100), 100) : 0;
+        const int e = m > 0.0f ? min(max(ilogbf(m) + 1, -100), 100) : 0;
         by = ldexpf(1.0f, -e), back = ldexpf(1.0f, e);
     }
     for (uint64_t i = block * kT + threadIdx.x; i < a.n; i += blocks * kT) a.weight[i] = of(i) * by;
