@@ -327,8 +327,9 @@ int sf_logps_rows(const float* logits, size_t ld, size_t rows, size_t vocab,
  * floats; order (or null): of rows + 1 integers, with which rows without a label
  * inside the vocabulary take no part in the product, where the hidden rows
  * span less than 4 GiB (SF_ETOOBIG).  keep (or null): [rows,
- * ld_keep] of dtype, every 2^(logit - m) of the rows that do, 0 behind the
- * vocabulary up to the next whole span, for sf_logps_keep_grad.
+ * ld_keep] of dtype, every 2^(logit - m) of the rows that do (of SF_DTYPE_F16
+ * times 2^14, as D below), 0 behind the vocabulary up to the next whole span,
+ * for sf_logps_keep_grad.
  * hidden_size is a multiple of 64, ldw and ldh (at most 2^22) and ld_keep of 8,
  * weight, hidden and keep start on 16-byte boundaries (SF_EALIGN). */
 #define SF_LOGPS_SPAN 256
@@ -342,8 +343,10 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab,
 /* The gradient of such logits is row_weight[i] * D[i, j], D = ((j == label) -
  * p) / (1 - p_label): 1 at the label.  row_weight = grad * scale * (1 -
  * p_label); 0 for an ignored row or a grad of 0, NaN for a label outside [0,
- * vocab).  norm (or null: 1): two floats; the weights are then divided by the power of two
- * norm[0] that leaves the largest in [1/2, 1), and norm[1] = 1. */
+ * vocab).  D of SF_DTYPE_F16 is held times 2^14, so that small probabilities are
+ * no subnormals.  norm (or null), for that type: two floats; the weights are then
+ * divided by the power of two that leaves the largest in [1/2, 1), and norm[0] =
+ * that power / 2^14, what both products are multiplied by; norm[1] = 1. */
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
                     int64_t ignore_index, size_t rows, size_t vocab,
                     float scale, float* row_weight, float* norm,
@@ -355,7 +358,8 @@ int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels,
  * `padded`.  ld is a multiple of SF_LOGPS_SPAN (SF_EALIGN).  all_rows (or 0): in
  * the same launch the row weights of that many rows, of which these are the
  * first, as sf_logps_weight makes them; with `normalise` as with its norm,
- * without it norm (or null) is set to 1, 1. */
+ * without it they are not divided: norm (or null) is then 1, of SF_DTYPE_F16
+ * 2^-14, and 1. */
 int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
                        size_t vocab, const void* parts, const int64_t* labels,
                        int64_t ignore_index, const float* lse2,

@@ -10,7 +10,8 @@ or an old policy without.
 Numerics: the logits stay fp32 (they are not rounded to 16 bits in between),
 maximum and sum of the softmax are fp32.  The gradient's products take 16-bit
 operands, fp32 of fp32 ones: the exponentials, kept to 16 bits relative to their
-span of the vocabulary, and their share of 1 - p, rounded again; the label's
+span of the vocabulary, and their share of 1 - p, rounded again (fp16 with a
+factor of 2^14, which keeps them out of its subnormals); the label's
 element is exact, and the rows' own factors stay fp32 up to the hidden rows of
 the weight gradient's product.
 """
@@ -119,7 +120,7 @@ def _forward_kernels(hidden, weight, labels, ignore_index, scale):
 
 
 def _row_weight(grad, logp, labels, vocab, ignore_index, scale, dtype):
-    """What multiplies the rows of D, and fp16's factor (``sf_logps_weight``)."""
+    """What multiplies the rows of D, and what takes out fp16's factors (``sf_logps_weight``)."""
     n = labels.shape[0]
     weight = torch.empty(n, dtype=torch.float32, device=grad.device)
     norm = torch.empty(2, dtype=torch.float32, device=grad.device) if dtype == torch.float16 else None
