@@ -54,8 +54,11 @@ __device__ __forceinline__ float lifted(float d) {   // d times kLift, not above
     return d;
 }
 
-// 1 - p of a log-probability.
-__device__ __forceinline__ float rest_of(float logp) { return fmaxf(-expm1f(logp), kLeastRest); }
+// 1 - p of a log-probability; NaN stays NaN.
+__device__ __forceinline__ float rest_of(float logp) {
+    const float rest = -expm1f(logp);
+    return rest < kLeastRest ? kLeastRest : rest;
+}
 
 // ---------------------------------------------------------------------
 // The product with the softmax's sums.  A workgroup has a tile of 256 words

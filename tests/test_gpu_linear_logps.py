@@ -405,3 +405,18 @@ def test_hidden_gradient_of_many_tiles_in_parts(dev, shape, parts, dtype):
     lp = linear_logps(hidden, weight, labels)
     for got, w, b in zip((lp.detach(), *torch.autograd.grad(lp, (hidden, weight), up)), want, bound):
         near(got, w, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 64, 300), (70, 64, 300), (1, 65, 300), (400, 128, 20_000)])
+def test_nan_in_the_weight(dev, shape, dtype):
+    """One NaN takes part in every token's softmax: nothing is left that is a number,
+    the label's own element of the gradient included."""
+    hidden, weight, labels, up = inputs(shape, dtype, dev)
+    labels[:] = 7
+    weight[5, 3] = math.nan
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    lp = linear_logps(hidden, weight, labels)
+    gh, gw = torch.autograd.grad(lp, (hidden, weight), up)
+    assert lp.isnan().all() and gh.isnan().all() and gw.isnan().all()
