@@ -228,12 +228,15 @@ def _label_kinds(labels, vocab, ignore_index):
     return valid, torch.where(valid & inside, labels, torch.zeros_like(labels)), valid & ~inside
 
 
-def _torch_logps(hidden, weight, labels, ignore_index, scale):
+def _torch_logps(hidden, weight, labels, ignore_index, scale, bias=None):
     with torch.autocast(hidden.device.type, enabled=False):
         valid, at, bad = _label_kinds(labels, weight.shape[0], ignore_index)
         # what ignored tokens hold does not reach the weight's gradient
         hidden = torch.where(valid.unsqueeze(-1), hidden, torch.zeros_like(hidden))
-        logp = torch.log_softmax(hidden.float() @ weight.float().t() * scale, dim=-1)
+        logits = hidden.float() @ weight.float().t()
+        if bias is not None:
+            logits = logits + bias.float()
+        logp = torch.log_softmax(logits * scale, dim=-1)
         logp = logp.gather(-1, at.unsqueeze(-1)).squeeze(-1)
         logp = logp * torch.where(bad, math.nan, 1.0)
         return torch.where(valid, logp, torch.zeros_like(logp))

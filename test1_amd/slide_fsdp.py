@@ -62,7 +62,7 @@ from .act8 import _check_format, act8_bytes
 from .config import SlideFSDPConfig
 from .distributed_sync import create_distributed_sync
 from .fused_ce import chunked_linear_cross_entropy
-from .linear_logps import linear_logps
+from .linear_logps import _torch_logps, linear_logps
 from .layer_state import GradSlotRing, LayerRuntimeState, StreamingRuntime
 from .optimizer import LayerAdam
 from .sliding_checkpoint import ActivationRing, KeptOnDevice, SlidingCheckpoint, StorageSpill, pin_or_keep
@@ -103,9 +103,13 @@ class OutputLayer(nn.Module):
 
     def token_logps(self, hidden_states: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
         """Log-probabilities of the shifted labels, [B, S - 1] fp32, 0 where
-        they are ignored; no logits are kept."""
-        return linear_logps(self.norm(hidden_states)[..., :-1, :], self.lm_head.weight, labels[..., 1:],
-                            self.loss_fn.ignore_index, temperature)
+        they are ignored; no logits are kept.  With a bias, which the kernels do
+        not add, they are made by torch operations from all logits."""
+        hidden_states, labels = self.norm(hidden_states)[..., :-1, :], labels[..., 1:]
+        ignore_index, bias = self.loss_fn.ignore_index, getattr(self.lm_head, "bias", None)
+        if bias is None:
+            return linear_logps(hidden_states, self.lm_head.weight, labels, ignore_index, temperature)
+        return _torch_logps(hidden_states, self.lm_head.weight, labels, ignore_index, 1.0 / temperature, bias)
 
     def forward(self, hidden_states: torch.Tensor, labels: Optional[torch.Tensor] = None):
         hidden_states = self.norm(hidden_states)

@@ -219,3 +219,26 @@ def test_parts_of_the_hidden_gradient():
             for v in (5000, 16_384, 32_000, 152_064):
                 p = _hidden_parts(n, Weight(v, h))
                 assert p in (1, 2, 4, 8, 16) and (p == 1 or v // p >= 1024)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+def test_token_logps_of_the_output_unit(bias):
+    """log_softmax of the logits that the unit's forward gives, at the next labels."""
+    from test1_amd.slide_fsdp import OutputLayer
+
+    torch.manual_seed(0)
+    unit = OutputLayer(torch.nn.LayerNorm(16), torch.nn.Linear(16, 50, bias=bias), 16)
+    hidden = torch.randn(3, 9, 16, requires_grad=True)
+    labels = torch.randint(0, 50, (3, 9))
+    labels[1, 2:6] = -100
+    got = unit.token_logps(hidden, labels, temperature=0.7)
+    logits = unit(hidden)[1][:, :-1].double()
+    want = torch.log_softmax(logits / 0.7, dim=-1).gather(-1, labels[:, 1:].clamp(min=0).unsqueeze(-1)).squeeze(-1)
+    want = torch.where(labels[:, 1:] == -100, torch.zeros_like(want), want)
+    assert got.shape == (3, 8) and got.dtype == torch.float32 and (got[1, 1:5] == 0).all()
+    assert torch.allclose(got.double(), want, atol=2e-6)   # a few roundings of logits up to 5
+    for a, b in zip(torch.autograd.grad(got.sum(), [hidden, *unit.lm_head.parameters()], retain_graph=True),
+                    torch.autograd.grad(want.sum(), [hidden, *unit.lm_head.parameters()])):
+        assert torch.allclose(a, b, atol=1e-4)
+    labels[0, 3] = 50
+    assert unit.token_logps(hidden, labels)[0, 2].isnan()
