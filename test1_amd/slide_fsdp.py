@@ -47,6 +47,7 @@ row-sparse embedding, bf16 H2D, SDMA gradient copies) change no bits.
 
 from __future__ import annotations
 
+import math
 import os
 import warnings
 from dataclasses import dataclass
@@ -716,34 +717,46 @@ class SlideFSDP(nn.Module):
         with the loss in its ``loss`` (``alignment.preference_loss`` and
         ``policy_loss`` do).  The step's backward starts from that loss, and
         the output is an ``ObjectiveOutput``."""
-        if objective is not None and labels is None:
-            raise ValueError("SlideFSDP: an objective needs labels")
+        if objective is not None:
+            if labels is None:
+                raise ValueError("SlideFSDP: an objective needs labels")
+            self._check_token_logps(input_ids, labels, temperature)
         hidden_states = self._run_decoders(input_ids, attention_mask)
         output_state = self.layer_states[-1]
-        hidden_states = self._PreLayerFunction.apply(hidden_states, output_state, None)
-        if objective is None:
-            loss, logits = self.output_layer(hidden_states, labels)
-        else:
-            labels = labels.to(hidden_states.device)
-            logps = self.output_layer.token_logps(hidden_states, labels, temperature)
-            logits, result = None, objective(logps, labels[..., 1:] != self.output_layer.loss_fn.ignore_index)
-            loss = result if isinstance(result, torch.Tensor) else result.loss
-        if loss is not None:
-            loss = self._PostLayerFunction.apply(loss, output_state, True)
-            if self._early_embedding_update and torch.is_grad_enabled() and loss.requires_grad:
-                # the backward below reaches the lookup: the embedding's
-                # gradient-free rows can be updated while it starts
-                self.layer_states[0].start_early_update()
-            try:
+        try:
+            hidden_states = self._PreLayerFunction.apply(hidden_states, output_state, None)
+            if objective is None:
+                loss, logits = self.output_layer(hidden_states, labels)
+            else:
+                labels = labels.to(hidden_states.device)
+                logps = self.output_layer.token_logps(hidden_states, labels, temperature)
+                logits, result = None, objective(logps, labels[..., 1:] != self.output_layer.loss_fn.ignore_index)
+                loss = result if isinstance(result, torch.Tensor) else result.loss
+            if loss is not None:
+                loss = self._PostLayerFunction.apply(loss, output_state, True)
+                if self._early_embedding_update and torch.is_grad_enabled() and loss.requires_grad:
+                    # the backward below reaches the lookup: the embedding's
+                    # gradient-free rows can be updated while it starts
+                    self.layer_states[0].start_early_update()
                 loss.backward()
-            except BaseException:
-                self._after_failed_backward()
-                raise
-            if isinstance(self.runtime.grad_ring, GradSlotRing) and not self._ring_grown:
-                self._ring_grow_pending = True
+        except BaseException:
+            self._after_failed_step()
+            raise
+        if loss is not None and isinstance(self.runtime.grad_ring, GradSlotRing) and not self._ring_grown:
+            self._ring_grow_pending = True
         if objective is not None:
             return ObjectiveOutput(loss=loss, logps=logps.detach(), result=result)
         return CausalLMOutputWithPast(loss=loss, logits=logits)
+
+    @staticmethod
+    def _check_token_logps(input_ids: torch.Tensor, labels: torch.Tensor, temperature: float) -> None:
+        """What can be refused before any decoder has run."""
+        if labels.shape != input_ids.shape:
+            raise ValueError(f"SlideFSDP: labels of {tuple(input_ids.shape)} expected, got {tuple(labels.shape)}")
+        if labels.dtype != torch.int64:
+            raise TypeError(f"SlideFSDP: int64 labels expected, got {labels.dtype}")
+        if not (temperature > 0 and math.isfinite(temperature)):
+            raise ValueError("SlideFSDP: temperature must be above 0")
 
     @torch.no_grad()
     def token_logps(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
@@ -752,15 +765,17 @@ class SlideFSDP(nn.Module):
         as it is, [B, S - 1] fp32, shifted by one, 0 where the label is -100:
         what a preference or policy objective takes of its reference policy or
         of the policy that sampled.  Nothing is kept for a backward."""
-        labels = (input_ids if labels is None else labels).to(self.device)
+        labels = input_ids if labels is None else labels
+        self._check_token_logps(input_ids, labels, temperature)
         hidden_states = self._run_decoders(input_ids, attention_mask)
-        hidden_states = self._PreLayerFunction.apply(hidden_states, self.layer_states[-1], None)
-        logps = self.output_layer.token_logps(hidden_states, labels, temperature)
-        # No backward follows, for which the last two units stay loaded: what
-        # they hold of the pool goes back to it, or the next forward waits for it.
-        for state in self.layer_states[-2:]:
-            state.to_offload_async(is_backward=False)
-        return logps
+        try:
+            hidden_states = self._PreLayerFunction.apply(hidden_states, self.layer_states[-1], None)
+            return self.output_layer.token_logps(hidden_states, labels.to(self.device), temperature)
+        finally:
+            # No backward follows, for which the last two units stay loaded: what
+            # they hold of the pool goes back to it, or the next forward waits for it.
+            for state in self.layer_states[-2:]:
+                state.to_offload_async(is_backward=False)
 
     def _run_decoders(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor]) -> torch.Tensor:
         """The lookup and every decoder: the last hidden states."""
@@ -871,10 +886,11 @@ class SlideFSDP(nn.Module):
             if embed_rows:
                 self.layer_states[0].alloc_host_buffers(batch_size * seq_length)
 
-    def _after_failed_backward(self) -> None:
-        """The backward raised part-way (a hook, an out-of-memory error, an
-        interrupt): the units it finished were offloaded and their updates
-        queued, the others never were.  Let the queued work finish, close the
+    def _after_failed_step(self) -> None:
+        """The step raised behind its decoders (the output unit, an objective), or
+        its backward part-way (a hook, an out-of-memory error, an interrupt):
+        the units it finished were offloaded and their updates queued, the
+        others never were.  Let the queued work finish, close the
         embedding's early update part (its late part will not come), give
         back every unit still on the device and drop gradients, so the next
         step starts from the masters as they are.  Errors here are secondary

@@ -201,3 +201,65 @@ def test_the_example_learns(dev):
     losses = main(["--steps", "3", "--pairs", "2", "--length", "64"])
     assert len(losses) == 6 and all(np.isfinite(losses))
     assert losses[2] < losses[0] and losses[5] < losses[3]
+
+
+class _Own(Exception):
+    """An objective's own error."""
+
+
+def _raise(lp, mask):
+    raise _Own
+
+
+def test_errors_behind_the_decoders_give_the_units_back(dev, monkeypatch):
+    """Two pool units and no unit with a buffer of its own: whatever raises
+    between the decoders and the backward, the next step is that of a trainer
+    where nothing had raised."""
+    from test1_amd import SlideFSDP, SlideFSDPConfig, slide_fsdp
+
+    model = make_model()
+    ids, labels, noise = batch(dev)
+    objective = objectives(noise, torch.full_like(noise, -7.0), labels)["preference"]
+    want = non_offloaded(model, dev, ids, labels, objective)
+    base = want[1]
+    sf = SlideFSDP(model, SlideFSDPConfig(device=dev, lr=LR, weight_decay=WD), wait_timeout=10, resident_layers=0)
+    for bad, error in ((_raise, _Own), (lambda lp, m: objective(lp[:, 1:], m), ValueError),
+                       (lambda lp, m: objective(lp, m).loss.detach(), RuntimeError)):
+        with pytest.raises(error):
+            sf(input_ids=ids, labels=labels, objective=bad)
+        assert torch.equal(sf.token_logps(ids, labels=labels), base)
+
+    def failing(*args):
+        raise _Own
+
+    with monkeypatch.context() as m:
+        m.setattr(slide_fsdp, "linear_logps", failing)
+        for call in (lambda: sf.token_logps(ids, labels=labels),
+                     lambda: sf(input_ids=ids, labels=labels, objective=objective)):
+            with pytest.raises(_Own):
+                call()
+    with monkeypatch.context() as m:
+        m.setattr(sf.output_layer, "forward", failing)
+        with pytest.raises(_Own):
+            sf(input_ids=ids, labels=labels)
+    check_step(sf, ids, labels, objective, want)
+    sf.close()
+
+
+def test_calls_refused_before_a_decoder_runs(dev, monkeypatch):
+    sf = slide(dev, make_model())
+    ids, labels, _ = batch(dev)
+
+    def ran(*args):
+        raise AssertionError("the decoders ran")
+
+    monkeypatch.setattr(sf, "_run_decoders", ran)
+    mean = lambda lp, m: -lp[m].mean()  # noqa: E731
+    for kw, error in ((dict(temperature=0.0), ValueError), (dict(temperature=float("nan")), ValueError),
+                      (dict(labels=labels[:, 1:]), ValueError), (dict(labels=labels.int()), TypeError)):
+        kw = dict(dict(labels=labels), **kw)
+        with pytest.raises(error):
+            sf.token_logps(ids, **kw)
+        with pytest.raises(error):
+            sf(input_ids=ids, objective=mean, **kw)
+    sf.close()
