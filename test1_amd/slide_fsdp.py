@@ -83,6 +83,17 @@ class ObjectiveOutput(CausalLMOutputWithPast):
     result: Any = None
 
 
+def _loss_of(result: Any) -> torch.Tensor:
+    """The loss in what an objective returned."""
+    loss = result if isinstance(result, torch.Tensor) else getattr(result, "loss", None)
+    if loss is None and isinstance(result, (tuple, list)) and len(result) > 0:
+        loss = result[0]
+    if not isinstance(loss, torch.Tensor):
+        raise TypeError("SlideFSDP: an objective returns the loss, something with a loss in its `loss`, or a tuple "
+                        f"that begins with the loss; got {type(result).__name__}")
+    return loss
+
+
 class OutputLayer(nn.Module):
     """Final norm + lm_head + shifted cross-entropy as one unit (reference
     slide_fsdp.py:45-113).  ``fused=False``: full logits and
@@ -713,9 +724,9 @@ class SlideFSDP(nn.Module):
         ``objective``: in place of the cross entropy, a callable of the
         labels' log-probabilities under the model, [B, S - 1] fp32 at
         ``temperature`` and shifted by one, and of the bool mask of those that
-        count (labels that are not -100); it returns the loss, or something
-        with the loss in its ``loss`` (``alignment.preference_loss`` and
-        ``policy_loss`` do).  The step's backward starts from that loss, and
+        count (labels that are not -100); it returns the loss, something with
+        the loss in its ``loss`` (``alignment.preference_loss`` and
+        ``policy_loss`` do), or a tuple whose first element it is.  The step's backward starts from that loss, and
         the output is an ``ObjectiveOutput``."""
         if objective is not None:
             if labels is None:
@@ -731,7 +742,7 @@ class SlideFSDP(nn.Module):
                 labels = labels.to(hidden_states.device)
                 logps = self.output_layer.token_logps(hidden_states, labels, temperature)
                 logits, result = None, objective(logps, labels[..., 1:] != self.output_layer.loss_fn.ignore_index)
-                loss = result if isinstance(result, torch.Tensor) else result.loss
+                loss = _loss_of(result)
             if loss is not None:
                 loss = self._PostLayerFunction.apply(loss, output_state, True)
                 if self._early_embedding_update and torch.is_grad_enabled() and loss.requires_grad:

@@ -242,3 +242,18 @@ def test_token_logps_of_the_output_unit(bias):
         assert torch.allclose(a, b, atol=1e-4)
     labels[0, 3] = 50
     assert unit.token_logps(hidden, labels)[0, 2].isnan()
+
+
+def test_what_an_objective_may_return():
+    from collections import namedtuple
+
+    from test1_amd.alignment import PreferenceLoss
+    from test1_amd.slide_fsdp import _loss_of
+
+    loss, other = torch.tensor(1.0), torch.tensor(2.0)
+    for result in (loss, (loss, other), [loss, {}], (loss,), PreferenceLoss(loss, other, other),
+                   namedtuple("Late", "metrics loss")(other, loss)):
+        assert _loss_of(result) is loss
+    for result in (None, 1.0, (), (1.0, loss), {"loss": loss}, namedtuple("Odd", "metrics loss")(other, 3.0)):
+        with pytest.raises(TypeError, match="objective returns"):
+            _loss_of(result)

@@ -263,3 +263,21 @@ def test_calls_refused_before_a_decoder_runs(dev, monkeypatch):
         with pytest.raises(error):
             sf(input_ids=ids, objective=mean, **kw)
     sf.close()
+
+
+def test_an_objective_that_returns_a_tuple(dev):
+    model = make_model()
+    ids, labels, noise = batch(dev)
+    objective = objectives(noise, torch.full_like(noise, -7.0), labels)["preference"]
+    want = non_offloaded(model, dev, ids, labels, objective)
+    sf = slide(dev, model)
+    with pytest.raises(TypeError, match="objective returns"):
+        sf(input_ids=ids, labels=labels, objective=lambda lp, m: None)
+    sf.runtime.capture = {}
+    out = sf(input_ids=ids, labels=labels, objective=lambda lp, m: (objective(lp, m).loss, {"tokens": int(m.sum())}))
+    sf.wait_for_updates()
+    cap, sf.runtime.capture = sf.runtime.capture, None
+    assert torch.equal(out.loss.detach(), want[0]) and out.result[1]["tokens"] == int((labels[:, 1:] != -100).sum())
+    for u, ref in enumerate(want[2]):
+        assert np.array_equal(u16(cap[u][0]), ref), u
+    sf.close()
