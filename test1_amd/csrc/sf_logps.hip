@@ -88,7 +88,8 @@ struct Tiles {
     const int64_t* labels;
     const int32_t* order;     // [tokens + 1] the rows with a label and their number, or null: all rows
     float scale2;             // scale * log2(e)
-    float2* parts;            // [tiles of words, tokens] maximum in base 2 and sum
+    float2* parts;            // [tiles of words, parts_row] maximum in base 2 and sum
+    uint64_t parts_row;       // tokens of the whole call, of which these are some
     float* target;            // [tokens] the label's product, unscaled
     uint16_t* keep;           // [tokens, ld_keep] or null
     uint64_t ld_keep;
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
             const uint32_t t = wt0 + j * 16 + l16;
 #pragma unroll
             for (int w = 1; w < kWV; ++w) sum[j] += shared[w * kBT + t];
-            if (t0 + t < count) a.parts[uint64_t(v0 / kSpan) * a.tokens + row[j]] = float2{top[j], sum[j]};
+            if (t0 + t < count) a.parts[uint64_t(v0 / kSpan) * a.parts_row + row[j]] = float2{top[j], sum[j]};
         }
 }
 
@@ -387,7 +388,8 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
 constexpr int kJoinThreads = 256;
 constexpr int kJoinTokens = 4;
 __global__ __launch_bounds__(kJoinThreads) void logps_join_kernel(const float2* __restrict__ parts, uint32_t spans,
-                                                                  uint32_t tokens, const float* __restrict__ target,
+                                                                  uint64_t parts_row, uint32_t tokens,
+                                                                  const float* __restrict__ target,
                                                                   const int64_t* __restrict__ labels,
                                                                   int64_t ignore_index, uint32_t vocab, float scale2,
                                                                   float* __restrict__ lse2, float* __restrict__ logp) {
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(kJoinThreads) void logps_join_kernel(const float2* 
     const RowKind kind = token < tokens ? row_kind(labels[token], ignore_index, vocab) : kIgnored;
     if (kind == kValid)   // the others may have no parts
         for (uint32_t k = threadIdx.x / kJoinTokens; k < spans; k += kJoinThreads / kJoinTokens) {
-            const float2 v = parts[uint64_t(k) * tokens + token];
+            const float2 v = parts[uint64_t(k) * parts_row + token];
             const float m = fmaxf(p.m, v.x), c = base(m);
             // an empty part stays empty whatever the bases are; a NaN sum stays NaN
             p.s = (p.s == 0.0f ? 0.0f : p.s * exp2f(base(p.m) - c)) + (v.y == 0.0f ? 0.0f : v.y * exp2f(base(v.x) - c));
@@ -1023,7 +1025,6 @@ template <typename Fmt, int kWV, int kWT, int kFV, int kFT, int kDeep>
 int launch_tiles(const Tiles& a, hipStream_t st) {
     constexpr uint32_t kBT = kWT * kFT * 16;
     const uint64_t tiles = uint64_t((a.vocab + kSpan - 1) / kSpan) * ((a.tokens + kBT - 1) / kBT);
-    if (tiles > kMaxLanes / (kWV * kWT * 64)) return SF_EINVAL;
     const auto all = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, kDeep, true, false>
                                        : logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, kDeep, false, false>;
     const auto some = a.keep != nullptr ? logps_tiles_kernel<Fmt, kWV, kWT, kFV, kFT, kDeep, true, true>
@@ -1052,14 +1053,14 @@ int launch_tiles(const Tiles& a, hipStream_t st) {
 // L2) 8.8 against 8.4.  With two tiles a unit, 4 buffers cost what the second
 // tile gives: 200 x 4096 x 32000 138 against 113 us.
 struct TileKind {
-    uint32_t tokens, slots;
+    uint32_t tokens, slots, lanes;
     float round, half, brief, brief_half;
 };
 constexpr TileKind kTileKinds[] = {
-    {256, 256, 1.00f, 1.00f, 1.00f, 1.00f},
-    {128, 256, 0.75f, 0.68f, 0.60f, 0.60f},
-    {64, 512, 0.76f, 0.66f, 0.60f, 0.57f},
-    {32, 512, 0.78f, 0.53f, 0.60f, 0.50f},
+    {256, 256, 512, 1.00f, 1.00f, 1.00f, 1.00f},
+    {128, 256, 512, 0.75f, 0.68f, 0.60f, 0.60f},
+    {64, 512, 256, 0.76f, 0.66f, 0.60f, 0.57f},
+    {32, 512, 256, 0.78f, 0.53f, 0.60f, 0.50f},
 };
 
 template <typename Fmt>
@@ -1071,6 +1072,7 @@ int dispatch_tiles(const Tiles& a, hipStream_t st) {
     float least = 0.0f;
     for (const TileKind& k : kTileKinds) {
         const uint64_t tiles = spans * ((a.tokens + k.tokens - 1) / k.tokens);
+        if (tiles > kMaxLanes / k.lanes) continue;   // never of the first kind
         const float one = tiles <= 256 ? (brief ? k.brief_half : k.half) : brief ? k.brief : k.round;
         const float time = one * float((tiles + k.slots - 1) / k.slots);
         if (best == 0 || time < least) best = k.tokens, least = time, alone = tiles <= 256;
@@ -1188,22 +1190,33 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab, const void* hid
         misaligned(hidden, 16) || misaligned(parts, 8) || misaligned(keep, 16) || ld_keep % kGroup != 0)
         return SF_EALIGN;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const Tiles a = {static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(hidden), uint32_t(ldw),
-                     uint32_t(ldh), uint32_t(vocab), uint32_t(rows), uint32_t(hidden_size / kTerms), labels, order,
-                     scale * kLog2e, static_cast<float2*>(parts), target, static_cast<uint16_t*>(keep), ld_keep};
-    int e = SF_OK;
-    if (order != nullptr) {   // 32-bit byte offsets of all rows
-        if (uint64_t(rows) * ldh * 2 > UINT32_MAX) return SF_ETOOBIG;
-        hipLaunchKernelGGL(logps_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, labels, ignore_index, a.vocab, a.tokens,
-                           order);
+    if (order != nullptr && uint64_t(rows) * ldh * 2 > UINT32_MAX) return SF_ETOOBIG;   // 32-bit byte offsets of all rows
+    // Rows of one launch: whole tiles of 256, as many as its lanes allow for the
+    // product (2.1 M rows of 128256 words) and the join.
+    constexpr uint64_t kTile = 256, kMostRows = kMaxLanes / kJoinThreads * kJoinTokens;
+    const uint64_t fit = kMaxLanes / kTileKinds[0].lanes / spans * kTile, most = fit < kMostRows ? fit : kMostRows;
+    for (uint64_t r = 0; r < rows; r += most) {
+        const uint32_t n = uint32_t(rows - r < most ? rows - r : most);
+        const Tiles a = {static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(hidden) + r * ldh,
+                         uint32_t(ldw), uint32_t(ldh), uint32_t(vocab), n, uint32_t(hidden_size / kTerms), labels + r,
+                         order == nullptr ? nullptr : order + r, scale * kLog2e, static_cast<float2*>(parts) + r, rows,
+                         target + r, keep == nullptr ? nullptr : static_cast<uint16_t*>(keep) + r * ld_keep, ld_keep};
+        int e = SF_OK;
+        if (order != nullptr) {   // its last element is the next launch's first, which is written behind this one's
+            hipLaunchKernelGGL(logps_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, a.labels, ignore_index, a.vocab, n,
+                               order + r);
+            e = status();
+            if (e != SF_OK) return e;
+        }
+        e = dtype == SF_DTYPE_BF16 ? dispatch_tiles<Bf16>(a, st) : dispatch_tiles<F16>(a, st);
+        if (e != SF_OK) return e;
+        hipLaunchKernelGGL(logps_join_kernel, dim3((n + kJoinTokens - 1) / kJoinTokens), dim3(kJoinThreads), 0, st,
+                           a.parts, uint32_t(spans), a.parts_row, n, a.target, a.labels, ignore_index, a.vocab, a.scale2,
+                           lse2 + r, logp + r);
         e = status();
         if (e != SF_OK) return e;
     }
-    e = dtype == SF_DTYPE_BF16 ? dispatch_tiles<Bf16>(a, st) : dispatch_tiles<F16>(a, st);
-    if (e != SF_OK) return e;
-    hipLaunchKernelGGL(logps_join_kernel, dim3((a.tokens + kJoinTokens - 1) / kJoinTokens), dim3(kJoinThreads), 0, st,
-                       a.parts, uint32_t(spans), a.tokens, target, labels, ignore_index, a.vocab, a.scale2, lse2, logp);
-    return status();
+    return SF_OK;
 }
 
 int sf_logps_keep_grad(void* keep, size_t ld, size_t rows, size_t padded, size_t vocab, const void* parts,

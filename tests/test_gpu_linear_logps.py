@@ -420,3 +420,28 @@ def test_nan_in_the_weight(dev, shape, dtype):
     lp = linear_logps(hidden, weight, labels)
     gh, gw = torch.autograd.grad(lp, (hidden, weight), up)
     assert lp.isnan().all() and gh.isnan().all() and gw.isnan().all()
+
+
+@pytest.mark.parametrize("few", [False, True])
+def test_more_tiles_than_one_launch_takes(dev, few):
+    """2^22 tiles of 256 words x 256 tokens and some more, with a label for every
+    token and for a few around where the second launch begins."""
+    n, h, v = 262_144 + 300, 64, 1 << 20
+    g = torch.Generator(device=dev).manual_seed(3)
+    hidden = torch.randn(n, h, generator=g, device=dev).bfloat16()
+    weight = torch.empty(v, h, dtype=torch.bfloat16, device=dev).normal_(0.0, 0.25, generator=g)
+    labels = torch.randint(0, v, (n,), generator=g, device=dev)
+    at = torch.tensor([0, 1, 255, 256, 1000, 262_142, 262_144, 262_145, n - 1], device=dev)
+    if few:
+        labels = torch.full_like(labels, -100).index_copy_(0, at, labels[at])
+        labels[262_143] = v
+    with torch.no_grad():
+        lp = linear_logps(hidden, weight, labels)
+    (want,), (bound,) = logps(hidden[at], weight, labels[at])
+    near(lp[at], want, bound)
+    if few:
+        assert lp[262_143].isnan() and int((lp != 0).sum()) == len(at) + 1
+    else:   # as the rows give by themselves in one launch
+        for s in (slice(0, 600), slice(262_000, n)):
+            (want,), (bound,) = logps(hidden[s], weight, labels[s])
+            near(lp[s], want, bound)
