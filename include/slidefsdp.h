@@ -420,8 +420,8 @@ int sf_logps_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab,
                          const void* hidden_t, size_t cols, const float* norm,
                          int dtype, void* out, sf_stream_t stream);
 
-/* As sf_ce_sum, also of one part, each row times row_weight[i], 0 where that
- * is, and times norm[0] where norm is not null. */
+/* As sf_ce_sum, also of one part, then of any size, each row times
+ * row_weight[i], 0 where that is, and times norm[0] where norm is not null. */
 int sf_logps_sum(const float* parts, int nparts, size_t rows, size_t cols,
                  void* out, int dtype, const void* d_tail, size_t ld,
                  const void* w_tail, size_t tail, const float* row_weight,

@@ -786,19 +786,24 @@ int sf_logps_sum(const float* parts, int nparts, size_t rows, size_t cols, void*
         return SF_EINVAL;
     if (tail >= size_t(kGroup) * size_t(nparts) || (tail > 0 && (d_tail == nullptr || w_tail == nullptr || ld < tail)))
         return SF_EINVAL;
-    if (cols > (size_t(1) << 31) || rows > (size_t(1) << 31) / cols) return SF_EINVAL;
+    // of one launch: 32-bit offsets of the elements
+    if (cols > (size_t(1) << 31)) return SF_EINVAL;
+    const size_t most = (size_t(1) << 31) / cols;
+    if (rows > most && nparts != 1) return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
     if (cols % kGroup != 0 || misaligned(parts, 16) || misaligned(out, 16) || (tail > 0 && misaligned(w_tail, 16)) ||
         (tail > 0 && misaligned(d_tail, 2)))
         return SF_EALIGN;
-    const uint32_t count = uint32_t(rows * cols);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == SF_DTYPE_BF16)
-        return launch_sum<Bf16, true>(nparts, parts, count, uint32_t(cols), out, d_tail, ld, w_tail, uint32_t(tail), st,
-                                      row_weight, norm);
-    if (dtype == SF_DTYPE_F16)
-        return launch_sum<F16, true>(nparts, parts, count, uint32_t(cols), out, d_tail, ld, w_tail, uint32_t(tail), st,
-                                     row_weight, norm);
-    return SF_EDTYPE;
+    for (size_t r = 0; r < rows; r += most) {
+        const uint32_t count = uint32_t((rows - r < most ? rows - r : most) * cols);
+        const auto launch = dtype == SF_DTYPE_BF16 ? launch_sum<Bf16, true> : launch_sum<F16, true>;
+        const int e = launch(nparts, parts + r * cols, count, uint32_t(cols), static_cast<uint16_t*>(out) + r * cols,
+                             tail > 0 ? static_cast<const uint16_t*>(d_tail) + r * ld : nullptr, ld, w_tail,
+                             uint32_t(tail), st, row_weight + r, norm);
+        if (e != SF_OK) return e;
+    }
+    return SF_OK;
 }
 
 int sf_ce_loss(const float* row_loss, const int64_t* labels, size_t n, int64_t ignore_index, float* loss,

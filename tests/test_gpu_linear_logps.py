@@ -445,3 +445,26 @@ def test_more_tiles_than_one_launch_takes(dev, few):
         for s in (slice(0, 600), slice(262_000, n)):
             (want,), (bound,) = logps(hidden[s], weight, labels[s])
             near(lp[s], want, bound)
+
+
+def test_hidden_gradients_of_more_than_2_31_elements(dev):
+    """A small vocabulary of many tokens: what is kept is small, the hidden rows are not."""
+    h, v = 4096, 512
+    n = (1 << 31) // h + 77
+    g = torch.Generator(device=dev).manual_seed(3)
+    hidden = torch.empty(n, h, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    weight = torch.empty(v, h, dtype=torch.bfloat16, device=dev).normal_(0.0, 2 / 64, generator=g)
+    labels = torch.randint(0, v, (n,), generator=g, device=dev)
+    up = torch.randn(n, generator=g, device=dev)
+    hidden.requires_grad_(True)
+    weight.requires_grad_(True)
+    gh, gw = torch.autograd.grad(linear_logps(hidden, weight, labels), (hidden, weight), up)
+    want_w = torch.zeros(v, h, dtype=torch.float64, device=dev)
+    bound_w = torch.zeros_like(want_w)
+    for s in range(0, n, 1 << 15):
+        part = slice(s, min(n, s + (1 << 15)))
+        want, bound = logps(hidden.detach()[part], weight.detach(), labels[part], grad=up[part])
+        near(gh[part], want[1], bound[1])
+        want_w += want[2]
+        bound_w += bound[2]
+    near(gw, want_w, bound_w)
