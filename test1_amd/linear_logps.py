@@ -41,14 +41,17 @@ _SPAN = _native.SF_LOGPS_SPAN
 # chunks takes does not grow with the tokens.
 _KEEP_BYTES = 8 << 30
 _AGAIN_BYTES = 2 << 30
+# Tiles of 64 x 64 hidden elements that the launch transposing them takes.
+_TURNED_TILES = 1 << 23
 
 
-def _backward_rows(n: int, vocab: int) -> Tuple[int, bool]:
+def _backward_rows(n: int, vocab: int, hidden: int) -> Tuple[int, bool]:
     """Rows that the backward takes at a time, and whether the forward keeps
     their exponentials for it (then all)."""
     row = 2 * (-(-vocab // _SPAN) * _SPAN)
-    step = max(64, _AGAIN_BYTES // row // 64 * 64)
-    return (n, True) if (n + 63) * row <= _KEEP_BYTES else (min(n, step), False)
+    most = _TURNED_TILES // -(-hidden // 64) * 64
+    step = min(max(64, _AGAIN_BYTES // row // 64 * 64), most)
+    return (n, True) if (n + 63) * row <= _KEEP_BYTES and n <= most else (min(n, step), False)
 
 
 def _hidden_parts(rows: int, weight: torch.Tensor) -> int:
@@ -283,7 +286,7 @@ def linear_logps(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tenso
     need_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
     step, keep, nparts = rows.shape[0], False, 1
     if need_grad:
-        step, keep = _backward_rows(step, weight.shape[0])
+        step, keep = _backward_rows(step, *weight.shape)
         nparts = _hidden_parts(step, weight)
     logp = _native.ops().linear_logps(rows, weight, flat, ignore_index, scale, nparts, step, keep)
     if logp is None:

@@ -257,3 +257,19 @@ def test_what_an_objective_may_return():
     for result in (None, 1.0, (), (1.0, loss), {"loss": loss}, namedtuple("Odd", "metrics loss")(other, 3.0)):
         with pytest.raises(TypeError, match="objective returns"):
             _loss_of(result)
+
+
+def test_rows_of_the_backward():
+    """All of them and kept up to 8 GiB, whole 64s otherwise, and never more hidden
+    elements than the launch that transposes them takes."""
+    from test1_amd.linear_logps import _backward_rows
+
+    assert _backward_rows(4092, 128_256, 4096) == (4092, True)
+    assert _backward_rows(40_000, 128_256, 4096) == (8320, False)
+    assert _backward_rows(1 << 23, 128, 4096) == (1 << 23, True)
+    assert _backward_rows((1 << 23) + 1, 128, 4096) == (1 << 22, False)   # 2 GiB of 256 words
+    assert _backward_rows(10_000, 128_256, 1 << 22) == (8192, False)
+    for n, v, h in ((1 << 24, 128, 4096), (40_000, 128_256, 1 << 22), (1 << 25, 64, 64), (100, 1 << 29, 64), (900, 64, 1 << 22)):
+        rows, kept = _backward_rows(n, v, h)
+        assert (rows == n if kept else rows % 64 == 0 or rows == n)
+        assert -(-rows // 64) * (h // 64) <= 1 << 23, (n, v, h)
