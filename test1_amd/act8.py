@@ -16,6 +16,7 @@ is not differentiable: a checkpoint's gradient is that of what it restores.
 
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Optional, Sequence
 
@@ -46,12 +47,20 @@ def _reads_memory(t: torch.Tensor) -> bool:
     return t.is_cuda and not _traced() and type(t) in _PLAIN and _memory_is_value(t)
 
 
+def _aligned(packed: torch.Tensor) -> bool:
+    return packed.data_ptr() % 16 == 0
+
+
+def _on(stream: Optional[torch.cuda.Stream]):
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
 def pack_act8(x: torch.Tensor, fmt: str = "int8", out: Optional[torch.Tensor] = None,
               stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """The elements of ``x`` (float32, bfloat16 or float16; in order, whatever
     its strides) packed into ``out``: uint8, ``act8_bytes(x.numel())`` of them,
-    contiguous, made here if not given.  Asynchronous on ``stream`` (default:
-    the current one)."""
+    contiguous, made here if not given (one that starts on no 16-byte boundary
+    takes a copy more).  Asynchronous on ``stream`` (default: the current one)."""
     code = _check_format(fmt)
     if x.dtype not in _CE_DTYPES:
         raise TypeError(f"pack_act8: float32, bfloat16 or float16 expected, got {x.dtype}")
@@ -71,23 +80,20 @@ def pack_act8(x: torch.Tensor, fmt: str = "int8", out: Optional[torch.Tensor] = 
     if x.device.index != torch.cuda.current_device():
         with torch.cuda.device(x.device):
             return pack_act8(x, fmt, out, stream)
-    if stream is not None and (out is None or not x.is_contiguous()):
-        with torch.cuda.stream(stream):   # what is made here belongs to that stream
-            out = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if out is None else out
-            x = x.contiguous()
-    elif out is None:
-        out = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    x = x.contiguous()
-    if n:
-        _native.check(_native.hip().sf_act8_pack(x.data_ptr(), _CE_DTYPES[x.dtype], n, out.data_ptr(), code,
-                                                 _stream_ptr(stream)), "sf_act8_pack")
-    return out
+    with _on(stream):   # what is made here belongs to that stream
+        packed = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if out is None or not _aligned(out) else out
+        x = x.contiguous()
+        if n:
+            _native.check(_native.hip().sf_act8_pack(x.data_ptr(), _CE_DTYPES[x.dtype], n, packed.data_ptr(), code,
+                                                     _stream_ptr(stream)), "sf_act8_pack")
+        return packed if out is None or packed is out else out.copy_(packed.view(out.shape))
 
 
 def unpack_act8(packed: torch.Tensor, shape: Sequence[int], dtype: torch.dtype = torch.bfloat16, fmt: str = "int8",
                 out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """What ``pack_act8`` packed, as a tensor of ``shape`` and ``dtype``, into
-    the contiguous ``out`` if given."""
+    the contiguous ``out`` if given.  A ``packed`` that starts on no 16-byte
+    boundary takes a copy more."""
     code = _check_format(fmt)
     if dtype not in _CE_DTYPES:
         raise TypeError(f"unpack_act8: float32, bfloat16 or float16 expected, got {dtype}")
@@ -108,15 +114,12 @@ def unpack_act8(packed: torch.Tensor, shape: Sequence[int], dtype: torch.dtype =
     if packed.device.index != torch.cuda.current_device():
         with torch.cuda.device(packed.device):
             return unpack_act8(packed, shape, dtype, fmt, out, stream)
-    if out is None:
-        if stream is not None:
-            with torch.cuda.stream(stream):
-                out = torch.empty(shape, dtype=dtype, device=packed.device)
-        else:
-            out = torch.empty(shape, dtype=dtype, device=packed.device)
-    if n:
-        _native.check(_native.hip().sf_act8_unpack(packed.data_ptr(), code, n, out.data_ptr(), _CE_DTYPES[dtype],
-                                                   _stream_ptr(stream)), "sf_act8_unpack")
+    with _on(stream):
+        out = torch.empty(shape, dtype=dtype, device=packed.device) if out is None else out
+        packed = packed if _aligned(packed) else packed.clone()
+        if n:
+            _native.check(_native.hip().sf_act8_unpack(packed.data_ptr(), code, n, out.data_ptr(), _CE_DTYPES[dtype],
+                                                       _stream_ptr(stream)), "sf_act8_unpack")
     return out
 
 

@@ -600,6 +600,7 @@ PyObject* act8_unpack(PyObject*, PyObject* args) {
     }
     const Tensor& packed = THPVariable_Unpack(p);
     if (packed.scalar_type() != at::kByte || !packed.is_contiguous() ||
+        reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 != 0 ||
         uint64_t(packed.numel()) != (n + SF_ACT8_BLOCK - 1) / SF_ACT8_BLOCK * SF_ACT8_BLOCK_BYTES)
         Py_RETURN_NONE;
     at::AutoDispatchBelowADInplaceOrView below;

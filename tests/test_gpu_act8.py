@@ -140,3 +140,25 @@ def test_entry_points_refuse(dev):
     assert hip.sf_act8_unpack(p.data_ptr(), 0, 256, x.data_ptr() + 1, bf, None) == 9001
     assert hip.sf_act8_pack(x.data_ptr(), bf, 256, x.data_ptr(), 0, None) == 9005
     assert act8._LEAST == 2.0 ** -100
+
+
+@pytest.mark.parametrize("off", [1, 2, 4, 8, 15])
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_packed_elements_on_any_byte(dev, fmt, off):
+    x = values(1000, torch.bfloat16).to(dev)
+    want = pack_act8(x, fmt)
+    back = unpack_act8(want, (1000,), torch.bfloat16, fmt)
+    room = torch.full((act8_bytes(1000) + 32,), 7, dtype=torch.uint8, device=dev)
+    at = room[off:off + act8_bytes(1000)]
+    assert pack_act8(x, fmt, out=at) is at and torch.equal(at, want)
+    assert (room[:off] == 7).all() and (room[off + act8_bytes(1000):] == 7).all()
+    assert torch.equal(unpack_act8(at, (1000,), torch.bfloat16, fmt), back)
+    out = torch.empty_like(x)
+    assert unpack_act8(at, (1000,), torch.bfloat16, fmt, out=out) is out and torch.equal(out, back)
+    at.zero_()
+    s = torch.cuda.Stream(device=dev)
+    s.wait_stream(torch.cuda.current_stream())
+    pack_act8(x, fmt, out=at, stream=s)
+    got = unpack_act8(at, (1000,), torch.bfloat16, fmt, stream=s)
+    s.synchronize()
+    assert torch.equal(at, want) and torch.equal(got, back)
