@@ -212,3 +212,22 @@ def test_transforms_take_torch_operations(dev):
     assert torch.allclose(tangent, want.sum(), rtol=1e-3, atol=1e-6)
     pref = lambda x: preference_loss(x, ref, mask).loss  # noqa: E731
     assert torch.allclose(torch.func.grad(pref)(lp.detach()), torch.autograd.grad(pref(lp), lp)[0], rtol=1e-4, atol=1e-8)
+
+
+@pytest.mark.parametrize("shape", [(6, 301), (40, 9000)])
+def test_gradients_under_strided_and_broadcast_inputs(dev, shape):
+    """Advantages with a stride between rows, one that rows share, and references
+    that every token shares: losses and gradients as of contiguous copies."""
+    mask, lp, old, ref, adv = tokens(shape, dev)
+    lp.requires_grad_(True)
+    strided = adv.t()[0]
+    assert strided.shape == shape[:1] and strided.stride() == (shape[1],)
+    calls = [(old, strided, ref), (old, adv[0, :1].expand(shape[0]), ref), (old, adv[:, :1].expand(shape), ref),
+             (old, strided, torch.zeros(1, 1, device=dev).expand(shape)), (old[:1].expand(shape), adv.t().contiguous().t(), None)]
+    for reduction in ("token", "sequence"):
+        for o, a, r in calls:
+            kw = dict(kl_coef=0.1, reduction=reduction)
+            got = policy_loss(lp, o, a, mask, r, **kw)
+            want = policy_loss(lp, o.contiguous(), a.contiguous(), mask, None if r is None else r.contiguous(), **kw)
+            assert torch.equal(got.loss, want.loss) and torch.equal(got.clip_fraction, want.clip_fraction)
+            assert torch.equal(torch.autograd.grad(got.loss, lp)[0], torch.autograd.grad(want.loss, lp)[0])
