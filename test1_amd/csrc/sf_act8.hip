@@ -28,8 +28,8 @@ constexpr int kBlock = SF_ACT8_BLOCK;
 // elements.  Restoring: one 128-bit store of 16-bit elements, so that a wave's
 // stores lie side by side (16 elements a lane, two stores with gaps: 16.8 M
 // elements 11.6 | 9.3 us, 41.9 M 27.8 | 23.8).  Both move 51 MB at 16.8 M, in
-// 9.4 and 9.3 us, 5.4 TB/s; a device copy reaches 5.4.  Stores past the caches
-// would take 8.2 us and cost the recompute that reads them next as much.
+// 9.8 and 9.7 us after each other, 5.2 TB/s (each repeated by itself 9.4 and 9.3);
+// a device copy reaches 5.4.  Stores past the caches would take 8.2 us and cost the recompute that reads them next as much.
 constexpr int kPack = 16;
 constexpr int kUnpack = 8;
 constexpr int kThreads = 256;

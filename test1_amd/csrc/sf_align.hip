@@ -5,9 +5,9 @@
 // elementwise and reduction operations, forward and backward, they are some 30
 // to 60 launches; here they are two or three, and the host's time for a forward
 // and a backward, 50 to 65 us with autograd's, is what bounds a call.  On the
-// device, parts | join | gradient, us: preference, 128 x 8191 tokens 3.7 | 4.0 |
-// 3.5, 9.4 MB and 5.2 MB; policy, 256 x 8191 with every input 9.6 | 4.1 | 4.8, 44
-// MB, 4.6 TB/s, and 17 MB.  The sums are taken in fp32 by each lane over its few tokens
+// device, parts | join | gradient, us: preference, 128 x 8191 tokens 4.2 | 4.7 |
+// 3.5, 9.4 MB and 5.2 MB; policy, 256 x 8191 with every input 11.3 | 4.0 | 4.9, 44
+// MB, 3.9 TB/s, and 17 MB.  The sums are taken in fp32 by each lane over its few tokens
 // and in fp64 from there on, in an order fixed by the shape alone: no atomics.
 // Masked tokens are selected away before any arithmetic, so NaN and infinities
 // there reach neither a sum nor a gradient.

@@ -8,7 +8,7 @@
 // (8 bytes for 256 logits), and the joined sums give the result.  Where a
 // gradient will be wanted the exponentials themselves are kept, relative to
 // their tile's maximum, 2 bytes a logit: from those a probability is off by a
-// rounding of itself, from logits in 16 bits by up to 2^-9 of the logit.
+// rounding of itself, from logits in 16 bits by up to 2^-8 of the logit.
 // Others (fp32, hidden sizes that are no multiple of 64, unaligned rows) have
 // their logits made by a library product in chunks of fp32 and read once.
 //
@@ -598,10 +598,12 @@ __global__ __launch_bounds__(kGradThreads) void logps_keep_grad_kernel(uint16_t*
 // the other: a lane reads 8 neighbouring dimensions of 8 words and turns them
 // around in registers, so that its operand for dimension j of the 8 is one
 // register from each pair of words, and it ends up with 8 neighbours of a token.
-// No LDS but for the waves' sums.  14 us at 126 x 512 x 4096, 15 at 128 x 2048 x
-// 4096, 32 at 250 x 4096 x 4096: the waits for W's words bind it, some 0.8 us a turn
-// of 256, whatever is on its way; 16 waves or 64 dimensions a workgroup took 14 and
-// 13 there.  A call this small waits longer for the host.
+// No LDS but for the waves' sums.  Inside a backward 17.5 us at 126 x 512 x 4096,
+// 18.4 at 128 x 2048 x 4096, 33.4 at 250 x 4096 x 4096: the waits for W's words bind
+// it, about 1 us a turn of 256, whatever is on its way (launched again and again on
+// operands that stay in the caches 14, 15 and 32, where 16 waves or 64 dimensions a
+// workgroup took 14 and 13 at the first).  A call this small waits longer for the
+// host.
 constexpr int kHgWaves = 8;
 constexpr int kHgTokens = 16;
 constexpr int kHgColumns = 128;
