@@ -502,6 +502,41 @@ int sf_act8_pack(const void* x, int dtype, size_t n, void* packed, int format,
 int sf_act8_unpack(const void* packed, int format, size_t n, void* x, int dtype,
                    sf_stream_t stream);
 
+/* Words that sf_top_logps gives at most, and that sf_sample_tokens' top_k has to be
+ * within for a row to need no second look at its logits. */
+#define SF_TOP_MOST 128
+
+/* Bytes of workspace of the next two for [rows, vocab] logits; 0 where a size is
+ * 0 or vocab over 2^30. */
+size_t sf_rows_work(size_t rows, size_t vocab, int dtype);
+
+/* The k (1 to SF_TOP_MOST, at most vocab) largest words of each row of logits
+ * (dtype SF_DTYPE_F32, SF_DTYPE_BF16 or SF_DTYPE_F16, ld elements from row to
+ * row, any element boundary): ids[i, :], by falling logit, the first of equals
+ * first, and logps[i, :] = x / T - log sum exp(x / T).  A row with a NaN or
+ * +infinity, or of -infinities alone: ids -1, logps NaN.  temperature is above 0.
+ * work: sf_rows_work(rows, vocab, dtype) bytes on a 16-byte boundary. */
+int sf_top_logps(const void* logits, int dtype, size_t ld, size_t rows,
+                 size_t vocab, int k, double temperature, void* work,
+                 float* logps, int64_t* ids, sf_stream_t stream);
+
+/* One word for each row of logits (as above).  Words by falling logit, the first
+ * of equals first, w = exp((x - max) / T): kept are the first top_k (0 or less:
+ * all), of those the words with less than top_p of their mass before them (1 or
+ * more: all; always the first), of those the words with w >= min_p (0 or less:
+ * all; always the largest).  ids[i] = the first kept word, by its index, with
+ * whom the sum of w exceeds uniforms[i] times the kept mass; logps[i] = its x / T -
+ * log sum exp(x / T), over all words.  A temperature that is not above 0 takes the
+ * first of the largest, its log-probability being that at temperature 1.  uniforms
+ * are in [0, 1).  temperatures, top_ks, top_ps, min_ps: one for each row, or null:
+ * the value beside it for all.  Rows that cannot be drawn from: ids -1, logps NaN. */
+int sf_sample_tokens(const void* logits, int dtype, size_t ld, size_t rows,
+                     size_t vocab, const float* uniforms, double temperature,
+                     const float* temperatures, int64_t top_k,
+                     const int64_t* top_ks, double top_p, const float* top_ps,
+                     double min_p, const float* min_ps, void* work,
+                     int64_t* ids, float* logps, sf_stream_t stream);
+
 /* ---------------------------------------------------------------------
  * Copies and pinned host memory (libsf_hip.so)
  * ------------------------------------------------------------------- */

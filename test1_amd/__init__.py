@@ -32,6 +32,9 @@ def __getattr__(name):
     if name in ("pack_act8", "unpack_act8", "act8_bytes"):
         from . import act8
         return getattr(act8, name)
+    if name in ("top_logps", "sample_tokens", "TopLogps", "SampledTokens"):
+        from . import sampling
+        return getattr(sampling, name)
     if name == "LayerAdam":
         from .optimizer import LayerAdam
         return LayerAdam

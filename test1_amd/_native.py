@@ -44,6 +44,7 @@ SF_ETIMEDOUT = 9009
 SF_STAGE_SCRATCH_ELEMS = 16 << 20
 SF_CE_LOSS_PARTS = 256
 SF_LOGPS_SPAN = 256
+SF_TOP_MOST = 128
 SF_PREF_SIGMOID = 0
 SF_PREF_HINGE = 1
 SF_PREF_IPO = 2
@@ -77,6 +78,7 @@ _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 _i = ctypes.c_int
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> (argtypes) for every entry point; restype is int unless listed in
 # _RESTYPES.
@@ -125,6 +127,9 @@ HIP_SIGNATURES = {
     "sf_policy_grad": [_vp, _vp, _vp, _sz, _sz, _vp, _vp],
     "sf_act8_pack": [_vp, _i, _sz, _vp, _i, _vp],
     "sf_act8_unpack": [_vp, _i, _sz, _vp, _i, _vp],
+    "sf_rows_work": [_sz, _sz, _i],
+    "sf_top_logps": [_vp, _i, _sz, _sz, _sz, _i, _d, _vp, _vp, _vp, _vp],
+    "sf_sample_tokens": [_vp, _i, _sz, _sz, _sz, _vp, _d, _vp, ctypes.c_int64, _vp, _d, _vp, _d, _vp, _vp, _vp, _vp, _vp],
     "sf_stage_f32_bf16": [_vp, _vp, _sz, _vp, _sz, _vp],
     "sf_stage_f32_bf16_noalloc": [_vp, _vp, _sz, _sz, _vp],
     "sf_memcpy_async": [_vp, _vp, _sz, _i, _vp],
@@ -178,7 +183,7 @@ _segs = None
 _ops = None
 
 _RESTYPES = {"sf_error_string": ctypes.c_char_p, "sf_dma_choose_engines": ctypes.c_uint32,
-             "sf_align_parts": ctypes.c_size_t}
+             "sf_align_parts": ctypes.c_size_t, "sf_rows_work": ctypes.c_size_t}
 
 
 def _bind(path: str, sigs: dict) -> ctypes.CDLL:

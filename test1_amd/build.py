@@ -31,7 +31,7 @@ INCLUDE = os.path.join(ROOT, "include")
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
 OFFLOAD_ARCH = "gfx950"
-HIP_SOURCES = ("sf_hip.hip", "sf_ce.hip", "sf_logps.hip", "sf_align.hip", "sf_act8.hip")
+HIP_SOURCES = ("sf_hip.hip", "sf_ce.hip", "sf_logps.hip", "sf_align.hip", "sf_act8.hip", "sf_sample.hip")
 
 
 def _run(cmd, verbose: bool) -> None:
@@ -51,7 +51,7 @@ def build_hip(verbose: bool = False) -> str:
     os.makedirs(LIB, exist_ok=True)
     out = os.path.join(LIB, "libsf_hip.so")
     tmp = _atomic_out(out)
-    _run([HIPCC, f"--offload-arch={OFFLOAD_ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", "-parallel-jobs=5",
+    _run([HIPCC, f"--offload-arch={OFFLOAD_ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", "-parallel-jobs=8",
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
           "-I", INCLUDE, "-o", tmp, *(os.path.join(CSRC, f) for f in HIP_SOURCES), "-lhsa-runtime64"], verbose)
     os.replace(tmp, out)

@@ -1,6 +1,6 @@
 // The calls and the autograd nodes of the losses over token log-probabilities,
-// of the log-probabilities themselves and of the 8-bit checkpoints, as a
-// CPython module over the C ABI.
+// of the log-probabilities themselves, of distillation, sampling and the 8-bit
+// checkpoints, as a CPython module over the C ABI.
 //
 // In Python a loss with its gradient took 125 us of host time for two to five
 // launches, the gradient's node alone 60: the engine runs it on a thread of its
@@ -613,12 +613,76 @@ PyObject* act8_unpack(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+// Rows of logits [.., vocab] as the kernels read them.
+int logits_type(const Tensor& t) {
+    return t.scalar_type() == at::kFloat ? SF_DTYPE_F32 : t.scalar_type() == at::kBFloat16 ? SF_DTYPE_BF16 : SF_DTYPE_F16;
+}
+Tensor as_rows(const Tensor& t) { return rows(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})); }
+Tensor rows_work(const Tensor& logits) {
+    const size_t bytes = sf_rows_work(logits.size(0), logits.size(1), logits_type(logits));
+    return at::empty({int64_t(bytes)}, logits.options().dtype(at::kByte));
+}
+
+// top_logps(logits, k, temperature): (logps, ids), or None
+PyObject* top_logps(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject* o;
+    int k;
+    double temperature;
+    if (!PyArg_ParseTuple(args, "Oid", &o, &k, &temperature)) return nullptr;
+    if (!plain(o)) Py_RETURN_NONE;
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor& given = THPVariable_Unpack(o);
+    if (given.size(-1) > (int64_t(1) << 30) || given.numel() / given.size(-1) >= (int64_t(1) << 31)) Py_RETURN_NONE;
+    const c10::DeviceGuard guard(given.device());
+    const Tensor x = as_rows(given), work = rows_work(x);
+    c10::SmallVector<int64_t, 6> shape(given.sizes().begin(), given.sizes().end());
+    shape.back() = k;
+    const Tensor logps = like(x, shape), ids = at::empty(shape, x.options().dtype(at::kLong));
+    check(sf_top_logps(x.data_ptr(), logits_type(x), ld(x), x.size(0), x.size(1), k, temperature, work.data_ptr(),
+                       at_ptr<float>(logps), at_ptr<int64_t>(ids), stream_of(x)),
+          "sf_top_logps");
+    return Py_BuildValue("NN", wrap(logps), wrap(ids));
+    END_HANDLE_TH_ERRORS
+}
+
+// sample_tokens(logits, uniforms, temperature, temperatures or None, top_k, top_ks or None, top_p, top_ps or None,
+// min_p, min_ps or None): (ids, logps), or None
+PyObject* sample_tokens(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject *l, *u, *own[4];
+    double t, p, m;
+    long long k;
+    if (!PyArg_ParseTuple(args, "OOdOLOdOdO", &l, &u, &t, &own[0], &k, &own[1], &p, &own[2], &m, &own[3])) return nullptr;
+    if (!plain(l) || !plain(u)) Py_RETURN_NONE;
+    for (PyObject* o : own)
+        if (o != Py_None && !plain(o)) Py_RETURN_NONE;
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor& given = THPVariable_Unpack(l);
+    if (given.size(-1) > (int64_t(1) << 30) || given.numel() / given.size(-1) >= (int64_t(1) << 31)) Py_RETURN_NONE;
+    const c10::DeviceGuard guard(given.device());
+    const Tensor x = as_rows(given), uniforms = THPVariable_Unpack(u).contiguous(), work = rows_work(x);
+    Tensor each[4];
+    for (int i = 0; i < 4; ++i)
+        if (own[i] != Py_None) each[i] = THPVariable_Unpack(own[i]).contiguous();
+    const Tensor ids = at::empty(uniforms.sizes(), x.options().dtype(at::kLong)), logps = like(x, uniforms.sizes());
+    check(sf_sample_tokens(x.data_ptr(), logits_type(x), ld(x), x.size(0), x.size(1), at_ptr<float>(uniforms), t,
+                           at_ptr<float>(each[0]), k, at_ptr<int64_t>(each[1]), p, at_ptr<float>(each[2]), m,
+                           at_ptr<float>(each[3]), work.data_ptr(), at_ptr<int64_t>(ids), at_ptr<float>(logps),
+                           stream_of(x)),
+          "sf_sample_tokens");
+    return Py_BuildValue("NN", wrap(ids), wrap(logps));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"pref_loss", pref_loss, METH_VARARGS, "(loss, chosen, rejected), or None."},
     {"policy_loss", policy_loss, METH_VARARGS, "(loss, kl, clipped), or None."},
     {"linear_logps", linear_logps, METH_VARARGS, "Log-probabilities, or None."},
     {"act8_pack", act8_pack, METH_VARARGS, "Packed elements, or None."},
     {"act8_unpack", act8_unpack, METH_VARARGS, "Restored elements, or None."},
+    {"top_logps", top_logps, METH_VARARGS, "(logps, ids), or None."},
+    {"sample_tokens", sample_tokens, METH_VARARGS, "(ids, logps), or None."},
     {nullptr, nullptr, 0, nullptr},
 };
 
