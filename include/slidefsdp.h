@@ -502,6 +502,85 @@ int sf_act8_pack(const void* x, int dtype, size_t n, void* packed, int format,
 int sf_act8_unpack(const void* packed, int format, size_t n, void* x, int dtype,
                    sf_stream_t stream);
 
+/* Distillation under the output unit (test1_amd/distillation.py): the divergence of
+ * p = softmax(scale * hidden weight^T) from a teacher's log-probabilities of up to
+ * SF_TOP_MOST words of each token.  Words are kept by rising index; spans are
+ * SF_LOGPS_SPAN words, or (whole) one of all.
+ *
+ * sf_distill_lists: from ids and logps [rows, k] (ld_ids, ld_logps elements from
+ * row to row; -infinity: no word, whatever its id) and mask (a byte a row, or null)
+ * each token's words and teacher [rows, k], starts [rows, spans + 1] (the first word
+ * of each span; the last: how many words), status [rows]: 0 masked or without words, 1,
+ * or 2 where an id is outside [0, vocab) or there twice. */
+#define SF_DISTILL_FORWARD 0 /* sum q (log q - log p) */
+#define SF_DISTILL_REVERSE 1 /* sum p (log p - log q) */
+int sf_distill_lists(const int64_t* ids, size_t ld_ids, const float* logps,
+                     size_t ld_logps, const uint8_t* mask, size_t rows, int k,
+                     size_t vocab, int whole, int32_t* words, float* teacher,
+                     uint8_t* starts, uint8_t* status, sf_stream_t stream);
+
+/* The product of 16-bit operands, as sf_logps_tiles takes them: picked [rows, k], each
+ * token's words' hidden . weight; parts, keep as there, of all other words
+ * (keep: 16 bits of -log2 relative to the span's
+ * maximum, of 128 octaves for bf16 and 32 for fp16).  order (rows + 1 elements, or null): only rows of
+ * status 1 take part. */
+int sf_distill_tiles(const void* weight, size_t ldw, size_t vocab,
+                     const void* hidden, size_t ldh, size_t rows,
+                     size_t hidden_size, const int32_t* words,
+                     const uint8_t* starts, const uint8_t* status, int k,
+                     float scale, int dtype, void* parts, float* picked,
+                     int32_t* order, void* keep, size_t ld_keep,
+                     sf_stream_t stream);
+
+/* The same from fp32 logits (ld elements from row to row), unscaled, with one part
+ * a row (whole); leaves -infinity at the words. */
+int sf_distill_rows(float* logits, size_t ld, size_t rows, size_t vocab,
+                    const int32_t* words, const uint8_t* starts, int k,
+                    float scale, void* parts, float* picked,
+                    sf_stream_t stream);
+
+/* Each token's loss (0 of status 0, NaN of status 2) from its parts (parts_row
+ * elements from span to span) and words.  rest: all words outside the teacher's
+ * count as one outcome, of mass 1 - sum q (reverse: at least 2^-24); not: the
+ * teacher's probabilities are divided by their sum (forward only).  hidden, weight
+ * (hidden_size elements a row, of dtype): the products of likely words are formed
+ * again.  slopes [rows, k] (or null: no gradient) and stats [3, stats_row]: the
+ * derivatives by the words' logits over the token's largest one; that one, log2 of
+ * the others' sum and the derivative they share over it. */
+int sf_distill_loss(const void* parts, size_t parts_row, int whole,
+                    const float* picked, const float* teacher,
+                    const uint8_t* starts, const uint8_t* status, size_t rows,
+                    int k, size_t vocab, double scale, int form, int rest,
+                    const void* hidden, size_t ldh, const void* weight,
+                    size_t ldw, size_t hidden_size, int dtype,
+                    const int32_t* words, float* loss, float* slopes,
+                    float* stats, size_t stats_row, sf_stream_t stream);
+
+/* row_weight[i]: 1, or 0 where a row's gradient is 0 (status 0, grad 0, stats 0).
+ * norm (or null; of 16-bit dtype): what D is divided by, its largest element, for
+ * fp16 times 2^-14; and 1. */
+int sf_distill_weight(const float* grad, const float* stats,
+                      const uint8_t* status, size_t rows, float scale,
+                      int dtype, float* row_weight, float* norm,
+                      sf_stream_t stream);
+
+/* D[i, j] = grad[i] * scale * derivative / norm[0] (norm null: not divided; fp16
+ * needs it) in place of what sf_distill_tiles kept; rows from `rows` to `padded` and
+ * those without gradient become 0.  parts: `rows` elements from span to span. */
+int sf_distill_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
+                         size_t vocab, const void* parts, const int32_t* words,
+                         const uint8_t* starts, const uint8_t* status, int k,
+                         const float* slopes, const float* stats,
+                         size_t stats_row, int dtype, const float* grad,
+                         float scale, const float* norm, sf_stream_t stream);
+
+/* D, fp32, in place of fp32 logits (as sf_distill_rows takes them, before it ran). */
+int sf_distill_grad(float* logits, size_t ld, size_t rows, size_t vocab,
+                    const int32_t* words, const uint8_t* starts,
+                    const uint8_t* status, int k, float scale,
+                    const float* slopes, const float* stats, size_t stats_row,
+                    const float* grad, sf_stream_t stream);
+
 /* Words that sf_top_logps gives at most, and that sf_sample_tokens' top_k has to be
  * within for a row to need no second look at its logits. */
 #define SF_TOP_MOST 128

@@ -35,6 +35,9 @@ def __getattr__(name):
     if name in ("top_logps", "sample_tokens", "TopLogps", "SampledTokens"):
         from . import sampling
         return getattr(sampling, name)
+    if name == "linear_distill":
+        from . import distillation
+        return distillation.linear_distill
     if name == "LayerAdam":
         from .optimizer import LayerAdam
         return LayerAdam

@@ -45,6 +45,8 @@ SF_STAGE_SCRATCH_ELEMS = 16 << 20
 SF_CE_LOSS_PARTS = 256
 SF_LOGPS_SPAN = 256
 SF_TOP_MOST = 128
+SF_DISTILL_FORWARD = 0
+SF_DISTILL_REVERSE = 1
 SF_PREF_SIGMOID = 0
 SF_PREF_HINGE = 1
 SF_PREF_IPO = 2
@@ -127,6 +129,14 @@ HIP_SIGNATURES = {
     "sf_policy_grad": [_vp, _vp, _vp, _sz, _sz, _vp, _vp],
     "sf_act8_pack": [_vp, _i, _sz, _vp, _i, _vp],
     "sf_act8_unpack": [_vp, _i, _sz, _vp, _i, _vp],
+    "sf_distill_lists": [_vp, _sz, _vp, _sz, _vp, _sz, _i, _sz, _i, _vp, _vp, _vp, _vp, _vp],
+    "sf_distill_tiles": [_vp, _sz, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _i, _f, _i, _vp, _vp, _vp, _vp, _sz, _vp],
+    "sf_distill_rows": [_vp, _sz, _sz, _sz, _vp, _vp, _i, _f, _vp, _vp, _vp],
+    "sf_distill_loss": [_vp, _sz, _i, _vp, _vp, _vp, _vp, _sz, _i, _sz, _d, _i, _i, _vp, _sz, _vp, _sz, _sz, _i, _vp, _vp,
+                        _vp, _vp, _sz, _vp],
+    "sf_distill_weight": [_vp, _vp, _vp, _sz, _f, _i, _vp, _vp, _vp],
+    "sf_distill_keep_grad": [_vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _i, _vp, _vp, _sz, _i, _vp, _f, _vp, _vp],
+    "sf_distill_grad": [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _i, _f, _vp, _vp, _sz, _vp, _vp],
     "sf_rows_work": [_sz, _sz, _i],
     "sf_top_logps": [_vp, _i, _sz, _sz, _sz, _i, _d, _vp, _vp, _vp, _vp],
     "sf_sample_tokens": [_vp, _i, _sz, _sz, _sz, _vp, _d, _vp, ctypes.c_int64, _vp, _d, _vp, _d, _vp, _vp, _vp, _vp, _vp],

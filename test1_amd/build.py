@@ -31,7 +31,7 @@ INCLUDE = os.path.join(ROOT, "include")
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
 OFFLOAD_ARCH = "gfx950"
-HIP_SOURCES = ("sf_hip.hip", "sf_ce.hip", "sf_logps.hip", "sf_align.hip", "sf_act8.hip", "sf_sample.hip")
+HIP_SOURCES = ("sf_hip.hip", "sf_ce.hip", "sf_logps.hip", "sf_align.hip", "sf_act8.hip", "sf_sample.hip", "sf_distill.hip")
 
 
 def _run(cmd, verbose: bool) -> None:

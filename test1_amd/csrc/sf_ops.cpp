@@ -237,6 +237,9 @@ struct LogpsArgs {
 };
 
 int type_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? SF_DTYPE_BF16 : SF_DTYPE_F16; }
+int logits_type(const Tensor& t) {
+    return t.scalar_type() == at::kFloat ? SF_DTYPE_F32 : t.scalar_type() == at::kBFloat16 ? SF_DTYPE_BF16 : SF_DTYPE_F16;
+}
 int64_t up(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 
 // As the kernel asks for it: 16-bit operands whose rows start on 16-byte
@@ -344,47 +347,37 @@ bool own_weight_grad(int64_t n, int64_t h, int64_t v, int64_t row, bool fp16) {
 // 16384 86 | 85, 32 x 2048 x 32000 61 | 142.
 bool own_hidden_grad(int64_t n, int64_t h, int64_t v) { return v <= 8192 && n * h * v <= int64_t(1) << 32; }
 
-// Both gradients (undefined where not needed).  What was kept turns into the
-// gradient of the logits in place; without it, it is made again, `step` rows at
-// a time.
-std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
-                                         const Tensor& labels, const Tensor& logp, const Tensor& lse2, Tensor keep,
-                                         Tensor parts, const LogpsArgs& a, bool need_hidden, bool need_weight) {
-    at::AutoDispatchBelowADInplaceOrView below;
+// Both gradients (undefined where not needed) from D, `step` rows at a time, all
+// of them where it was kept.  fill(first row, rows, rows padded, their hidden rows,
+// keep, row weights, norm or null) makes D of so many rows in keep's first, and with
+// the first rows the weights of all.  divided: bf16's D may be over norm too.
+template <typename Fill>
+std::pair<Tensor, Tensor> products(const Tensor& hidden, const Tensor& weight, Tensor keep, int64_t step, int64_t nparts,
+                                   bool need_hidden, bool need_weight, bool divided, const Fill& fill) {
     const int64_t n = hidden.size(0), h = hidden.size(1), v = weight.size(0), row = up(v, SF_LOGPS_SPAN);
-    const bool kept = keep.defined(), fp16 = hidden.scalar_type() == at::kHalf;
-    const int64_t step = kept ? n : std::min(n, a.step);
+    const bool fp16 = hidden.scalar_type() == at::kHalf;
     const bool one = step == n;
     const sf_stream_t st = stream_of(hidden);
     const int type = type_of(hidden);
-    const int64_t* y = at_ptr<int64_t>(labels);
-    const float *lp = at_ptr<float>(logp), *l2 = at_ptr<float>(lse2);
-    const Tensor by = like(hidden, {n}), norm = like(hidden, {2});
+    const Tensor by = like(hidden, {n}), norms = like(hidden, {2});
     const bool own = one && own_weight_grad(n, h, v, row, fp16);
-    Tensor gh, gw, again;
+    // What D is divided by leaves before the results are rounded: in the own products, or of few
+    // tiles with a pass over them.
+    const Tensor norm = fp16 || (divided && one && (own || tiles_of(h, v) < 96)) ? norms : Tensor();
+    Tensor gh, gw;
     if (need_hidden) gh = at::empty({n, h}, hidden.options());
-    if (need_weight) gw = at::empty({v, h}, own || (one && !fp16) ? weight.options() : weight.options().dtype(at::kFloat));
-    if (!kept) {
-        keep = at::empty({up(step, 64), row}, hidden.options());
-        again = like(hidden, {2, step});
-    }
+    if (need_weight) gw = at::empty({v, h}, own || (one && !norm.defined()) ? weight.options() : weight.options().dtype(at::kFloat));
+    if (!keep.defined()) keep = at::empty({up(step, 64), row}, hidden.options());
     for (int64_t s = 0; s < n; s += step) {
         const int64_t m = std::min(n - s, step), pad = up(m, 64);
         const Tensor hc = one ? hidden : hidden.narrow(0, s, m);
-        if (!kept) {
-            float* results = at_ptr<float>(again);
-            parts = tiles(hc, weight, y + s, a, keep, results, results + step);
-        }
-        check(sf_logps_keep_grad(keep.data_ptr(), row, m, pad, v, parts.data_ptr(), y + s, a.ignore_index, l2 + s, lp + s,
-                                 type, at_ptr<float>(grad) + s, s == 0 ? n : 0, float(a.scale), at_ptr<float>(by),
-                                 at_ptr<float>(norm), fp16, st),
-              "sf_logps_keep_grad");
+        fill(s, m, pad, hc, keep, at_ptr<float>(by), at_ptr<float>(norm));
         if (need_hidden && one && own_hidden_grad(n, h, v))
             check(sf_logps_hidden_grad(keep.data_ptr(), row, n, weight.data_ptr(), weight.stride(0), v, h,
-                                       at_ptr<float>(by), fp16 ? at_ptr<float>(norm) : nullptr, type, gh.data_ptr(), st),
+                                       at_ptr<float>(by), at_ptr<float>(norm), type, gh.data_ptr(), st),
                   "sf_logps_hidden_grad");
         else if (need_hidden)
-            hidden_product(keep, m, weight, a.nparts, at_ptr<float>(by) + s, fp16 ? norm : Tensor(),
+            hidden_product(keep, m, weight, nparts, at_ptr<float>(by) + s, norm,
                            one ? gh : gh.narrow(0, s, m));
         if (!need_weight) continue;
         if (fp16 && !own) {
@@ -403,19 +396,19 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
         check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, ht.data_ptr(), pad, st),
               "sf_logps_hidden");
         if (own) {
-            check(sf_logps_weight_grad(keep.data_ptr(), row, pad, v, ht.data_ptr(), h, fp16 ? at_ptr<float>(norm) : nullptr,
+            check(sf_logps_weight_grad(keep.data_ptr(), row, pad, v, ht.data_ptr(), h, at_ptr<float>(norm),
                                        type, gw.data_ptr(), st),
                   "sf_logps_weight_grad");
             break;
         }
         const Tensor dt = keep.as_strided({v, pad}, {1, row}), hp = ht.t();
-        if (one) at::mm_out(gw, dt, hp);
+        if (one && !norm.defined()) at::mm_out(gw, dt, hp);
         else if (s == 0) at::mm_out(gw, dt, hp, at::kFloat);
         else at::addmm_out(gw, gw, dt, hp, at::kFloat);
     }
     if (need_weight && gw.scalar_type() != weight.scalar_type()) {
-        // fp16's factor leaves before the rounding
-        if (fp16) {
+        // its factor leaves before the rounding
+        if (norm.defined()) {
             const Tensor out = at::empty({v, h}, weight.options());
             check(sf_ce_scale(at_ptr<float>(norm), at_ptr<float>(norm) + 1, nullptr, nullptr, 0, at_ptr<float>(gw),
                               out.data_ptr(), size_t(v * h), type, st),
@@ -426,6 +419,27 @@ std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidde
         }
     }
     return {gh, gw};
+}
+
+std::pair<Tensor, Tensor> logps_backward(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
+                                         const Tensor& labels, const Tensor& logp, const Tensor& lse2, const Tensor& keep,
+                                         Tensor parts, const LogpsArgs& a, bool need_hidden, bool need_weight) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t n = hidden.size(0), v = weight.size(0), row = up(v, SF_LOGPS_SPAN);
+    const bool kept = keep.defined();
+    const int64_t step = kept ? n : std::min(n, a.step);
+    const int type = type_of(hidden);
+    const int64_t* y = at_ptr<int64_t>(labels);
+    Tensor again;   // results of the product made again
+    if (!kept) again = like(hidden, {2, step});
+    return products(hidden, weight, keep, step, a.nparts, need_hidden, need_weight, false,
+                    [&](int64_t s, int64_t m, int64_t pad, const Tensor& hc, const Tensor& d, float* by, float* norm) {
+        if (!kept) parts = tiles(hc, weight, y + s, a, d, at_ptr<float>(again), at_ptr<float>(again) + step);
+        check(sf_logps_keep_grad(d.data_ptr(), row, m, pad, v, parts.data_ptr(), y + s, a.ignore_index,
+                                 at_ptr<float>(lse2) + s, at_ptr<float>(logp) + s, type, at_ptr<float>(grad) + s,
+                                 s == 0 ? n : 0, float(a.scale), by, norm, type == SF_DTYPE_F16, stream_of(hidden)),
+              "sf_logps_keep_grad");
+    });
 }
 
 struct LinearLogps : torch::autograd::Function<LinearLogps> {
@@ -490,6 +504,236 @@ struct LinearLogps : torch::autograd::Function<LinearLogps> {
         }
         variable_list r = once(g, {gh, gw});
         return {r[0], r[1], Tensor(), Tensor()};
+    }
+};
+
+// ---------------------------------------------------------------------------
+// Distillation.  16-bit operands as logps_tiles_kernel takes them go through it; of
+// others a library's product leaves fp32 logits, and the gradients' products are
+// fp32, in pieces of 1 GiB.
+struct DistillArgs {
+    int64_t form;
+    bool rest;
+    double scale;
+    int64_t nparts, step;   // as LogpsArgs
+    bool keep;
+};
+
+struct DistillOut {
+    Tensor loss, keep, parts;
+    // [n, k] or as include/slidefsdp.h says, for the backward
+    Tensor words, starts, status, slopes, stats;
+};
+
+// Rows of logits of one piece.
+int64_t piece_rows(int64_t n, int64_t v) { return std::min(n, std::max(int64_t(1), (int64_t(1) << 28) / v)); }
+
+void product32(const Tensor& out, const Tensor& hidden, const Tensor& weight) {
+    Tensor to = out;
+    if (hidden.scalar_type() == at::kFloat) at::mm_out(to, hidden, weight.t());
+    else at::mm_out(to, hidden, weight.t(), at::kFloat);
+}
+
+Tensor distill_tiles(const Tensor& hidden, const Tensor& weight, const Tensor& words, const Tensor& starts,
+                     const Tensor& status, int64_t first, double scale, const Tensor& keep, const Tensor& picked) {
+    const int64_t n = hidden.size(0), v = weight.size(0), k = words.size(1);
+    const int64_t held = 2 * n * ((v + SF_LOGPS_SPAN - 1) / SF_LOGPS_SPAN);
+    const bool skip = skips_rows(n, hidden.size(1), v) && 2 * n * hidden.stride(0) <= int64_t(UINT32_MAX);
+    const Tensor parts = like(hidden, {held + (skip ? n + 1 : 0)});
+    int32_t* order = skip ? reinterpret_cast<int32_t*>(at_ptr<float>(parts) + held) : nullptr;
+    check(sf_distill_tiles(weight.data_ptr(), weight.stride(0), v, hidden.data_ptr(), hidden.stride(0), n, hidden.size(1),
+                           at_ptr<int32_t>(words) + first * k, at_ptr<uint8_t>(starts) + first * starts.size(1),
+                           at_ptr<uint8_t>(status) + first, int(k), float(scale), type_of(hidden), parts.data_ptr(),
+                           at_ptr<float>(picked), order, keep.defined() ? keep.data_ptr() : nullptr,
+                           keep.defined() ? keep.stride(0) : 0, stream_of(hidden)),
+          "sf_distill_tiles");
+    return parts;
+}
+
+DistillOut distill_forward(const Tensor& hidden_, const Tensor& weight_, const Tensor& ids_, const Tensor& logps_,
+                           const Tensor& mask, const DistillArgs& a, bool grad) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor ids = rows(ids_), logps = rows(logps_), hidden = rows(hidden_), weight = rows(weight_);
+    const int64_t n = hidden.size(0), v = weight.size(0), k = ids.size(1);
+    const bool whole = !in_tiles(hidden_, weight_);
+    const int64_t spans = whole ? 1 : (v + SF_LOGPS_SPAN - 1) / SF_LOGPS_SPAN;
+    const sf_stream_t st = stream_of(hidden);
+    const auto bytes = hidden.options().dtype(at::kByte);
+    DistillOut o;
+    o.loss = like(hidden, {n});
+    o.words = at::empty({n, k}, hidden.options().dtype(at::kInt));
+    o.starts = at::empty({n, spans + 1}, bytes);
+    o.status = at::empty({n}, bytes);
+    const Tensor lists = like(hidden, {2, n, k});   // the teacher's, the products
+    float *teacher = at_ptr<float>(lists), *picked = teacher + n * k;
+    if (grad) o.slopes = like(hidden, {n, k}), o.stats = like(hidden, {3, n});
+    check(sf_distill_lists(at_ptr<int64_t>(ids), ld(ids), at_ptr<float>(logps), ld(logps), at_ptr<uint8_t>(mask), n, int(k), v,
+                           whole, at_ptr<int32_t>(o.words), teacher, at_ptr<uint8_t>(o.starts), at_ptr<uint8_t>(o.status), st),
+          "sf_distill_lists");
+    if (whole) {
+        const int64_t step = piece_rows(n, v);
+        const Tensor buf = like(hidden, {step, v});
+        o.parts = like(hidden, {n, 2});
+        for (int64_t s = 0; s < n; s += step) {
+            const int64_t m = std::min(step, n - s);
+            product32(buf.narrow(0, 0, m), hidden.narrow(0, s, m), weight);
+            check(sf_distill_rows(at_ptr<float>(buf), v, m, v, at_ptr<int32_t>(o.words) + s * k,
+                                  at_ptr<uint8_t>(o.starts) + s * 2, int(k), float(a.scale), at_ptr<float>(o.parts) + 2 * s,
+                                  picked + s * k, st),
+                  "sf_distill_rows");
+        }
+    } else {
+        if (a.keep && grad) o.keep = at::empty({up(n, 64), up(v, SF_LOGPS_SPAN)}, hidden.options());
+        o.parts = distill_tiles(hidden, weight, o.words, o.starts, o.status, 0, a.scale, o.keep, lists.select(0, 1));
+    }
+    check(sf_distill_loss(o.parts.data_ptr(), n, whole, picked, teacher, at_ptr<uint8_t>(o.starts), at_ptr<uint8_t>(o.status),
+                          n, int(k), v, a.scale, int(a.form), a.rest, hidden.data_ptr(), ld(hidden), weight.data_ptr(),
+                          ld(weight), hidden.size(1), logits_type(hidden), at_ptr<int32_t>(o.words), at_ptr<float>(o.loss), at_ptr<float>(o.slopes),
+                          at_ptr<float>(o.stats), n, st),
+          "sf_distill_loss");
+    return o;
+}
+
+// Both gradients by fp32 products of whole logits, in pieces.
+std::pair<Tensor, Tensor> distill_backward_whole(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
+                                                 const DistillOut& o, const DistillArgs& a, bool need_hidden,
+                                                 bool need_weight) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t n = hidden.size(0), v = weight.size(0), k = o.words.size(1), step = piece_rows(n, v);
+    const Tensor none = at::zeros({}, grad.options());
+    const Tensor by = at::where(o.status.eq(0).logical_or(grad.eq(0)), none, grad * a.scale * o.stats.select(0, 0)).unsqueeze(1);
+    const Tensor buf = like(hidden, {step, v});
+    const Tensor w32 = need_hidden ? weight.to(at::kFloat) : Tensor();
+    Tensor gh, gw;
+    if (need_hidden) gh = like(hidden, hidden.sizes());
+    if (need_weight) gw = at::zeros(weight.sizes(), grad.options());
+    for (int64_t s = 0; s < n; s += step) {
+        const int64_t m = std::min(step, n - s);
+        const Tensor d = buf.narrow(0, 0, m), f = by.narrow(0, s, m);
+        product32(d, hidden.narrow(0, s, m), weight);
+        check(sf_distill_grad(at_ptr<float>(buf), v, m, v, at_ptr<int32_t>(o.words) + s * k, at_ptr<uint8_t>(o.starts) + s * 2,
+                              at_ptr<uint8_t>(o.status) + s, int(k), float(a.scale), at_ptr<float>(o.slopes) + s * k,
+                              at_ptr<float>(o.stats) + s, n, at_ptr<float>(grad) + s, stream_of(hidden)),
+              "sf_distill_grad");
+        if (need_hidden) {
+            Tensor to = gh.narrow(0, s, m);
+            at::mm_out(to, d, w32);
+            to.mul_(f).masked_fill_(f == 0, 0);
+        }
+        if (need_weight) {
+            const Tensor h = hidden.narrow(0, s, m).to(at::kFloat).masked_fill(f == 0, 0) * f;
+            at::addmm_out(gw, gw, d.t(), h);
+        }
+    }
+    if (need_hidden) gh = gh.to(hidden.scalar_type());
+    if (need_weight) gw = gw.to(weight.scalar_type());
+    return {gh, gw};
+}
+
+std::pair<Tensor, Tensor> distill_backward(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
+                                           const DistillOut& o, const DistillArgs& a, bool need_hidden, bool need_weight) {
+    if (!in_tiles(hidden, weight)) return distill_backward_whole(grad, hidden, weight, o, a, need_hidden, need_weight);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t n = hidden.size(0), v = weight.size(0), k = o.words.size(1), row = up(v, SF_LOGPS_SPAN);
+    const bool kept = o.keep.defined();
+    const int64_t step = kept ? n : std::min(n, a.step);
+    const int type = type_of(hidden);
+    Tensor parts = o.parts, again;   // products of the words, made again
+    if (!kept) again = like(hidden, {step, k});
+    return products(hidden, weight, o.keep, step, a.nparts, need_hidden, need_weight, true,
+                    [&](int64_t s, int64_t m, int64_t pad, const Tensor& hc, const Tensor& d, float* by, float* norm) {
+        if (!kept) parts = distill_tiles(hc, weight, o.words, o.starts, o.status, s, a.scale, d, again);
+        if (s == 0)
+            check(sf_distill_weight(at_ptr<float>(grad), at_ptr<float>(o.stats), at_ptr<uint8_t>(o.status), n, float(a.scale),
+                                    type, by, norm, stream_of(hidden)),
+                  "sf_distill_weight");
+        check(sf_distill_keep_grad(d.data_ptr(), row, m, pad, v, parts.data_ptr(), at_ptr<int32_t>(o.words) + s * k,
+                                   at_ptr<uint8_t>(o.starts) + s * o.starts.size(1), at_ptr<uint8_t>(o.status) + s, int(k),
+                                   at_ptr<float>(o.slopes) + s * k, at_ptr<float>(o.stats) + s, n, type,
+                                   at_ptr<float>(grad) + s, float(a.scale), norm, stream_of(hidden)),
+              "sf_distill_keep_grad");
+    });
+}
+
+// The gradients by torch operations, where what was saved came back as something else.
+std::pair<Tensor, Tensor> distill_backward_torch(const Tensor& grad_, const Tensor& hidden, const Tensor& weight,
+                                                 const DistillOut& o, const DistillArgs& a, bool need_hidden,
+                                                 bool need_weight) {
+    const Tensor grad = grad_.to(at::kFloat), w = weight.to(at::kFloat), stats = o.stats.to(at::kFloat);
+    const Tensor taught = o.status.eq(1), bad = o.status.eq(2), counts = grad.ne(0).logical_and(o.status.ne(0));
+    const Tensor h = at::where(counts.unsqueeze(1), hidden.to(at::kFloat), at::zeros({}, w.options()));
+    const int64_t v = w.size(0), k = o.words.size(1);
+    // a token's words: those before its last count; the others' slots go to a column behind
+    const Tensor n = o.starts.select(1, o.starts.size(1) - 1).to(at::kLong).unsqueeze(1);
+    const Tensor there = at::arange(k, n.options()).unsqueeze(0) < n;
+    const Tensor at = at::where(there, o.words.to(at::kLong), at::full_like(n, v));
+    const Tensor z = at::matmul(h, w.t()) * (a.scale / std::log(2.0));
+    Tensor d = at::exp2(z - stats.select(0, 1).unsqueeze(1)) * stats.select(0, 2).unsqueeze(1);
+    d = at::cat({d, at::zeros({d.size(0), 1}, d.options())}, 1);
+    d = d.scatter(1, at, at::where(there, o.slopes.to(at::kFloat), at::zeros({}, d.options()))).narrow(1, 0, v);
+    d = d * (grad * a.scale * stats.select(0, 0)).unsqueeze(1);
+    d = at::where(counts.logical_and(taught).unsqueeze(1), d, at::zeros_like(d));
+    d = at::where(counts.logical_and(bad).unsqueeze(1), at::full_like(d, NAN), d);
+    Tensor gh, gw;
+    if (need_hidden) gh = at::matmul(d, w).to(hidden.scalar_type());
+    if (need_weight) gw = at::matmul(d.t(), h).to(weight.scalar_type());
+    return {gh, gw};
+}
+
+struct LinearDistill : torch::autograd::Function<LinearDistill> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
+                          const Tensor& logps, const c10::optional<Tensor>& mask, const DistillArgs& a) {
+        DistillOut o = distill_forward(hidden, weight, ids, logps, mask.has_value() ? *mask : Tensor(), a, true);
+        ctx->save_for_backward({hidden, weight, o.words, o.starts, o.status, o.slopes, o.stats});
+        ctx->set_materialize_grads(false);
+        // not among the saved tensors: the backward overwrites it, and gives it up
+        if (o.keep.defined()) {
+            ctx->saved_data["keep"] = o.keep;
+            ctx->saved_data["parts"] = o.parts;
+        }
+        ctx->saved_data["scale"] = a.scale;
+        ctx->saved_data["nparts"] = a.nparts;
+        ctx->saved_data["step"] = a.step;
+        return o.loss;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor& g = grads[0];
+        if (!g.defined()) return variable_list(6);
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &hidden = saved[0], &weight = saved[1];
+        DistillOut o;
+        o.words = saved[2], o.starts = saved[3], o.status = saved[4], o.slopes = saved[5], o.stats = saved[6];
+        auto& data = ctx->saved_data;
+        const DistillArgs a = {0, true, data["scale"].toDouble(), data["nparts"].toInt(), data["step"].toInt(), false};
+        const bool need_hidden = ctx->needs_input_grad(0), need_weight = ctx->needs_input_grad(1);
+        Tensor gh, gw;
+        {
+            at::NoGradGuard none;
+            const c10::Device dev = g.device();
+            const bool tiles = hidden.device() == dev && weight.device() == dev && in_tiles(hidden, weight);
+            const int64_t spans = tiles ? (weight.size(0) + SF_LOGPS_SPAN - 1) / SF_LOGPS_SPAN : 1;
+            if (dev.is_cuda() && memory_is_value(g) && hidden.device() == dev && weight.device() == dev &&
+                memory_is_value(hidden) && memory_is_value(weight) && weight.scalar_type() == hidden.scalar_type() &&
+                as_saved(o.words, at::kInt, dev) && as_saved(o.starts, at::kByte, dev) && o.starts.size(1) == spans + 1 &&
+                as_saved(o.status, at::kByte, dev) && as_saved(o.slopes, at::kFloat, dev) &&
+                as_saved(o.stats, at::kFloat, dev) && (!tiles || a.nparts == 1 || weight.is_contiguous())) {
+                const c10::DeviceGuard guard(dev);
+                if (auto it = data.find("keep"); it != data.end()) {
+                    o.keep = it->second.toTensor();
+                    o.parts = data["parts"].toTensor();
+                    // a second backward of a retained graph makes it again
+                    data.erase("keep");
+                    data.erase("parts");
+                }
+                std::tie(gh, gw) = distill_backward(g.to(at::kFloat).contiguous(), hidden, weight, o, a, need_hidden,
+                                                    need_weight);
+            } else {
+                std::tie(gh, gw) = distill_backward_torch(g, hidden, weight, o, a, need_hidden, need_weight);
+            }
+        }
+        variable_list r = once(g, {gh, gw});
+        return {r[0], r[1], Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -564,6 +808,29 @@ PyObject* linear_logps(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+// linear_distill(hidden, weight, ids, logps, mask or None, form, rest, scale, nparts, step, keep): each token's
+// loss, or None
+PyObject* linear_distill(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject *h, *w, *i, *l, *m;
+    int form, rest, keep;
+    double scale;
+    long long nparts, step;
+    if (!PyArg_ParseTuple(args, "OOOOOipdLLp", &h, &w, &i, &l, &m, &form, &rest, &scale, &nparts, &step, &keep)) return nullptr;
+    if (!plain(h) || !plain(w) || !plain(i) || !plain(l) || (m != Py_None && !plain(m))) Py_RETURN_NONE;
+    const Tensor &hidden = THPVariable_Unpack(h), &weight = THPVariable_Unpack(w);
+    const Tensor &ids = THPVariable_Unpack(i), &logps = THPVariable_Unpack(l);
+    if (hidden.numel() == 0) Py_RETURN_NONE;
+    const c10::DeviceGuard guard(hidden.device());
+    const Tensor mask = m == Py_None ? Tensor() : THPVariable_Unpack(m).contiguous();
+    const bool grad = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad());
+    const DistillArgs a = {form, rest != 0, scale, nparts, step, keep != 0};
+    if (!grad) return wrap(distill_forward(hidden, weight, ids, logps, mask, a, false).loss);
+    const c10::optional<Tensor> given = mask.defined() ? c10::optional<Tensor>(mask) : c10::nullopt;
+    return wrap(LinearDistill::apply(hidden, weight, ids, logps, given, a));
+    END_HANDLE_TH_ERRORS
+}
+
 // act8_pack(x, dtype, format, bytes): packed, or None
 PyObject* act8_pack(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
@@ -614,9 +881,6 @@ PyObject* act8_unpack(PyObject*, PyObject* args) {
 }
 
 // Rows of logits [.., vocab] as the kernels read them.
-int logits_type(const Tensor& t) {
-    return t.scalar_type() == at::kFloat ? SF_DTYPE_F32 : t.scalar_type() == at::kBFloat16 ? SF_DTYPE_BF16 : SF_DTYPE_F16;
-}
 Tensor as_rows(const Tensor& t) { return rows(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})); }
 Tensor rows_work(const Tensor& logits) {
     const size_t bytes = sf_rows_work(logits.size(0), logits.size(1), logits_type(logits));
@@ -679,6 +943,7 @@ PyMethodDef methods[] = {
     {"pref_loss", pref_loss, METH_VARARGS, "(loss, chosen, rejected), or None."},
     {"policy_loss", policy_loss, METH_VARARGS, "(loss, kl, clipped), or None."},
     {"linear_logps", linear_logps, METH_VARARGS, "Log-probabilities, or None."},
+    {"linear_distill", linear_distill, METH_VARARGS, "Each token's loss, or None."},
     {"act8_pack", act8_pack, METH_VARARGS, "Packed elements, or None."},
     {"act8_unpack", act8_unpack, METH_VARARGS, "Restored elements, or None."},
     {"top_logps", top_logps, METH_VARARGS, "(logps, ids), or None."},
