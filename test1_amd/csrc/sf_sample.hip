@@ -13,7 +13,10 @@
 // its mass relative to that, and what the row's border will need: the words that
 // may be among the k largest of it, or a histogram of its masses.  The chip is
 // filled by parts, whatever the rows.  A workgroup for each row then joins its
-// parts and finds the border and the word, reading again what it needs.  Rows
+// parts.  The k largest are picked from the parts' lists by one wave, without a
+// barrier.  A border by mass lies in one bin of the joined histograms, whose few
+// hundred words are read and binned again; the histograms also say how much of its
+// mass each part keeps, so that the word is looked for in one part alone.  Rows
 // whose words tie or spread so that this does not do (more candidates than their
 // lists hold, a border below the histogram) find their border by radix passes
 // over the row.
@@ -36,10 +39,12 @@ namespace {
 constexpr uint32_t kMost = SF_TOP_MOST;   // words that the parts' lists are made for
 constexpr uint32_t kPartLanes = 256;
 constexpr uint32_t kPartVectors = 8;      // of a lane
-constexpr uint32_t kList = 512;           // candidates of a part, of a row's only part twice as many
-constexpr uint32_t kBins = 256;           // of a part's histogram, T / kBinsOfT of logit each
-constexpr float kBinsOfT = 16.0f;
-constexpr uint32_t kSorted = 4096;        // candidates that a row sorts in LDS
+constexpr uint32_t kBins = 512;           // of a part's histogram, T / kBinsOfT of logit each
+constexpr float kBinsOfT = 32.0f;
+constexpr uint32_t kList = kBins + kBins / 4;   // candidates of a part, of a row's only part twice as many
+constexpr uint32_t kSubBins = 1024;       // of a bin
+constexpr uint32_t kDigit = 8;            // bits of a radix pass
+constexpr uint32_t kMostParts = 64;       // of a row that goes by histograms
 constexpr float kNegInf = -__builtin_inff();
 
 // fp32 rows beside the 16-bit formats: what a 16-byte vector holds.
@@ -143,7 +148,6 @@ struct Rows {
     int64_t top_k;
     const float *temperatures, *top_ps, *min_ps;
     const int64_t* top_ks;
-    bool top_only;              // no draw: the k largest
     float* logps;
     int64_t* ids;
     const float* uniforms;
@@ -153,9 +157,11 @@ struct Settings {
     double t, top_p, min_p;
     uint32_t k;       // vocab: every word
     bool listed;      // by the parts' lists, else by masses
-    bool filtered;    // of the latter: not every word is kept
-    bool bins;        // of those: a border to find
+    bool filtered;    // of the latter: not every word is kept, and the parts leave histograms
 };
+// What the host knows of a call's rows: kListed and kFiltered as above, kWhole neither.
+enum Kind { kEither, kListed, kFiltered, kWhole };
+template <Kind kKind>
 __device__ __forceinline__ Settings settings(const Rows& a, uint64_t row) {
     Settings s;
     s.t = a.temperatures != nullptr ? double(a.temperatures[row]) : a.temperature;
@@ -165,10 +171,8 @@ __device__ __forceinline__ Settings settings(const Rows& a, uint64_t row) {
     s.k = k <= 0 || k >= int64_t(a.vocab) ? a.vocab : uint32_t(k);
     if (!(s.t > 0.0)) s.t = 1.0, s.k = 1;   // the largest
     s.t = fmin(fmax(s.t, 1e-30), 1e30);     // so that neither it nor its inverse is infinite in fp32
-    s.listed = a.top_only || s.k <= kMost;
-    if (a.top_only) s.k = uint32_t(a.top_k);
-    s.bins = s.top_p < 1.0 || s.k < a.vocab;
-    s.filtered = s.bins || s.min_p > 0.0;
+    s.listed = kKind == kListed || (kKind == kEither && s.k <= kMost);
+    s.filtered = kKind == kFiltered || (kKind != kWhole && (s.top_p < 1.0 || s.k < a.vocab || s.min_p > 0.0));
     return s;
 }
 
@@ -196,7 +200,14 @@ struct Add {
 __device__ __forceinline__ float bin_scale(double t) { return float(double(kBinsOfT) / t); }
 
 // ---------------------------------------------------------------------
-template <typename E, uint32_t kV>
+// What was read is used once more: no converted copies of it stay in registers meanwhile.
+template <uint32_t kV>
+__device__ __forceinline__ void afresh(u32x4 (&x)[kV]) {
+#pragma unroll
+    for (uint32_t i = 0; i < kV; ++i) asm volatile("" : "+v"(x[i]));
+}
+
+template <typename E, uint32_t kV, Kind kKind>
 __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
     constexpr uint32_t kN = kOf<E>;
     __shared__ float shared_m[kPartLanes / 64];
@@ -208,7 +219,6 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
     float* const most = reinterpret_cast<float*>(mass);   // [kPartLanes]
     const uint64_t row = blockIdx.x / a.parts;
     const uint32_t part = blockIdx.x % a.parts;
-    const Settings s = settings(a, a.first + row);
     const Row<E> r(a.logits, a.ld, a.first + row, a.vocab);
     u32x4 x[kV];
 #pragma unroll
@@ -216,6 +226,7 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
         const uint32_t in = i * kPartLanes + threadIdx.x, v = part * a.per + in;
         x[i] = in < a.per && v < r.vectors ? r.load(v) : nothing<E>();
     }
+    const Settings s = settings<kKind>(a, a.first + row);
     float mine = kNegInf;
 #pragma unroll
     for (uint32_t i = 0; i < kV; ++i)
@@ -226,18 +237,31 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
     Part* const out = a.part + row * a.parts + part;
     uint64_t* const list = a.lists + (row * a.parts + part) * a.list;
     const float from = base(m);
+    afresh(x);
 
     if (s.listed) {
+        // 2^(c x - from c), from c rounded, which the sum makes up for at its end; of a largest
+        // logit near the type's lowest value, where that is infinite, 2^(c (x - from))
         const float c = float(double(kLog2e) / s.t);
+        const bool far = !(fabsf(from * c) < 0x1p100f);
+        const float less = far ? 0.0f : from * c;
         float sum = 0.0f;
+        if (far) {
 #pragma unroll
-        for (uint32_t i = 0; i < kV; ++i)
+            for (uint32_t i = 0; i < kV; ++i)
 #pragma unroll
-            for (uint32_t j = 0; j < kN; ++j) sum += __builtin_amdgcn_exp2f((item<E>(x[i], j) - from) * c);
+                for (uint32_t j = 0; j < kN; ++j) sum += __builtin_amdgcn_exp2f((item<E>(x[i], j) - from) * c);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kV; ++i)
+#pragma unroll
+                for (uint32_t j = 0; j < kN; ++j) sum += __builtin_amdgcn_exp2f(fmaf(item<E>(x[i], j), c, -less));
+        }
+        afresh(x);
         // A bound with k words of the part or more above it: the k-th largest of the
         // lanes' maxima, to 16 bits.  Of 256 lanes about 256 ln(256 / (256 - k)) words are.
         most[threadIdx.x] = mine;
-        const double total = block_all<kPartLanes>(double(sum), shared_s, Add{});
+        const double total = block_all<kPartLanes>(double(sum), shared_s, Add{}) * (far ? 1.0 : exp2_wide(double(less) - double(from) * double(c)));
         if (threadIdx.x < 64) {
             uint32_t keys[kPartLanes / 64];
 #pragma unroll
@@ -250,6 +274,7 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
 #pragma unroll
                 for (uint32_t i = 0; i < kPartLanes / 64; ++i) n += __popcll(__ballot(keys[i] >= with));
                 if (n >= s.k) bound = with;
+                if (n == s.k) break;
             }
             if (threadIdx.x == 0) bound_of = float_of(bound << 16);
         }
@@ -273,22 +298,23 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
     }
     const double c = 1.4426950408889634073599 / s.t;
     const float scale = bin_scale(s.t), top_bin = floorf(m * scale);
-    if (s.bins) {
-        mass[threadIdx.x] = 0, number[threadIdx.x] = 0;
+    if (s.filtered) {
+        for (uint32_t i = threadIdx.x; i < kBins; i += kPartLanes) mass[i] = 0, number[i] = 0;
         __syncthreads();
     }
     // a part has at most 2^14 words: whole numbers of 2^-48
     double sum = 0.0;
     bool nan = false;
 #pragma unroll
-    for (uint32_t i = 0; i < kV; ++i)
+    for (uint32_t i = 0; i < kV; ++i) {
+        asm volatile("" : "+v"(x[i]), "+v"(sum));   // a vector's words after the last one's: few registers
 #pragma unroll
         for (uint32_t j = 0; j < kN; ++j) {
             const float f = item<E>(x[i], j);
             nan |= f != f;
             const double w = exp2_wide((double(f) - double(from)) * c);
             sum += w;
-            if (s.bins) {
+            if (s.filtered) {
                 const float bin = top_bin - floorf(f * scale);
                 if (bin >= 0.0f && bin < float(kBins)) {
                     atomicAdd(reinterpret_cast<unsigned long long*>(&mass[uint32_t(bin)]),
@@ -297,13 +323,14 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
                 }
             }
         }
+    }
     if (nan) sum = __builtin_nan("");
     sum = block_all<kPartLanes>(sum, shared_s, Add{});
-    if (s.bins) {
-        static_assert(kBins + kBins / 2 <= kList, "a list holds them");
-        list[threadIdx.x] = mass[threadIdx.x];
-        reinterpret_cast<uint32_t*>(list + kBins)[threadIdx.x] = number[threadIdx.x];
-    }
+    if (s.filtered)
+        for (uint32_t i = threadIdx.x; i < kBins; i += kPartLanes) {
+            list[i] = mass[i];
+            reinterpret_cast<uint16_t*>(list + kBins)[i] = uint16_t(number[i]);
+        }
     if (threadIdx.x == 0) *out = Part{m, 0, sum};
 }
 
@@ -314,69 +341,64 @@ struct Joined {
     double sum;   // of exp((x - m) / T)
     bool bad;     // a NaN, an infinity, nothing but -inf
 };
+__device__ __forceinline__ double mass_of(const Part& p, float m, double c) {   // in that of the row's largest weight
+    return p.m > kNegInf || p.sum != p.sum ? p.sum * exp2_wide((double(p.m) - double(m)) * c) : 0.0;
+}
 template <uint32_t kT>
 __device__ Joined join_parts(const Rows& a, const Part* part, double c, double* shared) {
-    float m = kNegInf;
-    for (uint32_t p = threadIdx.x; p < a.parts; p += kT) m = fmaxf(m, part[p].m);
+    const Part own = threadIdx.x < a.parts ? part[threadIdx.x] : Part{kNegInf, 0, 0.0};
+    float m = own.m;
+    for (uint32_t p = threadIdx.x + kT; p < a.parts; p += kT) m = fmaxf(m, part[p].m);
     m = block_all<kT>(m, reinterpret_cast<float*>(shared), Max{});
     if (__builtin_isinf(m)) return {m, 0.0, true};
-    double sum = 0.0;
-    for (uint32_t p = threadIdx.x; p < a.parts; p += kT)
-        if (part[p].m > kNegInf || part[p].sum != part[p].sum) sum += part[p].sum * exp2_wide((double(part[p].m) - double(m)) * c);
+    double sum = mass_of(own, m, c);
+    for (uint32_t p = threadIdx.x + kT; p < a.parts; p += kT) sum += mass_of(part[p], m, c);
     sum = block_all<kT>(sum, shared, Add{});
     return {m, sum, !(sum > 0.0)};
 }
 
-// places[0 .. n), n a power of two, by falling place.
-template <uint32_t kT>
-__device__ void sort_places(uint64_t* places, uint32_t n) {
-    for (uint32_t size = 2; size <= n; size <<= 1)
-        for (uint32_t d = size >> 1; d > 0; d >>= 1) {
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < n / 2; i += kT) {
-                const uint32_t lo = (i & ~(d - 1)) << 1 | (i & (d - 1)), hi = lo | d;
-                const uint64_t u = places[lo], v = places[hi];
-                if ((u < v) == ((lo & size) == 0)) places[lo] = v, places[hi] = u;
-            }
-        }
-    __syncthreads();
-}
-template <uint32_t kT>
-__device__ uint32_t sort_padded(uint64_t* places, uint32_t n) {
-    uint32_t pad = 2;
-    while (pad < n) pad <<= 1;
-    for (uint32_t i = n + threadIdx.x; i < pad; i += kT) places[i] = 0;
-    sort_places<kT>(places, pad);
-    return pad;
-}
-
 // What a row's workgroup has in LDS.
+template <uint32_t kSorted_>
 struct Shared {
+    static constexpr uint32_t kSorted = kSorted_;   // candidates that it holds
     union {
         uint64_t places[kSorted];
         struct {
-            uint64_t mass[2048];
-            uint32_t number[2048];
+            uint64_t mass[1 << kDigit];
+            uint32_t number[1 << kDigit];
         } digits;
-        struct {
-            uint64_t mass[kBins];
-            uint32_t number[kBins];
-        } bins;
     };
-    double waves[16];
+    uint64_t few[256];       // the k largest, sorted, or a border's neighbours
     double weights[kMost];
-    uint32_t count, found_index;
+    double waves[16];        // of the block's sums
+    uint64_t scan_m[16];
+    uint32_t scan_n[16];
+    uint32_t count, found_index, found_count, tied, held;
     uint64_t found;
     double found_mass;
-    uint32_t found_count, tied;
+};
+// What a row that goes by histograms has beside it.
+struct Bins {
+    union {
+        uint64_t mass[kBins];
+        uint64_t sub_mass[kSubBins];
+    };
+    union {
+        uint32_t number[kBins];
+        uint32_t sub_number[kSubBins];
+    };
+    uint64_t kept[kMostParts];    // mass of each part
+    double factor[kMostParts];    // 2^-44 of the row's largest weight in 2^-48 of the part's
+    float offset[kMostParts];     // bins from the row's first to the part's
+    float bin;                    // whose words are held; -1: none
 };
 
 // The bin, of kN in falling order, in which a running count or mass first comes to `reach`,
 // `before` of it ahead of all bins; kN where none does.  Left in sh with what comes before it
 // and its number of words.
-template <uint32_t kT, uint32_t kN>
+template <uint32_t kT, uint32_t kN, typename Sh>
 __device__ void find_bin(const uint64_t* mass, const uint32_t* number, bool by_mass, uint64_t reach, uint64_t before_mass,
-                         uint32_t before, Shared& sh) {
+                         uint32_t before, Sh& sh) {
     constexpr uint32_t kEach = (kN + kT - 1) / kT;
     const uint32_t bin0 = threadIdx.x * kEach;
     uint64_t m = 0;
@@ -391,15 +413,13 @@ __device__ void find_bin(const uint64_t* mass, const uint32_t* number, bool by_m
         const uint32_t below_n = __shfl_up(upto_n, d);
         if ((threadIdx.x & 63) >= uint32_t(d)) upto_m += below_m, upto_n += below_n;
     }
-    uint64_t* const waves_m = reinterpret_cast<uint64_t*>(sh.waves);
-    uint32_t* const waves_n = reinterpret_cast<uint32_t*>(sh.weights);
     __syncthreads();
-    if ((threadIdx.x & 63) == 63) waves_m[threadIdx.x >> 6] = upto_m, waves_n[threadIdx.x >> 6] = upto_n;
+    if ((threadIdx.x & 63) == 63) sh.scan_m[threadIdx.x >> 6] = upto_m, sh.scan_n[threadIdx.x >> 6] = upto_n;
     if (threadIdx.x == 0) sh.found_index = kN;
     __syncthreads();
     uint64_t at_m = before_mass + upto_m - m;
     uint32_t at_n = upto_n - n;   // of these bins
-    for (uint32_t w = 0; w < threadIdx.x >> 6; ++w) at_m += waves_m[w], at_n += waves_n[w];
+    for (uint32_t w = 0; w < threadIdx.x >> 6; ++w) at_m += sh.scan_m[w], at_n += sh.scan_n[w];
     for (uint32_t i = 0; i < kEach && bin0 + i < kN; ++i) {
         const uint64_t next_m = at_m + mass[bin0 + i];
         const uint32_t next_n = at_n + number[bin0 + i];
@@ -417,8 +437,8 @@ __device__ void find_bin(const uint64_t* mass, const uint32_t* number, bool by_m
 // added up, and the first word that takes the sum above `target` is found; where rounding
 // leaves none, the last with a weight.  Every wave has a run of the row's vectors from v0
 // to v1.  share: the target is that of the whole sum.
-template <typename E, uint32_t kT, typename Weight>
-__device__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double target, bool share, Weight weight, Shared& sh) {
+template <typename E, uint32_t kT, typename Weight, typename Sh>
+__device__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double target, bool share, Weight weight, Sh& sh) {
     constexpr uint32_t kWaves = kT / 64;
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t each = (v1 - v0 + kWaves - 1) / kWaves;
@@ -515,12 +535,13 @@ __device__ __forceinline__ void each_word(const Row<E>& r, F f) {
     }
 }
 
-// The border of a row by three passes over the digits of its words' keys: the place of the last
+// The border of a row by passes over the digits of its words' keys: the place of the last
 // word of the prefix that a count (so many words) or a mass (the words with less than `reach`
 // before them) asks for, 0 for every word.  prefix_mass: of the prefix, or null.
-template <typename E, uint32_t kT>
+template <typename E, uint32_t kT, typename Sh>
 __device__ uint64_t border_by_digits(const Row<E>& r, float m, double c, bool by_mass, double reach, double* prefix_mass,
-                                     Shared& sh) {
+                                     Sh& sh) {
+    constexpr uint32_t kDigits = 1 << kDigit;
     // masses in whole numbers whose sum 62 bits hold
     const int bits = 62 - (32 - __builtin_clz(r.vocab));
     const double one = ldexp(1.0, bits);
@@ -528,25 +549,25 @@ __device__ uint64_t border_by_digits(const Row<E>& r, float m, double c, bool by
     const uint64_t target = by_mass ? uint64_t(ceil(fmax(reach, 0.0) * one)) : uint64_t(reach);
     uint32_t prefix = 0, known = 0, before = 0;
     uint64_t before_mass = 0;
-    for (int pass = 0; pass < 3; ++pass) {
-        const uint32_t width = pass < 2 ? 11 : 10, left = 32 - known - width;
+    while (known < 32) {
+        const uint32_t left = 32 - known - kDigit;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < 2048; i += kT) sh.digits.mass[i] = 0, sh.digits.number[i] = 0;
+        for (uint32_t i = threadIdx.x; i < kDigits; i += kT) sh.digits.mass[i] = 0, sh.digits.number[i] = 0;
         __syncthreads();
         each_word<E, kT>(r, [&](float f, uint32_t) {
             if (!(f > kNegInf)) return;
             const uint32_t key = key_of(f);
             if (known > 0 && (key >> (32 - known)) != prefix) return;
-            const uint32_t bin = 2047 - ((key >> left) & ((1u << width) - 1));   // falling
+            const uint32_t bin = kDigits - 1 - ((key >> left) & (kDigits - 1));   // falling
             atomicAdd(&sh.digits.number[bin], 1u);
             atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits.mass[bin]), static_cast<unsigned long long>(whole(f)));
         });
         __syncthreads();
-        find_bin<kT, 2048>(sh.digits.mass, sh.digits.number, by_mass, target, before_mass, before, sh);
+        find_bin<kT, kDigits>(sh.digits.mass, sh.digits.number, by_mass, target, before_mass, before, sh);
         const uint32_t bin = sh.found_index;
-        if (bin == 2048) return 0;   // the row has less
-        prefix = prefix << width | ((2047 - bin) & ((1u << width) - 1));
-        known += width;
+        if (bin == kDigits) return 0;   // the row has less
+        prefix = prefix << kDigit | (kDigits - 1 - bin);
+        known += kDigit;
         before = sh.found_count, before_mass = sh.found;
     }
     const uint32_t tied = sh.tied;
@@ -563,111 +584,256 @@ __device__ uint64_t border_by_digits(const Row<E>& r, float m, double c, bool by
     return uint64_t(prefix) << 32 | uint32_t(~index);
 }
 
-// The same from the parts' histograms: the bin with the border, whose words are sorted.
-// false: what is looked for lies below them, or the bin holds too many.
-template <typename E, uint32_t kT>
+// What the histograms of a row's parts say of it together.
+__device__ __forceinline__ bool bins_do(const Rows& a, float top_bin) {
+    // whole numbers of 2^-44 of a row of up to 2^18 words; bins that floats tell apart
+    return a.vocab <= (1u << 18) && a.parts <= kMostParts && fabsf(top_bin) < 0x1p22f;
+}
+template <uint32_t kT>
+__device__ void join_bins(const Rows& a, const Part* part, const uint64_t* lists, float m, double c, float scale, float top_bin,
+                          Bins& bins) {
+    for (uint32_t i = threadIdx.x; i < kBins; i += kT) bins.mass[i] = 0, bins.number[i] = 0;
+    if (threadIdx.x < a.parts) {
+        const float mp = part[threadIdx.x].m;
+        bins.factor[threadIdx.x] = mp > kNegInf ? exp2_wide((double(mp) - double(m)) * c) * 0x1p-4 : 0.0;
+        bins.offset[threadIdx.x] = mp > kNegInf ? top_bin - floorf(mp * scale) : 2.0f * kBins;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.parts * kBins; i += kT) {
+        const uint32_t p = i / kBins, bin = i % kBins;
+        const float at = bins.offset[p] + float(bin);
+        if (!(at < float(kBins))) continue;
+        const uint32_t number = reinterpret_cast<const uint16_t*>(lists + uint64_t(p) * a.list + kBins)[bin];
+        if (number == 0) continue;
+        atomicAdd(&bins.number[uint32_t(at)], number);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&bins.mass[uint32_t(at)]),
+                  static_cast<unsigned long long>(double(lists[uint64_t(p) * a.list + bin]) * bins.factor[p] + 0.5));
+    }
+    __syncthreads();
+}
+
+// The border, as border_by_digits gives it, from the parts' histograms: the bin it lies in,
+// whose words are binned again, and of those a few sorted.  Leaves the bin's words in
+// sh.places, sh.held of them, and its number in bins.bin.  false: what is looked for lies
+// below the histograms, or the bin holds too many.
+template <typename E, uint32_t kT, typename Sh>
 __device__ bool border_by_bins(const Rows& a, const Part* part, const uint64_t* lists, const Row<E>& r, float m, double t,
-                               bool by_mass, double reach, uint64_t* border, double* prefix_mass, Shared& sh) {
+                               bool by_mass, double reach, uint64_t* border, double* prefix_mass, Sh& sh, Bins& bins) {
     const double c = 1.4426950408889634073599 / t;
     const float scale = bin_scale(t), top_bin = floorf(m * scale);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kBins; i += kT) sh.bins.mass[i] = 0, sh.bins.number[i] = 0;
-    __syncthreads();
-    if (!(fabsf(top_bin) < 0x1p23f)) return false;   // bins that floats do not tell apart
-    // 2^-44 of the largest weight: a row of up to 2^18 words; longer ones by digits
-    if (r.vocab > (1u << 18)) return false;
-    for (uint32_t i = threadIdx.x; i < a.parts * kBins; i += kT) {
-        const uint32_t p = i / kBins, bin = i % kBins;
-        if (!(part[p].m > kNegInf)) continue;
-        const float offset = top_bin - floorf(part[p].m * scale) + float(bin);
-        const uint32_t number = reinterpret_cast<const uint32_t*>(lists + uint64_t(p) * a.list + kBins)[bin];
-        if (number == 0 || !(offset < float(kBins))) continue;
-        const double by = exp2_wide((double(part[p].m) - double(m)) * c) * 0x1p-4;
-        atomicAdd(&sh.bins.number[uint32_t(offset)], number);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins.mass[uint32_t(offset)]),
-                  static_cast<unsigned long long>(double(lists[uint64_t(p) * a.list + bin]) * by + 0.5));
-    }
-    __syncthreads();
-    find_bin<kT, kBins>(sh.bins.mass, sh.bins.number, by_mass,
-                        by_mass ? uint64_t(ceil(fmax(reach, 0.0) * 0x1p44)) : uint64_t(reach), 0, 0, sh);
+    if (threadIdx.x == 0) bins.bin = -1.0f;
+    if (!bins_do(a, top_bin)) return false;
+    const uint64_t target = by_mass ? uint64_t(ceil(fmax(reach, 0.0) * 0x1p44)) : uint64_t(reach);
+    join_bins<kT>(a, part, lists, m, c, scale, top_bin, bins);
+    find_bin<kT, kBins>(bins.mass, bins.number, by_mass, target, 0, 0, sh);
     const uint32_t bin = sh.found_index, n = sh.tied, before = sh.found_count;
-    const double before_mass = double(sh.found) * 0x1p-44;
-    if (bin == kBins || n > kSorted) return false;
+    const uint64_t before_mass = sh.found;
+    if (bin == kBins || n > Sh::kSorted) return false;
     __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
+    for (uint32_t i = threadIdx.x; i < kSubBins; i += kT) bins.sub_mass[i] = 0, bins.sub_number[i] = 0;
+    if (threadIdx.x == 0) sh.count = 0, sh.held = n, bins.bin = float(bin);
     __syncthreads();
+    const float lo = top_bin - float(bin);   // floor(v) == lo
     each_word<E, kT>(r, [&](float f, uint32_t index) {
-        if (f > kNegInf && top_bin - floorf(f * scale) == float(bin)) {
+        const float v = f * scale;
+        if (v >= lo && v < lo + 1.0f) {
             const uint32_t at = atomicAdd(&sh.count, 1u);
-            if (at < kSorted) sh.places[at] = place_of(f, index);
+            if (at < Sh::kSorted) sh.places[at] = place_of(f, index);
         }
     });
     __syncthreads();
     if (sh.count != n) return false;
-    sort_padded<kT>(sh.places, n);
-    // one wave along the sorted words, 64 at a time
-    if (threadIdx.x < 64) {
-        double before_here = before_mass;
-        uint64_t last = 0;
-        double mass = 0.0;
-        for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-            const uint32_t i = i0 + threadIdx.x;
-            const uint64_t place = i < n ? sh.places[i] : 0;
-            const double w = i < n ? exp2_wide((double(logit_of(place)) - double(m)) * c) : 0.0;
-            double upto = w;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double below = __shfl_up(upto, d);
-                if (threadIdx.x >= uint32_t(d)) upto += below;
-            }
-            const bool in = i < n && (by_mass ? before_here + (upto - w) < reach || (before + i == 0) : double(before + i) < reach);
-            const uint64_t took = __ballot(in);
-            if (took == 0) break;
-            const int end = 63 - __builtin_clzll(took);
-            last = __shfl(place, end);
-            mass = before_here + __shfl(upto, end);
-            before_here += __shfl(upto, 63);
-        }
-        if (threadIdx.x == 0) sh.found = last, sh.found_mass = mass;
+    const auto sub_of = [&](float f) { return kSubBins - 1 - min(uint32_t((f * scale - lo) * float(kSubBins)), kSubBins - 1); };
+    const auto weight = [&](float f) { return exp2_wide((double(f) - double(m)) * c); };
+    for (uint32_t i = threadIdx.x; i < n; i += kT) {
+        const float f = logit_of(sh.places[i]);
+        atomicAdd(&bins.sub_number[sub_of(f)], 1u);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&bins.sub_mass[sub_of(f)]),
+                  static_cast<unsigned long long>(weight(f) * 0x1p44 + 0.5));
     }
     __syncthreads();
-    // a bin is reached before its first word where masses were rounded: then that is the border
-    *border = sh.found != 0 ? sh.found : sh.places[0];
+    find_bin<kT, kSubBins>(bins.sub_mass, bins.sub_number, by_mass, target, before_mass, before, sh);
+    const uint32_t sub = sh.found_index, few = sh.tied, before_sub = sh.found_count;
+    const double mass_sub = double(sh.found) * 0x1p-44;
+    if (sub == kSubBins) return false;   // a rounding at the end of the bin
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kT)
+        if (sub_of(logit_of(sh.places[i])) == sub) {
+            const uint32_t at = atomicAdd(&sh.count, 1u);
+            if (at < 64) sh.few[at] = sh.places[i];
+        }
+    __syncthreads();
+    if (few > 64) {
+        // Equal words, as 16-bit logits have them by the hundreds: as many as are asked for, by
+        // their index, whose bits are binned in turn.
+        const uint32_t key = uint32_t(sh.few[0] >> 32);
+        const double w = weight(float_of(key));
+        double more = by_mass ? ceil((reach - mass_sub) / w) : reach - double(before_sub);
+        const uint32_t take = more < 1.0 ? 1 : more < double(few) ? uint32_t(more) : few;
+        const uint32_t shift = max(0, 32 - 10 - __builtin_clz(max(r.vocab - 1, 1u)));   // of an index, to 1024 bins
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < kSubBins; i += kT) bins.sub_mass[i] = 0, bins.sub_number[i] = 0;
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+        bool other = false;
+        for (uint32_t i = threadIdx.x; i < n; i += kT) {
+            const uint64_t place = sh.places[i];
+            if (uint32_t(place >> 32) == key) atomicAdd(&bins.sub_number[index_of(place) >> shift], 1u);
+            else other |= sub_of(logit_of(place)) == sub;
+        }
+        if (__syncthreads_or(other)) return false;
+        find_bin<kT, kSubBins>(bins.sub_mass, bins.sub_number, false, take, 0, 0, sh);
+        const uint32_t among = sh.found_index, ahead = sh.found_count;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += kT)
+            if (uint32_t(sh.places[i] >> 32) == key && index_of(sh.places[i]) >> shift == among)
+                sh.few[atomicAdd(&sh.count, 1u)] = sh.places[i];   // at most 2^8 indices
+        __syncthreads();
+        if (threadIdx.x < sh.count) {
+            const uint64_t own = sh.few[threadIdx.x];
+            uint32_t rank = 0;
+            for (uint32_t i = 0; i < sh.count; ++i) rank += sh.few[i] > own;
+            if (ahead + rank + 1 == take) sh.found = own;
+        }
+        if (threadIdx.x == 0) sh.found_mass = mass_sub + w * take;
+    } else if (threadIdx.x < 64) {
+        const uint32_t lane = threadIdx.x;
+        const uint64_t own = lane < few ? sh.few[lane] : 0;
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < few; ++i) rank += sh.few[i] > own;
+        if (lane < few) sh.few[64 + rank] = own;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint64_t place = lane < few ? sh.few[64 + lane] : 0;
+        const double w = lane < few ? weight(logit_of(place)) : 0.0;
+        double upto = w;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double below = __shfl_up(upto, d);
+            if (lane >= uint32_t(d)) upto += below;
+        }
+        // the first of them at least: their bin was reached
+        const bool in = lane < few && (lane == 0 || (by_mass ? mass_sub + (upto - w) < reach : double(before_sub + lane) < reach));
+        const int end = 63 - __builtin_clzll(__ballot(in));
+        const uint64_t last = __shfl(place, end);
+        const double mass = mass_sub + __shfl(upto, end);
+        if (lane == 0) sh.found = last, sh.found_mass = mass;
+    }
+    __syncthreads();
+    *border = sh.found;
     if (prefix_mass != nullptr) *prefix_mass = sh.found_mass;
     __syncthreads();
     return true;
 }
 
-// The words of the parts' lists, sorted in sh.places; their number, or kSorted + 1 where a list
-// or this one did not hold them.
-template <uint32_t kT>
-__device__ uint32_t sorted_lists(const Rows& a, const Part* part, const uint64_t* lists, Shared& sh) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
-    for (uint32_t p = threadIdx.x / 64; p < a.parts; p += kT / 64) {
-        const uint32_t n = part[p].count;
+// ---------------------------------------------------------------------
+// The k largest words of a row, sorted in sh.few; how many there are (-inf are none).
+//
+// One wave picks them from the parts' lists, up to 16 words a lane at a time: the key that k
+// of them reach, bit by bit, by counting ballots; what reaches it, k and ties, goes on to the
+// next lists and is ranked by counting in the end.  Others than the first wave wait.
+// ---------------------------------------------------------------------
+constexpr uint32_t kPicked = 1024;
+template <typename Sh>
+__device__ bool pick_largest(const Rows& a, const Part* part, const uint64_t* lists, uint32_t k, Sh& sh) {
+    static_assert(Sh::kSorted >= kPicked, "it holds them");
+    constexpr uint32_t kEach = kPicked / 64;
+    const uint32_t lane = threadIdx.x;
+    uint32_t n = 0, p = 0;
+    do {
+        // the next lists, as many of up to 64 as fit, a word a lane in turn; all on their way at once
+        const uint32_t in = p + lane < a.parts ? part[p + lane].count : 0;
+        if (__ballot(in > a.list) != 0) return false;
+        uint32_t end = in;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t below = __shfl_up(end, d);
+            if (lane >= uint32_t(d)) end += below;
+        }
+        const uint32_t took = min(uint32_t(__popcll(__ballot(n + end <= kPicked))), a.parts - p);   // ends only rise
+        const uint32_t more = took > 0 ? __shfl(end, took - 1) : 0;
+        uint64_t next[kEach];
+        uint32_t of[kEach], from[kEach];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) of[i] = from[i] = 0;
+        for (uint32_t q = 0; q + 1 < took; ++q) {
+            const uint32_t edge = __builtin_amdgcn_readlane(end, q);
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i)
+                if (i * 64 + lane >= edge) of[i] = q + 1, from[i] = edge;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t at = i * 64 + lane;
+            next[i] = at < more ? lists[uint64_t(p + of[i]) * a.list + at - from[i]] : 0;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i)
+            if (i * 64 + lane < more) sh.places[n + i * 64 + lane] = next[i];
+        p += took, n += more;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (n <= k && p < a.parts) return false;   // a list does not fit beside so few
+        if (n <= k) break;
+        uint32_t keys[kEach];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) keys[i] = i * 64 + lane < n ? uint32_t(sh.places[i * 64 + lane] >> 32) : 0;
+        // from the first bit on in which they differ
+        uint32_t low = ~0u, high = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) high = max(high, keys[i]), low = min(low, i * 64 + lane < n ? keys[i] : ~0u);
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            high = max(high, uint32_t(__shfl_xor(int(high), d)));
+            low = min(low, uint32_t(__shfl_xor(int(low), d)));
+        }
+        const int differ = high == low ? -1 : 31 - __builtin_clz(high ^ low);
+        uint32_t bound = differ < 0 ? low : differ == 31 ? 0 : low >> (differ + 1) << (differ + 1), reached = n;
+#pragma unroll 1
+        for (int bit = differ; bit >= 0 && reached != k; --bit) {
+            const uint32_t with = bound | 1u << bit;
+            uint32_t have = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; ++i) have += __popcll(__ballot(keys[i] >= with));
+            if (have >= k) bound = with, reached = have;
+        }
+        if (reached > kMost) return false;   // ties
+        // in any order, each before where it was
         uint32_t at = 0;
-        if ((threadIdx.x & 63) == 0) at = atomicAdd(&sh.count, n <= a.list ? n : kSorted + 1);
-        at = __shfl(at, 0);
-        for (uint32_t i = threadIdx.x & 63; i < min(n, a.list); i += 64)
-            if (at + i < kSorted) sh.places[at + i] = lists[uint64_t(p) * a.list + i];
-        if (at > kSorted) break;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const bool in = i * 64 + lane < n && keys[i] >= bound;
+            const uint64_t place = in ? sh.places[i * 64 + lane] : 0, those = __ballot(in);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (in) sh.places[at + __popcll(those & ((uint64_t(1) << lane) - 1))] = place;
+            at += __popcll(those);
+        }
+        n = reached;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } while (p < a.parts);
+    static_assert(kMost == 128, "two words a lane");
+    const uint64_t own0 = lane < n ? sh.places[lane] : 0, own1 = lane + 64 < n ? sh.places[lane + 64] : 0;
+    uint32_t rank0 = 0, rank1 = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        const uint64_t other = sh.places[i];
+        rank0 += other > own0, rank1 += other > own1;
+    }
+    if (lane < n && rank0 < k) sh.few[rank0] = own0;
+    if (lane + 64 < n && rank1 < k) sh.few[rank1] = own1;
+    if (lane == 0) sh.held = min(n, k);
+    return true;
+}
+template <typename E, uint32_t kT, typename Sh>
+__device__ uint32_t largest(const Rows& a, const Part* part, const uint64_t* lists, const Row<E>& r, float m, double c, uint32_t k,
+                            Sh& sh) {
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const bool done = pick_largest(a, part, lists, k, sh);
+        if (threadIdx.x == 0 && !done) sh.held = ~0u;
     }
     __syncthreads();
-    const uint32_t n = sh.count;
-    if (n > kSorted) return kSorted + 1;
-    sort_padded<kT>(sh.places, n);
-    return n;
-}
-
-// The k largest words of a row, sorted in sh.places, by whatever finds them; how many there are
-// (-inf are none).
-template <typename E, uint32_t kT>
-__device__ uint32_t largest(const Rows& a, const Part* part, const uint64_t* lists, const Row<E>& r, float m, double c, uint32_t k,
-                            Shared& sh) {
-    uint32_t n = sorted_lists<kT>(a, part, lists, sh);
-    if (n <= kSorted) return min(n, k);
+    if (sh.held != ~0u) return sh.held;
     const uint64_t border = border_by_digits<E, kT>(r, m, c, false, double(k), nullptr, sh);
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
@@ -675,41 +841,47 @@ __device__ uint32_t largest(const Rows& a, const Part* part, const uint64_t* lis
     each_word<E, kT>(r, [&](float f, uint32_t index) {
         if (f > kNegInf && place_of(f, index) >= border) {
             const uint32_t at = atomicAdd(&sh.count, 1u);
-            if (at < kSorted) sh.places[at] = place_of(f, index);
+            if (at < kMost) sh.few[128 + at] = place_of(f, index);
         }
     });
     __syncthreads();
-    n = min(sh.count, kSorted);
-    sort_padded<kT>(sh.places, n);
-    return min(n, k);
+    const uint32_t n = min(sh.count, k);
+    for (uint32_t i = threadIdx.x; i < n; i += kT) {
+        const uint64_t own = sh.few[128 + i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; ++j) rank += sh.few[128 + j] > own;
+        sh.few[rank] = own;
+    }
+    __syncthreads();
+    return n;
 }
 
-constexpr uint32_t kTopLanes = 256;
+constexpr uint32_t kListedLanes = 64;
 template <typename E>
-__global__ __launch_bounds__(kTopLanes) void top_rows_kernel(const Rows a) {
-    __shared__ Shared sh;
+__global__ __launch_bounds__(kListedLanes) void top_rows_kernel(const Rows a) {
+    __shared__ Shared<kPicked> sh;
     const uint64_t row = blockIdx.x, of = a.first + row;
     const Part* const part = a.part + row * a.parts;
     const uint64_t* const lists = a.lists + row * a.parts * a.list;
-    const Settings s = settings(a, of);
+    const Settings s = settings<kListed>(a, of);
+    const uint32_t k = uint32_t(a.top_k);
     const double c = 1.4426950408889634073599 / s.t;
-    const Joined j = join_parts<kTopLanes>(a, part, c, sh.waves);
-    float* const logps = a.logps + of * s.k;
-    int64_t* const ids = a.ids + of * s.k;
+    const Joined j = join_parts<kListedLanes>(a, part, c, sh.waves);
+    float* const logps = a.logps + of * k;
+    int64_t* const ids = a.ids + of * k;
     if (j.bad) {
-        for (uint32_t i = threadIdx.x; i < s.k; i += kTopLanes) logps[i] = __builtin_nanf(""), ids[i] = -1;
+        for (uint32_t i = threadIdx.x; i < k; i += kListedLanes) logps[i] = __builtin_nanf(""), ids[i] = -1;
         return;
     }
     const Row<E> r(a.logits, a.ld, of, a.vocab);
-    const uint32_t n = largest<E, kTopLanes>(a, part, lists, r, j.m, c, s.k, sh);
+    const uint32_t n = largest<E, kListedLanes>(a, part, lists, r, j.m, c, k, sh);
     const double lse = log(j.sum);
-    for (uint32_t i = threadIdx.x; i < n; i += kTopLanes) {
-        logps[i] = float((double(logit_of(sh.places[i])) - double(j.m)) / s.t - lse);
-        ids[i] = index_of(sh.places[i]);
+    for (uint32_t i = threadIdx.x; i < n; i += kListedLanes) {
+        logps[i] = float((double(logit_of(sh.few[i])) - double(j.m)) / s.t - lse);
+        ids[i] = index_of(sh.few[i]);
     }
     // words of probability 0 in the order of their index
-    for (uint32_t done = n, v0 = 0; done < s.k; v0 += kTopLanes) {
-        uint32_t found = 0;
+    for (uint32_t done = n, v0 = 0; done < k && v0 < a.vocab; v0 += 64) {
         const uint32_t index = v0 + threadIdx.x;
         bool none = false;
         if (index < a.vocab) {
@@ -717,129 +889,272 @@ __global__ __launch_bounds__(kTopLanes) void top_rows_kernel(const Rows a) {
             else none = r.x[index] == E::kNegInf;
         }
         const uint64_t those = __ballot(none);
-        uint32_t* const waves = reinterpret_cast<uint32_t*>(sh.waves);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = __popcll(those);
-        __syncthreads();
-        uint32_t at = done + __popcll(those & ((uint64_t(1) << (threadIdx.x & 63)) - 1));
-        for (uint32_t w = 0; w < kTopLanes / 64; ++w) {
-            if (w < threadIdx.x >> 6) at += waves[w];
-            found += waves[w];
-        }
-        if (none && at < s.k) logps[at] = kNegInf, ids[at] = index;
-        done += found;
-        if (v0 >= a.vocab) break;
+        const uint32_t at = done + __popcll(those & ((uint64_t(1) << threadIdx.x) - 1));
+        if (none && at < k) logps[at] = kNegInf, ids[at] = index;
+        done += __popcll(those);
     }
 }
 
-constexpr uint32_t kDrawLanes = 1024;
+// ---------------------------------------------------------------------
+// A draw from the k largest words, by the first wave: two words a lane, in their order.
+template <typename E, uint32_t kT, typename Sh>
+__device__ void draw_listed(const Rows& a, uint64_t of, const Settings& s, const Part* part, const uint64_t* lists,
+                            const Joined& j, double c, double u, double least, double lse, Sh& sh) {
+    const Row<E> r(a.logits, a.ld, of, a.vocab);
+    const uint32_t n = largest<E, kT>(a, part, lists, r, j.m, c, s.k, sh);
+    if (threadIdx.x >= 64) return;
+    const uint32_t lane = threadIdx.x;
+    uint64_t place[2];
+    double d[2], w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const uint32_t i = 2 * lane + e;
+        place[e] = i < n ? sh.few[i] : 0;
+        d[e] = i < n ? double(logit_of(place[e])) - double(j.m) : 0.0;
+        w[e] = i < n ? exp2_wide(d[e] * c) : 0.0;
+    }
+    double upto = w[0] + w[1];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double below = __shfl_up(upto, d);
+        if (lane >= uint32_t(d)) upto += below;
+    }
+    const double total = __shfl(upto, 63);
+    const double before[2] = {upto - w[1] - w[0], upto - w[1]};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const uint32_t i = 2 * lane + e;
+        const bool kept = i < n && (i == 0 || !(s.top_p < 1.0) || before[e] < s.top_p * total) && d[e] >= least;
+        w[e] = kept ? w[e] : 0.0;
+        sh.weights[i] = w[e];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint32_t index[2] = {index_of(place[0]), index_of(place[1])};
+    double mass = 0.0, sums[2] = {0.0, 0.0};   // in one order everywhere
+    for (uint32_t i = 0; i < n; ++i) {
+        const double v = sh.weights[i];
+        const uint32_t at = index_of(sh.few[i]);
+        mass += v;
+        if (at <= index[0]) sums[0] += v;
+        if (at <= index[1]) sums[1] += v;
+    }
+    // the first word above the target, by its index; where rounding leaves none, the last
+    uint32_t first = ~0u, last = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (w[e] > 0.0) {
+            if (sums[e] > u * mass) first = min(first, index[e]);
+            last = max(last, index[e]);
+        }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        first = min(first, uint32_t(__shfl_xor(int(first), d)));
+        last = max(last, uint32_t(__shfl_xor(int(last), d)));
+    }
+    const uint32_t chosen = first != ~0u ? first : last;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (w[e] > 0.0 && index[e] == chosen) a.ids[of] = chosen, a.logps[of] = float(d[e] / s.t - lse);
+}
+
+// What a draw is by: its share of the mass, below 1 (what is no number is 0), and the least x -
+// max that min_p allows.
+__device__ __forceinline__ double share_of(float u) { return u > 0.0f ? double(fminf(u, 0x1.fffffep-1f)) : 0.0; }
+__device__ __forceinline__ double least_of(const Settings& s) {
+    return s.min_p > 0.0 ? fmin(log(s.min_p), 0.0) * s.t : -__builtin_inf();
+}
+
 template <typename E>
-__global__ __launch_bounds__(kDrawLanes) void draw_rows_kernel(const Rows a) {
-    __shared__ Shared sh;
+__global__ __launch_bounds__(kListedLanes) void draw_listed_kernel(const Rows a) {
+    __shared__ Shared<kPicked> sh;
     const uint64_t row = blockIdx.x, of = a.first + row;
     const Part* const part = a.part + row * a.parts;
     const uint64_t* const lists = a.lists + row * a.parts * a.list;
-    const Settings s = settings(a, of);
+    const Settings s = settings<kListed>(a, of);
+    const double c = 1.4426950408889634073599 / s.t;
+    const Joined j = join_parts<kListedLanes>(a, part, c, sh.waves);
+    if (j.bad) {
+        if (threadIdx.x == 0) a.ids[of] = -1, a.logps[of] = __builtin_nanf("");
+        return;
+    }
+    draw_listed<E, kListedLanes>(a, of, s, part, lists, j, c, share_of(a.uniforms[of]), least_of(s), log(j.sum), sh);
+}
+
+// The mass that each part keeps with a border in bin `at`: its bins above, and of that bin's words
+// those up to the border.
+template <typename E, uint32_t kT, typename Sh>
+__device__ void kept_by_parts(const Rows& a, const uint64_t* lists, const Row<E>& r, float m, double c, float scale, float top_bin,
+                              float at, uint64_t border, Sh& sh, Bins& bins) {
+    __syncthreads();
+    if (threadIdx.x < a.parts) bins.kept[threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t i0 = 0; i0 < a.parts * kBins; i0 += kT) {   // a wave has bins of one part
+        const uint32_t i = i0 + threadIdx.x, p = i / kBins, bin = i % kBins;
+        uint64_t mass = 0;
+        if (p < a.parts && bins.offset[p] + float(bin) < at)
+            mass = uint64_t(double(lists[uint64_t(p) * a.list + bin]) * bins.factor[p] + 0.5);
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) mass += __shfl_xor(mass, d);
+        if ((threadIdx.x & 63) == 0 && mass != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&bins.kept[p]), static_cast<unsigned long long>(mass));
+    }
+    const auto add = [&](uint64_t place) {
+        const uint64_t mass = uint64_t(exp2_wide((double(logit_of(place)) - double(m)) * c) * 0x1p44 + 0.5);
+        const uint32_t p = (index_of(place) + r.shift) / kOf<E> / a.per;
+        atomicAdd(reinterpret_cast<unsigned long long*>(&bins.kept[p]), static_cast<unsigned long long>(mass));
+    };
+    if (bins.bin == at) {
+        for (uint32_t i = threadIdx.x; i < sh.held; i += kT)
+            if (sh.places[i] >= border) add(sh.places[i]);
+    } else {
+        const float lo = top_bin - at;
+        each_word<E, kT>(r, [&](float f, uint32_t index) {
+            const float v = f * scale;
+            if (v >= lo && v < lo + 1.0f && place_of(f, index) >= border) add(place_of(f, index));
+        });
+    }
+    __syncthreads();
+}
+
+template <typename E>
+__device__ void write_draw(const Rows& a, uint64_t of, const Row<E>& r, uint32_t index, const Joined& j, const Settings& s) {
+    float f;
+    if constexpr (std::is_same_v<E, F32>) f = __uint_as_float(r.x[index]);
+    else f = E::lo(r.x[index]);
+    a.ids[of] = index;
+    a.logps[of] = float((double(f) - double(j.m)) / s.t - log(j.sum));
+}
+
+// The part in which the running mass exceeds u times all (sum_up: their sum, of up to 64 parts), and
+// what of that mass lies within it; where rounding leaves none, the last with a mass and infinity.
+template <typename Mass, typename Sh>
+__device__ double choose_part(const Rows& a, double u, bool sum_up, double all, Mass mass, uint32_t* chosen, Sh& sh) {
+    if (threadIdx.x < 64) {
+        const uint32_t lane = threadIdx.x;
+        double before = 0.0, rest = __builtin_inf();
+        uint32_t last = 0;
+        for (uint32_t p = 0; p < a.parts; p += 64) {
+            const double own = p + lane < a.parts ? mass(p + lane) : 0.0;
+            double upto = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const double below = __shfl_up(upto, d);
+                if (lane >= uint32_t(d)) upto += below;
+            }
+            const double total = __shfl(upto, 63);
+            if (sum_up) all = total;
+            const uint64_t some = __ballot(own > 0.0), over = __ballot(own > 0.0 && before + upto > u * all);
+            if (over != 0) {
+                const int at = __ffsll(static_cast<unsigned long long>(over)) - 1;
+                last = p + at;
+                rest = u * all - (before + __shfl(upto, at) - __shfl(own, at));
+                break;
+            }
+            if (some != 0) last = p + 63 - __builtin_clzll(some);
+            before += total;
+        }
+        if (lane == 0) sh.found_index = last, sh.found_mass = rest;
+    }
+    __syncthreads();
+    *chosen = sh.found_index;
+    const double rest = sh.found_mass;
+    __syncthreads();
+    return rest;
+}
+
+// A draw from all of a row's words.
+constexpr uint32_t kWholeLanes = 256;
+template <typename E>
+__global__ __launch_bounds__(kWholeLanes) void draw_whole_kernel(const Rows a) {
+    __shared__ Shared<1> sh;
+    const uint64_t row = blockIdx.x, of = a.first + row;
+    const Part* const part = a.part + row * a.parts;
+    const Settings s = settings<kWhole>(a, of);
+    const double c = 1.4426950408889634073599 / s.t;
+    const Joined j = join_parts<kWholeLanes>(a, part, c, sh.waves);
+    if (j.bad) {
+        if (threadIdx.x == 0) a.ids[of] = -1, a.logps[of] = __builtin_nanf("");
+        return;
+    }
+    const Row<E> r(a.logits, a.ld, of, a.vocab);
+    uint32_t v0;
+    const double target = choose_part(a, share_of(a.uniforms[of]), false, j.sum, [&](uint32_t p) { return mass_of(part[p], j.m, c); }, &v0, sh);
+    v0 = min(v0 * a.per, r.vectors);
+    const uint32_t index = min(find_word<E, kWholeLanes>(
+        r, v0, min(v0 + a.per, r.vectors), target, false,
+        [&](float f, uint32_t) { return exp2_wide((double(f) - double(j.m)) * c); }, sh), a.vocab - 1);
+    if (threadIdx.x == 0) write_draw(a, of, r, index, j, s);
+}
+
+constexpr uint32_t kDrawLanes = 1024;
+template <typename E, Kind kKind>
+__global__ __launch_bounds__(kDrawLanes) void draw_rows_kernel(const Rows a) {
+    __shared__ Shared<8192> sh;
+    __shared__ Bins bins;
+    const uint64_t row = blockIdx.x, of = a.first + row;
+    const Part* const part = a.part + row * a.parts;
+    const uint64_t* const lists = a.lists + row * a.parts * a.list;
+    const Settings s = settings<kKind>(a, of);
     const double c = 1.4426950408889634073599 / s.t;
     const Joined j = join_parts<kDrawLanes>(a, part, c, sh.waves);
     if (j.bad) {
         if (threadIdx.x == 0) a.ids[of] = -1, a.logps[of] = __builtin_nanf("");
         return;
     }
+    const double u = share_of(a.uniforms[of]), least = least_of(s);
+    if (kKind == kEither && s.listed)
+        return draw_listed<E, kDrawLanes>(a, of, s, part, lists, j, c, u, least, log(j.sum), sh);
     const Row<E> r(a.logits, a.ld, of, a.vocab);
-    // a share of the mass below 1; what is no number is 0
-    float u = a.uniforms[of];
-    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-    const double least = s.min_p > 0.0 ? fmin(log(s.min_p), 0.0) * s.t : -__builtin_inf();   // of x - max
-    const double lse = log(j.sum);
-
-    if (s.listed) {
-        const uint32_t n = largest<E, kDrawLanes>(a, part, lists, r, j.m, c, s.k, sh);
-        // n <= kMost words, one each for the first lanes
-        const bool mine = threadIdx.x < n;
-        const uint64_t place = mine ? sh.places[threadIdx.x] : 0;
-        const double d = mine ? double(logit_of(place)) - double(j.m) : 0.0, w = mine ? exp2_wide(d * c) : 0.0;
-        if (mine) sh.weights[threadIdx.x] = w;
-        __syncthreads();
-        double before = 0.0, total = 0.0;
-        if (mine)
-            for (uint32_t i = 0; i < n; ++i) {
-                if (i == threadIdx.x) before = total;
-                total += sh.weights[i];
-            }
-        const bool kept = mine && (!(s.top_p < 1.0) || threadIdx.x == 0 || before < s.top_p * total) && d >= least;
-        __syncthreads();
-        if (mine) sh.weights[threadIdx.x] = kept ? w : 0.0;
-        if (threadIdx.x == 0) sh.found = 0;
-        __syncthreads();
-        if (kept && w > 0.0) {
-            const uint32_t index = index_of(place);
-            double mass = 0.0, upto = 0.0;
-            for (uint32_t i = 0; i < n; ++i) {
-                const double v = sh.weights[i];
-                mass += v;
-                if (index_of(sh.places[i]) <= index) upto += v;
-            }
-            // the first word above the target; where rounding leaves none, the last
-            const bool over = upto > double(u) * mass;
-            atomicMax(reinterpret_cast<unsigned long long*>(&sh.found),
-                      uint64_t(over) << 63 | uint64_t(over ? ~index : index) << 16 | threadIdx.x);
-        }
-        __syncthreads();
-        const uint32_t chosen = uint32_t(sh.found & 0xFFFF);
-        if (threadIdx.x == chosen) a.ids[of] = index_of(place), a.logps[of] = float(d / s.t - lse);
-        return;
-    }
-    uint32_t index;
-    if (!s.filtered) {
-        // the part, then the word within it
-        const double target = double(u) * j.sum;
-        double before = 0.0;
-        uint32_t chosen = a.parts, fallback = 0;
-        for (uint32_t p = 0; p < a.parts && chosen == a.parts; ++p) {
-            if (!(part[p].m > kNegInf)) continue;
-            const double mass = part[p].sum * exp2_wide((double(part[p].m) - double(j.m)) * c);
-            if (mass > 0.0) fallback = p;
-            if (before + mass > target) chosen = p;
-            else before += mass;
-        }
-        const bool none = chosen == a.parts;
-        if (none) chosen = fallback;
-        const uint32_t v0 = min(chosen * a.per, r.vectors), v1 = min(v0 + a.per, r.vectors);
-        index = find_word<E, kDrawLanes>(
-            r, v0, v1, none ? __builtin_inf() : target - before, false,
-            [&](float f, uint32_t) { return exp2_wide((double(f) - double(j.m)) * c); }, sh);
-    } else {
-        uint64_t border = 0;
+    const auto weight = [&](float f) { return exp2_wide((double(f) - double(j.m)) * c); };
+    uint64_t border = 0;
+    bool by_parts = true;   // their masses say which one it is in
+    if (s.filtered) {
         double mass = j.sum;
         if (s.k < a.vocab) {
-            if (!border_by_bins<E, kDrawLanes>(a, part, lists, r, j.m, s.t, false, double(s.k), &border, &mass, sh))
+            if (!border_by_bins<E, kDrawLanes>(a, part, lists, r, j.m, s.t, false, double(s.k), &border, &mass, sh, bins)) {
                 border = border_by_digits<E, kDrawLanes>(r, j.m, c, false, double(s.k), &mass, sh);
+                if (threadIdx.x == 0) bins.bin = -1.0f;   // its words are no longer there
+            }
             if (border == 0) mass = j.sum;
         }
         if (s.top_p < 1.0) {
             const double reach = s.top_p * mass;
             uint64_t nucleus = 0;
-            if (!border_by_bins<E, kDrawLanes>(a, part, lists, r, j.m, s.t, true, reach, &nucleus, nullptr, sh))
+            if (!border_by_bins<E, kDrawLanes>(a, part, lists, r, j.m, s.t, true, reach, &nucleus, nullptr, sh, bins)) {
                 nucleus = border_by_digits<E, kDrawLanes>(r, j.m, c, true, reach, nullptr, sh);
+                if (threadIdx.x == 0) bins.bin = -1.0f;
+            }
             border = max(border, nucleus);
+        } else if (s.k == a.vocab) {
+            if (threadIdx.x == 0) bins.bin = -1.0f;
         }
-        index = find_word<E, kDrawLanes>(
-            r, 0, r.vectors, double(u), true,
-            [&](float f, uint32_t i) {
-                const double d = double(f) - double(j.m);
-                return f > kNegInf && d >= least && place_of(f, i) >= border ? exp2_wide(d * c) : 0.0;
-            },
-            sh);
+        if (s.min_p > 0.0) {   // the least logit that it allows
+            const double x = double(j.m) + least;
+            float f = float(x);
+            if (double(f) - double(j.m) < least) f = float_of(key_of(f) + 1);
+            border = max(border, uint64_t(key_of(f)) << 32);
+        }
+        const float scale = bin_scale(s.t), top_bin = floorf(j.m * scale);
+        const float at = border != 0 ? top_bin - floorf(logit_of(border) * scale) : float(kBins);
+        by_parts = bins_do(a, top_bin) && at < float(kBins);
+        if (by_parts) {
+            if (s.k == a.vocab && !(s.top_p < 1.0)) join_bins<kDrawLanes>(a, part, lists, j.m, c, scale, top_bin, bins);
+            kept_by_parts<E, kDrawLanes>(a, lists, r, j.m, c, scale, top_bin, at, border, sh, bins);
+        }
     }
-    if (threadIdx.x == 0) {
-        index = min(index, a.vocab - 1);
-        float f;
-        if constexpr (std::is_same_v<E, F32>) f = __uint_as_float(r.x[index]);
-        else f = E::lo(r.x[index]);
-        a.ids[of] = index;
-        a.logps[of] = float((double(f) - double(j.m)) / s.t - lse);
+    uint32_t v0 = 0, v1 = r.vectors;
+    double target = u;
+    if (by_parts) {
+        if (s.filtered)
+            target = choose_part(a, u, true, 0.0, [&](uint32_t p) { return double(bins.kept[p]) * 0x1p-44; }, &v0, sh);
+        else
+            target = choose_part(a, u, false, j.sum, [&](uint32_t p) { return mass_of(part[p], j.m, c); }, &v0, sh);
+        v0 = min(v0 * a.per, r.vectors), v1 = min(v0 + a.per, r.vectors);
     }
+    const float from = border != 0 ? logit_of(border) : kNegInf;
+    const uint32_t index = find_word<E, kDrawLanes>(
+        r, v0, v1, target, !by_parts,
+        [&](float f, uint32_t i) { return f > kNegInf && f >= from && place_of(f, i) >= border ? weight(f) : 0.0; }, sh);
+    if (threadIdx.x == 0) write_draw(a, of, r, min(index, a.vocab - 1), j, s);
 }
 
 // ---------------------------------------------------------------------
@@ -859,27 +1174,41 @@ uint64_t rows_at_once(const Plan& p) {
     return rows > 0 ? rows : 1;
 }
 
-template <typename E>
-int launch_parts(const Rows& a, uint32_t rows, uint32_t lane, hipStream_t st) {
-    const auto kernel = lane == 1   ? rows_parts_kernel<E, 1>
-                        : lane == 2 ? rows_parts_kernel<E, 2>
-                        : lane == 4 ? rows_parts_kernel<E, 4>
-                                    : rows_parts_kernel<E, 8>;
+template <typename E, Kind kKind>
+int launch_rows(const Rows& a, uint32_t rows, uint32_t lane, bool top, hipStream_t st) {
+    const auto kernel = lane == 1   ? rows_parts_kernel<E, 1, kKind>
+                        : lane == 2 ? rows_parts_kernel<E, 2, kKind>
+                        : lane == 4 ? rows_parts_kernel<E, 4, kKind>
+                                    : rows_parts_kernel<E, 8, kKind>;
     hipLaunchKernelGGL(kernel, dim3(rows * a.parts), dim3(kPartLanes), 0, st, a);
+    const int e = status();
+    if (e != SF_OK) return e;
+    if constexpr (kKind == kListed) {
+        const auto join = top ? top_rows_kernel<E> : draw_listed_kernel<E>;
+        hipLaunchKernelGGL(join, dim3(rows), dim3(kListedLanes), 0, st, a);
+    } else if constexpr (kKind == kWhole) {
+        hipLaunchKernelGGL(draw_whole_kernel<E>, dim3(rows), dim3(kWholeLanes), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((draw_rows_kernel<E, kKind>), dim3(rows), dim3(kDrawLanes), 0, st, a);
+    }
     return status();
 }
 
 template <typename E>
-int run_rows(Rows a, const Plan& p, hipStream_t st) {
+int run_rows(Rows a, const Plan& p, bool top, hipStream_t st) {
+    // a row's own temperature may ask for its largest word, its own top_k for a list
+    const bool either = a.temperatures != nullptr || a.top_ks != nullptr;
+    const bool filtered = a.top_ps != nullptr || a.min_ps != nullptr || a.top_p < 1.0 || a.min_p > 0.0 ||
+                          (a.top_k > 0 && a.top_k < int64_t(a.vocab));
+    const bool listed = !(a.temperature > 0.0) || (a.top_k > 0 && a.top_k <= int64_t(kMost)) || a.vocab <= kMost;
     const uint64_t most = rows_at_once(p);
     for (uint64_t r = 0; r < a.rows; r += most) {
         const uint32_t n = uint32_t(a.rows - r < most ? a.rows - r : most);
         a.first = r;
-        int e = launch_parts<E>(a, n, p.lane, st);
-        if (e != SF_OK) return e;
-        if (a.top_only) hipLaunchKernelGGL(top_rows_kernel<E>, dim3(n), dim3(kTopLanes), 0, st, a);
-        else hipLaunchKernelGGL(draw_rows_kernel<E>, dim3(n), dim3(kDrawLanes), 0, st, a);
-        e = status();
+        const int e = either     ? launch_rows<E, kEither>(a, n, p.lane, top, st)
+                      : listed   ? launch_rows<E, kListed>(a, n, p.lane, top, st)
+                      : filtered ? launch_rows<E, kFiltered>(a, n, p.lane, top, st)
+                                 : launch_rows<E, kWhole>(a, n, p.lane, top, st);
         if (e != SF_OK) return e;
     }
     return SF_OK;
@@ -893,15 +1222,15 @@ int check_rows(const Rows& a, int dtype, const void* work) {
     return SF_OK;
 }
 
-int dispatch_rows(Rows a, int dtype, void* work, hipStream_t st) {
+int dispatch_rows(Rows a, int dtype, void* work, bool top, hipStream_t st) {
     const Plan p = plan_of(a.vocab, dtype);
     const uint64_t most = rows_at_once(p), held = a.rows < most ? a.rows : most;
     a.parts = p.parts, a.per = p.per, a.list = p.list;
     a.part = static_cast<Part*>(work);
     a.lists = reinterpret_cast<uint64_t*>(a.part + held * p.parts);
-    if (dtype == SF_DTYPE_BF16) return run_rows<Bf16>(a, p, st);
-    if (dtype == SF_DTYPE_F16) return run_rows<F16>(a, p, st);
-    return run_rows<F32>(a, p, st);
+    if (dtype == SF_DTYPE_BF16) return run_rows<Bf16>(a, p, top, st);
+    if (dtype == SF_DTYPE_F16) return run_rows<F16>(a, p, top, st);
+    return run_rows<F32>(a, p, top, st);
 }
 
 }  // namespace
@@ -922,10 +1251,10 @@ int sf_top_logps(const void* logits, int dtype, size_t ld, size_t rows, size_t v
         return SF_EINVAL;
     Rows a = {};
     a.logits = logits, a.ld = ld, a.rows = rows, a.vocab = uint32_t(vocab);
-    a.temperature = temperature, a.top_p = 1.0, a.top_k = k, a.top_only = true;
+    a.temperature = temperature, a.top_p = 1.0, a.top_k = k;
     a.logps = logps, a.ids = ids;
     const int e = check_rows(a, dtype, work);
-    return e != SF_OK ? e : dispatch_rows(a, dtype, work, reinterpret_cast<hipStream_t>(stream));
+    return e != SF_OK ? e : dispatch_rows(a, dtype, work, true, reinterpret_cast<hipStream_t>(stream));
 }
 
 int sf_sample_tokens(const void* logits, int dtype, size_t ld, size_t rows, size_t vocab, const float* uniforms,
@@ -940,7 +1269,7 @@ int sf_sample_tokens(const void* logits, int dtype, size_t ld, size_t rows, size
     a.top_p = top_p, a.top_ps = top_ps, a.min_p = min_p, a.min_ps = min_ps;
     a.uniforms = uniforms, a.logps = logps, a.ids = ids;
     const int e = check_rows(a, dtype, work);
-    return e != SF_OK ? e : dispatch_rows(a, dtype, work, reinterpret_cast<hipStream_t>(stream));
+    return e != SF_OK ? e : dispatch_rows(a, dtype, work, false, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
