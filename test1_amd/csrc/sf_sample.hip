@@ -39,8 +39,11 @@ namespace {
 constexpr uint32_t kMost = SF_TOP_MOST;   // words that the parts' lists are made for
 constexpr uint32_t kPartLanes = 256;
 constexpr uint32_t kPartVectors = 8;      // of a lane
-constexpr uint32_t kBins = 512;           // of a part's histogram, T / kBinsOfT of logit each
-constexpr float kBinsOfT = 32.0f;
+// Of a part's histogram, T / kBinsOfT of logit each: down to e^-32 of the largest weight.  A
+// vocabulary's many small ones are beyond e^-16 of a sure word and still a thousandth of the
+// mass together.
+constexpr uint32_t kBins = 512;
+constexpr float kBinsOfT = 16.0f;
 constexpr uint32_t kList = kBins + kBins / 4;   // candidates of a part, of a row's only part twice as many
 constexpr uint32_t kSubBins = 1024;       // of a bin
 constexpr uint32_t kDigit = 8;            // bits of a radix pass
@@ -75,39 +78,84 @@ __device__ __forceinline__ uint64_t place_of(float x, uint32_t index) {
 __device__ __forceinline__ float logit_of(uint64_t place) { return float_of(uint32_t(place >> 32)); }
 __device__ __forceinline__ uint32_t index_of(uint64_t place) { return ~uint32_t(place); }
 
-// 2^y for y <= 0 or so: 2^n times the series of e^(f ln 2) to its 11th power, off
-// by 6e-15 of itself.
+// 2^y for finite y <= 0 or so: 2^n times the series of e^(f ln 2) to its 10th power, off
+// by 2^-42 of itself.
+constexpr int kPowers = 10;
 struct Series {
-    double c[12];
+    double c[kPowers + 1];
     constexpr Series() : c() {
         c[0] = 1.0;
-        for (int i = 1; i < 12; ++i) c[i] = c[i - 1] * 0.69314718055994530941723212145818 / i;
+        for (int i = 1; i <= kPowers; ++i) c[i] = c[i - 1] * 0.69314718055994530941723212145818 / i;
     }
 };
 __constant__ constexpr Series kSeries{};
 __device__ __forceinline__ double exp2_wide(double y) {
-    y = fmax(y, -1100.0);
     const double n = rint(y), f = y - n;
-    double p = kSeries.c[11];
+    double p = kSeries.c[kPowers];
 #pragma unroll
-    for (int i = 10; i >= 0; --i) p = fma(p, f, kSeries.c[i]);
+    for (int i = kPowers - 1; i >= 0; --i) p = fma(p, f, kSeries.c[i]);
     return ldexp(p, int(n));
 }
+// A logit's weight, exp((x - from) / T) as 2^(c x - c from); 0 of -inf.
+struct Weigh {
+    double c, less;
+    __device__ Weigh(double c_, float from) : c(c_), less(double(from) * c_) {}
+    __device__ double operator()(float x) const {
+        return exp2_wide(fma(double(fmaxf(x, -0x1.fffffep127f)), c, -less));
+    }
+};
 
-// A row's vectors: whole 16-byte ones, its first and last may lie partly outside
-// and are then read by elements, -inf where they are not the row's.
+template <typename E>
+__device__ __forceinline__ u32x4 nothing() {
+    const uint32_t w = std::is_same_v<E, F32> ? 0xFF800000u : std::is_same_v<E, Bf16> ? Bf16::kNegInf2 : F16::kNegInf2;
+    return u32x4{w, w, w, w};
+}
+
+// A row's vectors: whole 16-byte ones but for its first and its last, which may lie
+// partly outside and are read by elements, -inf where they are not the row's.
 template <typename E>
 struct Row {
     const Item<E>* x;
     uint32_t vocab, shift, vectors;   // the row begins `shift` elements into vector 0
+    uint32_t first, end;              // whole vectors
     __device__ Row(const void* logits, uint64_t ld, uint64_t row, uint32_t vocab_) : vocab(vocab_) {
         x = static_cast<const Item<E>*>(logits) + row * ld;
         shift = uint32_t(reinterpret_cast<uintptr_t>(x) % 16) / sizeof(Item<E>);
         vectors = (vocab + shift + kOf<E> - 1) / kOf<E>;
+        first = shift > 0 ? 1 : 0, end = max((vocab + shift) / kOf<E>, first);
     }
-    __device__ u32x4 load(uint32_t v) const {
+    // kN vectors, that(i) each: all whole ones on their way at once, without a branch between
+    // them, which would wait; from `vectors` on -inf.  Vector 0 is the first, if any.
+    template <uint32_t kN, typename That>
+    __device__ __forceinline__ void load(u32x4 (&r)[kN], That that) const {
+        if (end > first) {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) {
+                const uint32_t v = that(i), u = min(max(v, first), end - 1);
+                r[i] = reinterpret_cast<const u32x4*>(x - shift)[u];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i)
+                if (that(i) != min(max(that(i), first), end - 1)) r[i] = nothing<E>();
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) r[i] = nothing<E>();
+        }
+        if (first > 0 && that(0) == 0) r[0] = edge(0);
+        if (end < vectors) {
+            bool has = false;
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) has |= that(i) == vectors - 1;
+            if (has) {
+                const u32x4 last = edge(vectors - 1);
+#pragma unroll
+                for (uint32_t i = 0; i < kN; ++i)
+                    if (that(i) == vectors - 1) r[i] = last;
+            }
+        }
+    }
+    __device__ u32x4 edge(uint32_t v) const {
         const int64_t at = int64_t(v) * kOf<E> - shift;
-        if (at >= 0 && at + kOf<E> <= vocab) return *reinterpret_cast<const u32x4*>(x + at);
         u32x4 r;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
@@ -123,11 +171,6 @@ struct Row {
     }
     __device__ uint32_t index(uint32_t v, uint32_t i) const { return v * kOf<E> + i - shift; }
 };
-template <typename E>
-__device__ __forceinline__ u32x4 nothing() {
-    const uint32_t w = std::is_same_v<E, F32> ? 0xFF800000u : std::is_same_v<E, Bf16> ? Bf16::kNegInf2 : F16::kNegInf2;
-    return u32x4{w, w, w, w};
-}
 
 // What a part leaves.
 struct Part {
@@ -212,27 +255,30 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
     constexpr uint32_t kN = kOf<E>;
     __shared__ float shared_m[kPartLanes / 64];
     __shared__ double shared_s[kPartLanes / 64];
-    __shared__ uint32_t count;
+    __shared__ uint32_t count, hits;
     __shared__ float bound_of;
-    __shared__ uint64_t mass[kBins];
+    __shared__ __attribute__((aligned(16))) uint64_t mass[kBins];
     __shared__ uint32_t number[kBins];
+    static_assert(kPartLanes * 16 <= sizeof(mass) && kPartLanes <= kBins, "the vectors with candidates");
     float* const most = reinterpret_cast<float*>(mass);   // [kPartLanes]
     const uint64_t row = blockIdx.x / a.parts;
     const uint32_t part = blockIdx.x % a.parts;
     const Row<E> r(a.logits, a.ld, a.first + row, a.vocab);
     u32x4 x[kV];
+    r.load(x, [&](uint32_t i) {
+        const uint32_t in = i * kPartLanes + threadIdx.x;
+        return in < a.per ? part * a.per + in : ~0u;
+    });
+    const Settings s = settings<kKind>(a, a.first + row);
+    float mine = kNegInf, each[kV];   // the largest of each vector
 #pragma unroll
     for (uint32_t i = 0; i < kV; ++i) {
-        const uint32_t in = i * kPartLanes + threadIdx.x, v = part * a.per + in;
-        x[i] = in < a.per && v < r.vectors ? r.load(v) : nothing<E>();
+        each[i] = item<E>(x[i], 0);
+#pragma unroll
+        for (uint32_t j = 1; j < kN; ++j) each[i] = fmaxf(each[i], item<E>(x[i], j));
+        mine = fmaxf(mine, each[i]);
     }
-    const Settings s = settings<kKind>(a, a.first + row);
-    float mine = kNegInf;
-#pragma unroll
-    for (uint32_t i = 0; i < kV; ++i)
-#pragma unroll
-        for (uint32_t j = 0; j < kN; ++j) mine = fmaxf(mine, item<E>(x[i], j));
-    if (threadIdx.x == 0) count = 0;
+    if (threadIdx.x == 0) count = 0, hits = 0;
     const float m = block_all<kPartLanes>(mine, shared_m, Max{});
     Part* const out = a.part + row * a.parts + part;
     uint64_t* const list = a.lists + (row * a.parts + part) * a.list;
@@ -278,25 +324,46 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
             }
             if (threadIdx.x == 0) bound_of = float_of(bound << 16);
         }
-        __syncthreads();
+        __syncthreads();   // also: the lanes' maxima have been read
         const float bound = bound_of;
-        // a bound of NaN's bits is that of fewer lanes than k: every word
-        if (mine >= bound || bound != bound)
+        const auto keep = [&](u32x4 v, uint32_t of, uint32_t at_v, uint32_t j) {
+            const float f = item<E>(v, of);
+            if (f > kNegInf && !(f < bound)) {
+                const uint32_t at = atomicAdd(&count, 1u);
+                if (at < a.list) list[at] = place_of(f, r.index(at_v, j));
+            }
+        };
+        // Few vectors have a candidate: those go to LDS, and then every lane looks at one word at a
+        // time.  A bound of NaN's bits is that of fewer lanes than k: every word.
+        u32x4* const found = reinterpret_cast<u32x4*>(mass);
+        uint32_t* const found_v = number;
+#pragma unroll
+        for (uint32_t i = 0; i < kV; ++i)
+            if (!(each[i] < bound) && each[i] > kNegInf) {
+                const uint32_t at = atomicAdd(&hits, 1u);
+                if (at < kPartLanes) found[at] = x[i], found_v[at] = part * a.per + i * kPartLanes + threadIdx.x;
+            }
+        __syncthreads();
+        const uint32_t n = hits;
+        if (n <= kPartLanes) {
+            for (uint32_t i = threadIdx.x; i < n * kN; i += kPartLanes) {
+                const u32x4 v = found[i / kN];
+                uint32_t word = v[0];   // of the vector's four, or of its pairs
+#pragma unroll
+                for (uint32_t w = 1; w < 4; ++w) word = i % kN / (kN / 4) == w ? v[w] : word;
+                keep(u32x4{word, 0, 0, 0}, kN == 4 ? 0 : i % 2, found_v[i / kN], i % kN);
+            }
+        } else {
 #pragma unroll
             for (uint32_t i = 0; i < kV; ++i)
 #pragma unroll
-                for (uint32_t j = 0; j < kN; ++j) {
-                    const float f = item<E>(x[i], j);
-                    if (f > kNegInf && !(f < bound)) {
-                        const uint32_t at = atomicAdd(&count, 1u);
-                        if (at < a.list) list[at] = place_of(f, r.index(part * a.per + i * kPartLanes + threadIdx.x, j));
-                    }
-                }
+                for (uint32_t j = 0; j < kN; ++j) keep(x[i], j, part * a.per + i * kPartLanes + threadIdx.x, j);
+        }
         __syncthreads();
         if (threadIdx.x == 0) *out = Part{m, count, total};
         return;
     }
-    const double c = 1.4426950408889634073599 / s.t;
+    const Weigh weigh(1.4426950408889634073599 / s.t, from);
     const float scale = bin_scale(s.t), top_bin = floorf(m * scale);
     if (s.filtered) {
         for (uint32_t i = threadIdx.x; i < kBins; i += kPartLanes) mass[i] = 0, number[i] = 0;
@@ -312,7 +379,7 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
         for (uint32_t j = 0; j < kN; ++j) {
             const float f = item<E>(x[i], j);
             nan |= f != f;
-            const double w = exp2_wide((double(f) - double(from)) * c);
+            const double w = weigh(f);
             sum += w;
             if (s.filtered) {
                 const float bin = top_bin - floorf(f * scale);
@@ -345,7 +412,7 @@ __device__ __forceinline__ double mass_of(const Part& p, float m, double c) {   
     return p.m > kNegInf || p.sum != p.sum ? p.sum * exp2_wide((double(p.m) - double(m)) * c) : 0.0;
 }
 template <uint32_t kT>
-__device__ Joined join_parts(const Rows& a, const Part* part, double c, double* shared) {
+__device__ __forceinline__ Joined join_parts(const Rows& a, const Part* part, double c, double* shared) {
     const Part own = threadIdx.x < a.parts ? part[threadIdx.x] : Part{kNegInf, 0, 0.0};
     float m = own.m;
     for (uint32_t p = threadIdx.x + kT; p < a.parts; p += kT) m = fmaxf(m, part[p].m);
@@ -397,7 +464,7 @@ struct Bins {
 // `before` of it ahead of all bins; kN where none does.  Left in sh with what comes before it
 // and its number of words.
 template <uint32_t kT, uint32_t kN, typename Sh>
-__device__ void find_bin(const uint64_t* mass, const uint32_t* number, bool by_mass, uint64_t reach, uint64_t before_mass,
+__device__ __forceinline__ void find_bin(const uint64_t* mass, const uint32_t* number, bool by_mass, uint64_t reach, uint64_t before_mass,
                          uint32_t before, Sh& sh) {
     constexpr uint32_t kEach = (kN + kT - 1) / kT;
     const uint32_t bin0 = threadIdx.x * kEach;
@@ -438,7 +505,7 @@ __device__ void find_bin(const uint64_t* mass, const uint32_t* number, bool by_m
 // leaves none, the last with a weight.  Every wave has a run of the row's vectors from v0
 // to v1.  share: the target is that of the whole sum.
 template <typename E, uint32_t kT, typename Weight, typename Sh>
-__device__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double target, bool share, Weight weight, Sh& sh) {
+__device__ __forceinline__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double target, bool share, Weight weight, Sh& sh) {
     constexpr uint32_t kWaves = kT / 64;
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t each = (v1 - v0 + kWaves - 1) / kWaves;
@@ -447,8 +514,7 @@ __device__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double 
     uint32_t last = 0;   // index + 1 of the last with a weight
     for (uint32_t v = from + lane; v < to; v += 256) {
         u32x4 x[4];
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) x[u] = v + u * 64 < to ? r.load(v + u * 64) : nothing<E>();
+        r.load(x, [&](uint32_t u) { return v + u * 64 < to ? v + u * 64 : ~0u; });
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u)
 #pragma unroll
@@ -484,7 +550,9 @@ __device__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double 
         uint32_t found = last;
         double rest = target - before;
         for (uint32_t v = from + lane; !whole && v - lane < to; v += 64) {
-            const u32x4 x = v < to ? r.load(v) : nothing<E>();
+            u32x4 one[1];
+            r.load(one, [&](uint32_t) { return v < to ? v : ~0u; });
+            const u32x4 x = one[0];
             double own = 0.0;
 #pragma unroll
             for (uint32_t j = 0; j < kOf<E>; ++j) own += weight(item<E>(x, j), r.index(v, j));
@@ -524,12 +592,12 @@ __device__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double 
 // For every word of the row.
 template <typename E, uint32_t kT, typename F>
 __device__ __forceinline__ void each_word(const Row<E>& r, F f) {
-    for (uint32_t v = threadIdx.x; v < r.vectors; v += kT * 4) {
-        u32x4 x[4];
+    constexpr uint32_t kAtOnce = 8;
+    for (uint32_t v = threadIdx.x; v < r.vectors; v += kT * kAtOnce) {
+        u32x4 x[kAtOnce];
+        r.load(x, [&](uint32_t u) { return v + u * kT; });
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) x[u] = v + u * kT < r.vectors ? r.load(v + u * kT) : nothing<E>();
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)
+        for (uint32_t u = 0; u < kAtOnce; ++u)
 #pragma unroll
             for (uint32_t j = 0; j < kOf<E>; ++j) f(item<E>(x[u], j), r.index(v + u * kT, j));
     }
@@ -539,13 +607,14 @@ __device__ __forceinline__ void each_word(const Row<E>& r, F f) {
 // word of the prefix that a count (so many words) or a mass (the words with less than `reach`
 // before them) asks for, 0 for every word.  prefix_mass: of the prefix, or null.
 template <typename E, uint32_t kT, typename Sh>
-__device__ uint64_t border_by_digits(const Row<E>& r, float m, double c, bool by_mass, double reach, double* prefix_mass,
+__device__ __forceinline__ uint64_t border_by_digits(const Row<E>& r, float m, double c, bool by_mass, double reach, double* prefix_mass,
                                      Sh& sh) {
     constexpr uint32_t kDigits = 1 << kDigit;
     // masses in whole numbers whose sum 62 bits hold
     const int bits = 62 - (32 - __builtin_clz(r.vocab));
     const double one = ldexp(1.0, bits);
-    const auto whole = [&](float f) { return uint64_t(exp2_wide((double(f) - double(m)) * c) * one + 0.5); };
+    const Weigh weigh(c, m);
+    const auto whole = [&](float f) { return uint64_t(weigh(f) * one + 0.5); };
     const uint64_t target = by_mass ? uint64_t(ceil(fmax(reach, 0.0) * one)) : uint64_t(reach);
     uint32_t prefix = 0, known = 0, before = 0;
     uint64_t before_mass = 0;
@@ -590,7 +659,7 @@ __device__ __forceinline__ bool bins_do(const Rows& a, float top_bin) {
     return a.vocab <= (1u << 18) && a.parts <= kMostParts && fabsf(top_bin) < 0x1p22f;
 }
 template <uint32_t kT>
-__device__ void join_bins(const Rows& a, const Part* part, const uint64_t* lists, float m, double c, float scale, float top_bin,
+__device__ __forceinline__ void join_bins(const Rows& a, const Part* part, const uint64_t* lists, float m, double c, float scale, float top_bin,
                           Bins& bins) {
     for (uint32_t i = threadIdx.x; i < kBins; i += kT) bins.mass[i] = 0, bins.number[i] = 0;
     if (threadIdx.x < a.parts) {
@@ -617,7 +686,7 @@ __device__ void join_bins(const Rows& a, const Part* part, const uint64_t* lists
 // sh.places, sh.held of them, and its number in bins.bin.  false: what is looked for lies
 // below the histograms, or the bin holds too many.
 template <typename E, uint32_t kT, typename Sh>
-__device__ bool border_by_bins(const Rows& a, const Part* part, const uint64_t* lists, const Row<E>& r, float m, double t,
+__device__ __forceinline__ bool border_by_bins(const Rows& a, const Part* part, const uint64_t* lists, const Row<E>& r, float m, double t,
                                bool by_mass, double reach, uint64_t* border, double* prefix_mass, Sh& sh, Bins& bins) {
     const double c = 1.4426950408889634073599 / t;
     const float scale = bin_scale(t), top_bin = floorf(m * scale);
@@ -645,7 +714,7 @@ __device__ bool border_by_bins(const Rows& a, const Part* part, const uint64_t* 
     __syncthreads();
     if (sh.count != n) return false;
     const auto sub_of = [&](float f) { return kSubBins - 1 - min(uint32_t((f * scale - lo) * float(kSubBins)), kSubBins - 1); };
-    const auto weight = [&](float f) { return exp2_wide((double(f) - double(m)) * c); };
+    const Weigh weight(c, m);
     for (uint32_t i = threadIdx.x; i < n; i += kT) {
         const float f = logit_of(sh.places[i]);
         atomicAdd(&bins.sub_number[sub_of(f)], 1u);
@@ -737,7 +806,7 @@ __device__ bool border_by_bins(const Rows& a, const Part* part, const uint64_t* 
 // ---------------------------------------------------------------------
 constexpr uint32_t kPicked = 1024;
 template <typename Sh>
-__device__ bool pick_largest(const Rows& a, const Part* part, const uint64_t* lists, uint32_t k, Sh& sh) {
+__device__ __forceinline__ bool pick_largest(const Rows& a, const Part* part, const uint64_t* lists, uint32_t k, Sh& sh) {
     static_assert(Sh::kSorted >= kPicked, "it holds them");
     constexpr uint32_t kEach = kPicked / 64;
     const uint32_t lane = threadIdx.x;
@@ -825,7 +894,7 @@ __device__ bool pick_largest(const Rows& a, const Part* part, const uint64_t* li
     return true;
 }
 template <typename E, uint32_t kT, typename Sh>
-__device__ uint32_t largest(const Rows& a, const Part* part, const uint64_t* lists, const Row<E>& r, float m, double c, uint32_t k,
+__device__ __forceinline__ uint32_t largest(const Rows& a, const Part* part, const uint64_t* lists, const Row<E>& r, float m, double c, uint32_t k,
                             Sh& sh) {
     __syncthreads();
     if (threadIdx.x < 64) {
@@ -898,7 +967,7 @@ __global__ __launch_bounds__(kListedLanes) void top_rows_kernel(const Rows a) {
 // ---------------------------------------------------------------------
 // A draw from the k largest words, by the first wave: two words a lane, in their order.
 template <typename E, uint32_t kT, typename Sh>
-__device__ void draw_listed(const Rows& a, uint64_t of, const Settings& s, const Part* part, const uint64_t* lists,
+__device__ __forceinline__ void draw_listed(const Rows& a, uint64_t of, const Settings& s, const Part* part, const uint64_t* lists,
                             const Joined& j, double c, double u, double least, double lse, Sh& sh) {
     const Row<E> r(a.logits, a.ld, of, a.vocab);
     const uint32_t n = largest<E, kT>(a, part, lists, r, j.m, c, s.k, sh);
@@ -983,7 +1052,7 @@ __global__ __launch_bounds__(kListedLanes) void draw_listed_kernel(const Rows a)
 // The mass that each part keeps with a border in bin `at`: its bins above, and of that bin's words
 // those up to the border.
 template <typename E, uint32_t kT, typename Sh>
-__device__ void kept_by_parts(const Rows& a, const uint64_t* lists, const Row<E>& r, float m, double c, float scale, float top_bin,
+__device__ __forceinline__ void kept_by_parts(const Rows& a, const uint64_t* lists, const Row<E>& r, float m, double c, float scale, float top_bin,
                               float at, uint64_t border, Sh& sh, Bins& bins) {
     __syncthreads();
     if (threadIdx.x < a.parts) bins.kept[threadIdx.x] = 0;
@@ -997,8 +1066,9 @@ __device__ void kept_by_parts(const Rows& a, const uint64_t* lists, const Row<E>
         for (int d = 32; d > 0; d >>= 1) mass += __shfl_xor(mass, d);
         if ((threadIdx.x & 63) == 0 && mass != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&bins.kept[p]), static_cast<unsigned long long>(mass));
     }
+    const Weigh weigh(c, m);
     const auto add = [&](uint64_t place) {
-        const uint64_t mass = uint64_t(exp2_wide((double(logit_of(place)) - double(m)) * c) * 0x1p44 + 0.5);
+        const uint64_t mass = uint64_t(weigh(logit_of(place)) * 0x1p44 + 0.5);
         const uint32_t p = (index_of(place) + r.shift) / kOf<E> / a.per;
         atomicAdd(reinterpret_cast<unsigned long long*>(&bins.kept[p]), static_cast<unsigned long long>(mass));
     };
@@ -1016,7 +1086,7 @@ __device__ void kept_by_parts(const Rows& a, const uint64_t* lists, const Row<E>
 }
 
 template <typename E>
-__device__ void write_draw(const Rows& a, uint64_t of, const Row<E>& r, uint32_t index, const Joined& j, const Settings& s) {
+__device__ __forceinline__ void write_draw(const Rows& a, uint64_t of, const Row<E>& r, uint32_t index, const Joined& j, const Settings& s) {
     float f;
     if constexpr (std::is_same_v<E, F32>) f = __uint_as_float(r.x[index]);
     else f = E::lo(r.x[index]);
@@ -1027,7 +1097,7 @@ __device__ void write_draw(const Rows& a, uint64_t of, const Row<E>& r, uint32_t
 // The part in which the running mass exceeds u times all (sum_up: their sum, of up to 64 parts), and
 // what of that mass lies within it; where rounding leaves none, the last with a mass and infinity.
 template <typename Mass, typename Sh>
-__device__ double choose_part(const Rows& a, double u, bool sum_up, double all, Mass mass, uint32_t* chosen, Sh& sh) {
+__device__ __forceinline__ double choose_part(const Rows& a, double u, bool sum_up, double all, Mass mass, uint32_t* chosen, Sh& sh) {
     if (threadIdx.x < 64) {
         const uint32_t lane = threadIdx.x;
         double before = 0.0, rest = __builtin_inf();
@@ -1079,9 +1149,10 @@ __global__ __launch_bounds__(kWholeLanes) void draw_whole_kernel(const Rows a) {
     uint32_t v0;
     const double target = choose_part(a, share_of(a.uniforms[of]), false, j.sum, [&](uint32_t p) { return mass_of(part[p], j.m, c); }, &v0, sh);
     v0 = min(v0 * a.per, r.vectors);
+    const Weigh weigh(c, j.m);
     const uint32_t index = min(find_word<E, kWholeLanes>(
         r, v0, min(v0 + a.per, r.vectors), target, false,
-        [&](float f, uint32_t) { return exp2_wide((double(f) - double(j.m)) * c); }, sh), a.vocab - 1);
+        [&](float f, uint32_t) { return weigh(f); }, sh), a.vocab - 1);
     if (threadIdx.x == 0) write_draw(a, of, r, index, j, s);
 }
 
@@ -1104,7 +1175,7 @@ __global__ __launch_bounds__(kDrawLanes) void draw_rows_kernel(const Rows a) {
     if (kKind == kEither && s.listed)
         return draw_listed<E, kDrawLanes>(a, of, s, part, lists, j, c, u, least, log(j.sum), sh);
     const Row<E> r(a.logits, a.ld, of, a.vocab);
-    const auto weight = [&](float f) { return exp2_wide((double(f) - double(j.m)) * c); };
+    const Weigh weight(c, j.m);
     uint64_t border = 0;
     bool by_parts = true;   // their masses say which one it is in
     if (s.filtered) {
