@@ -78,7 +78,7 @@ __device__ __forceinline__ uint64_t place_of(float x, uint32_t index) {
 __device__ __forceinline__ float logit_of(uint64_t place) { return float_of(uint32_t(place >> 32)); }
 __device__ __forceinline__ uint32_t index_of(uint64_t place) { return ~uint32_t(place); }
 
-// 2^y for finite y <= 0 or so: 2^n times the series of e^(f ln 2) to its 10th power, off
+// 2^y for y <= 0 or so, 0 of -inf: 2^n times the series of e^(f ln 2) to its 10th power, off
 // by 2^-42 of itself.
 constexpr int kPowers = 10;
 struct Series {
@@ -90,18 +90,19 @@ struct Series {
 };
 __constant__ constexpr Series kSeries{};
 __device__ __forceinline__ double exp2_wide(double y) {
+    y = fmax(y, -1100.0);
     const double n = rint(y), f = y - n;
     double p = kSeries.c[kPowers];
 #pragma unroll
     for (int i = kPowers - 1; i >= 0; --i) p = fma(p, f, kSeries.c[i]);
     return ldexp(p, int(n));
 }
-// A logit's weight, exp((x - from) / T) as 2^(c x - c from); 0 of -inf.
+// A logit's weight, exp((x - from) / T) as 2^(c (x - from)); 0 of -inf.
 struct Weigh {
-    double c, less;
-    __device__ Weigh(double c_, float from) : c(c_), less(double(from) * c_) {}
+    double c, from;
+    __device__ Weigh(double c_, float from_) : c(c_), from(from_) {}
     __device__ double operator()(float x) const {
-        return exp2_wide(fma(double(fmaxf(x, -0x1.fffffep127f)), c, -less));
+        return exp2_wide((double(x) - from) * c);
     }
 };
 
@@ -185,7 +186,7 @@ struct Rows {
     uint32_t vocab, parts, per; // per: vectors of a part
     uint32_t list;              // places that a part's list holds
     Part* part;                 // [rows, parts]
-    uint64_t* lists;            // [rows, parts, list]: places, or masses and counts of bins
+    uint64_t* lists;            // [rows, parts, list]: places, or masses up to each bin and counts of bins
     // settings: of all rows, or of each
     double temperature, top_p, min_p;
     int64_t top_k;
@@ -393,11 +394,24 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
     }
     if (nan) sum = __builtin_nan("");
     sum = block_all<kPartLanes>(sum, shared_s, Add{});
-    if (s.filtered)
-        for (uint32_t i = threadIdx.x; i < kBins; i += kPartLanes) {
-            list[i] = mass[i];
-            reinterpret_cast<uint16_t*>(list + kBins)[i] = uint16_t(number[i]);
+    if (s.filtered) {
+        // the masses of all bins up to each
+        static_assert(kBins == 2 * kPartLanes, "two bins a lane");
+        const uint64_t one = mass[2 * threadIdx.x], two = one + mass[2 * threadIdx.x + 1];
+        uint64_t upto = two;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint64_t below = __shfl_up(upto, d);
+            if ((threadIdx.x & 63) >= uint32_t(d)) upto += below;
         }
+        uint64_t* const waves = reinterpret_cast<uint64_t*>(shared_s);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = upto;
+        __syncthreads();
+        for (uint32_t w = 0; w < threadIdx.x >> 6; ++w) upto += waves[w];
+        list[2 * threadIdx.x] = upto - two + one, list[2 * threadIdx.x + 1] = upto;
+        reinterpret_cast<uint32_t*>(list + kBins)[threadIdx.x] = number[2 * threadIdx.x] | number[2 * threadIdx.x + 1] << 16;
+    }
     if (threadIdx.x == 0) *out = Part{m, 0, sum};
 }
 
@@ -668,15 +682,26 @@ __device__ __forceinline__ void join_bins(const Rows& a, const Part* part, const
         bins.offset[threadIdx.x] = mp > kNegInf ? top_bin - floorf(mp * scale) : 2.0f * kBins;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < a.parts * kBins; i += kT) {
-        const uint32_t p = i / kBins, bin = i % kBins;
-        const float at = bins.offset[p] + float(bin);
-        if (!(at < float(kBins))) continue;
-        const uint32_t number = reinterpret_cast<const uint16_t*>(lists + uint64_t(p) * a.list + kBins)[bin];
-        if (number == 0) continue;
-        atomicAdd(&bins.number[uint32_t(at)], number);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&bins.mass[uint32_t(at)]),
-                  static_cast<unsigned long long>(double(lists[uint64_t(p) * a.list + bin]) * bins.factor[p] + 0.5));
+    constexpr uint32_t kAtOnce = 4;
+    for (uint32_t i0 = threadIdx.x; i0 < a.parts * kBins; i0 += kT * kAtOnce) {
+        uint64_t upto[kAtOnce], below[kAtOnce];
+        uint32_t number[kAtOnce];
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            const uint32_t i = min(i0 + u * kT, a.parts * kBins - 1), p = i / kBins, bin = i % kBins;
+            const uint64_t* const of = lists + uint64_t(p) * a.list;
+            upto[u] = of[bin], below[u] = bin > 0 ? of[bin - 1] : 0;
+            number[u] = reinterpret_cast<const uint16_t*>(of + kBins)[bin];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            const uint32_t i = i0 + u * kT, p = min(i / kBins, a.parts - 1);
+            const float at = bins.offset[p] + float(i % kBins);
+            if (i >= a.parts * kBins || number[u] == 0 || !(at < float(kBins))) continue;
+            atomicAdd(&bins.number[uint32_t(at)], number[u]);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&bins.mass[uint32_t(at)]),
+                      static_cast<unsigned long long>(double(upto[u] - below[u]) * bins.factor[p] + 0.5));
+        }
     }
     __syncthreads();
 }
@@ -764,7 +789,9 @@ __device__ __forceinline__ bool border_by_bins(const Rows& a, const Part* part, 
         if (threadIdx.x < sh.count) {
             const uint64_t own = sh.few[threadIdx.x];
             uint32_t rank = 0;
-            for (uint32_t i = 0; i < sh.count; ++i) rank += sh.few[i] > own;
+            const uint32_t all = sh.count;
+#pragma unroll 8
+            for (uint32_t i = 0; i < all; ++i) rank += sh.few[i] > own;
             if (ahead + rank + 1 == take) sh.found = own;
         }
         if (threadIdx.x == 0) sh.found_mass = mass_sub + w * take;
@@ -772,6 +799,7 @@ __device__ __forceinline__ bool border_by_bins(const Rows& a, const Part* part, 
         const uint32_t lane = threadIdx.x;
         const uint64_t own = lane < few ? sh.few[lane] : 0;
         uint32_t rank = 0;
+#pragma unroll 8
         for (uint32_t i = 0; i < few; ++i) rank += sh.few[i] > own;
         if (lane < few) sh.few[64 + rank] = own;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -884,6 +912,7 @@ __device__ __forceinline__ bool pick_largest(const Rows& a, const Part* part, co
     static_assert(kMost == 128, "two words a lane");
     const uint64_t own0 = lane < n ? sh.places[lane] : 0, own1 = lane + 64 < n ? sh.places[lane + 64] : 0;
     uint32_t rank0 = 0, rank1 = 0;
+#pragma unroll 8
     for (uint32_t i = 0; i < n; ++i) {
         const uint64_t other = sh.places[i];
         rank0 += other > own0, rank1 += other > own1;
@@ -1000,6 +1029,7 @@ __device__ __forceinline__ void draw_listed(const Rows& a, uint64_t of, const Se
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const uint32_t index[2] = {index_of(place[0]), index_of(place[1])};
     double mass = 0.0, sums[2] = {0.0, 0.0};   // in one order everywhere
+#pragma unroll 8
     for (uint32_t i = 0; i < n; ++i) {
         const double v = sh.weights[i];
         const uint32_t at = index_of(sh.few[i]);
@@ -1055,17 +1085,12 @@ template <typename E, uint32_t kT, typename Sh>
 __device__ __forceinline__ void kept_by_parts(const Rows& a, const uint64_t* lists, const Row<E>& r, float m, double c, float scale, float top_bin,
                               float at, uint64_t border, Sh& sh, Bins& bins) {
     __syncthreads();
-    if (threadIdx.x < a.parts) bins.kept[threadIdx.x] = 0;
-    __syncthreads();
-    for (uint32_t i0 = 0; i0 < a.parts * kBins; i0 += kT) {   // a wave has bins of one part
-        const uint32_t i = i0 + threadIdx.x, p = i / kBins, bin = i % kBins;
-        uint64_t mass = 0;
-        if (p < a.parts && bins.offset[p] + float(bin) < at)
-            mass = uint64_t(double(lists[uint64_t(p) * a.list + bin]) * bins.factor[p] + 0.5);
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) mass += __shfl_xor(mass, d);
-        if ((threadIdx.x & 63) == 0 && mass != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&bins.kept[p]), static_cast<unsigned long long>(mass));
+    if (threadIdx.x < a.parts) {
+        const float above = at - bins.offset[threadIdx.x];   // bins of the part
+        bins.kept[threadIdx.x] = !(above >= 1.0f) ? 0 : uint64_t(
+            double(lists[uint64_t(threadIdx.x) * a.list + uint32_t(above) - 1]) * bins.factor[threadIdx.x] + 0.5);
     }
+    __syncthreads();
     const Weigh weigh(c, m);
     const auto add = [&](uint64_t place) {
         const uint64_t mass = uint64_t(weigh(logit_of(place)) * 0x1p44 + 0.5);

@@ -94,6 +94,19 @@ def test_rows_that_are_no_distribution(dev):
         assert (top.ids[[3, 5]] >= 0).all()
 
 
+def test_rows_of_the_lowest_value(dev):
+    """Logits that are all the type's lowest, or that and infinities: their differences count."""
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        for vocab in (100, 500, 40_001):
+            x = torch.full((4, vocab), torch.finfo(dtype).min, dtype=dtype, device=dev)
+            x[1, ::2] = -math.inf
+            x[2] = torch.finfo(dtype).max
+            x[3, 1:] = -math.inf
+            for s in (dict(), dict(k=20), dict(p=0.5), dict(k=300, m=0.5), dict(t=0.5)):
+                u = torch.tensor([0.3, 0.999, 0.7, 0.5], device=dev)
+                against(x, u.cpu(), sample_tokens(x, u, s.get("t", 1.0), s.get("k", 0), s.get("p", 1.0), s.get("m", 0.0)), **s)
+
+
 def test_strides_shapes_and_rows_behind_others(dev):
     x = rows("plain", 12, 1000, torch.bfloat16, dev)
     u = torch.rand(12, device=dev)
