@@ -1,8 +1,8 @@
 """Distillation from a teacher's top log-probabilities under the output unit,
 without keeping its [N, V] logits: each token's divergence of
 ``softmax(hidden @ weight.T / temperature)`` from what a teacher leaves of it
-(``sampling.top_logps``, ``SlideFSDP.top_logps``), with the gradients of the
-hidden rows and of the weight.
+(``linear_top_logps``, ``sampling.top_logps``, ``SlideFSDP.top_logps``), with the
+gradients of the hidden rows and of the weight.
 
 The reference's output unit trains on labels alone (slide_fsdp.py:77-113).
 
@@ -23,8 +23,8 @@ import torch
 
 from . import _native
 from .fused_ce import _DTYPES, _PLAIN, _memory_is_value, _traced
-from .linear_logps import _backward_rows, _hidden_parts, _label_kinds
-from .sampling import TOP_MOST
+from .linear_logps import _backward_rows, _chunk_rows, _f32_out, _hidden_parts, _label_kinds
+from .sampling import TOP_MOST, TopLogps, top_logps
 
 _FORMS = {"forward": _native.SF_DISTILL_FORWARD, "reverse": _native.SF_DISTILL_REVERSE}
 _LEAST_REST = 2.0 ** -24
@@ -85,6 +85,30 @@ def _kernels_take(hidden, weight, ids, logps, mask) -> bool:
             and ids.numel() // ids.shape[-1] < 1 << 31 and all(type(t) in _PLAIN and _memory_is_value(t) for t in given))
 
 
+def _check_taught(shape, device, ids, logps, mask, temperature, kind, rest) -> None:
+    """What a teacher leaves of ``shape`` tokens, and how it is to be taken."""
+    if ids.shape != logps.shape or ids.dim() < 1 or ids.shape[:-1] != shape:
+        raise ValueError("linear_distill: teacher_ids and teacher_logps of [..., K] expected, one row for each hidden row")
+    if not 1 <= ids.shape[-1] <= TOP_MOST:
+        raise ValueError(f"linear_distill: from 1 to {TOP_MOST} words of each token expected, got {ids.shape[-1]}")
+    if ids.dtype != torch.int64 or logps.dtype != torch.float32:
+        raise TypeError(f"linear_distill: int64 ids and float32 log-probabilities expected, got {ids.dtype}, {logps.dtype}")
+    if mask is not None and mask.dtype != torch.bool:
+        raise TypeError(f"linear_distill: a bool mask expected, got {mask.dtype}")
+    if mask is not None and mask.shape != shape:
+        raise ValueError(f"linear_distill: the mask has to be {tuple(shape)}")
+    if any(t is not None and t.device != device for t in (ids, logps, mask)):
+        raise ValueError("linear_distill: all tensors have to be on one device")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError("linear_distill: temperature must be above 0")
+    if kind not in _FORMS:
+        raise ValueError(f"linear_distill: kind must be one of {sorted(_FORMS)}, got {kind!r}")
+    if kind == "reverse" and not rest:
+        raise ValueError("linear_distill: kind 'reverse' needs the rest: a student's words outside the teacher's have no q")
+    if logps.requires_grad and torch.is_grad_enabled():
+        raise ValueError("linear_distill: teacher_logps takes no gradient; detach it")
+
+
 def linear_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logps: torch.Tensor,
                    mask: Optional[torch.Tensor] = None, temperature: float = 1.0, kind: str = "forward",
                    rest: bool = True) -> torch.Tensor:
@@ -114,31 +138,13 @@ def linear_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
     it.  It is not multiplied by temperature^2."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError("linear_distill: hidden [..., H] and weight [V, H] expected")
-    if teacher_ids.shape != teacher_logps.shape or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != hidden.shape[:-1]:
-        raise ValueError("linear_distill: teacher_ids and teacher_logps of [..., K] expected, one row for each hidden row")
-    if not 1 <= teacher_ids.shape[-1] <= TOP_MOST:
-        raise ValueError(f"linear_distill: from 1 to {TOP_MOST} words of each token expected, got {teacher_ids.shape[-1]}")
     if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
         raise TypeError(f"linear_distill: hidden and weight of one float type expected, got {hidden.dtype}, {weight.dtype}")
-    if teacher_ids.dtype != torch.int64 or teacher_logps.dtype != torch.float32:
-        raise TypeError(f"linear_distill: int64 ids and float32 log-probabilities expected, got {teacher_ids.dtype}, "
-                        f"{teacher_logps.dtype}")
-    if mask is not None and mask.dtype != torch.bool:
-        raise TypeError(f"linear_distill: a bool mask expected, got {mask.dtype}")
-    if mask is not None and mask.shape != hidden.shape[:-1]:
-        raise ValueError(f"linear_distill: the mask has to be {tuple(hidden.shape[:-1])}")
-    if any(t.device != hidden.device for t in (weight, teacher_ids, teacher_logps, *(() if mask is None else (mask,)))):
+    if weight.device != hidden.device:
         raise ValueError("linear_distill: all tensors have to be on one device")
     if weight.shape[0] == 0:
         raise ValueError("linear_distill: an empty vocabulary")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError("linear_distill: temperature must be above 0")
-    if kind not in _FORMS:
-        raise ValueError(f"linear_distill: kind must be one of {sorted(_FORMS)}, got {kind!r}")
-    if kind == "reverse" and not rest:
-        raise ValueError("linear_distill: kind 'reverse' needs the rest: a student's words outside the teacher's have no q")
-    if teacher_logps.requires_grad and torch.is_grad_enabled():
-        raise ValueError("linear_distill: teacher_logps takes no gradient; detach it")
+    _check_taught(hidden.shape[:-1], hidden.device, teacher_ids, teacher_logps, mask, temperature, kind, rest)
     scale = 1.0 / float(temperature)
     if not _kernels_take(hidden, weight, teacher_ids, teacher_logps, mask):
         return _torch_distill(hidden, weight, teacher_ids, teacher_logps, mask, scale, kind, rest)
@@ -153,3 +159,36 @@ def linear_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
     if loss is None:
         return _torch_distill(hidden, weight, teacher_ids, teacher_logps, mask, scale, kind, rest)
     return loss.view(hidden.shape[:-1])
+
+
+# ---------------------------------------------------------------------------
+def _logits32(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``hidden @ weight.T + bias`` of a few rows, not rounded to 16 bits in between."""
+    if hidden.is_cuda and hidden.dim() == 2 and hidden.numel() > 0 and type(hidden) in _PLAIN and not _traced():
+        z = torch.mm(hidden, weight.t(), **_f32_out(hidden.dtype))
+    else:
+        z = hidden.float() @ weight.float().t()
+    return z if bias is None else z.add_(bias)
+
+
+@torch.no_grad()
+def linear_top_logps(hidden: torch.Tensor, weight: torch.Tensor, k: int, temperature: float = 1.0,
+                     bias: Optional[torch.Tensor] = None) -> TopLogps:
+    """``top_logps`` of ``hidden @ weight.T + bias``, whose logits are fp32 and
+    made 1 GiB at a time.  ``hidden`` [..., H] and ``weight`` [V, H] of one
+    float type, ``bias`` [V] or None.  No gradient."""
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError("linear_top_logps: hidden [..., H] and weight [V, H] expected")
+    if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
+        raise TypeError(f"linear_top_logps: hidden and weight of one float type expected, got {hidden.dtype}, {weight.dtype}")
+    if weight.device != hidden.device or (bias is not None and bias.device != hidden.device):
+        raise ValueError("linear_top_logps: all tensors have to be on one device")
+    if weight.shape[0] == 0 or (bias is not None and bias.shape != weight.shape[:1]):
+        raise ValueError(f"linear_top_logps: a vocabulary and a bias of it expected, got {tuple(weight.shape)}")
+    rows = hidden.reshape(-1, hidden.shape[-1])
+    step = _chunk_rows(weight.shape[0])
+    with torch.autocast(hidden.device.type, enabled=False):
+        parts = [top_logps(_logits32(rows[s:s + step], weight, bias), k, temperature)
+                 for s in range(0, max(1, rows.shape[0]), step)]
+    logps, ids = (torch.cat(t) if len(parts) > 1 else t[0] for t in zip(*parts))
+    return TopLogps(logps.view(*hidden.shape[:-1], k), ids.view(*hidden.shape[:-1], k))

@@ -114,11 +114,11 @@ def _sample_torch(logits, uniforms, temperature, top_k, top_p, min_p):
     return SampledTokens(torch.where(bad, -1, ids).squeeze(-1), torch.where(bad, math.nan, logps).squeeze(-1))
 
 
-def _setting(name: str, x, logits: torch.Tensor, dtype, least: float, most: float):
+def _setting(name: str, x, shape, device, dtype, least: float, most: float):
     """(value for all rows, value of each row or None)."""
     if isinstance(x, torch.Tensor) and x.dim() > 0:
-        if x.shape != logits.shape[:-1] or x.device != logits.device:
-            raise ValueError(f"sample_tokens: {name} of every row has to be {tuple(logits.shape[:-1])} on {logits.device}")
+        if x.shape != shape or x.device != device:
+            raise ValueError(f"sample_tokens: {name} of every row has to be {tuple(shape)} on {device}")
         if x.dtype != dtype:
             raise TypeError(f"sample_tokens: {dtype} {name} of every row expected, got {x.dtype}")
         return 0, x.detach()
@@ -126,6 +126,18 @@ def _setting(name: str, x, logits: torch.Tensor, dtype, least: float, most: floa
     if not (least <= value <= most and math.isfinite(value)) or value != x:
         raise ValueError(f"sample_tokens: {name} from {least} to {most} expected, got {x}")
     return value, None
+
+
+def _check_draw(shape, device, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The settings of a draw for ``shape`` rows, each (value for all, value of each row or None)."""
+    if uniforms.shape != shape or uniforms.device != device:
+        raise ValueError(f"sample_tokens: uniforms have to be {tuple(shape)} on {device}")
+    if uniforms.dtype != torch.float32:
+        raise TypeError(f"sample_tokens: float32 uniforms expected, got {uniforms.dtype}")
+    return (_setting("temperature", temperature, shape, device, torch.float32, 0.0, 3.0e38),
+            _setting("top_k", top_k, shape, device, torch.int64, 0, 2 ** 62),
+            _setting("top_p", top_p, shape, device, torch.float32, 0.0, 1.0),
+            _setting("min_p", min_p, shape, device, torch.float32, 0.0, 1.0))
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0,
@@ -152,14 +164,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Uni
     A row with a NaN or +infinity, or of -infinities alone, gives -1 and NaN.
     No gradient."""
     _check_logits("sample_tokens", logits)
-    if uniforms.shape != logits.shape[:-1] or uniforms.device != logits.device:
-        raise ValueError(f"sample_tokens: uniforms have to be {tuple(logits.shape[:-1])} on {logits.device}")
-    if uniforms.dtype != torch.float32:
-        raise TypeError(f"sample_tokens: float32 uniforms expected, got {uniforms.dtype}")
-    t, ts = _setting("temperature", temperature, logits, torch.float32, 0.0, 3.0e38)
-    k, ks = _setting("top_k", top_k, logits, torch.int64, 0, 2 ** 62)
-    p, ps = _setting("top_p", top_p, logits, torch.float32, 0.0, 1.0)
-    m, ms = _setting("min_p", min_p, logits, torch.float32, 0.0, 1.0)
+    (t, ts), (k, ks), (p, ps), (m, ms) = _check_draw(logits.shape[:-1], logits.device, uniforms, temperature, top_k, top_p,
+                                                     min_p)
     logits, uniforms = logits.detach(), uniforms.detach()
     if logits.is_cuda and logits.numel() > 0 and not _traced():
         out = _native.ops().sample_tokens(logits, uniforms, t, ts, k, ks, p, ps, m, ms)

@@ -61,11 +61,13 @@ from transformers.modeling_outputs import CausalLMOutputWithPast
 from . import _native, kernels
 from .act8 import _check_format, act8_bytes
 from .config import SlideFSDPConfig
+from .distillation import _check_taught, _logits32, _torch_distill, linear_distill, linear_top_logps
 from .distributed_sync import create_distributed_sync
 from .fused_ce import chunked_linear_cross_entropy
 from .linear_logps import _torch_logps, linear_logps
 from .layer_state import GradSlotRing, LayerRuntimeState, StreamingRuntime
 from .optimizer import LayerAdam
+from .sampling import TOP_MOST, SampledTokens, TopLogps, _check_draw, sample_tokens
 from .sliding_checkpoint import ActivationRing, KeptOnDevice, SlidingCheckpoint, StorageSpill, pin_or_keep
 
 
@@ -77,10 +79,13 @@ except ImportError:  # older versions keep the decoder's _update_causal_mask
 @dataclass
 class ObjectiveOutput(CausalLMOutputWithPast):
     """What a step on an ``objective`` returns: the loss, the log-probabilities
-    it was computed from, [B, S - 1], and what the objective returned."""
+    it was computed from, [B, S - 1], and what the objective returned.  Of a step
+    with a ``teacher``: the loss, each token's divergence, [B, S - 1], and what
+    the objective returned, if there was one."""
 
     logps: Optional[torch.Tensor] = None
     result: Any = None
+    divergences: Optional[torch.Tensor] = None
 
 
 def _loss_of(result: Any) -> torch.Tensor:
@@ -122,6 +127,29 @@ class OutputLayer(nn.Module):
         if bias is None:
             return linear_logps(hidden_states, self.lm_head.weight, labels, ignore_index, temperature)
         return _torch_logps(hidden_states, self.lm_head.weight, labels, ignore_index, 1.0 / temperature, bias)
+
+    def top_logps(self, hidden_states: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogps:
+        """The k largest log-probabilities of each next token and their words,
+        [B, S - 1, k]."""
+        hidden_states = self.norm(hidden_states)[..., :-1, :]
+        return linear_top_logps(hidden_states, self.lm_head.weight, k, temperature, getattr(self.lm_head, "bias", None))
+
+    def divergences(self, hidden_states: torch.Tensor, teacher: TopLogps, mask: Optional[torch.Tensor],
+                    temperature: float = 1.0, kind: str = "forward", rest: bool = True) -> torch.Tensor:
+        """Each next token's divergence from a teacher's, [B, S - 1] fp32, 0 where
+        the mask is False; no logits are kept.  With a bias, which the kernels do
+        not add, by torch operations from all logits."""
+        hidden_states, bias = self.norm(hidden_states)[..., :-1, :], getattr(self.lm_head, "bias", None)
+        if bias is None:
+            return linear_distill(hidden_states, self.lm_head.weight, teacher.ids, teacher.logps, mask, temperature, kind, rest)
+        return _torch_distill(hidden_states, self.lm_head.weight, teacher.ids, teacher.logps, mask, 1.0 / temperature, kind,
+                              rest, bias)
+
+    def sample_tokens(self, hidden_states: torch.Tensor, at: torch.Tensor, uniforms: torch.Tensor, **settings) -> SampledTokens:
+        """One token behind position ``at[i]`` of row i."""
+        rows = hidden_states[torch.arange(len(at), device=at.device), at]
+        logits = _logits32(self.norm(rows), self.lm_head.weight, getattr(self.lm_head, "bias", None))
+        return sample_tokens(logits, uniforms, **settings)
 
     def forward(self, hidden_states: torch.Tensor, labels: Optional[torch.Tensor] = None):
         hidden_states = self.norm(hidden_states)
@@ -718,7 +746,8 @@ class SlideFSDP(nn.Module):
 
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 labels: Optional[torch.Tensor] = None, objective: Optional[Callable] = None,
-                temperature: float = 1.0, **kwargs) -> CausalLMOutputWithPast:
+                temperature: float = 1.0, teacher: Optional[TopLogps] = None, teacher_kind: str = "forward",
+                teacher_rest: bool = True, **kwargs) -> CausalLMOutputWithPast:
         """One training step (reference slide_fsdp.py:507-640).
 
         ``objective``: in place of the cross entropy, a callable of the
@@ -727,8 +756,17 @@ class SlideFSDP(nn.Module):
         count (labels that are not -100); it returns the loss, something with
         the loss in its ``loss`` (``alignment.preference_loss`` and
         ``policy_loss`` do), or a tuple whose first element it is.  The step's backward starts from that loss, and
-        the output is an ``ObjectiveOutput``."""
-        if objective is not None:
+        the output is an ``ObjectiveOutput``.
+
+        ``teacher``: in place of labels' log-probabilities, (logps, ids) of
+        [B, S - 1, K] as ``top_logps`` gives them of the same input.  Each next
+        token's divergence from it (``distillation.linear_distill`` with
+        ``teacher_kind`` and ``teacher_rest``, at ``temperature``) counts where
+        the label is not -100 (without ``labels``: everywhere).  The loss is their
+        mean, or what an ``objective`` makes of the divergences and the mask."""
+        if teacher is not None:
+            teacher = self._check_teacher(input_ids, labels, temperature, teacher, teacher_kind, teacher_rest)
+        elif objective is not None:
             if labels is None:
                 raise ValueError("SlideFSDP: an objective needs labels")
             self._check_token_logps(input_ids, labels, temperature)
@@ -736,7 +774,14 @@ class SlideFSDP(nn.Module):
         output_state = self.layer_states[-1]
         try:
             hidden_states = self._PreLayerFunction.apply(hidden_states, output_state, None)
-            if objective is None:
+            if teacher is not None:
+                mask = torch.ones(teacher.ids.shape[:-1], dtype=torch.bool, device=self.device)
+                if labels is not None:
+                    mask = labels.to(self.device)[..., 1:] != self.output_layer.loss_fn.ignore_index
+                each = self.output_layer.divergences(hidden_states, teacher, mask, temperature, teacher_kind, teacher_rest)
+                logits, result = None, None if objective is None else objective(each, mask)
+                loss = each.sum() / mask.sum() if objective is None else _loss_of(result)
+            elif objective is None:
                 loss, logits = self.output_layer(hidden_states, labels)
             else:
                 labels = labels.to(hidden_states.device)
@@ -755,6 +800,8 @@ class SlideFSDP(nn.Module):
             raise
         if loss is not None and isinstance(self.runtime.grad_ring, GradSlotRing) and not self._ring_grown:
             self._ring_grow_pending = True
+        if teacher is not None:
+            return ObjectiveOutput(loss=loss, divergences=each.detach(), result=result)
         if objective is not None:
             return ObjectiveOutput(loss=loss, logps=logps.detach(), result=result)
         return CausalLMOutputWithPast(loss=loss, logits=logits)
@@ -769,6 +816,73 @@ class SlideFSDP(nn.Module):
         if not (temperature > 0 and math.isfinite(temperature)):
             raise ValueError("SlideFSDP: temperature must be above 0")
 
+    def _check_teacher(self, input_ids, labels, temperature, teacher, kind, rest) -> TopLogps:
+        """What can be refused before any decoder has run; the teacher on the device."""
+        if labels is not None:
+            self._check_token_logps(input_ids, labels, temperature)
+        if not (isinstance(teacher, (tuple, list)) and len(teacher) == 2
+                and all(isinstance(t, torch.Tensor) for t in teacher)):
+            raise TypeError("SlideFSDP: a teacher is (logps, ids), as top_logps gives them")
+        teacher = TopLogps(*(t.to(self.device) for t in teacher))
+        want = (input_ids.shape[0], input_ids.shape[1] - 1)
+        for t in teacher:
+            if t.dim() != 3 or t.shape[:2] != want:
+                raise ValueError(f"SlideFSDP: a teacher of {want} tokens expected, got {tuple(t.shape)}")
+        _check_taught(torch.Size(want), teacher.ids.device, teacher.ids, teacher.logps, None, temperature, kind, rest)
+        return teacher
+
+    @torch.no_grad()
+    def top_logps(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None, k: int = 64,
+                  temperature: float = 1.0) -> TopLogps:
+        """The ``k`` largest log-probabilities of each next token under the model
+        as it is, and their words, [B, S - 1, k] (``sampling.top_logps``): what
+        this model leaves, as a teacher, for ``forward(teacher=...)`` of another.
+        Nothing is kept for a backward."""
+        if not 1 <= k <= min(TOP_MOST, self.output_layer.lm_head.weight.shape[0]):
+            raise ValueError(f"SlideFSDP: k from 1 to {TOP_MOST} and the vocabulary expected, got {k}")
+        if not (temperature > 0 and math.isfinite(temperature)):
+            raise ValueError("SlideFSDP: temperature must be above 0")
+        hidden_states = self._run_decoders(input_ids, attention_mask)
+        return self._evaluate(lambda: self.output_layer.top_logps(self._at_output(hidden_states), k, temperature))
+
+    @torch.no_grad()
+    def sample_tokens(self, input_ids: torch.Tensor, uniforms: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
+                      **settings) -> SampledTokens:
+        """One token behind each row's last one (with ``attention_mask`` the last
+        whose mask is not 0) under the model as it is, drawn by ``uniforms`` [B],
+        with its log-probability; ``settings`` as ``sampling.sample_tokens`` takes
+        them.  Its log-probabilities are what ``policy_loss`` takes as
+        ``old_logps``.  A token takes a whole forward: there is no cache of keys
+        and values."""
+        rows, length = input_ids.shape
+        if length < 1:
+            raise ValueError("SlideFSDP: a token to sample behind expected")
+        uniforms = uniforms.to(self.device)
+        settings = {n: x.to(self.device) if isinstance(x, torch.Tensor) else x for n, x in settings.items()}
+        _check_draw((rows,), uniforms.device, uniforms, **settings)   # before any decoder runs
+        at = torch.full((rows,), length - 1, device=self.device)
+        if attention_mask is not None:
+            if attention_mask.shape != input_ids.shape:
+                raise ValueError(f"SlideFSDP: an attention mask of {tuple(input_ids.shape)} expected")
+            seen = attention_mask.to(self.device) != 0
+            at = torch.where(seen, torch.arange(length, device=self.device), 0).amax(dim=1)
+        hidden_states = self._run_decoders(input_ids, attention_mask)
+        return self._evaluate(lambda: self.output_layer.sample_tokens(self._at_output(hidden_states), at,
+                                                                      uniforms, **settings))
+
+    def _at_output(self, hidden_states: torch.Tensor) -> torch.Tensor:
+        return self._PreLayerFunction.apply(hidden_states, self.layer_states[-1], None)
+
+    def _evaluate(self, run: Callable):
+        """The output unit's part of a forward that no backward follows, for which
+        the last two units stay loaded: what they hold of the pool goes back to
+        it, or the next forward waits for it."""
+        try:
+            return run()
+        finally:
+            for state in self.layer_states[-2:]:
+                state.to_offload_async(is_backward=False)
+
     @torch.no_grad()
     def token_logps(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                     labels: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
@@ -779,14 +893,8 @@ class SlideFSDP(nn.Module):
         labels = input_ids if labels is None else labels
         self._check_token_logps(input_ids, labels, temperature)
         hidden_states = self._run_decoders(input_ids, attention_mask)
-        try:
-            hidden_states = self._PreLayerFunction.apply(hidden_states, self.layer_states[-1], None)
-            return self.output_layer.token_logps(hidden_states, labels.to(self.device), temperature)
-        finally:
-            # No backward follows, for which the last two units stay loaded: what
-            # they hold of the pool goes back to it, or the next forward waits for it.
-            for state in self.layer_states[-2:]:
-                state.to_offload_async(is_backward=False)
+        return self._evaluate(lambda: self.output_layer.token_logps(self._at_output(hidden_states), labels.to(self.device),
+                                                                    temperature))
 
     def _run_decoders(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor]) -> torch.Tensor:
         """The lookup and every decoder: the last hidden states."""
