@@ -63,6 +63,15 @@ __device__ __forceinline__ float item(u32x4 v, uint32_t i) {
     else return i % 2 ? E::hi(v[i / 2]) : E::lo(v[i / 2]);
 }
 
+template <typename E>
+__device__ __forceinline__ float item_at(u32x4 v, uint32_t i) {
+    constexpr uint32_t kA = std::is_same_v<E, F32> ? 1 : 2;   // of a word
+    uint32_t word = v[0];
+#pragma unroll
+    for (uint32_t w = 1; w < 4; ++w) word = i / kA == w ? v[w] : word;
+    return item<E>(u32x4{word, 0, 0, 0}, kA == 1 ? 0 : i % 2);
+}
+
 // Order-preserving words of floats; -0 as 0.
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
@@ -327,8 +336,7 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
         }
         __syncthreads();   // also: the lanes' maxima have been read
         const float bound = bound_of;
-        const auto keep = [&](u32x4 v, uint32_t of, uint32_t at_v, uint32_t j) {
-            const float f = item<E>(v, of);
+        const auto keep = [&](float f, uint32_t at_v, uint32_t j) {
             if (f > kNegInf && !(f < bound)) {
                 const uint32_t at = atomicAdd(&count, 1u);
                 if (at < a.list) list[at] = place_of(f, r.index(at_v, j));
@@ -348,17 +356,13 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
         const uint32_t n = hits;
         if (n <= kPartLanes) {
             for (uint32_t i = threadIdx.x; i < n * kN; i += kPartLanes) {
-                const u32x4 v = found[i / kN];
-                uint32_t word = v[0];   // of the vector's four, or of its pairs
-#pragma unroll
-                for (uint32_t w = 1; w < 4; ++w) word = i % kN / (kN / 4) == w ? v[w] : word;
-                keep(u32x4{word, 0, 0, 0}, kN == 4 ? 0 : i % 2, found_v[i / kN], i % kN);
+                keep(item_at<E>(found[i / kN], i % kN), found_v[i / kN], i % kN);
             }
         } else {
 #pragma unroll
             for (uint32_t i = 0; i < kV; ++i)
 #pragma unroll
-                for (uint32_t j = 0; j < kN; ++j) keep(x[i], j, part * a.per + i * kPartLanes + threadIdx.x, j);
+                for (uint32_t j = 0; j < kN; ++j) keep(item<E>(x[i], j), part * a.per + i * kPartLanes + threadIdx.x, j);
         }
         __syncthreads();
         if (threadIdx.x == 0) *out = Part{m, count, total};
@@ -500,7 +504,9 @@ __device__ __forceinline__ void find_bin(const uint64_t* mass, const uint32_t* n
     __syncthreads();
     uint64_t at_m = before_mass + upto_m - m;
     uint32_t at_n = upto_n - n;   // of these bins
-    for (uint32_t w = 0; w < threadIdx.x >> 6; ++w) at_m += sh.scan_m[w], at_n += sh.scan_n[w];
+#pragma unroll
+    for (uint32_t w = 0; w < kT / 64; ++w)
+        if (w < threadIdx.x >> 6) at_m += sh.scan_m[w], at_n += sh.scan_n[w];
     for (uint32_t i = 0; i < kEach && bin0 + i < kN; ++i) {
         const uint64_t next_m = at_m + mass[bin0 + i];
         const uint32_t next_n = at_n + number[bin0 + i];
@@ -526,11 +532,12 @@ __device__ __forceinline__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint
     const uint32_t from = min(v0 + wave * each, v1), to = min(from + each, v1);
     double sum = 0.0;
     uint32_t last = 0;   // index + 1 of the last with a weight
-    for (uint32_t v = from + lane; v < to; v += 256) {
-        u32x4 x[4];
+    constexpr uint32_t kAtOnce = 2;
+    for (uint32_t v = from + lane; v < to; v += 64 * kAtOnce) {
+        u32x4 x[kAtOnce];
         r.load(x, [&](uint32_t u) { return v + u * 64 < to ? v + u * 64 : ~0u; });
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u)
+        for (uint32_t u = 0; u < kAtOnce; ++u)
 #pragma unroll
             for (uint32_t j = 0; j < kOf<E>; ++j) {
                 const uint32_t index = r.index(v + u * 64, j);
@@ -667,6 +674,37 @@ __device__ __forceinline__ uint64_t border_by_digits(const Row<E>& r, float m, d
     return uint64_t(prefix) << 32 | uint32_t(~index);
 }
 
+// The words with lo <= scale x < lo + 1, into sh.places as many as it holds; how many there are.
+// A vector's words at once: an addition to the counter for each of them would be waited for.
+template <typename E, uint32_t kT, typename Sh>
+__device__ __forceinline__ uint32_t gather_bin(const Row<E>& r, float scale, float lo, Sh& sh) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    constexpr uint32_t kAtOnce = 8;
+    for (uint32_t v = threadIdx.x; v < r.vectors; v += kT * kAtOnce) {
+        u32x4 x[kAtOnce];
+        r.load(x, [&](uint32_t u) { return v + u * kT; });
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            uint32_t those = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kOf<E>; ++j) {
+                const float f = item<E>(x[u], j) * scale;
+                those |= uint32_t(f >= lo && f < lo + 1.0f) << j;
+            }
+            if (those == 0) continue;
+            uint32_t at = atomicAdd(&sh.count, uint32_t(__popc(those)));
+            for (; those != 0; those &= those - 1, ++at) {
+                const uint32_t j = __ffs(those) - 1;
+                if (at < Sh::kSorted) sh.places[at] = place_of(item_at<E>(x[u], j), r.index(v + u * kT, j));
+            }
+        }
+    }
+    __syncthreads();
+    return sh.count;
+}
+
 // What the histograms of a row's parts say of it together.
 __device__ __forceinline__ bool bins_do(const Rows& a, float top_bin) {
     // whole numbers of 2^-44 of a row of up to 2^18 words; bins that floats tell apart
@@ -726,18 +764,9 @@ __device__ __forceinline__ bool border_by_bins(const Rows& a, const Part* part, 
     if (bin == kBins || n > Sh::kSorted) return false;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kSubBins; i += kT) bins.sub_mass[i] = 0, bins.sub_number[i] = 0;
-    if (threadIdx.x == 0) sh.count = 0, sh.held = n, bins.bin = float(bin);
-    __syncthreads();
     const float lo = top_bin - float(bin);   // floor(v) == lo
-    each_word<E, kT>(r, [&](float f, uint32_t index) {
-        const float v = f * scale;
-        if (v >= lo && v < lo + 1.0f) {
-            const uint32_t at = atomicAdd(&sh.count, 1u);
-            if (at < Sh::kSorted) sh.places[at] = place_of(f, index);
-        }
-    });
-    __syncthreads();
-    if (sh.count != n) return false;
+    if (gather_bin<E, kT>(r, scale, lo, sh) != n) return false;
+    if (threadIdx.x == 0) sh.held = n, bins.bin = float(bin);
     const auto sub_of = [&](float f) { return kSubBins - 1 - min(uint32_t((f * scale - lo) * float(kSubBins)), kSubBins - 1); };
     const Weigh weight(c, m);
     for (uint32_t i = threadIdx.x; i < n; i += kT) {
@@ -828,9 +857,9 @@ __device__ __forceinline__ bool border_by_bins(const Rows& a, const Part* part, 
 // ---------------------------------------------------------------------
 // The k largest words of a row, sorted in sh.few; how many there are (-inf are none).
 //
-// One wave picks them from the parts' lists, up to 16 words a lane at a time: the key that k
-// of them reach, bit by bit, by counting ballots; what reaches it, k and ties, goes on to the
-// next lists and is ranked by counting in the end.  Others than the first wave wait.
+// One wave picks them from the parts' lists, up to 16 words a lane at a time: a key that k and
+// at most 128 of them reach, bit by bit, by counting ballots; those go on to the next lists and
+// are ranked by counting in the end.  Others than the first wave wait.
 // ---------------------------------------------------------------------
 constexpr uint32_t kPicked = 1024;
 template <typename Sh>
@@ -888,7 +917,7 @@ __device__ __forceinline__ bool pick_largest(const Rows& a, const Part* part, co
         const int differ = high == low ? -1 : 31 - __builtin_clz(high ^ low);
         uint32_t bound = differ < 0 ? low : differ == 31 ? 0 : low >> (differ + 1) << (differ + 1), reached = n;
 #pragma unroll 1
-        for (int bit = differ; bit >= 0 && reached != k; --bit) {
+        for (int bit = differ; bit >= 0 && reached > kMost; --bit) {
             const uint32_t with = bound | 1u << bit;
             uint32_t have = 0;
 #pragma unroll
@@ -1097,8 +1126,10 @@ __device__ __forceinline__ void kept_by_parts(const Rows& a, const uint64_t* lis
         const uint32_t p = (index_of(place) + r.shift) / kOf<E> / a.per;
         atomicAdd(reinterpret_cast<unsigned long long*>(&bins.kept[p]), static_cast<unsigned long long>(mass));
     };
-    if (bins.bin == at) {
-        for (uint32_t i = threadIdx.x; i < sh.held; i += kT)
+    uint32_t n = sh.held;
+    if (bins.bin != at) n = gather_bin<E, kT>(r, scale, top_bin - at, sh);
+    if (n <= Sh::kSorted) {
+        for (uint32_t i = threadIdx.x; i < n; i += kT)
             if (sh.places[i] >= border) add(sh.places[i]);
     } else {
         const float lo = top_bin - at;
