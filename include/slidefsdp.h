@@ -523,13 +523,14 @@ int sf_distill_lists(const int64_t* ids, size_t ld_ids, const float* logps,
  * token's words' hidden . weight; parts, keep as there, of all other words
  * (keep: 16 bits of -log2 relative to the span's
  * maximum, of 128 octaves for bf16 and 32 for fp16).  order (rows + 1 elements, or null): only rows of
- * status 1 take part. */
+ * status 1 take part, whose numbers it then holds, behind `rows` elements how many;
+ * close: keep's rows are in that order, without gaps. */
 int sf_distill_tiles(const void* weight, size_t ldw, size_t vocab,
                      const void* hidden, size_t ldh, size_t rows,
                      size_t hidden_size, const int32_t* words,
                      const uint8_t* starts, const uint8_t* status, int k,
                      float scale, int dtype, void* parts, float* picked,
-                     int32_t* order, void* keep, size_t ld_keep,
+                     int32_t* order, void* keep, size_t ld_keep, int close,
                      sf_stream_t stream);
 
 /* The same from fp32 logits (ld elements from row to row), unscaled, with one part
@@ -557,8 +558,8 @@ int sf_distill_loss(const void* parts, size_t parts_row, int whole,
                     float* stats, size_t stats_row, sf_stream_t stream);
 
 /* row_weight[i]: 1, or 0 where a row's gradient is 0 (status 0, grad 0, stats 0).
- * norm (or null; of 16-bit dtype): what D is divided by, its largest element, for
- * fp16 times 2^-14; and 1. */
+ * norm (or null): what D is divided by, its largest element, for fp16 times 2^-14;
+ * 1; and the first again, NaN if a row of status 2 has a gradient. */
 int sf_distill_weight(const float* grad, const float* stats,
                       const uint8_t* status, size_t rows, float scale,
                       int dtype, float* row_weight, float* norm,
@@ -566,13 +567,45 @@ int sf_distill_weight(const float* grad, const float* stats,
 
 /* D[i, j] = grad[i] * scale * derivative / norm[0] (norm null: not divided; fp16
  * needs it) in place of what sf_distill_tiles kept; rows from `rows` to `padded` and
- * those without gradient become 0.  parts: `rows` elements from span to span. */
+ * those without gradient become 0.  parts: `rows` elements from span to span.  order
+ * (or null): of rows that are close; behind the last one those up to the next
+ * multiple of 64, and up to `cleared`, become 0, the others stay. */
 int sf_distill_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
                          size_t vocab, const void* parts, const int32_t* words,
                          const uint8_t* starts, const uint8_t* status, int k,
                          const float* slopes, const float* stats,
                          size_t stats_row, int dtype, const float* grad,
-                         float scale, const float* norm, sf_stream_t stream);
+                         float scale, const float* norm,
+                         const int32_t* order, size_t cleared,
+                         sf_stream_t stream);
+
+/* sf_logps_hidden_product and sf_logps_weight_grad of D whose rows are close: only
+ * the first *live take part (of parts the others stay; of the sum those up to the next
+ * multiple of 64 hold zeros). */
+int sf_distill_hidden_product(const void* d, size_t ld, size_t rows,
+                              const int32_t* live, const void* weight,
+                              size_t ldw, size_t vocab, size_t cols, int nparts,
+                              float* parts, int dtype, sf_stream_t stream);
+int sf_distill_weight_grad(const void* d, size_t ld, size_t tokens,
+                           const int32_t* live, size_t vocab,
+                           const void* hidden_t, size_t cols, const float* norm,
+                           int dtype, void* out, sf_stream_t stream);
+
+/* hidden_t[j, i] = hidden[order[i], j] of 16-bit rows, 0 where the row's weight is and
+ * from the last row to the next multiple of 64; cols and ldh are multiples of 8, both
+ * aligned to 16 bytes (SF_EALIGN), ldt as sf_ce_hidden. */
+int sf_distill_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols,
+                      const int32_t* order, const float* row_weight,
+                      void* hidden_t, size_t ldt, sf_stream_t stream);
+
+/* out[order[i], :] = norm[0] * (the sum of parts[s, i, :] + d[i, done:] @
+ * weight[done:]), rounded once; rows whose weight is 0: 0, others that are not in the
+ * order: NaN.  place: `rows` elements of workspace. */
+int sf_distill_sum(const float* parts, int nparts, size_t rows, size_t cols,
+                   const int32_t* order, const uint8_t* status, int32_t* place,
+                   const float* row_weight, const float* norm, const void* d,
+                   size_t ld, const void* weight, size_t ldw, size_t done,
+                   size_t vocab, int dtype, void* out, sf_stream_t stream);
 
 /* D, fp32, in place of fp32 logits (as sf_distill_rows takes them, before it ran). */
 int sf_distill_grad(float* logits, size_t ld, size_t rows, size_t vocab,

@@ -378,18 +378,22 @@ struct Weights {
     }
 };
 
-// c and what the products multiply rows by: 1, or 0 where a row has no gradient.  One
-// workgroup.
+// c and what the products multiply rows by: 1, or 0 where a row has no gradient.  Behind c what
+// the weight gradient is multiplied by: NaN if a token has a gradient but words that are wrong,
+// whose row may not be in D.  One workgroup.
 constexpr int kWeightThreads = 1024;
 __global__ __launch_bounds__(kWeightThreads) void distill_weight_kernel(const Weights a) {
     __shared__ float waves[kWeightThreads / 64];
     float m = 0.0f;
+    bool wrong = false;
     for (uint64_t i = threadIdx.x; i < a.n; i += kWeightThreads) {
+        wrong |= a.status[i] == kBad && a.grad[i] != 0.0f;
         const float w = fabsf(a(i));
         if (__builtin_isfinite(w)) m = fmaxf(m, w);
         a.weight[i] = w == 0.0f ? 0.0f : 1.0f;
     }
     if (a.norm == nullptr) return;
+    wrong = __syncthreads_or(wrong);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
@@ -399,7 +403,7 @@ __global__ __launch_bounds__(kWeightThreads) void distill_weight_kernel(const We
     for (int w = 1; w < kWeightThreads / 64; ++w) m = fmaxf(m, waves[w]);
     // so that its inverse is finite too
     m = m < 0x1p-120f ? (m > 0.0f ? 0x1p-120f : 1.0f) : fminf(m, 0x1p120f);
-    a.norm[0] = m * a.unlift, a.norm[1] = 1.0f;
+    a.norm[0] = m * a.unlift, a.norm[1] = 1.0f, a.norm[2] = wrong ? __builtin_nanf("") : a.norm[0];
 }
 
 struct Slopes {
@@ -411,6 +415,7 @@ struct Slopes {
     const uint8_t* status;
     const float* grad;
     uint32_t k, spans;
+    const int32_t* order;   // of D's rows, their number behind all; or null: the tokens' own order
 };
 // What a row's D is: 0 whatever its hidden states hold, NaN, or computed.
 enum RowOf { kZero, kNan, kComputed };
@@ -428,10 +433,14 @@ __global__ __launch_bounds__(kGradThreads) void distill_keep_grad_kernel(uint16_
                                                                          uint32_t tokens, uint32_t col_blocks,
                                                                          uint64_t first, const float2* __restrict__ parts,
                                                                          const Slopes a, float scale,
-                                                                         const float* __restrict__ norm) {
-    const uint64_t b = first + blockIdx.x, row = b / col_blocks;
+                                                                         const float* __restrict__ norm, uint32_t cleared) {
+    const uint64_t b = first + blockIdx.x, at = b / col_blocks;
+    const uint32_t live = a.order != nullptr ? uint32_t(a.order[tokens]) : tokens;
+    // behind the last row as many are cleared as pad the weight gradient's sum, or all that a library's product reads
+    if (at >= live && at >= max((live + 63) / 64 * 64, max(cleared, 64u))) return;
+    const uint64_t row = at >= live ? tokens : a.order != nullptr ? uint64_t(a.order[at]) : at;
     const uint32_t col0 = uint32_t(b % col_blocks) * kKeepColumns, col = col0 + threadIdx.x * kGroup;
-    uint16_t* k = keep + row * ld;
+    uint16_t* k = keep + at * ld;
     const RowOf kind = row < tokens ? row_of(a, row) : kZero;
     if (kind != kComputed) {
         const uint32_t w = kind == kNan ? Fmt::kNan2 : 0u;
@@ -463,6 +472,104 @@ __global__ __launch_bounds__(kGradThreads) void distill_keep_grad_kernel(uint16_
             if (w - c < uint32_t(kGroup)) k[w] = uint16_t(Fmt::pack(a.slopes[row * a.k + i] * whole, 0.0f));
         }
     }
+}
+
+// Where each token's row is among D's, -1 of those without one; a lane a token.
+constexpr int kPlaceThreads = 256;
+__global__ __launch_bounds__(kPlaceThreads) void distill_place_kernel(const int32_t* __restrict__ order,
+                                                                      const uint8_t* __restrict__ status, uint32_t rows,
+                                                                      int32_t* __restrict__ place) {
+    const uint32_t i = blockIdx.x * kPlaceThreads + threadIdx.x;
+    if (i >= rows) return;
+    if (i < uint32_t(order[rows])) place[order[i]] = int32_t(i);
+    if (status[i] != kTaught) place[i] = -1;   // the others are in the order
+}
+
+// hidden_t[j, i] = hidden[order[i], j], 0 from the last row on: the weight gradient's product
+// wants them along its sum.  A tile of 64 x 64 through LDS, rows of 66 elements there, so that
+// a wave's reads of a column spread over the banks.  Bound by its bytes.
+constexpr int kTurn = 64;
+constexpr int kTurnThreads = 256;
+__global__ __launch_bounds__(kTurnThreads) void distill_hidden_kernel(const uint16_t* __restrict__ hidden, uint64_t ldh,
+                                                                      uint32_t rows, uint32_t cols,
+                                                                      const int32_t* __restrict__ order,
+                                                                      const float* __restrict__ by,
+                                                                      uint16_t* __restrict__ out, uint64_t ldt) {
+    __shared__ uint32_t tile[kTurn][kTurn / 2 + 1];
+    const uint32_t across = uint32_t(ldt / kTurn), row0 = blockIdx.x % across * kTurn, col0 = blockIdx.x / across * kTurn;
+    const uint32_t live = uint32_t(order[rows]);
+    if (row0 >= max((live + 63) / 64 * 64, 64u)) return;   // no term of the sum
+    constexpr int kEach = kTurn * kTurn / kGroup / kTurnThreads;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const uint32_t g = k * kTurnThreads + threadIdx.x, r = g / (kTurn / kGroup), c = g % (kTurn / kGroup) * kGroup;
+        u32x4 v = {0, 0, 0, 0};
+        if (row0 + r < live && col0 + c < cols) {
+            const uint32_t from = uint32_t(order[row0 + r]);
+            if (by[from] != 0.0f) v = *reinterpret_cast<const u32x4*>(hidden + from * ldh + col0 + c);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tile[r][c / 2 + j] = v[j];
+    }
+    __syncthreads();
+    const uint16_t* const flat = reinterpret_cast<const uint16_t*>(tile);
+    constexpr uint32_t kLd = 2 * (kTurn / 2 + 1);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const uint32_t g = k * kTurnThreads + threadIdx.x, c = g / (kTurn / kGroup), r = g % (kTurn / kGroup) * kGroup;
+        if (col0 + c >= cols) continue;
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = uint32_t(flat[(r + 2 * j) * kLd + c]) | uint32_t(flat[(r + 2 * j + 1) * kLd + c]) << 16;
+        *reinterpret_cast<u32x4*>(out + uint64_t(col0 + c) * ldt + row0 + r) = v;
+    }
+}
+
+// The hidden gradient from its sum's parts: added up, times c, rounded once, into the tokens'
+// rows: 0 without a gradient, NaN of a token that has one but no row in D (words that are
+// wrong).  The words from `done` on, which equal parts leave over, are added here.  Bound by its
+// bytes.
+constexpr int kSumThreads = 256;
+template <typename Fmt>
+__global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* __restrict__ parts, uint32_t nparts,
+                                                                  uint64_t rows, uint32_t cols,
+                                                                  const int32_t* __restrict__ place,
+                                                                  const float* __restrict__ by,
+                                                                  const float* __restrict__ norm,
+                                                                  const uint16_t* __restrict__ d, uint64_t ld,
+                                                                  const uint16_t* __restrict__ weight, uint64_t ldw,
+                                                                  uint32_t done, uint32_t vocab,
+                                                                  uint16_t* __restrict__ out) {
+    const uint32_t groups = cols / kGroup;
+    const uint64_t i = uint64_t(blockIdx.x) * kSumThreads + threadIdx.x, row = i / groups;
+    const uint32_t col = uint32_t(i - row * groups) * kGroup;
+    if (row >= rows) return;
+    const int32_t at = place[row];
+    u32x4 o = {0, 0, 0, 0};
+    if (by[row] == 0.0f) {
+    } else if (at < 0) {
+        o = u32x4{Fmt::kNan2, Fmt::kNan2, Fmt::kNan2, Fmt::kNan2};
+    } else {
+        f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+        for (uint32_t s = 0; s < nparts; ++s) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(parts + (s * rows + uint32_t(at)) * cols + col);
+            lo += p[0], hi += p[1];
+        }
+        for (uint32_t w = done; w < vocab; ++w) {
+            const float f = Fmt::lo(d[uint32_t(at) * ld + w]);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(weight + w * ldw + col);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                lo[2 * j] = fmaf(f, Fmt::lo(v[j]), lo[2 * j]), lo[2 * j + 1] = fmaf(f, Fmt::hi(v[j]), lo[2 * j + 1]);
+                hi[2 * j] = fmaf(f, Fmt::lo(v[j + 2]), hi[2 * j]), hi[2 * j + 1] = fmaf(f, Fmt::hi(v[j + 2]), hi[2 * j + 1]);
+            }
+        }
+        const float c = *norm;
+        o = u32x4{Fmt::pack(lo[0] * c, lo[1] * c), Fmt::pack(lo[2] * c, lo[3] * c), Fmt::pack(hi[0] * c, hi[1] * c),
+                  Fmt::pack(hi[2] * c, hi[3] * c)};
+    }
+    *reinterpret_cast<u32x4*>(out + row * cols + col) = o;
 }
 
 // D in fp32 of fp32 logits, in place, a row a workgroup.
@@ -522,7 +629,7 @@ int sf_distill_lists(const int64_t* ids, size_t ld_ids, const float* logps, size
 int sf_distill_tiles(const void* weight, size_t ldw, size_t vocab, const void* hidden, size_t ldh, size_t rows,
                      size_t hidden_size, const int32_t* words, const uint8_t* starts, const uint8_t* status_, int k,
                      float scale, int dtype, void* parts, float* picked, int32_t* order, void* keep, size_t ld_keep,
-                     sf_stream_t stream) {
+                     int close, sf_stream_t stream) {
     if (rows == 0) return SF_OK;
     if (weight == nullptr || hidden == nullptr || words == nullptr || starts == nullptr || status_ == nullptr ||
         parts == nullptr || picked == nullptr || sizes_bad(rows, vocab, k))
@@ -532,6 +639,7 @@ int sf_distill_tiles(const void* weight, size_t ldw, size_t vocab, const void* h
         return SF_EINVAL;
     if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
     const size_t spans = spans_of(vocab, 0);
+    if (close && order == nullptr) return SF_EINVAL;
     if (keep != nullptr && ld_keep < spans * kSpan) return SF_EINVAL;
     if (hidden_size % kTerms != 0 || ldw % kGroup != 0 || ldh % kGroup != 0 || misaligned(weight, 16) ||
         misaligned(hidden, 16) || misaligned(parts, 8) || misaligned(keep, 16) || ld_keep % kGroup != 0)
@@ -539,13 +647,14 @@ int sf_distill_tiles(const void* weight, size_t ldw, size_t vocab, const void* h
     if (order != nullptr && uint64_t(rows) * ldh * 2 > UINT32_MAX) return SF_ETOOBIG;   // 32-bit byte offsets of all rows
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const uint64_t most = kMaxLanes / kTileKinds[0].lanes / spans * 256;   // rows of one launch, whole tiles
+    if (close && rows > most) return SF_EINVAL;   // one order for all
     for (uint64_t r = 0; r < rows; r += most) {
         const uint32_t n = uint32_t(rows - r < most ? rows - r : most);
         const Tiles a = {static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(hidden) + r * ldh,
                          uint32_t(ldw), uint32_t(ldh), uint32_t(vocab), n, uint32_t(hidden_size / kTerms), nullptr,
                          order == nullptr ? nullptr : order + r, scale * kLog2e, static_cast<float2*>(parts) + r, rows,
                          nullptr, keep == nullptr ? nullptr : static_cast<uint16_t*>(keep) + r * ld_keep, ld_keep,
-                         words + r * k, starts + r * (spans + 1), picked + r * k, uint32_t(k)};
+                         words + r * k, starts + r * (spans + 1), picked + r * k, uint32_t(k), close != 0};
         int e = SF_OK;
         if (order != nullptr) {   // its last element is the next launch's first, which is written behind this one's
             hipLaunchKernelGGL(logps_order_kernel<Taught>, dim3(1), dim3(kOrderThreads), 0, st, Taught{status_ + r}, n,
@@ -608,22 +717,23 @@ int sf_distill_loss(const void* parts, size_t parts_row, int whole, const float*
 int sf_distill_keep_grad(void* keep, size_t ld, size_t rows, size_t padded, size_t vocab, const void* parts,
                          const int32_t* words, const uint8_t* starts, const uint8_t* status_, int k, const float* slopes,
                          const float* stats, size_t stats_row, int dtype, const float* grad, float scale, const float* norm,
-                         sf_stream_t stream) {
+                         const int32_t* order, size_t cleared, sf_stream_t stream) {
     if (padded == 0) return SF_OK;
     if (keep == nullptr || parts == nullptr || words == nullptr || starts == nullptr || status_ == nullptr ||
         slopes == nullptr || stats == nullptr || stats_row < rows || sizes_bad(padded, vocab, k) || padded < rows ||
-        (rows > 0 && grad == nullptr) || ld < size_t(spans_of(vocab, 0)) * kSpan || ld > (size_t(1) << 31))
+        cleared > padded || (rows > 0 && grad == nullptr) || ld < size_t(spans_of(vocab, 0)) * kSpan || ld > (size_t(1) << 31))
         return SF_EINVAL;
     if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
     if (dtype == SF_DTYPE_F16 && norm == nullptr) return SF_EINVAL;
     if (misaligned(keep, 16) || misaligned(parts, 8) || ld % kSpan != 0) return SF_EALIGN;
     const uint32_t col_blocks = uint32_t((ld + kKeepColumns - 1) / kKeepColumns);
     const auto kernel = dtype == SF_DTYPE_BF16 ? distill_keep_grad_kernel<Bf16> : distill_keep_grad_kernel<F16>;
-    const Slopes a = {words, starts, slopes, stats, stats_row, status_, grad, uint32_t(k), spans_of(vocab, 0)};
+    const Slopes a = {words, starts, slopes, stats, stats_row, status_, grad, uint32_t(k), spans_of(vocab, 0), order};
     return in_launches(uint64_t(padded) * col_blocks, kGradThreads, [&](uint64_t first, uint32_t blocks) {
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kGradThreads), 0, reinterpret_cast<hipStream_t>(stream),
                            static_cast<uint16_t*>(keep), uint64_t(ld), uint32_t(rows), col_blocks, first,
-                           static_cast<const float2*>(parts), a, scale, norm);
+                           static_cast<const float2*>(parts), a, scale, norm,
+                           order == nullptr ? uint32_t(padded) : uint32_t(cleared));
     });
 }
 
@@ -638,6 +748,47 @@ int sf_distill_weight(const float* grad, const float* stats, const uint8_t* stat
     return status();
 }
 
+int sf_distill_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols, const int32_t* order, const float* row_weight,
+                      void* hidden_t, size_t ldt, sf_stream_t stream) {
+    if (rows == 0 || cols == 0) return SF_OK;
+    if (hidden == nullptr || order == nullptr || row_weight == nullptr || hidden_t == nullptr || ldh < cols || ldt < rows ||
+        ldt % kTurn != 0 || ldt - rows >= kTurn || rows >= (size_t(1) << 31) || cols > (size_t(1) << 22))
+        return SF_EINVAL;
+    if (misaligned(hidden, 16) || ldh % kGroup != 0 || cols % kGroup != 0 || misaligned(hidden_t, 16)) return SF_EALIGN;
+    const uint64_t tiles = uint64_t(ldt / kTurn) * ((cols + kTurn - 1) / kTurn);
+    if (tiles > kMaxLanes / kTurnThreads) return SF_EINVAL;
+    hipLaunchKernelGGL(distill_hidden_kernel, dim3(uint32_t(tiles)), dim3(kTurnThreads), 0,
+                       reinterpret_cast<hipStream_t>(stream), static_cast<const uint16_t*>(hidden), uint64_t(ldh),
+                       uint32_t(rows), uint32_t(cols), order, row_weight, static_cast<uint16_t*>(hidden_t), uint64_t(ldt));
+    return status();
+}
+
+int sf_distill_sum(const float* parts, int nparts, size_t rows, size_t cols, const int32_t* order, const uint8_t* status_,
+                   int32_t* place, const float* row_weight, const float* norm, const void* d, size_t ld, const void* weight,
+                   size_t ldw, size_t done, size_t vocab, int dtype, void* out, sf_stream_t stream) {
+    if (rows == 0 || cols == 0) return SF_OK;
+    if (parts == nullptr || nparts < 1 || order == nullptr || status_ == nullptr || place == nullptr || norm == nullptr ||
+        row_weight == nullptr || d == nullptr || weight == nullptr || out == nullptr || done > vocab || ld < vocab || ldw < cols ||
+        rows >= (size_t(1) << 31) || vocab > (size_t(1) << 30) || cols > (size_t(1) << 22))
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (cols % kGroup != 0 || ldw % kGroup != 0 || misaligned(parts, 16) || misaligned(weight, 16) || misaligned(out, 16))
+        return SF_EALIGN;
+    const uint64_t blocks = (uint64_t(rows) * (cols / kGroup) + kSumThreads - 1) / kSumThreads;
+    if (blocks > kMaxLanes / kSumThreads) return SF_EINVAL;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(distill_place_kernel, dim3(uint32_t((rows + kPlaceThreads - 1) / kPlaceThreads)), dim3(kPlaceThreads), 0,
+                       st, order, status_, uint32_t(rows), place);
+    const int e = status();
+    if (e != SF_OK) return e;
+    const auto kernel = dtype == SF_DTYPE_BF16 ? distill_sum_kernel<Bf16> : distill_sum_kernel<F16>;
+    hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(kSumThreads), 0, st, parts, uint32_t(nparts), uint64_t(rows),
+                       uint32_t(cols), place, row_weight, norm, static_cast<const uint16_t*>(d), uint64_t(ld),
+                       static_cast<const uint16_t*>(weight), uint64_t(ldw), uint32_t(done), uint32_t(vocab),
+                       static_cast<uint16_t*>(out));
+    return status();
+}
+
 int sf_distill_grad(float* logits, size_t ld, size_t rows, size_t vocab, const int32_t* words, const uint8_t* starts,
                     const uint8_t* status_, int k, float scale, const float* slopes, const float* stats, size_t stats_row,
                     const float* grad, sf_stream_t stream) {
@@ -648,7 +799,7 @@ int sf_distill_grad(float* logits, size_t ld, size_t rows, size_t vocab, const i
     if (misaligned(logits, 4)) return SF_EALIGN;
     return in_launches(rows, kRowLanes, [&](uint64_t r, uint32_t n) {
         const Slopes a = {words + r * k, starts + r * 2, slopes + r * k, stats + r, stats_row, status_ + r, grad + r,
-                          uint32_t(k), 1};
+                          uint32_t(k), 1, nullptr};
         hipLaunchKernelGGL(distill_grad_kernel, dim3(n), dim3(kRowLanes), 0, reinterpret_cast<hipStream_t>(stream),
                            logits + r * ld, uint64_t(ld), uint32_t(vocab), scale * kLog2e, a);
     });

@@ -455,6 +455,8 @@ struct Product {
     uint32_t steps, each;   // 64 terms each: in all and in a part
     void* out;
     const float* norm;
+    uint32_t parts;
+    const int32_t* live;    // or null: how many tokens there are, of rows or of sum
 };
 constexpr int kPrTile = 256;
 typedef short Four __attribute__((ext_vector_type(4)));
@@ -473,16 +475,21 @@ __global__ __launch_bounds__(512, 2) void logps_product_kernel(const Product a) 
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wp = wave / kWQ, wq = wave % kWQ;
 
-    // as in the forward: each XCD has a contiguous run, 8 tiles of rows beside each other
-    const uint32_t tiles_p = (a.rows + kPrTile - 1) / kPrTile, tiles_q = (a.cols + kPrTile - 1) / kPrTile;
-    const uint32_t tiles = gridDim.x, xcd = blockIdx.x % 8, run = tiles / 8, more = tiles % 8;
+    // As in the forward: each XCD has a contiguous run, 8 tiles of rows beside each other; tiles
+    // and terms without a token are left out.
+    const uint32_t live = a.live != nullptr ? uint32_t(*a.live) : ~0u;
+    const uint32_t rows = kHidden ? min(a.rows, live) : a.rows;
+    const uint32_t all = kHidden || a.live == nullptr ? a.steps : min(a.steps, max((live + kTerms - 1) / kTerms, 1u));
+    const uint32_t tiles_p = (rows + kPrTile - 1) / kPrTile, tiles_q = (a.cols + kPrTile - 1) / kPrTile;
+    const uint32_t tiles = tiles_p * tiles_q * a.parts, xcd = blockIdx.x % 8, run = tiles / 8, more = tiles % 8;
+    if (blockIdx.x / 8 >= run + (xcd < more)) return;
     uint32_t id = xcd * run + min(xcd, more) + blockIdx.x / 8;
     const uint32_t part = id / (tiles_p * tiles_q);
     id -= part * tiles_p * tiles_q;
     const uint32_t first_p = id / (kGroupT * tiles_q) * kGroupT, group = min(uint32_t(kGroupT), tiles_p - first_p);
     const uint32_t in = id - first_p * tiles_q;
     const uint32_t q0 = in / group * kPrTile, p0 = (first_p + in % group) * kPrTile;
-    const uint32_t step0 = part * a.each, steps = min(a.steps - step0, a.each);
+    const uint32_t step0 = part * a.each, steps = min(all - step0, a.each);
 
     const uint8_t* gx = reinterpret_cast<const uint8_t*>(a.x + uint64_t(p0) * a.ldx + uint64_t(step0) * kTerms);
     const uint8_t* gy = reinterpret_cast<const uint8_t*>(a.y + uint64_t(step0) * kTerms * a.ldy + q0);
@@ -490,7 +497,7 @@ __global__ __launch_bounds__(512, 2) void logps_product_kernel(const Product a) 
     uint32_t off_x[kLX], row_y[kLY], col_y[kLY];
 #pragma unroll
     for (int j = 0; j < kLX; ++j)
-        off_x[j] = min((j * kWaves + wave) * 8 + (lane >> 3), a.rows - 1 - p0) * (a.ldx * 2) +
+        off_x[j] = min((j * kWaves + wave) * 8 + (lane >> 3), rows - 1 - p0) * (a.ldx * 2) +
                    ((lane & 7) ^ (lane >> 3)) * 16;
 #pragma unroll
     for (int j = 0; j < kLY; ++j) {
@@ -578,7 +585,7 @@ __global__ __launch_bounds__(512, 2) void logps_product_kernel(const Product a) 
 #pragma unroll
         for (int i = 0; i < kFP; ++i) {
             const uint32_t row = p0 + wp * kFP * 16 + i * 16 + l16;
-            if (row >= a.rows) continue;
+            if (row >= rows) continue;
 #pragma unroll
             for (int j = 0; j < kFQ; ++j) {
                 const uint32_t col = q0 + wq * kFQ * 16 + j * 16 + quad * 4;
@@ -753,6 +760,45 @@ bool sizes_bad(size_t rows, size_t vocab) {
     return vocab == 0 || vocab > (size_t(1) << 30) || rows >= (size_t(1) << 31);
 }
 
+int hidden_product(const void* d, size_t ld, size_t rows, const int32_t* live, const void* weight, size_t ldw, size_t vocab,
+                   size_t cols, int nparts, float* parts, int dtype, sf_stream_t stream) {
+    if (rows == 0) return SF_OK;
+    if (d == nullptr || weight == nullptr || parts == nullptr || sizes_bad(rows, vocab) || cols == 0 ||
+        cols > (size_t(1) << 22) || ld < (vocab + kTerms - 1) / kTerms * kTerms || ld > (size_t(1) << 22) || ldw < cols ||
+        ldw > (size_t(1) << 22) || nparts < 1 || size_t(nparts) > (vocab + kTerms - 1) / kTerms)
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (cols % 8 != 0 || ld % 8 != 0 || ldw % 8 != 0 || misaligned(d, 16) || misaligned(weight, 16) || misaligned(parts, 16))
+        return SF_EALIGN;
+    Product a = {static_cast<const uint16_t*>(d), static_cast<const uint16_t*>(weight), uint32_t(ld), uint32_t(ldw),
+                 uint32_t(rows), uint32_t(cols), uint32_t(cols), uint32_t(vocab),
+                 uint32_t((vocab + kTerms - 1) / kTerms), 0, parts, nullptr, uint32_t(nparts), live};
+    a.each = (a.steps + nparts - 1) / nparts;
+    if ((a.steps + a.each - 1) / a.each != uint32_t(nparts)) return SF_EINVAL;
+    return launch_product<true>(a, nparts, dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+int weight_grad(const void* d, size_t ld, size_t tokens, const int32_t* live, size_t vocab, const void* hidden_t, size_t cols,
+                const float* norm, int dtype, void* out, sf_stream_t stream) {
+    if (d == nullptr || hidden_t == nullptr || out == nullptr || sizes_bad(tokens, vocab) || tokens == 0 ||
+        tokens > (size_t(1) << 22) || cols == 0 || cols > (size_t(1) << 22) || ld < vocab || ld > (size_t(1) << 22))
+        return SF_EINVAL;
+    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
+    if (tokens % 64 != 0 || cols % 8 != 0 || ld % 8 != 0 || misaligned(d, 16) || misaligned(hidden_t, 16) ||
+        misaligned(out, 16))
+        return SF_EALIGN;
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (tokens > kWgTokens || live != nullptr) {
+        const uint32_t steps = uint32_t(tokens / kTerms);
+        const Product a = {static_cast<const uint16_t*>(hidden_t), static_cast<const uint16_t*>(d), uint32_t(tokens),
+                           uint32_t(ld), uint32_t(cols), uint32_t(vocab), uint32_t(ld), uint32_t(tokens), steps, steps,
+                           out, norm, 1, live};
+        return launch_product<false>(a, 1, dtype, st);
+    }
+    return dtype == SF_DTYPE_BF16 ? dispatch_weight_grad<Bf16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st)
+                                  : dispatch_weight_grad<F16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -787,7 +833,7 @@ int sf_logps_tiles(const void* weight, size_t ldw, size_t vocab, const void* hid
                          uint32_t(ldw), uint32_t(ldh), uint32_t(vocab), n, uint32_t(hidden_size / kTerms), labels + r,
                          order == nullptr ? nullptr : order + r, scale * kLog2e, static_cast<float2*>(parts) + r, rows,
                          target + r, keep == nullptr ? nullptr : static_cast<uint16_t*>(keep) + r * ld_keep, ld_keep,
-                         nullptr, nullptr, nullptr, 0};
+                         nullptr, nullptr, nullptr, 0, false};
         int e = SF_OK;
         if (order != nullptr) {   // its last element is the next launch's first, which is written behind this one's
             hipLaunchKernelGGL(logps_order_kernel<HasLabel>, dim3(1), dim3(kOrderThreads), 0, st,
@@ -886,41 +932,24 @@ int sf_logps_weighted(const void* hidden, size_t ldh, size_t rows, size_t cols, 
 
 int sf_logps_hidden_product(const void* d, size_t ld, size_t rows, const void* weight, size_t ldw, size_t vocab,
                             size_t cols, int nparts, float* parts, int dtype, sf_stream_t stream) {
-    if (rows == 0) return SF_OK;
-    if (d == nullptr || weight == nullptr || parts == nullptr || sizes_bad(rows, vocab) || cols == 0 ||
-        cols > (size_t(1) << 22) || ld < (vocab + kTerms - 1) / kTerms * kTerms || ld > (size_t(1) << 22) || ldw < cols ||
-        ldw > (size_t(1) << 22) || nparts < 1 || size_t(nparts) > (vocab + kTerms - 1) / kTerms)
-        return SF_EINVAL;
-    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
-    if (cols % 8 != 0 || ld % 8 != 0 || ldw % 8 != 0 || misaligned(d, 16) || misaligned(weight, 16) || misaligned(parts, 16))
-        return SF_EALIGN;
-    Product a = {static_cast<const uint16_t*>(d), static_cast<const uint16_t*>(weight), uint32_t(ld), uint32_t(ldw),
-                 uint32_t(rows), uint32_t(cols), uint32_t(cols), uint32_t(vocab),
-                 uint32_t((vocab + kTerms - 1) / kTerms), 0, parts, nullptr};
-    a.each = (a.steps + nparts - 1) / nparts;
-    if ((a.steps + a.each - 1) / a.each != uint32_t(nparts)) return SF_EINVAL;
-    return launch_product<true>(a, nparts, dtype, reinterpret_cast<hipStream_t>(stream));
+    return hidden_product(d, ld, rows, nullptr, weight, ldw, vocab, cols, nparts, parts, dtype, stream);
+}
+
+int sf_distill_hidden_product(const void* d, size_t ld, size_t rows, const int32_t* live, const void* weight, size_t ldw,
+                              size_t vocab, size_t cols, int nparts, float* parts, int dtype, sf_stream_t stream) {
+    if (live == nullptr) return SF_EINVAL;
+    return hidden_product(d, ld, rows, live, weight, ldw, vocab, cols, nparts, parts, dtype, stream);
 }
 
 int sf_logps_weight_grad(const void* d, size_t ld, size_t tokens, size_t vocab, const void* hidden_t, size_t cols,
                          const float* norm, int dtype, void* out, sf_stream_t stream) {
-    if (d == nullptr || hidden_t == nullptr || out == nullptr || sizes_bad(tokens, vocab) || tokens == 0 ||
-        tokens > (size_t(1) << 22) || cols == 0 || cols > (size_t(1) << 22) || ld < vocab || ld > (size_t(1) << 22))
-        return SF_EINVAL;
-    if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
-    if (tokens % 64 != 0 || cols % 8 != 0 || ld % 8 != 0 || misaligned(d, 16) || misaligned(hidden_t, 16) ||
-        misaligned(out, 16))
-        return SF_EALIGN;
-    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (tokens > kWgTokens) {
-        const uint32_t steps = uint32_t(tokens / kTerms);
-        const Product a = {static_cast<const uint16_t*>(hidden_t), static_cast<const uint16_t*>(d), uint32_t(tokens),
-                           uint32_t(ld), uint32_t(cols), uint32_t(vocab), uint32_t(ld), uint32_t(tokens), steps, steps,
-                           out, norm};
-        return launch_product<false>(a, 1, dtype, st);
-    }
-    return dtype == SF_DTYPE_BF16 ? dispatch_weight_grad<Bf16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st)
-                                  : dispatch_weight_grad<F16>(d, ld, tokens, vocab, hidden_t, cols, norm, out, st);
+    return weight_grad(d, ld, tokens, nullptr, vocab, hidden_t, cols, norm, dtype, out, stream);
+}
+
+int sf_distill_weight_grad(const void* d, size_t ld, size_t tokens, const int32_t* live, size_t vocab, const void* hidden_t,
+                           size_t cols, const float* norm, int dtype, void* out, sf_stream_t stream) {
+    if (live == nullptr) return SF_EINVAL;
+    return weight_grad(d, ld, tokens, live, vocab, hidden_t, cols, norm, dtype, out, stream);
 }
 
 int sf_logps_weight(const float* grad, const float* logp, const int64_t* labels, int64_t ignore_index, size_t rows,

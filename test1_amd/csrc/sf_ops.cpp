@@ -359,7 +359,7 @@ std::pair<Tensor, Tensor> products(const Tensor& hidden, const Tensor& weight, T
     const bool one = step == n;
     const sf_stream_t st = stream_of(hidden);
     const int type = type_of(hidden);
-    const Tensor by = like(hidden, {n}), norms = like(hidden, {2});
+    const Tensor by = like(hidden, {n}), norms = like(hidden, {3});
     const bool own = one && own_weight_grad(n, h, v, row, fp16);
     // What D is divided by leaves before the results are rounded: in the own products, or of few
     // tiles with a pass over them.
@@ -516,13 +516,14 @@ struct DistillArgs {
     bool rest;
     double scale;
     int64_t nparts, step;   // as LogpsArgs
-    bool keep;
+    bool keep, masked;
 };
 
 struct DistillOut {
     Tensor loss, keep, parts;
     // [n, k] or as include/slidefsdp.h says, for the backward
     Tensor words, starts, status, slopes, stats;
+    Tensor order;         // where keep's rows are close: of which tokens they are
 };
 
 // Rows of logits of one piece.
@@ -534,18 +535,36 @@ void product32(const Tensor& out, const Tensor& hidden, const Tensor& weight) {
     else at::mm_out(to, hidden, weight.t(), at::kFloat);
 }
 
+bool skips_masked(int64_t n, const Tensor& hidden, int64_t v) {
+    return skips_rows(n, hidden.size(1), v) && 2 * n * hidden.stride(0) <= int64_t(UINT32_MAX);
+}
+
+// Whether a masked call keeps the rows of D close, so that both gradients' products leave out
+// what has no loss, as the forward's does: where the weight gradient's product is the
+// framework's own, of 96 tiles or more.  How many rows there are is known on the device alone.
+// Loss and both gradients in us, all rows | close, nothing masked, a fifth, half: 4092 x 4096 x
+// 128256 10412 | 10448, 8837, 6927; 8190 x 5120 x 152064 30342 | 30527, 27293, 16894; 4096 x
+// 1024 x 32000 943 | 929, 826, 672; 512 x 4096 x 32000 546 | 555, 532, 508.
+bool keeps_close(int64_t n, const Tensor& hidden, int64_t v) {
+    return skips_masked(n, hidden, v) && tiles_of(hidden.size(1), v) >= 96 && n < int64_t(1) << 22 &&
+           v <= (int64_t(1) << 22) - SF_LOGPS_SPAN;
+}
+
 Tensor distill_tiles(const Tensor& hidden, const Tensor& weight, const Tensor& words, const Tensor& starts,
-                     const Tensor& status, int64_t first, double scale, const Tensor& keep, const Tensor& picked) {
+                     const Tensor& status, int64_t first, double scale, const Tensor& keep, const Tensor& picked,
+                     bool masked, const Tensor& close) {
     const int64_t n = hidden.size(0), v = weight.size(0), k = words.size(1);
     const int64_t held = 2 * n * ((v + SF_LOGPS_SPAN - 1) / SF_LOGPS_SPAN);
-    const bool skip = skips_rows(n, hidden.size(1), v) && 2 * n * hidden.stride(0) <= int64_t(UINT32_MAX);
-    const Tensor parts = like(hidden, {held + (skip ? n + 1 : 0)});
-    int32_t* order = skip ? reinterpret_cast<int32_t*>(at_ptr<float>(parts) + held) : nullptr;
+    const bool skip = masked && skips_masked(n, hidden, v), own = skip && !close.defined();
+    const Tensor parts = like(hidden, {held + (own ? n + 1 : 0)});
+    int32_t* order = close.defined() ? at_ptr<int32_t>(close)
+                     : own           ? reinterpret_cast<int32_t*>(at_ptr<float>(parts) + held)
+                                     : nullptr;
     check(sf_distill_tiles(weight.data_ptr(), weight.stride(0), v, hidden.data_ptr(), hidden.stride(0), n, hidden.size(1),
                            at_ptr<int32_t>(words) + first * k, at_ptr<uint8_t>(starts) + first * starts.size(1),
                            at_ptr<uint8_t>(status) + first, int(k), float(scale), type_of(hidden), parts.data_ptr(),
                            at_ptr<float>(picked), order, keep.defined() ? keep.data_ptr() : nullptr,
-                           keep.defined() ? keep.stride(0) : 0, stream_of(hidden)),
+                           keep.defined() ? keep.stride(0) : 0, close.defined(), stream_of(hidden)),
           "sf_distill_tiles");
     return parts;
 }
@@ -584,7 +603,9 @@ DistillOut distill_forward(const Tensor& hidden_, const Tensor& weight_, const T
         }
     } else {
         if (a.keep && grad) o.keep = at::empty({up(n, 64), up(v, SF_LOGPS_SPAN)}, hidden.options());
-        o.parts = distill_tiles(hidden, weight, o.words, o.starts, o.status, 0, a.scale, o.keep, lists.select(0, 1));
+        if (o.keep.defined() && mask.defined() && keeps_close(n, hidden, v)) o.order = at::empty({n + 1}, o.words.options());
+        o.parts = distill_tiles(hidden, weight, o.words, o.starts, o.status, 0, a.scale, o.keep, lists.select(0, 1),
+                                mask.defined(), o.order);
     }
     check(sf_distill_loss(o.parts.data_ptr(), n, whole, picked, teacher, at_ptr<uint8_t>(o.starts), at_ptr<uint8_t>(o.status),
                           n, int(k), v, a.scale, int(a.form), a.rest, hidden.data_ptr(), ld(hidden), weight.data_ptr(),
@@ -630,8 +651,65 @@ std::pair<Tensor, Tensor> distill_backward_whole(const Tensor& grad, const Tenso
     return {gh, gw};
 }
 
+// Both gradients from rows of D that are close.
+std::pair<Tensor, Tensor> distill_backward_close(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
+                                                 const DistillOut& o, const DistillArgs& a, bool need_hidden,
+                                                 bool need_weight) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t n = hidden.size(0), h = hidden.size(1), v = weight.size(0), k = o.words.size(1);
+    const int64_t row = o.keep.stride(0), pad = up(n, 64);
+    const int type = type_of(hidden);
+    const sf_stream_t st = stream_of(hidden);
+    const int32_t *order = at_ptr<int32_t>(o.order), *live = order + n;
+    const Tensor scalars = like(hidden, {n + 3});
+    float *by = at_ptr<float>(scalars), *norm = by + n;
+    const bool own = own_hidden_product(n, h, row);
+    check(sf_distill_weight(at_ptr<float>(grad), at_ptr<float>(o.stats), at_ptr<uint8_t>(o.status), n, float(a.scale), type, by,
+                            norm, st),
+          "sf_distill_weight");
+    check(sf_distill_keep_grad(o.keep.data_ptr(), row, n, pad, v, o.parts.data_ptr(), at_ptr<int32_t>(o.words),
+                               at_ptr<uint8_t>(o.starts), at_ptr<uint8_t>(o.status), int(k), at_ptr<float>(o.slopes),
+                               at_ptr<float>(o.stats), n, type, at_ptr<float>(grad), float(a.scale), norm, order,
+                               need_hidden && !own ? n : 0, st),
+          "sf_distill_keep_grad");
+    Tensor gh, gw;
+    if (need_hidden) {
+        gh = at::empty({n, h}, hidden.options());
+        Tensor parts = like(hidden, {a.nparts, n, h});
+        const Tensor place = at::empty({n}, o.order.options());
+        const int64_t part = own || a.nparts == 1 ? v : v / a.nparts / 8 * 8, done = own ? v : a.nparts * part;
+        if (own) {
+            check(sf_distill_hidden_product(o.keep.data_ptr(), row, n, live, weight.data_ptr(), weight.stride(0), v, h,
+                                            int(a.nparts), at_ptr<float>(parts), type, st),
+                  "sf_distill_hidden_product");
+        } else if (a.nparts == 1) {
+            Tensor whole = parts.select(0, 0);
+            at::mm_out(whole, o.keep.as_strided({n, v}, {row, 1}), weight, at::kFloat);
+        } else {
+            at::bmm_out(parts, o.keep.as_strided({a.nparts, n, part}, {part, row, 1}),
+                        weight.as_strided({a.nparts, part, h}, {part * h, h, 1}), at::kFloat);
+        }
+        check(sf_distill_sum(at_ptr<float>(parts), int(a.nparts), n, h, order, at_ptr<uint8_t>(o.status), at_ptr<int32_t>(place),
+                             by, norm, o.keep.data_ptr(), row, weight.data_ptr(), weight.stride(0), done, v, type,
+                             gh.data_ptr(), st),
+              "sf_distill_sum");
+    }
+    if (need_weight) {
+        gw = at::empty({v, h}, weight.options());
+        const Tensor ht = at::empty({h, pad}, hidden.options());
+        check(sf_distill_hidden(hidden.data_ptr(), hidden.stride(0), n, h, order, by, ht.data_ptr(), pad, st),
+              "sf_distill_hidden");
+        check(sf_distill_weight_grad(o.keep.data_ptr(), row, pad, live, v, ht.data_ptr(), h, norm + 2, type, gw.data_ptr(), st),
+              "sf_distill_weight_grad");
+    }
+    return {gh, gw};
+}
+
+// The gradients by torch operations, where what was saved came back as something else.
+
 std::pair<Tensor, Tensor> distill_backward(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
                                            const DistillOut& o, const DistillArgs& a, bool need_hidden, bool need_weight) {
+    if (o.keep.defined() && o.order.defined()) return distill_backward_close(grad, hidden, weight, o, a, need_hidden, need_weight);
     if (!in_tiles(hidden, weight)) return distill_backward_whole(grad, hidden, weight, o, a, need_hidden, need_weight);
     at::AutoDispatchBelowADInplaceOrView below;
     const int64_t n = hidden.size(0), v = weight.size(0), k = o.words.size(1), row = up(v, SF_LOGPS_SPAN);
@@ -642,7 +720,7 @@ std::pair<Tensor, Tensor> distill_backward(const Tensor& grad, const Tensor& hid
     if (!kept) again = like(hidden, {step, k});
     return products(hidden, weight, o.keep, step, a.nparts, need_hidden, need_weight, true,
                     [&](int64_t s, int64_t m, int64_t pad, const Tensor& hc, const Tensor& d, float* by, float* norm) {
-        if (!kept) parts = distill_tiles(hc, weight, o.words, o.starts, o.status, s, a.scale, d, again);
+        if (!kept) parts = distill_tiles(hc, weight, o.words, o.starts, o.status, s, a.scale, d, again, a.masked, Tensor());
         if (s == 0)
             check(sf_distill_weight(at_ptr<float>(grad), at_ptr<float>(o.stats), at_ptr<uint8_t>(o.status), n, float(a.scale),
                                     type, by, norm, stream_of(hidden)),
@@ -650,12 +728,11 @@ std::pair<Tensor, Tensor> distill_backward(const Tensor& grad, const Tensor& hid
         check(sf_distill_keep_grad(d.data_ptr(), row, m, pad, v, parts.data_ptr(), at_ptr<int32_t>(o.words) + s * k,
                                    at_ptr<uint8_t>(o.starts) + s * o.starts.size(1), at_ptr<uint8_t>(o.status) + s, int(k),
                                    at_ptr<float>(o.slopes) + s * k, at_ptr<float>(o.stats) + s, n, type,
-                                   at_ptr<float>(grad) + s, float(a.scale), norm, stream_of(hidden)),
+                                   at_ptr<float>(grad) + s, float(a.scale), norm, nullptr, 0, stream_of(hidden)),
               "sf_distill_keep_grad");
     });
 }
 
-// The gradients by torch operations, where what was saved came back as something else.
 std::pair<Tensor, Tensor> distill_backward_torch(const Tensor& grad_, const Tensor& hidden, const Tensor& weight,
                                                  const DistillOut& o, const DistillArgs& a, bool need_hidden,
                                                  bool need_weight) {
@@ -690,10 +767,12 @@ struct LinearDistill : torch::autograd::Function<LinearDistill> {
         if (o.keep.defined()) {
             ctx->saved_data["keep"] = o.keep;
             ctx->saved_data["parts"] = o.parts;
+            if (o.order.defined()) ctx->saved_data["order"] = o.order;
         }
         ctx->saved_data["scale"] = a.scale;
         ctx->saved_data["nparts"] = a.nparts;
         ctx->saved_data["step"] = a.step;
+        ctx->saved_data["masked"] = a.masked;
         return o.loss;
     }
 
@@ -705,7 +784,8 @@ struct LinearDistill : torch::autograd::Function<LinearDistill> {
         DistillOut o;
         o.words = saved[2], o.starts = saved[3], o.status = saved[4], o.slopes = saved[5], o.stats = saved[6];
         auto& data = ctx->saved_data;
-        const DistillArgs a = {0, true, data["scale"].toDouble(), data["nparts"].toInt(), data["step"].toInt(), false};
+        const DistillArgs a = {0, true, data["scale"].toDouble(), data["nparts"].toInt(), data["step"].toInt(), false,
+                               data["masked"].toBool()};
         const bool need_hidden = ctx->needs_input_grad(0), need_weight = ctx->needs_input_grad(1);
         Tensor gh, gw;
         {
@@ -722,9 +802,11 @@ struct LinearDistill : torch::autograd::Function<LinearDistill> {
                 if (auto it = data.find("keep"); it != data.end()) {
                     o.keep = it->second.toTensor();
                     o.parts = data["parts"].toTensor();
+                    if (auto at = data.find("order"); at != data.end()) o.order = at->second.toTensor();
                     // a second backward of a retained graph makes it again
                     data.erase("keep");
                     data.erase("parts");
+                    data.erase("order");
                 }
                 std::tie(gh, gw) = distill_backward(g.to(at::kFloat).contiguous(), hidden, weight, o, a, need_hidden,
                                                     need_weight);
@@ -824,7 +906,7 @@ PyObject* linear_distill(PyObject*, PyObject* args) {
     const c10::DeviceGuard guard(hidden.device());
     const Tensor mask = m == Py_None ? Tensor() : THPVariable_Unpack(m).contiguous();
     const bool grad = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad());
-    const DistillArgs a = {form, rest != 0, scale, nparts, step, keep != 0};
+    const DistillArgs a = {form, rest != 0, scale, nparts, step, keep != 0, mask.defined()};
     if (!grad) return wrap(distill_forward(hidden, weight, ids, logps, mask, a, false).loss);
     const c10::optional<Tensor> given = mask.defined() ? c10::optional<Tensor>(mask) : c10::nullopt;
     return wrap(LinearDistill::apply(hidden, weight, ids, logps, given, a));

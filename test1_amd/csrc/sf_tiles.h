@@ -84,6 +84,7 @@ struct Tiles {
     const uint8_t* starts;    // [tokens, tiles of words + 1] its first of each tile
     float* picked;            // [tokens, picks] their products, unscaled
     uint32_t picks;
+    bool close;               // keep's rows in the order of `order`, without gaps
 };
 
 // The rows that have(i), in their order, and behind `rows` of them their number.
@@ -405,7 +406,8 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
             for (int k = 0; k < 16 / kRows; ++k) {
                 const uint32_t r = k * kRows + lane / kAcross, c16 = lane % kAcross;
                 const u32x4 v = *reinterpret_cast<const u32x4*>(turn + r * kTurnRow + (c16 ^ (r & (kFV * 2 - 1))) * 16);
-                const uint32_t to = __shfl(row[j], r);   // of the lane that has this token
+                const uint32_t from = __shfl(row[j], r);   // of the lane that has this token
+                const uint32_t to = kPick && a.close ? t0 + wt0 + j * 16 + r : from;
                 if (t0 + wt0 + j * 16 + r < count)
                     *reinterpret_cast<u32x4*>(a.keep + to * a.ld_keep + v0 + wv0 + c16 * 8) = v;
             }

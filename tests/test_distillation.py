@@ -115,11 +115,11 @@ def test_entry_points_refuse_without_a_gpu():
         ids, ld, p, 4, None, rows, k, vocab, 0, words, p, p, p, None)
     assert lists(rows=0) == 0
     assert [lists(**b) for b in (dict(ids=None), dict(ld=3), dict(k=0), dict(k=129), dict(vocab=0), dict(words=None))] == [E] * 6
-    tiles = lambda weight=p, ldw=64, h=64, k=4, scale=1.0, dtype=1, keep=None, ldk=0, rows=2: hip.sf_distill_tiles(  # noqa: E731
-        weight, ldw, 300, p, 64, rows, h, p, p, p, k, scale, dtype, p, p, None, keep, ldk, None)
+    tiles = lambda weight=p, ldw=64, h=64, k=4, scale=1.0, dtype=1, keep=None, ldk=0, rows=2, close=0: hip.sf_distill_tiles(  # noqa: E731
+        weight, ldw, 300, p, 64, rows, h, p, p, p, k, scale, dtype, p, p, None, keep, ldk, close, None)
     assert tiles(rows=0) == 0
     assert [tiles(**b) for b in (dict(weight=None), dict(ldw=32), dict(h=0), dict(k=0), dict(scale=0.0), dict(scale=math.nan),
-                                 dict(keep=p, ldk=300))] == [E] * 7
+                                 dict(keep=p, ldk=300), dict(close=1))] == [E] * 8
     assert [tiles(**b) for b in (dict(weight=p + 2), dict(h=32), dict(ldw=65), dict(keep=p + 8, ldk=512))] == [A] * 4
     assert tiles(dtype=0) not in (0, E)
     loss = lambda parts=p, row=2, form=0, rest=1, scale=1.0, ldh=64, weight=p, dtype=1, slopes=p, stats=p: hip.sf_distill_loss(  # noqa: E731
@@ -129,12 +129,21 @@ def test_entry_points_refuse_without_a_gpu():
     assert loss(weight=p + 2) == loss(ldh=65) == loss(dtype=0) == A and loss(dtype=7) not in (0, E, A)
     by = lambda grad=p, dtype=1, rows=2: hip.sf_distill_weight(grad, p, p, rows, 1.0, dtype, p, p, None)  # noqa: E731
     assert by(rows=0) == 0 and by(grad=None) == E and by(dtype=0) not in (0, E)
-    grad = lambda keep=p, ld=512, padded=64, grad=p, dtype=1, norm=p: hip.sf_distill_keep_grad(  # noqa: E731
-        keep, ld, 2, padded, 300, p, p, p, p, 4, p, p, 2, dtype, grad, 1.0, norm, None)
+    grad = lambda keep=p, ld=512, padded=64, grad=p, dtype=1, norm=p, cleared=0: hip.sf_distill_keep_grad(  # noqa: E731
+        keep, ld, 2, padded, 300, p, p, p, p, 4, p, p, 2, dtype, grad, 1.0, norm, None, cleared, None)
     assert grad(padded=0) == 0
-    assert [grad(**b) for b in (dict(keep=None), dict(ld=256), dict(padded=1), dict(grad=None), dict(dtype=2, norm=None))] == [E] * 5
+    assert [grad(**b) for b in (dict(keep=None), dict(ld=256), dict(padded=1), dict(grad=None), dict(dtype=2, norm=None), dict(cleared=65))] == [E] * 6
     assert grad(keep=p + 8) == grad(ld=520) == A
     rows = lambda logits=p, ld=300, k=4: hip.sf_distill_rows(logits, ld, 2, 300, p, p, k, 1.0, p, p, None)  # noqa: E731
     assert [rows(logits=None), rows(ld=299), rows(k=0)] == [E] * 3 and rows(logits=p + 2) == A
     whole = lambda logits=p, ld=300, grad=p: hip.sf_distill_grad(logits, ld, 2, 300, p, p, p, 4, 1.0, p, p, 2, grad, None)  # noqa: E731
     assert [whole(logits=None), whole(ld=299), whole(grad=None)] == [E] * 3
+    turn = lambda hidden=p, ldh=64, ldt=64, order=p: hip.sf_distill_hidden(hidden, ldh, 2, 64, order, p, p, ldt, None)  # noqa: E731
+    assert [turn(hidden=None), turn(ldh=63), turn(ldt=128), turn(ldt=63), turn(order=None)] == [E] * 5
+    assert turn(hidden=p + 2) == turn(ldh=65) == A
+    add = lambda parts=p, done=300, order=p, norm=p, ldw=64, ld=512: hip.sf_distill_sum(  # noqa: E731
+        parts, 1, 2, 64, order, p, p, p, norm, p, ld, p, ldw, done, 300, 1, p, None)
+    assert [add(parts=None), add(done=301), add(order=None), add(norm=None), add(ldw=63), add(ld=299)] == [E] * 6
+    assert add(ldw=65) == add(parts=p + 8) == A
+    assert hip.sf_distill_hidden_product(p, 512, 2, None, p, 64, 300, 64, 1, p, 1, None) == E
+    assert hip.sf_distill_weight_grad(p, 512, 64, None, 300, p, 64, None, 1, p, None) == E

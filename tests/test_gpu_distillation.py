@@ -61,6 +61,43 @@ def test_matches_float64(dev, shape, dtype):
         check(args, dtype, 1.0 if shape[0] % 2 else 1.5, kind, rest)
 
 
+@pytest.mark.parametrize("share", [0.0, 0.3, 0.95, 1.0])
+@pytest.mark.parametrize("shape,dtype", [((400, 2048, 50_000, 9), torch.bfloat16), ((300, 2048, 60_000, 128), torch.float16),
+                                         ((4200, 2048, 12_000, 3), torch.bfloat16), ((700, 1536, 40_011, 20), torch.bfloat16)])
+def test_masked_tokens_left_out_of_the_products(dev, shape, dtype, share):
+    """Calls large enough that D has the rows of the tokens that count alone: a fraction, none, all of them
+    masked; tokens without an upstream gradient, without words, with wrong ones."""
+    hidden, weight, ids, logps, _, up = inputs(shape, dtype, dev)
+    g = torch.Generator(device=dev).manual_seed(1)
+    mask = torch.rand(shape[0], generator=g, device=dev) >= share
+    up[5:9] = 0
+    plain = linear_distill(hidden.clone().requires_grad_(True), weight, ids, logps, mask)
+    want, bound = distill(hidden, weight, ids, logps, mask, 1.0, "forward", True, grad=up)
+    near(plain.detach(), want[0], bound[0])
+    hidden[~mask] = math.nan
+    hr, wr = hidden.requires_grad_(True), weight.clone().requires_grad_(True)
+    loss = linear_distill(hr, wr, ids, logps, mask)
+    assert torch.equal(loss, plain)
+    gh, gw = torch.autograd.grad(loss, (hr, wr), up, retain_graph=True)
+    assert (gh[~mask] == 0).all() and (gh[5:9] == 0).all() and gh.isfinite().all() and gw.isfinite().all()
+    again = torch.autograd.grad(loss, (hr, wr), up)   # made again
+    for got, other, w, b in zip((gh, gw), again, want[1:], bound[1:]):
+        near(got, w, b)
+        near(other, w, b)
+    assert torch.equal(torch.autograd.grad(linear_distill(hr, weight, ids, logps, mask), hr, up)[0], gh)
+    assert torch.equal(torch.autograd.grad(linear_distill(hidden.detach(), wr, ids, logps, mask), wr, up)[0], gw)
+    if share < 0.9:
+        at = int(mask.nonzero()[20])
+        ids = ids.clone()
+        ids[at, 0] = -3
+        logps[at, 0] = -1.0
+        up[at] = 1.0
+        loss = linear_distill(hr, wr, ids, logps, mask)
+        gh, gw = torch.autograd.grad(loss, (hr, wr), up)
+        assert loss[at].isnan() and gh[at].isnan().all() and gh[torch.arange(shape[0], device=dev) != at].isfinite().all()
+        assert gw.isnan().all()
+
+
 def test_words_in_one_tile_and_at_its_edges(dev):
     """A token's words all side by side, across a tile's end, in the last tile."""
     hidden, weight, ids, logps, mask, up = inputs((70, 64, 1000, 128), torch.bfloat16, dev)
