@@ -580,7 +580,8 @@ int sf_distill_keep_grad(void* keep, size_t ld, size_t rows, size_t padded,
                          sf_stream_t stream);
 
 /* sf_logps_hidden_product and sf_logps_weight_grad of D whose rows are close: only
- * the first *live take part (of parts the others stay; of the sum those up to the next
+ * the first *live take part (of parts, as many of nparts, up to 16, as suit them, the
+ * others stay; of the sum those up to the next
  * multiple of 64 hold zeros). */
 int sf_distill_hidden_product(const void* d, size_t ld, size_t rows,
                               const int32_t* live, const void* weight,
@@ -600,9 +601,10 @@ int sf_distill_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols,
 
 /* out[order[i], :] = norm[0] * (the sum of parts[s, i, :] + d[i, done:] @
  * weight[done:]), rounded once; rows whose weight is 0: 0, others that are not in the
- * order: NaN.  place: `rows` elements of workspace. */
-int sf_distill_sum(const float* parts, int nparts, size_t rows, size_t cols,
-                   const int32_t* order, const uint8_t* status, int32_t* place,
+ * order: NaN.  place: `rows` elements of workspace.  by_live: of the parts there are as
+ * many as sf_distill_hidden_product took, and done is vocab. */
+int sf_distill_sum(const float* parts, int nparts, int by_live, size_t rows,
+                   size_t cols, const int32_t* order, const uint8_t* status, int32_t* place,
                    const float* row_weight, const float* norm, const void* d,
                    size_t ld, const void* weight, size_t ldw, size_t done,
                    size_t vocab, int dtype, void* out, sf_stream_t stream);

@@ -140,7 +140,7 @@ HIP_SIGNATURES = {
     "sf_distill_hidden_product": [_vp, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _i, _vp, _i, _vp],
     "sf_distill_weight_grad": [_vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _i, _vp, _vp],
     "sf_distill_hidden": [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp],
-    "sf_distill_sum": [_vp, _i, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _i, _vp, _vp],
+    "sf_distill_sum": [_vp, _i, _i, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _i, _vp, _vp],
     "sf_distill_grad": [_vp, _sz, _sz, _sz, _vp, _vp, _vp, _i, _f, _vp, _vp, _sz, _vp, _vp],
     "sf_rows_work": [_sz, _sz, _i],
     "sf_top_logps": [_vp, _i, _sz, _sz, _sz, _i, _d, _vp, _vp, _vp, _vp],

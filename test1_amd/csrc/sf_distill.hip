@@ -528,12 +528,13 @@ __global__ __launch_bounds__(kTurnThreads) void distill_hidden_kernel(const uint
 
 // The hidden gradient from its sum's parts: added up, times c, rounded once, into the tokens'
 // rows: 0 without a gradient, NaN of a token that has one but no row in D (words that are
-// wrong).  The words from `done` on, which equal parts leave over, are added here.  Bound by its
-// bytes.
+// wrong).  The words from `done` on, which equal parts leave over, are added here.  live: how many
+// parts there are hangs on it.  Bound by its bytes.
 constexpr int kSumThreads = 256;
 template <typename Fmt>
 __global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* __restrict__ parts, uint32_t nparts,
                                                                   uint64_t rows, uint32_t cols,
+                                                                  const int32_t* __restrict__ live,
                                                                   const int32_t* __restrict__ place,
                                                                   const float* __restrict__ by,
                                                                   const float* __restrict__ norm,
@@ -544,6 +545,7 @@ __global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* _
     const uint32_t groups = cols / kGroup;
     const uint64_t i = uint64_t(blockIdx.x) * kSumThreads + threadIdx.x, row = i / groups;
     const uint32_t col = uint32_t(i - row * groups) * kGroup;
+    if (live != nullptr) nparts = parts_of_rows(uint32_t(*live), cols, (vocab + kTerms - 1) / kTerms, nparts);
     if (row >= rows) return;
     const int32_t at = place[row];
     u32x4 o = {0, 0, 0, 0};
@@ -763,12 +765,12 @@ int sf_distill_hidden(const void* hidden, size_t ldh, size_t rows, size_t cols, 
     return status();
 }
 
-int sf_distill_sum(const float* parts, int nparts, size_t rows, size_t cols, const int32_t* order, const uint8_t* status_,
+int sf_distill_sum(const float* parts, int nparts, int by_live, size_t rows, size_t cols, const int32_t* order, const uint8_t* status_,
                    int32_t* place, const float* row_weight, const float* norm, const void* d, size_t ld, const void* weight,
                    size_t ldw, size_t done, size_t vocab, int dtype, void* out, sf_stream_t stream) {
     if (rows == 0 || cols == 0) return SF_OK;
     if (parts == nullptr || nparts < 1 || order == nullptr || status_ == nullptr || place == nullptr || norm == nullptr ||
-        row_weight == nullptr || d == nullptr || weight == nullptr || out == nullptr || done > vocab || ld < vocab || ldw < cols ||
+        row_weight == nullptr || d == nullptr || weight == nullptr || out == nullptr || done > vocab || (by_live && (done < vocab || nparts > int(kMostLiveParts))) || ld < vocab || ldw < cols ||
         rows >= (size_t(1) << 31) || vocab > (size_t(1) << 30) || cols > (size_t(1) << 22))
         return SF_EINVAL;
     if (dtype != SF_DTYPE_BF16 && dtype != SF_DTYPE_F16) return SF_EDTYPE;
@@ -783,7 +785,7 @@ int sf_distill_sum(const float* parts, int nparts, size_t rows, size_t cols, con
     if (e != SF_OK) return e;
     const auto kernel = dtype == SF_DTYPE_BF16 ? distill_sum_kernel<Bf16> : distill_sum_kernel<F16>;
     hipLaunchKernelGGL(kernel, dim3(uint32_t(blocks)), dim3(kSumThreads), 0, st, parts, uint32_t(nparts), uint64_t(rows),
-                       uint32_t(cols), place, row_weight, norm, static_cast<const uint16_t*>(d), uint64_t(ld),
+                       uint32_t(cols), by_live ? order + rows : nullptr, place, row_weight, norm, static_cast<const uint16_t*>(d), uint64_t(ld),
                        static_cast<const uint16_t*>(weight), uint64_t(ldw), uint32_t(done), uint32_t(vocab),
                        static_cast<uint16_t*>(out));
     return status();

@@ -455,7 +455,7 @@ struct Product {
     uint32_t steps, each;   // 64 terms each: in all and in a part
     void* out;
     const float* norm;
-    uint32_t parts;
+    uint32_t parts;         // with live, of the hidden gradient: at most
     const int32_t* live;    // or null: how many tokens there are, of rows or of sum
 };
 constexpr int kPrTile = 256;
@@ -481,7 +481,9 @@ __global__ __launch_bounds__(512, 2) void logps_product_kernel(const Product a) 
     const uint32_t rows = kHidden ? min(a.rows, live) : a.rows;
     const uint32_t all = kHidden || a.live == nullptr ? a.steps : min(a.steps, max((live + kTerms - 1) / kTerms, 1u));
     const uint32_t tiles_p = (rows + kPrTile - 1) / kPrTile, tiles_q = (a.cols + kPrTile - 1) / kPrTile;
-    const uint32_t tiles = tiles_p * tiles_q * a.parts, xcd = blockIdx.x % 8, run = tiles / 8, more = tiles % 8;
+    uint32_t parts = a.parts, each = a.each;
+    if (kHidden && a.live != nullptr) parts = parts_of_rows(rows, a.cols, a.steps, a.parts), each = (a.steps + parts - 1) / parts;
+    const uint32_t tiles = tiles_p * tiles_q * parts, xcd = blockIdx.x % 8, run = tiles / 8, more = tiles % 8;
     if (blockIdx.x / 8 >= run + (xcd < more)) return;
     uint32_t id = xcd * run + min(xcd, more) + blockIdx.x / 8;
     const uint32_t part = id / (tiles_p * tiles_q);
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(512, 2) void logps_product_kernel(const Product a) 
     const uint32_t first_p = id / (kGroupT * tiles_q) * kGroupT, group = min(uint32_t(kGroupT), tiles_p - first_p);
     const uint32_t in = id - first_p * tiles_q;
     const uint32_t q0 = in / group * kPrTile, p0 = (first_p + in % group) * kPrTile;
-    const uint32_t step0 = part * a.each, steps = min(all - step0, a.each);
+    const uint32_t step0 = part * each, steps = min(all - step0, each);
 
     const uint8_t* gx = reinterpret_cast<const uint8_t*>(a.x + uint64_t(p0) * a.ldx + uint64_t(step0) * kTerms);
     const uint8_t* gy = reinterpret_cast<const uint8_t*>(a.y + uint64_t(step0) * kTerms * a.ldy + q0);
@@ -937,7 +939,7 @@ int sf_logps_hidden_product(const void* d, size_t ld, size_t rows, const void* w
 
 int sf_distill_hidden_product(const void* d, size_t ld, size_t rows, const int32_t* live, const void* weight, size_t ldw,
                               size_t vocab, size_t cols, int nparts, float* parts, int dtype, sf_stream_t stream) {
-    if (live == nullptr) return SF_EINVAL;
+    if (live == nullptr || nparts > int(kMostLiveParts)) return SF_EINVAL;
     return hidden_product(d, ld, rows, live, weight, ldw, vocab, cols, nparts, parts, dtype, stream);
 }
 

@@ -543,8 +543,8 @@ bool skips_masked(int64_t n, const Tensor& hidden, int64_t v) {
 // what has no loss, as the forward's does: where the weight gradient's product is the
 // framework's own, of 96 tiles or more.  How many rows there are is known on the device alone.
 // Loss and both gradients in us, all rows | close, nothing masked, a fifth, half: 4092 x 4096 x
-// 128256 10412 | 10448, 8837, 6927; 8190 x 5120 x 152064 30342 | 30527, 27293, 16894; 4096 x
-// 1024 x 32000 943 | 929, 826, 672; 512 x 4096 x 32000 546 | 555, 532, 508.
+// 128256 10450 | 10516, 8968, 5499; 8190 x 5120 x 152064 30584 | 30915, 26577, 15796; 4096 x
+// 1024 x 32000 923 | 924, 817, 620; 512 x 4096 x 32000 542 | 549, 532, 502.
 bool keeps_close(int64_t n, const Tensor& hidden, int64_t v) {
     return skips_masked(n, hidden, v) && tiles_of(hidden.size(1), v) >= 96 && n < int64_t(1) << 22 &&
            v <= (int64_t(1) << 22) - SF_LOGPS_SPAN;
@@ -675,21 +675,24 @@ std::pair<Tensor, Tensor> distill_backward_close(const Tensor& grad, const Tenso
     Tensor gh, gw;
     if (need_hidden) {
         gh = at::empty({n, h}, hidden.options());
-        Tensor parts = like(hidden, {a.nparts, n, h});
+        // of the framework's own product as many as 1 GiB holds, of which the device takes what suits the rows
+        const int64_t most = std::min<int64_t>({16, (v + 1999) / 2000, (int64_t(1) << 28) / (n * h)});
+        const int64_t nparts = own ? std::max<int64_t>(most, 1) : a.nparts;
+        Tensor parts = like(hidden, {nparts, n, h});
         const Tensor place = at::empty({n}, o.order.options());
-        const int64_t part = own || a.nparts == 1 ? v : v / a.nparts / 8 * 8, done = own ? v : a.nparts * part;
+        const int64_t part = own || nparts == 1 ? v : v / nparts / 8 * 8, done = own ? v : nparts * part;
         if (own) {
             check(sf_distill_hidden_product(o.keep.data_ptr(), row, n, live, weight.data_ptr(), weight.stride(0), v, h,
-                                            int(a.nparts), at_ptr<float>(parts), type, st),
+                                            int(nparts), at_ptr<float>(parts), type, st),
                   "sf_distill_hidden_product");
-        } else if (a.nparts == 1) {
+        } else if (nparts == 1) {
             Tensor whole = parts.select(0, 0);
             at::mm_out(whole, o.keep.as_strided({n, v}, {row, 1}), weight, at::kFloat);
         } else {
-            at::bmm_out(parts, o.keep.as_strided({a.nparts, n, part}, {part, row, 1}),
-                        weight.as_strided({a.nparts, part, h}, {part * h, h, 1}), at::kFloat);
+            at::bmm_out(parts, o.keep.as_strided({nparts, n, part}, {part, row, 1}),
+                        weight.as_strided({nparts, part, h}, {part * h, h, 1}), at::kFloat);
         }
-        check(sf_distill_sum(at_ptr<float>(parts), int(a.nparts), n, h, order, at_ptr<uint8_t>(o.status), at_ptr<int32_t>(place),
+        check(sf_distill_sum(at_ptr<float>(parts), int(nparts), own, n, h, order, at_ptr<uint8_t>(o.status), at_ptr<int32_t>(place),
                              by, norm, o.keep.data_ptr(), row, weight.data_ptr(), weight.stride(0), done, v, type,
                              gh.data_ptr(), st),
               "sf_distill_sum");

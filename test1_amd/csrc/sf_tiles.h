@@ -114,6 +114,24 @@ __global__ __launch_bounds__(kOrderThreads) void logps_order_kernel(const Have h
     if (threadIdx.x == kOrderThreads - 1) order[rows] = int32_t(before);
 }
 
+// Parts of the hidden gradient's sum over `steps` of 64 words, at most `most`, where the device
+// alone knows the rows: by rounds of 256 compute units that the tiles of 256 x 256 take, and by
+// what adding a part up costs, as much as 20 steps of its tiles.  Product and sum in us, the
+// host's parts for all rows | these, a fifth of the rows masked: 4092 x 4096 x 128256 2923 (1) |
+// 2849 (6), 8190 x 5120 x 152064 9728 (2) | 8870 (6); a step with half of them masked 6927 | 5499
+// and 16894 | 15796, 16384 x 2048 x 50257 5995 | 4767.  Whole numbers: the product and the sum
+// come to the same.  All lanes of a wave call it, each weighs a number of its own.
+constexpr uint32_t kMostLiveParts = 16;
+__device__ __forceinline__ uint32_t parts_of_rows(uint32_t rows, uint32_t cols, uint32_t steps, uint32_t most) {
+    const uint32_t p = (threadIdx.x & (kMostLiveParts - 1)) + 1, each = (steps + p - 1) / p;
+    const uint64_t tiles = uint64_t((rows + 255) / 256) * ((cols + 255) / 256);
+    uint64_t least = ((tiles * p + 255) / 256 * each * 256 + tiles * p * 20) << 5 | p;
+    if (p > most || (steps + each - 1) / each != p) least = ~uint64_t(0) << 5 | 1;   // or a part would be empty
+#pragma unroll
+    for (int d = 1; d < int(kMostLiveParts); d <<= 1) least = min(least, uint64_t(__shfl_xor(least, d)));
+    return uint32_t(least) & 31;
+}
+
 // Interleaves what a half's products run beside: kLoads copies into LDS, then
 // kReads reads of it, two products each; all else after.
 template <int kReads, int kMul, int kLoads>

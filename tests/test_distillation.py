@@ -141,9 +141,10 @@ def test_entry_points_refuse_without_a_gpu():
     turn = lambda hidden=p, ldh=64, ldt=64, order=p: hip.sf_distill_hidden(hidden, ldh, 2, 64, order, p, p, ldt, None)  # noqa: E731
     assert [turn(hidden=None), turn(ldh=63), turn(ldt=128), turn(ldt=63), turn(order=None)] == [E] * 5
     assert turn(hidden=p + 2) == turn(ldh=65) == A
-    add = lambda parts=p, done=300, order=p, norm=p, ldw=64, ld=512: hip.sf_distill_sum(  # noqa: E731
-        parts, 1, 2, 64, order, p, p, p, norm, p, ld, p, ldw, done, 300, 1, p, None)
-    assert [add(parts=None), add(done=301), add(order=None), add(norm=None), add(ldw=63), add(ld=299)] == [E] * 6
+    add = lambda parts=p, done=300, order=p, norm=p, ldw=64, ld=512, live=0: hip.sf_distill_sum(  # noqa: E731
+        parts, 1, live, 2, 64, order, p, p, p, norm, p, ld, p, ldw, done, 300, 1, p, None)
+    assert [add(parts=None), add(done=301), add(order=None), add(norm=None), add(ldw=63), add(ld=299),
+            add(done=299, live=1)] == [E] * 7
     assert add(ldw=65) == add(parts=p + 8) == A
     assert hip.sf_distill_hidden_product(p, 512, 2, None, p, 64, 300, 64, 1, p, 1, None) == E
     assert hip.sf_distill_weight_grad(p, 512, 64, None, 300, p, 64, None, 1, p, None) == E
