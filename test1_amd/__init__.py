@@ -6,6 +6,9 @@ Public API, matching the reference's:
 and beside it the operators of preference and policy fine-tuning:
     preference_loss, policy_loss, pack_act8, unpack_act8 and
     ``linear_logps.linear_logps``
+of distillation and of answering:
+    linear_distill, top_logps, sample_tokens and
+    ``distillation.linear_top_logps``
 The device work runs in hand-written HIP kernels for gfx950 behind the C ABI
 declared in include/slidefsdp.h (``test1_amd/lib/libsf_hip.so``); the host
 AdamW runs in ``test1_amd/lib/libsf_cpu.so``.

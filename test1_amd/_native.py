@@ -261,7 +261,7 @@ def _load_segs():
 
 def ops():
     """The module with the calls and autograd nodes of the losses, the token
-    log-probabilities and the 8-bit checkpoints.  They have no other form on a
+    log-probabilities, distillation, sampling and the 8-bit checkpoints.  They have no other form on a
     GPU: it raises where the module is missing or built against another torch."""
     global _ops
     if _ops is None:

@@ -1,5 +1,5 @@
-// What the device sources of the output unit, the losses and the checkpoints
-// share: vector types, the 16-bit formats, matrix products of 16 x 16 x 32, and
+// What the device sources of the output unit, the losses, sampling and the
+// checkpoints share: vector types, the 16-bit formats, matrix products of 16 x 16 x 32, and
 // the host side's checks.
 
 #pragma once

@@ -49,7 +49,8 @@ enum Status : uint8_t { kNone, kTaught, kBad };
 // ---------------------------------------------------------------------
 // Each token's words by rising index, with its teacher's log-probabilities, and where
 // those of each tile begin.  A wave takes a token, two words a lane, and ranks them by
-// counting.
+// counting: 128 comparisons a lane at most, where a sort would be 28 steps with a wait
+// each.  4092 tokens of 64 words, 502 tiles, 19 us; 8190 of 32 23; 126 4.4.
 // ---------------------------------------------------------------------
 struct Lists {
     const int64_t* ids;     // ld_ids
@@ -132,7 +133,8 @@ struct Taught {
 
 // ---------------------------------------------------------------------
 // fp32 logits that a library product has left, a row a workgroup: the words picked out,
-// -inf in their place, the others' maximum and sum as one part.
+// -inf in their place, the others' maximum and sum as one part.  fp32 calls and rows that the
+// tiles cannot take; next to the library product bound by its bytes.
 // ---------------------------------------------------------------------
 constexpr int kRowLanes = 256;
 __global__ __launch_bounds__(kRowLanes) void distill_rows_kernel(float* logits, uint64_t ld, uint32_t vocab,
@@ -228,7 +230,10 @@ __device__ __forceinline__ double product_of(const Loss& a, uint64_t token, uint
         return wave_sum(s);
     }
 }
-constexpr double kLikely = 1.0 / 64;
+// A wave a token: its tiles' maxima and sums joined, its words' terms two a lane.  Bound by the
+// latency of the joining and of each likely word's product: 4092 tokens of 502 tiles 43 us, 8190
+// of 595 88, 126 8.
+constexpr double kLikely = 1.0 / 64;   // from which a word's logit is summed again
 constexpr int kLossTokens = 4;
 constexpr int kLossLanes = kLossTokens * 64;
 template <typename E>
@@ -380,7 +385,7 @@ struct Weights {
 
 // c and what the products multiply rows by: 1, or 0 where a row has no gradient.  Behind c what
 // the weight gradient is multiplied by: NaN if a token has a gradient but words that are wrong,
-// whose row may not be in D.  One workgroup.
+// whose row may not be in D.  One workgroup: 4092 tokens 5 us.
 constexpr int kWeightThreads = 1024;
 __global__ __launch_bounds__(kWeightThreads) void distill_weight_kernel(const Weights a) {
     __shared__ float waves[kWeightThreads / 64];
@@ -425,7 +430,8 @@ __device__ __forceinline__ RowOf row_of(const Slopes& a, uint64_t row) {
 }
 
 // D from what the product kept, in place; as logps_keep_grad_kernel, but that a token's
-// own words follow over what their lane has just stored.
+// own words follow over what their lane has just stored.  Bound by its bytes, 2 read and 2
+// written a logit: a fifth of the rows masked, 4092 x 128256 286 us, 8190 x 152064 720, 5.5 TB/s.
 constexpr int kGradThreads = 256;
 constexpr int kKeepColumns = kGradThreads * kGroup * 2;
 template <typename Fmt>
@@ -487,7 +493,8 @@ __global__ __launch_bounds__(kPlaceThreads) void distill_place_kernel(const int3
 
 // hidden_t[j, i] = hidden[order[i], j], 0 from the last row on: the weight gradient's product
 // wants them along its sum.  A tile of 64 x 64 through LDS, rows of 66 elements there, so that
-// a wave's reads of a column spread over the banks.  Bound by its bytes.
+// a wave's reads of a column spread over the banks.  Bound by its bytes: 4092 x 4096, a fifth of
+// the rows masked, 14 us, 3.8 TB/s.
 constexpr int kTurn = 64;
 constexpr int kTurnThreads = 256;
 __global__ __launch_bounds__(kTurnThreads) void distill_hidden_kernel(const uint16_t* __restrict__ hidden, uint64_t ldh,
@@ -529,7 +536,7 @@ __global__ __launch_bounds__(kTurnThreads) void distill_hidden_kernel(const uint
 // The hidden gradient from its sum's parts: added up, times c, rounded once, into the tokens'
 // rows: 0 without a gradient, NaN of a token that has one but no row in D (words that are
 // wrong).  The words from `done` on, which equal parts leave over, are added here.  live: how many
-// parts there are hangs on it.  Bound by its bytes.
+// parts there are hangs on it.  Bound by its bytes: 4092 x 4096 from 6 parts 64 us, 5.6 TB/s.
 constexpr int kSumThreads = 256;
 template <typename Fmt>
 __global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* __restrict__ parts, uint32_t nparts,
