@@ -712,8 +712,9 @@ std::pair<Tensor, Tensor> distill_backward_close(const Tensor& grad, const Tenso
 
 std::pair<Tensor, Tensor> distill_backward(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
                                            const DistillOut& o, const DistillArgs& a, bool need_hidden, bool need_weight) {
-    if (o.keep.defined() && o.order.defined()) return distill_backward_close(grad, hidden, weight, o, a, need_hidden, need_weight);
     if (!in_tiles(hidden, weight)) return distill_backward_whole(grad, hidden, weight, o, a, need_hidden, need_weight);
+    if (o.keep.defined() && o.order.defined())
+        return distill_backward_close(grad, hidden, weight, o, a, need_hidden, need_weight);
     at::AutoDispatchBelowADInplaceOrView below;
     const int64_t n = hidden.size(0), v = weight.size(0), k = o.words.size(1), row = up(v, SF_LOGPS_SPAN);
     const bool kept = o.keep.defined();

@@ -99,8 +99,8 @@ def _check_taught(shape, device, ids, logps, mask, temperature, kind, rest) -> N
         raise ValueError(f"linear_distill: the mask has to be {tuple(shape)}")
     if any(t is not None and t.device != device for t in (ids, logps, mask)):
         raise ValueError("linear_distill: all tensors have to be on one device")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError("linear_distill: temperature must be above 0")
+    if not 1e-30 <= temperature <= 1e30:   # neither it nor its inverse leaves fp32
+        raise ValueError(f"linear_distill: a temperature above 0, from 1e-30 to 1e30, expected, got {temperature}")
     if kind not in _FORMS:
         raise ValueError(f"linear_distill: kind must be one of {sorted(_FORMS)}, got {kind!r}")
     if kind == "reverse" and not rest:

@@ -56,7 +56,8 @@ def _bad(logits: torch.Tensor) -> torch.Tensor:
 def _top_torch(logits, k, temperature):
     bad = _bad(logits).unsqueeze(-1)
     order = torch.where(bad, torch.zeros_like(logits), logits).sort(dim=-1, descending=True, stable=True).indices[..., :k]
-    z = logits.double() / temperature
+    z = torch.where(bad, 0.0, logits.double())
+    z = (z - z.amax(dim=-1, keepdim=True)) / temperature   # or a low temperature's lse loses the sum
     logps = (z.gather(-1, order) - _lse(z)).float()
     return TopLogps(torch.where(bad, math.nan, logps), torch.where(bad, -1, order))
 
@@ -79,7 +80,7 @@ def top_logps(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogp
         out = _native.ops().top_logps(logits, k, float(temperature))
         if out is not None:
             return TopLogps(*out)
-    return _top_torch(logits, k, float(temperature))
+    return _top_torch(logits, k, min(max(float(temperature), 1e-30), 1e30))   # as the kernels take it
 
 
 # ---------------------------------------------------------------------------

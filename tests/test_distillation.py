@@ -97,6 +97,14 @@ def test_refusals():
             linear_distill(**{**good, **bad})
 
 
+def test_temperatures_that_leave_fp32():
+    hidden, weight, ids, logps = inputs(6, 16, 40, 3)
+    for t in (1e-39, 1e39, -1.0, math.nan):
+        with pytest.raises(ValueError):
+            linear_distill(hidden, weight, ids, logps, temperature=t)
+    assert linear_distill(hidden, weight, ids, logps, temperature=1e30).isfinite().all()
+
+
 def test_shapes_and_no_rows():
     hidden, weight, ids, logps = inputs(12, 16, 40, 3)
     flat = linear_distill(hidden, weight, ids, logps)

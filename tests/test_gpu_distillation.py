@@ -264,6 +264,34 @@ def test_graph_replays_with_an_eager_graph_alive(dev):
     assert alive.isfinite().all()
 
 
+@pytest.mark.parametrize("shape", [(4200, 2048, 12_000, 3), (400, 2048, 50_000, 9)])
+def test_graph_replays_with_other_masks(dev, shape):
+    """How many rows the products take is known on the device alone: a captured step replayed with more of
+    them, fewer, none and all."""
+    hidden, weight, ids, logps, mask, up = inputs(shape, torch.bfloat16, dev)
+    hidden.requires_grad_(True), weight.requires_grad_(True)
+
+    def step(h, w):
+        loss = linear_distill(h, w, ids, logps, mask)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w), up))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(hidden, weight)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(hidden, weight)
+    g = torch.Generator(device=dev).manual_seed(2)
+    for share in (0.5, 0.0, 1.0, 0.9, 0.1):
+        mask.copy_(torch.rand(shape[0], generator=g, device=dev) >= share)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step(hidden.detach().clone().requires_grad_(True), weight.detach().clone().requires_grad_(True))
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
 def test_transforms_take_torch_operations(dev):
     hidden, weight, ids, logps, mask, _ = inputs((12, 64, 300, 6), torch.float32, dev)
     out = torch.vmap(lambda h, i, l: linear_distill(h, weight, i, l))(hidden.view(3, 4, 64), ids.view(3, 4, 6), logps.view(3, 4, 6))

@@ -76,6 +76,13 @@ def test_uniforms_at_the_ends():
     assert sample_tokens(x, u, top_p=0.0).ids.tolist() == [0] * 6
 
 
+def test_a_temperature_below_all_that_tells_words_apart():
+    x = torch.tensor([[1.0, 3.0, 3.0, 2.0]])
+    got = top_logps(x, 4, temperature=1e-45)
+    assert got.ids.tolist() == [[1, 2, 3, 0]] and got.logps[0, :2].allclose(torch.tensor(0.5).log())
+    assert got.logps[0, 2:].tolist() == [torch.tensor(-1e30).item(), torch.tensor(-2e30).item()]
+
+
 def test_no_rows_and_no_gradient():
     out = sample_tokens(torch.zeros(0, 5, requires_grad=True), torch.zeros(0))
     assert out.ids.shape == (0,) and not out.logps.requires_grad
