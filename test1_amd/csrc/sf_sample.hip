@@ -179,6 +179,10 @@ struct Row {
         }
         return r;
     }
+    __device__ float at(uint32_t index) const {
+        if constexpr (std::is_same_v<E, F32>) return __uint_as_float(x[index]);
+        else return E::lo(x[index]);
+    }
     __device__ uint32_t index(uint32_t v, uint32_t i) const { return v * kOf<E> + i - shift; }
 };
 
@@ -524,30 +528,46 @@ __device__ __forceinline__ void find_bin(const uint64_t* mass, const uint32_t* n
     __syncthreads();
 }
 
-// The words of a row in the order of their index: what `weight` (0: not taken) gives is
+// The words of a row in the order of their index: the weights of those that are `kept` are
 // added up, and the first word that takes the sum above `target` is found; where rounding
 // leaves none, the last with a weight.  Every wave has a run of the row's vectors from v0
-// to v1.  share: the target is that of the whole sum.
-template <typename E, uint32_t kT, typename Weight, typename Sh>
-__device__ __forceinline__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double target, bool share, Weight weight, Sh& sh) {
-    constexpr uint32_t kWaves = kT / 64;
+// to v1.  share: the target is that of the whole sum.  kFew: a weight costs 20 operations in
+// 64 bits, so a lane goes over its kept words alone; where every word is kept that is slower.
+template <typename E, uint32_t kT, bool kFew, typename Weight, typename Kept, typename Sh>
+__device__ __forceinline__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint32_t v1, double target, bool share, Weight weigh,
+                                              Kept kept, Sh& sh) {
+    const auto each_kept = [&](const u32x4& x, uint32_t v, auto f) {   // f(weight, index), by rising index
+        if constexpr (kFew) {
+            uint32_t those = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kOf<E>; ++j) those |= uint32_t(kept(item<E>(x, j), r.index(v, j))) << j;
+            for (; those != 0; those &= those - 1) {
+                const uint32_t j = __ffs(those) - 1;
+                f(weigh(item_at<E>(x, j)), r.index(v, j));
+            }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kOf<E>; ++j) f(weigh(item<E>(x, j)), r.index(v, j));
+        }
+    };
+    constexpr uint32_t kWaves = kT / 64, kAtOnce = 2;
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t each = (v1 - v0 + kWaves - 1) / kWaves;
     const uint32_t from = min(v0 + wave * each, v1), to = min(from + each, v1);
-    double sum = 0.0;
+    const bool once = each <= 64 * kAtOnce;   // a part's run: what is read and weighed first is kept
+    double sum = 0.0, own[kAtOnce] = {};
+    u32x4 x[kAtOnce];
     uint32_t last = 0;   // index + 1 of the last with a weight
-    constexpr uint32_t kAtOnce = 2;
     for (uint32_t v = from + lane; v < to; v += 64 * kAtOnce) {
-        u32x4 x[kAtOnce];
         r.load(x, [&](uint32_t u) { return v + u * 64 < to ? v + u * 64 : ~0u; });
 #pragma unroll
-        for (uint32_t u = 0; u < kAtOnce; ++u)
-#pragma unroll
-            for (uint32_t j = 0; j < kOf<E>; ++j) {
-                const uint32_t index = r.index(v + u * 64, j);
-                const double w = weight(item<E>(x[u], j), index);
-                if (w > 0.0) sum += w, last = index + 1;
-            }
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            own[u] = 0.0;
+            each_kept(x[u], v + u * 64, [&](double w, uint32_t index) {
+                if (w > 0.0) own[u] += w, last = index + 1;
+            });
+            sum += own[u];
+        }
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -574,33 +594,42 @@ __device__ __forceinline__ uint32_t find_word(const Row<E>& r, uint32_t v0, uint
     if (wave == chosen) {
         uint32_t found = last;
         double rest = target - before;
-        for (uint32_t v = from + lane; !whole && v - lane < to; v += 64) {
-            u32x4 one[1];
-            r.load(one, [&](uint32_t) { return v < to ? v : ~0u; });
-            const u32x4 x = one[0];
-            double own = 0.0;
-#pragma unroll
-            for (uint32_t j = 0; j < kOf<E>; ++j) own += weight(item<E>(x, j), r.index(v, j));
-            double upto = own;
+        for (uint32_t v = from + lane, t = 0; !whole && v - lane < to; v += 64, ++t) {
+            u32x4 one[1] = {t == 0 ? x[0] : x[1]};
+            double mine = t == 0 ? own[0] : own[1];
+            if (!once) {
+                r.load(one, [&](uint32_t) { return v < to ? v : ~0u; });
+                mine = 0.0;
+                each_kept(one[0], v, [&](double w, uint32_t) { mine += w; });
+            } else if (v >= to) {
+                mine = 0.0;
+            }
+            double upto = mine;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double below = __shfl_up(upto, d);
                 if (lane >= uint32_t(d)) upto += below;
             }
-            const uint64_t over = __ballot(upto > rest && own > 0.0);
-            if (over != 0) {
-                const uint32_t at = __ffsll(static_cast<unsigned long long>(over)) - 1;
-                if (lane == at) {
-                    double c = upto - own;
-                    uint32_t pick = 0;
+            const uint64_t over = __ballot(upto > rest && mine > 0.0);
+            if (over != 0) {   // its words, one a lane
+                const int at = __ffsll(static_cast<unsigned long long>(over)) - 1;
+                u32x4 those;
 #pragma unroll
-                    for (uint32_t j = 0; j < kOf<E>; ++j) {
-                        const double w = weight(item<E>(x, j), r.index(v, j));
-                        if (w > 0.0 && (pick == 0 || c <= rest)) pick = r.index(v, j) + 1;
-                        c += w;
-                    }
-                    sh.found_index = pick;
+                for (uint32_t w = 0; w < 4; ++w) those[w] = __shfl(one[0][w], at);
+                const uint32_t index = r.index(v - lane + at, lane);
+                const float f = item_at<E>(those, lane % kOf<E>);
+                const double w = lane < kOf<E> && kept(f, index) ? weigh(f) : 0.0;
+                const double ahead = __shfl(upto, at) - __shfl(mine, at);
+                double c = w;
+#pragma unroll
+                for (int d = 1; d < int(kOf<E>); d <<= 1) {
+                    const double below = __shfl_up(c, d);
+                    if (lane >= uint32_t(d)) c += below;
                 }
+                // the last of those whose forerunners do not exceed it, the first at least
+                const uint64_t some = __ballot(w > 0.0), in = __ballot(w > 0.0 && ahead + (c - w) <= rest);
+                const int pick = in != 0 ? 63 - __builtin_clzll(in) : __ffsll(static_cast<unsigned long long>(some)) - 1;
+                if (int(lane) == pick) sh.found_index = index + 1;
                 found = 0;
                 break;
             }
@@ -673,40 +702,95 @@ __device__ __forceinline__ uint64_t border_by_digits(const Row<E>& r, float m, d
     if (prefix_mass != nullptr) *prefix_mass = double(before_mass + w * take) / one;
     __syncthreads();
     if (take >= tied) return uint64_t(prefix) << 32;
-    const uint32_t index = find_word<E, kT>(
-        r, 0, r.vectors, double(take) - 0.5, false, [&](float f, uint32_t) { return f > kNegInf && key_of(f) == prefix ? 1.0 : 0.0; }, sh);
+    const uint32_t index = find_word<E, kT, true>(
+        r, 0, r.vectors, double(take) - 0.5, false, [](float) { return 1.0; },
+        [&](float f, uint32_t) { return f > kNegInf && key_of(f) == prefix; }, sh);
     return uint64_t(prefix) << 32 | uint32_t(~index);
 }
 
+// How many of the codes of 16-bit floats, in their order (code_of), lie below `t` times 1 / scale:
+// those with scale x < t, rounded as the histograms have it.  Every wave by itself.
+template <typename E>
+__device__ __forceinline__ uint32_t codes_below(float t, float scale) {
+    constexpr uint32_t kInf = (E::kNegInf & 0x7FFFu) | 0x8000u;   // +infinity's
+    uint32_t below = 0;
+#pragma unroll
+    for (uint32_t step = 1024; step > 0; step = step == 1024 ? 16 : step == 16 ? 1 : 0) {
+        const uint32_t lane = threadIdx.x & 63, u = below + lane * step + step - 1;
+        const float x = E::lo(u & 0x8000u ? u & 0x7FFFu : ~u & 0xFFFFu);
+        below += uint32_t(__popcll(__ballot(u < kInf && (step > 1 || lane < 16) && !(x * scale >= t)))) * step;
+    }
+    return below;
+}
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+// Of a pair of 16-bit floats a bit each, 0 and 16: whether its code is among `many` from `from` on.
+__device__ __forceinline__ uint32_t codes_in(uint32_t pair, u16x2 from, u16x2 many) {
+    const uint32_t sign = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, pair) >> i16x2{15, 15});
+    const u16x2 code = __builtin_bit_cast(u16x2, pair ^ (sign | 0x80008000u));   // all bits of a negative one turned
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_elementwise_sub_sat(many, u16x2(code - from)), u16x2{1, 1}));
+}
+
 // The words with lo <= scale x < lo + 1, into sh.places as many as it holds; how many there are.
-// A vector's words at once: an addition to the counter for each of them would be waited for.
+// Found by bits, of 16-bit words two at a time by their codes, and put in place by one addition of
+// a wave to the counter for 8 vectors of each lane: the index first, the logit read again.
 template <typename E, uint32_t kT, typename Sh>
 __device__ __forceinline__ uint32_t gather_bin(const Row<E>& r, float scale, float lo, Sh& sh) {
+    constexpr bool kCodes = !std::is_same_v<E, F32>;
+    constexpr uint32_t kAtOnce = 8, kMasks = kOf<E> / 4;   // of 32 bits: 8 vectors of 4, or 4 of 8
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    constexpr uint32_t kAtOnce = 8;
-    for (uint32_t v = threadIdx.x; v < r.vectors; v += kT * kAtOnce) {
+    u16x2 from, many;
+    if constexpr (kCodes) {
+        const uint32_t a = codes_below<E>(lo, scale), b = codes_below<E>(lo + 1.0f, scale);
+        from = u16x2{uint16_t(a), uint16_t(a)}, many = u16x2{uint16_t(b - a), uint16_t(b - a)};
+    }
+    for (uint32_t v0 = 0; v0 < r.vectors; v0 += kT * kAtOnce) {
+        const uint32_t v = v0 + threadIdx.x;
         u32x4 x[kAtOnce];
         r.load(x, [&](uint32_t u) { return v + u * kT; });
+        uint32_t those[kMasks] = {}, n = 0;
 #pragma unroll
-        for (uint32_t u = 0; u < kAtOnce; ++u) {
-            uint32_t those = 0;
+        for (uint32_t u = 0; u < kAtOnce; ++u)
 #pragma unroll
-            for (uint32_t j = 0; j < kOf<E>; ++j) {
-                const float f = item<E>(x[u], j) * scale;
-                those |= uint32_t(f >= lo && f < lo + 1.0f) << j;
+            for (uint32_t w = 0; w < 4; ++w) {
+                if constexpr (kCodes) {
+                    those[u / 4] |= codes_in(x[u][w], from, many) << (u % 4 * 4 + w);
+                } else {
+                    const float f = item<E>(x[u], w) * scale;
+                    those[0] |= uint32_t(f >= lo && f < lo + 1.0f) << (u * 4 + w);
+                }
             }
-            if (those == 0) continue;
-            uint32_t at = atomicAdd(&sh.count, uint32_t(__popc(those)));
-            for (; those != 0; those &= those - 1, ++at) {
-                const uint32_t j = __ffs(those) - 1;
-                if (at < Sh::kSorted) sh.places[at] = place_of(item_at<E>(x[u], j), r.index(v + u * kT, j));
-            }
+#pragma unroll
+        for (uint32_t k = 0; k < kMasks; ++k) n += __popc(those[k]);
+        uint32_t at = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t below = __shfl_up(at, d);
+            if ((threadIdx.x & 63) >= uint32_t(d)) at += below;
         }
+        const uint32_t all = __shfl(at, 63);
+        if (all == 0) continue;
+        uint32_t before = 0;
+        if ((threadIdx.x & 63) == 0) before = atomicAdd(&sh.count, all);
+        at += __shfl(before, 0) - n;
+#pragma unroll
+        for (uint32_t k = 0; k < kMasks; ++k)
+            for (uint32_t m = those[k]; m != 0; m &= m - 1, ++at) {
+                const uint32_t bit = __ffs(m) - 1, u = kCodes ? k * 4 + bit % 16 / 4 : bit / 4;
+                const uint32_t j = kCodes ? bit % 4 * 2 + bit / 16 : bit % 4;
+                if (at < Sh::kSorted) sh.places[at] = r.index(v + u * kT, j);
+            }
     }
     __syncthreads();
-    return sh.count;
+    const uint32_t n = sh.count;
+    for (uint32_t i = threadIdx.x; i < min(n, Sh::kSorted); i += kT) {
+        const uint32_t index = uint32_t(sh.places[i]);
+        sh.places[i] = place_of(r.at(index), index);
+    }
+    __syncthreads();
+    return n;
 }
 
 // What the histograms of a row's parts say of it together.
@@ -862,7 +946,8 @@ __device__ __forceinline__ bool border_by_bins(const Rows& a, const Part* part, 
 // The k largest words of a row, sorted in sh.few; how many there are (-inf are none).
 //
 // One wave picks them from the parts' lists, up to 16 words a lane at a time: a key that k and
-// at most 128 of them reach, bit by bit, by counting ballots; those go on to the next lists and
+// at most 128 of them reach, bit by bit, by counting ballots, and where more are equal the bits of
+// their index (by passes over the row such a row took 110 us); those go on to the next lists and
 // are ranked by counting in the end.  Others than the first wave wait.
 // ---------------------------------------------------------------------
 constexpr uint32_t kPicked = 1024;
@@ -928,13 +1013,25 @@ __device__ __forceinline__ bool pick_largest(const Rows& a, const Part* part, co
             for (uint32_t i = 0; i < kEach; ++i) have += __popcll(__ballot(keys[i] >= with));
             if (have >= k) bound = with, reached = have;
         }
-        if (reached > kMost) return false;   // ties
+        uint32_t bound_low = 0;
+        if (reached > kMost) {   // equal words, the first of them by the bits of their index
+            bound_low = ~0u << (32 - __builtin_clz(max(a.vocab - 1, 1u)));
+#pragma unroll 1
+            for (uint32_t bit = ~bound_low / 2 + 1; reached > kMost; bit /= 2) {
+                const uint64_t with = uint64_t(bound) << 32 | bound_low | bit;
+                uint32_t have = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < kEach; ++i) have += __popcll(__ballot(i * 64 + lane < n && sh.places[i * 64 + lane] >= with));
+                if (have >= k) bound_low |= bit, reached = have;
+            }
+        }
         // in any order, each before where it was
         uint32_t at = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const bool in = i * 64 + lane < n && keys[i] >= bound;
-            const uint64_t place = in ? sh.places[i * 64 + lane] : 0, those = __ballot(in);
+            const uint64_t own = i * 64 + lane < n ? sh.places[i * 64 + lane] : 0;
+            const bool in = i * 64 + lane < n && own >= (uint64_t(bound) << 32 | bound_low);
+            const uint64_t place = in ? own : 0, those = __ballot(in);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (in) sh.places[at + __popcll(those & ((uint64_t(1) << lane) - 1))] = place;
             at += __popcll(those);
@@ -1150,11 +1247,8 @@ __device__ __forceinline__ void kept_by_parts(const Rows& a, const uint64_t* lis
 
 template <typename E>
 __device__ __forceinline__ void write_draw(const Rows& a, uint64_t of, const Row<E>& r, uint32_t index, const Joined& j, const Settings& s) {
-    float f;
-    if constexpr (std::is_same_v<E, F32>) f = __uint_as_float(r.x[index]);
-    else f = E::lo(r.x[index]);
     a.ids[of] = index;
-    a.logps[of] = float((double(f) - double(j.m)) / s.t - log(j.sum));
+    a.logps[of] = float((double(r.at(index)) - double(j.m)) / s.t - log(j.sum));
 }
 
 // The part in which the running mass exceeds u times all (sum_up: their sum, of up to 64 parts), and
@@ -1214,20 +1308,18 @@ __global__ __launch_bounds__(kWholeLanes) void draw_whole_kernel(const Rows a) {
     const double target = choose_part(a, share_of(a.uniforms[of]), false, j.sum, [&](uint32_t p) { return mass_of(part[p], j.m, c); }, &v0, sh);
     v0 = min(v0 * a.per, r.vectors);
     const Weigh weigh(c, j.m);
-    const uint32_t index = min(find_word<E, kWholeLanes>(
-        r, v0, min(v0 + a.per, r.vectors), target, false,
-        [&](float f, uint32_t) { return weigh(f); }, sh), a.vocab - 1);
+    const uint32_t index = min(find_word<E, kWholeLanes, false>(
+        r, v0, min(v0 + a.per, r.vectors), target, false, weigh, [](float, uint32_t) { return true; }, sh), a.vocab - 1);
     if (threadIdx.x == 0) write_draw(a, of, r, index, j, s);
 }
 
 // A draw by masses, or by each row's own settings.  Bound by latency, a workgroup a row: 64 rows of
-// 128256 bf16, top_p 0.95, 48 us, of which the border bin's words 13 (the row read again), the
-// histograms joined and searched about 15, the word found in its part 10; 255 rows of 50257 fp16
-// with settings of their own 46.  1024 lanes, so that a row is read in as few waits as may be.
-constexpr uint32_t kDrawLanes = 1024;
-template <typename E, Kind kKind>
+// 128256 bf16, top_p 0.95, 40 us, of which the histograms joined and searched 7, the border bin's
+// words 9 to 11 (the row read again), those binned and sorted 5 to 9, the word found in its part 6 to
+// 10; 255 rows of 50257 fp16 with settings of their own 43.
+template <typename E, Kind kKind, uint32_t kDrawLanes>
 __global__ __launch_bounds__(kDrawLanes) void draw_rows_kernel(const Rows a) {
-    __shared__ Shared<8192> sh;
+    __shared__ Shared<7680> sh;
     __shared__ Bins bins;
     const uint64_t row = blockIdx.x, of = a.first + row;
     const Part* const part = a.part + row * a.parts;
@@ -1290,9 +1382,9 @@ __global__ __launch_bounds__(kDrawLanes) void draw_rows_kernel(const Rows a) {
         v0 = min(v0 * a.per, r.vectors), v1 = min(v0 + a.per, r.vectors);
     }
     const float from = border != 0 ? logit_of(border) : kNegInf;
-    const uint32_t index = find_word<E, kDrawLanes>(
-        r, v0, v1, target, !by_parts,
-        [&](float f, uint32_t i) { return f > kNegInf && f >= from && place_of(f, i) >= border ? weight(f) : 0.0; }, sh);
+    const uint32_t index = find_word<E, kDrawLanes, true>(
+        r, v0, v1, target, !by_parts, weight,
+        [&](float f, uint32_t i) { return f > kNegInf && f >= from && place_of(f, i) >= border; }, sh);
     if (threadIdx.x == 0) write_draw(a, of, r, min(index, a.vocab - 1), j, s);
 }
 
@@ -1307,6 +1399,11 @@ Plan plan_of(size_t vocab, int dtype) {
     while (lane * kPartLanes < per) lane *= 2;
     return {uint32_t(parts), uint32_t(per), parts == 1 ? 2 * kList : kList, lane};
 }
+// Rows of more than 8192 vectors, not more of them than compute units, are drawn from by 1024 lanes:
+// few waits to read a row. Otherwise 512, of which a compute unit has two rows and whose registers
+// hold all.  A call in us, 512 | 1024: 64 x 128256 bf16 62.8 | 58.2, 1 x 139482 fp32 52.5 | 50.4;
+// 377 x 121933 bf16 139 | 157, 351 x 2572 fp32 41 | 58, 221 x 1313 bf16 28 | 32.
+constexpr uint32_t kWideRows = 256, kWideParts = 5;
 // Rows of one pair of launches: 256 MiB of lists.
 uint64_t rows_at_once(const Plan& p) {
     const uint64_t rows = (uint64_t(256) << 20) / (uint64_t(p.parts) * (8 * p.list + sizeof(Part)));
@@ -1328,7 +1425,9 @@ int launch_rows(const Rows& a, uint32_t rows, uint32_t lane, bool top, hipStream
     } else if constexpr (kKind == kWhole) {
         hipLaunchKernelGGL(draw_whole_kernel<E>, dim3(rows), dim3(kWholeLanes), 0, st, a);
     } else {
-        hipLaunchKernelGGL((draw_rows_kernel<E, kKind>), dim3(rows), dim3(kDrawLanes), 0, st, a);
+        const bool wide = rows <= kWideRows && a.parts >= kWideParts;
+        hipLaunchKernelGGL((wide ? draw_rows_kernel<E, kKind, 1024> : draw_rows_kernel<E, kKind, 512>), dim3(rows),
+                           dim3(wide ? 1024 : 512), 0, st, a);
     }
     return status();
 }

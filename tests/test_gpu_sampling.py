@@ -81,6 +81,42 @@ def test_largest(dev, vocab, dtype):
                 assert all(close(a, b) for a, b in zip(got[~same], logps[~same])), (kind, k)
 
 
+@pytest.mark.parametrize("k", [1, 100, 127, 128])
+@pytest.mark.parametrize("vocab", [600, 9000, 40_003])
+def test_equal_words_at_the_end_of_a_list(dev, vocab, k):
+    """More words equal the k-th than a list has room for: the first of them by their index, in the lists
+    and in a draw of each row's own top_k."""
+    g = torch.Generator(device=dev).manual_seed(vocab + k)
+    x = torch.where(torch.rand(7, vocab, generator=g, device=dev) < 400 / vocab, 2.0, 0.0)
+    x = x + torch.where(torch.rand(7, vocab, generator=g, device=dev) < 60 / vocab, 1.0, 0.0)
+    x = x.to(torch.bfloat16)
+    order = x.sort(dim=-1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(top_logps(x, k).ids, order)
+    u = torch.full((7,), 1 - 2.0 ** -24, device=dev)   # the kept word of the largest index
+    ks = torch.full((7,), k, device=dev)
+    assert torch.equal(sample_tokens(x, u, top_k=ks).ids, order.amax(dim=-1))
+    assert torch.equal(sample_tokens(x, u, top_k=k).ids, order.amax(dim=-1))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(300, 70_000), (5, 70_001), (260, 3001)])
+def test_borders_at_zero_and_below(dev, rows, vocab, dtype):
+    """Bins of a border that hold both zeros, subnormal and negative logits; rows drawn from by as many lanes
+    as their number and length ask for."""
+    g = torch.Generator(device=dev).manual_seed(rows + vocab)
+    x = torch.randn(rows, vocab, generator=g, device=dev) * 0.02
+    x[:, ::3] = 0.0
+    x[:, 1::9] = -0.0
+    x[:, 5::7] = 1e-7
+    x[:, 6::7] = -1e-7
+    x = x.to(dtype)
+    u = torch.rand(rows, generator=g, device=dev)
+    for p in (0.3, 0.55, 0.95):
+        out = sample_tokens(x, u, top_p=p)
+        some = torch.arange(0, rows, max(1, rows // 6))
+        against(x[some], u[some], type(out)(*(t[some] for t in out)), p=p)
+
+
 def test_rows_that_are_no_distribution(dev):
     for dtype in (torch.bfloat16, torch.float32):
         x = rows("plain", 6, 20_001, dtype, dev)
