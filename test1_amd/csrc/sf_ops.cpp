@@ -304,7 +304,7 @@ bool own_hidden_product(int64_t n, int64_t h, int64_t row) {
 
 // out = row weight * (d @ weight), rounded once.
 void hidden_product(const Tensor& keep, int64_t n, const Tensor& weight, int64_t nparts, const float* row_weight,
-                    const Tensor& norm, const Tensor& out) {
+                    const float* norm, const Tensor& out) {
     const int64_t v = weight.size(0), h = weight.size(1), row = keep.stride(0);
     const bool own = own_hidden_product(n, h, row);
     const int64_t part = own || nparts == 1 ? v : v / nparts / 8 * 8, done = own ? v : nparts * part;
@@ -322,7 +322,7 @@ void hidden_product(const Tensor& keep, int64_t n, const Tensor& weight, int64_t
     }
     const char *d = static_cast<const char*>(keep.data_ptr()), *w = static_cast<const char*>(weight.data_ptr());
     check(sf_logps_sum(at_ptr<float>(parts), int(nparts), n, h, out.data_ptr(), type_of(keep), d + 2 * done, row,
-                       w + 2 * done * h, v - done, row_weight, at_ptr<float>(norm), stream_of(keep)),
+                       w + 2 * done * h, v - done, row_weight, norm, stream_of(keep)),
           "sf_logps_sum");
 }
 
@@ -359,31 +359,32 @@ std::pair<Tensor, Tensor> products(const Tensor& hidden, const Tensor& weight, T
     const bool one = step == n;
     const sf_stream_t st = stream_of(hidden);
     const int type = type_of(hidden);
-    const Tensor by = like(hidden, {n}), norms = like(hidden, {3});
+    const Tensor scalars = like(hidden, {n + 3});
+    float* const by = at_ptr<float>(scalars);
     const bool own = one && own_weight_grad(n, h, v, row, fp16);
     // What D is divided by leaves before the results are rounded: in the own products, or of few
     // tiles with a pass over them.
-    const Tensor norm = fp16 || (divided && one && (own || tiles_of(h, v) < 96)) ? norms : Tensor();
+    float* const norm = fp16 || (divided && one && (own || tiles_of(h, v) < 96)) ? by + n : nullptr;
     Tensor gh, gw;
     if (need_hidden) gh = at::empty({n, h}, hidden.options());
-    if (need_weight) gw = at::empty({v, h}, own || (one && !norm.defined()) ? weight.options() : weight.options().dtype(at::kFloat));
+    if (need_weight) gw = at::empty({v, h}, own || (one && norm == nullptr) ? weight.options() : weight.options().dtype(at::kFloat));
     if (!keep.defined()) keep = at::empty({up(step, 64), row}, hidden.options());
     for (int64_t s = 0; s < n; s += step) {
         const int64_t m = std::min(n - s, step), pad = up(m, 64);
         const Tensor hc = one ? hidden : hidden.narrow(0, s, m);
-        fill(s, m, pad, hc, keep, at_ptr<float>(by), at_ptr<float>(norm));
+        fill(s, m, pad, hc, keep, by, norm);
         if (need_hidden && one && own_hidden_grad(n, h, v))
             check(sf_logps_hidden_grad(keep.data_ptr(), row, n, weight.data_ptr(), weight.stride(0), v, h,
-                                       at_ptr<float>(by), at_ptr<float>(norm), type, gh.data_ptr(), st),
+                                       by, norm, type, gh.data_ptr(), st),
                   "sf_logps_hidden_grad");
         else if (need_hidden)
-            hidden_product(keep, m, weight, nparts, at_ptr<float>(by) + s, norm,
+            hidden_product(keep, m, weight, nparts, by + s, norm,
                            one ? gh : gh.narrow(0, s, m));
         if (!need_weight) continue;
         if (fp16 && !own) {
             // into fp32, of rows as they lie: 4096 x 4096 x 128256 4.2 ms, of transposed ones 28.8
             const Tensor weighted = at::empty({m, h}, hidden.options());
-            check(sf_logps_weighted(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, weighted.data_ptr(), st),
+            check(sf_logps_weighted(hc.data_ptr(), hc.stride(0), m, h, by + s, type, weighted.data_ptr(), st),
                   "sf_logps_weighted");
             const Tensor dt = keep.as_strided({v, m}, {1, row});
             if (s == 0) at::mm_out(gw, dt, weighted, at::kFloat);
@@ -393,24 +394,24 @@ std::pair<Tensor, Tensor> products(const Tensor& hidden, const Tensor& weight, T
         // transposed: of bf16 the product with an operand laid out along the sum is
         // faster, 3.3 ms there instead of 4.0
         const Tensor ht = at::empty({h, pad}, hidden.options());
-        check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, at_ptr<float>(by) + s, type, ht.data_ptr(), pad, st),
+        check(sf_logps_hidden(hc.data_ptr(), hc.stride(0), m, h, by + s, type, ht.data_ptr(), pad, st),
               "sf_logps_hidden");
         if (own) {
-            check(sf_logps_weight_grad(keep.data_ptr(), row, pad, v, ht.data_ptr(), h, at_ptr<float>(norm),
+            check(sf_logps_weight_grad(keep.data_ptr(), row, pad, v, ht.data_ptr(), h, norm,
                                        type, gw.data_ptr(), st),
                   "sf_logps_weight_grad");
             break;
         }
         const Tensor dt = keep.as_strided({v, pad}, {1, row}), hp = ht.t();
-        if (one && !norm.defined()) at::mm_out(gw, dt, hp);
+        if (one && norm == nullptr) at::mm_out(gw, dt, hp);
         else if (s == 0) at::mm_out(gw, dt, hp, at::kFloat);
         else at::addmm_out(gw, gw, dt, hp, at::kFloat);
     }
     if (need_weight && gw.scalar_type() != weight.scalar_type()) {
         // its factor leaves before the rounding
-        if (norm.defined()) {
+        if (norm != nullptr) {
             const Tensor out = at::empty({v, h}, weight.options());
-            check(sf_ce_scale(at_ptr<float>(norm), at_ptr<float>(norm) + 1, nullptr, nullptr, 0, at_ptr<float>(gw),
+            check(sf_ce_scale(norm, norm + 1, nullptr, nullptr, 0, at_ptr<float>(gw),
                               out.data_ptr(), size_t(v * h), type, st),
                   "sf_ce_scale");
             gw = out;
