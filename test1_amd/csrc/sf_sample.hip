@@ -304,10 +304,11 @@ __global__ __launch_bounds__(kPartLanes) void rows_parts_kernel(const Rows a) {
     afresh(x);
 
     if (s.listed) {
-        // 2^(c x - from c), from c rounded, which the sum makes up for at its end; of a largest
-        // logit near the type's lowest value, where that is infinite, 2^(c (x - from))
+        // 2^(c x - from c), from c rounded, which the sum makes up for at its end: below 2^24 that
+        // is half an octave at most.  Of larger ones, a part of a finite mask's value or a low
+        // temperature, 2^(c (x - from)): from 2^31 on the rounding alone leaves an exponential's range.
         const float c = float(double(kLog2e) / s.t);
-        const bool far = !(fabsf(from * c) < 0x1p100f);
+        const bool far = !(fabsf(from * c) < 0x1p24f);
         const float less = far ? 0.0f : from * c;
         float sum = 0.0f;
         if (far) {

@@ -1,0 +1,73 @@
+"""Token sampling and largest log-probabilities on the GPU where logits over the
+temperature are large: masks of finite values over whole parts of a row, low
+temperatures."""
+
+import numpy as np
+import pytest
+import torch
+
+import sampling_reference as reference
+from test1_amd.sampling import sample_tokens, top_logps
+from test_gpu_sampling import against, close, rows
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+# of up to 16,384 words of 16 bits or 8,192 of 32 a row is one part; these have 1, 3 and 5, and 8 and 16
+LENGTHS = [700, 40_003, 128_256]
+
+
+def largest_are(x, k, t):
+    out = top_logps(x, k, temperature=t)
+    for i in range(x.shape[0]):
+        logps, ids = reference.top(x[i].double().cpu().numpy(), k, t)
+        assert np.array_equal(out.ids[i].cpu().numpy(), ids), (k, t)
+        assert all(close(a, b) for a, b in zip(out.logps[i].double().cpu().numpy(), logps)), (k, t)
+
+
+def draws_are(x, g, **s):
+    u = torch.rand(x.shape[0], generator=g, device=x.device)
+    out = sample_tokens(x, u, s.get("t", 1.0), s.get("k", 0), s.get("p", 1.0), s.get("m", 0.0))
+    against(x, u.cpu(), out, **s)
+    # the same by settings of every row
+    every = lambda name, least, kind: torch.full_like(u, s.get(name, least), dtype=kind)  # noqa: E731
+    own = sample_tokens(x, u, every("t", 1.0, torch.float32), every("k", 0, torch.int64), every("p", 1.0, torch.float32),
+                        every("m", 0.0, torch.float32))
+    settings = {n: (v if n == "k" else float(torch.tensor(v))) for n, v in s.items()}
+    against(x, u.cpu(), own, **settings)
+
+
+@pytest.mark.parametrize("t", [1.0, 0.3, 0.1])
+@pytest.mark.parametrize("mask", [-3e4, -1e9, -1e10, -1e12, -1e20, -1e30])
+@pytest.mark.parametrize("vocab", LENGTHS)
+def test_whole_parts_of_a_finite_mask(dev, vocab, mask, t):
+    """A few hundred neighbouring words are allowed, fewer than asked for in one row, none in the last: the
+    others hold a mask's value, whole parts of it."""
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    for dtype in TYPES:
+        if abs(mask) > torch.finfo(dtype).max:
+            continue
+        x = torch.full((3, vocab), mask, device=dev)
+        x[0, vocab // 2:vocab // 2 + 300] = torch.randn(300, generator=g, device=dev) * 2.5
+        x[1, vocab // 3:vocab // 3 + 5] = torch.randn(5, generator=g, device=dev)
+        x = x.to(dtype)
+        for k in (1, 20, 128):
+            largest_are(x, k, t)
+        for s in (dict(t=0.0), dict(t=t, k=1), dict(t=t, k=50, p=0.95), dict(t=t, k=128), dict(t=t, k=128, m=0.01),
+                  dict(t=t, k=300), dict(t=t, p=0.9), dict(t=t, m=0.05), dict(t=t)):
+            draws_are(x, g, **s)
+
+
+@pytest.mark.parametrize("t", [0.3, 0.02, 1e-3, 1e-6, 1e-8, 1e-9, 1e-10, 1e-12, 1e-20, 1e-30])
+@pytest.mark.parametrize("vocab", LENGTHS)
+def test_low_temperatures(dev, vocab, t):
+    t = max(float(torch.tensor(t)), 1e-30)   # what fp32 settings hold of it
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    for dtype in TYPES:
+        x = rows("plain", 3, vocab, dtype, dev, seed=1)
+        x[1] += 300.0
+        x[2] -= 3000.0
+        for k in (1, 20, 128):
+            largest_are(x, k, t)
+        for s in (dict(t=t, k=1), dict(t=t, k=50, p=0.95), dict(t=t, k=128, m=0.01), dict(t=t, k=300), dict(t=t, p=0.9), dict(t=t)):
+            draws_are(x, g, **s)
