@@ -1,6 +1,6 @@
 """Token sampling and largest log-probabilities on the GPU where logits over the
 temperature are large: masks of finite values over whole parts of a row, low
-temperatures."""
+temperatures; and all kinds of rows over several parts."""
 
 import numpy as np
 import pytest
@@ -8,7 +8,7 @@ import torch
 
 import sampling_reference as reference
 from test1_amd.sampling import sample_tokens, top_logps
-from test_gpu_sampling import against, close, rows
+from test_gpu_sampling import KINDS, SETTINGS, against, close, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,15 @@ def test_low_temperatures(dev, vocab, t):
             largest_are(x, k, t)
         for s in (dict(t=t, k=1), dict(t=t, k=50, p=0.95), dict(t=t, k=128, m=0.01), dict(t=t, k=300), dict(t=t, p=0.9), dict(t=t)):
             draws_are(x, g, **s)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [40_003, 128_256, 270_001])
+def test_all_kinds_of_rows_over_several_parts(dev, vocab, dtype):
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    for kind in KINDS:
+        x = rows(kind, 2, vocab, dtype, dev, seed=7)
+        for s in SETTINGS if vocab < 200_000 else SETTINGS[2:10:2]:
+            u = torch.rand(2, generator=g, device=dev)
+            out = sample_tokens(x, u, s.get("t", 1.0), s.get("k", 0), s.get("p", 1.0), s.get("m", 0.0))
+            against(x, u.cpu(), out, **s)
