@@ -520,8 +520,8 @@ int sf_distill_lists(const int64_t* ids, size_t ld_ids, const float* logps,
                      uint8_t* starts, uint8_t* status, sf_stream_t stream);
 
 /* The product of 16-bit operands, as sf_logps_tiles takes them: picked [rows, k], each
- * token's words' hidden . weight; parts, keep as there, of all other words
- * (keep: 16 bits of -log2 relative to the span's
+ * token's words' hidden . weight; parts, keep as there, of all other words, but that a
+ * part's maximum is not scaled (keep: 16 bits of -log2 relative to the span's
  * maximum, of 128 octaves for bf16 and 32 for fp16).  order (rows + 1 elements, or null): only rows of
  * status 1 take part, whose numbers it then holds, behind `rows` elements how many;
  * close: keep's rows are in that order, without gaps. */
@@ -545,9 +545,10 @@ int sf_distill_rows(float* logits, size_t ld, size_t rows, size_t vocab,
  * count as one outcome, of mass 1 - sum q (reverse: at least 2^-24); not: the
  * teacher's probabilities are divided by their sum (forward only).  hidden, weight
  * (hidden_size elements a row, of dtype): the products of likely words are formed
- * again.  slopes [rows, k] (or null: no gradient) and stats [3, stats_row]: the
- * derivatives by the words' logits over the token's largest one; that one, log2 of
- * the others' sum and the derivative they share over it. */
+ * again.  slopes [rows, k] (or null: no gradient) and stats [4, stats_row]: the
+ * derivatives by the words' logits over the token's largest one; that one, the largest
+ * of the others' hidden . weight, log2 of their sum relative to it and the derivative
+ * they share over it. */
 int sf_distill_loss(const void* parts, size_t parts_row, int whole,
                     const float* picked, const float* teacher,
                     const uint8_t* starts, const uint8_t* status, size_t rows,

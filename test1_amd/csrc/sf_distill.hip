@@ -158,10 +158,10 @@ __global__ __launch_bounds__(kRowLanes) void distill_rows_kernel(float* logits, 
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3])) * scale2;
+    m = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
     const float c = base(m);
     float s = 0.0f;
-    for (uint32_t j = threadIdx.x; j < vocab; j += kRowLanes) s += exp2f(fmaf(x[j], scale2, -c));
+    for (uint32_t j = threadIdx.x; j < vocab; j += kRowLanes) s += exp2f((x[j] - c) * scale2);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
     __syncthreads();
@@ -191,7 +191,7 @@ struct Loss {
     uint32_t terms;
     float* loss;
     float* slopes;         // [rows, k] v_k / r, or null
-    float* stats;          // [3, stats_row] r, log2 of the others' sum, v_r / r
+    float* stats;          // [4, stats_row] r, the others' maximum, log2 of their sum over it, v_r / r
     uint64_t stats_row;
 };
 template <typename V>
@@ -241,10 +241,12 @@ __global__ __launch_bounds__(kLossLanes) void distill_loss_kernel(const Loss a) 
     __shared__ Lse waves[kLossTokens][kLossTokens];
     {
         const uint32_t t = threadIdx.x % kLossTokens, token = blockIdx.x * kLossTokens + t;
+        const float scale2 = float(a.scale * kLog2ed);
         Lse p = {-__builtin_inff(), 0.0f};
-        const auto merge = [](Lse p, Lse q) {
+        const auto merge = [=](Lse p, Lse q) {
             const float m = fmaxf(p.m, q.m), c = base(m);
-            return Lse{m, (p.s == 0.0f ? 0.0f : p.s * exp2f(base(p.m) - c)) + (q.s == 0.0f ? 0.0f : q.s * exp2f(base(q.m) - c))};
+            return Lse{m, (p.s == 0.0f ? 0.0f : p.s * exp2f((base(p.m) - c) * scale2)) +
+                              (q.s == 0.0f ? 0.0f : q.s * exp2f((base(q.m) - c) * scale2))};
         };
         if (token < a.rows && a.status[token] == kTaught)   // the others may have no parts
             for (uint32_t k = threadIdx.x / kLossTokens; k < a.spans; k += kLossLanes / kLossTokens) {
@@ -269,7 +271,8 @@ __global__ __launch_bounds__(kLossLanes) void distill_loss_kernel(const Loss a) 
     if (status != kTaught) {
         if (lane == 0) {
             a.loss[token] = status == kBad ? __builtin_nanf("") : 0.0f;
-            if (a.slopes != nullptr) r_out[0] = a.loss[token], r_out[a.stats_row] = 0.0f, r_out[2 * a.stats_row] = 0.0f;
+            if (a.slopes != nullptr)
+                r_out[0] = a.loss[token], r_out[a.stats_row] = r_out[2 * a.stats_row] = r_out[3 * a.stats_row] = 0.0f;
         }
         return;
     }
@@ -278,7 +281,8 @@ __global__ __launch_bounds__(kLossLanes) void distill_loss_kernel(const Loss a) 
     const bool outside = n < a.vocab;
     double z[2], t[2], q[2];
     bool mine[2];
-    double top = others.s == 0.0f ? -__builtin_inf() : double(base(others.m));
+    const double top_others = others.s == 0.0f ? -__builtin_inf() : double(base(others.m)) * a.scale * kLog2ed;
+    double top = top_others;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const uint32_t i = e * 64 + lane;
@@ -288,34 +292,34 @@ __global__ __launch_bounds__(kLossLanes) void distill_loss_kernel(const Loss a) 
         q[e] = mine[e] ? exp(t[e]) : 0.0;
         top = fmax(top, z[e]);
     }
-    // the student
-    double rest_sum, sum, lse2;
+    // the student; all relative to the largest, beside which a logarithm may be nothing
+    double rest_sum, sum, log_sum;
     const auto join = [&] {
         top = wave_max(top);
-        rest_sum = others.s == 0.0f ? 0.0 : double(others.s) * exp2(double(base(others.m)) - top);
+        rest_sum = others.s == 0.0f ? 0.0 : double(others.s) * exp2(top_others - top);
         sum = 0.0;
 #pragma unroll
         for (int e = 0; e < 2; ++e) sum += mine[e] ? exp2(z[e] - top) : 0.0;
         sum = wave_sum(sum) + rest_sum;
-        lse2 = top + log2(sum);
+        log_sum = log2(sum);
     };
     join();
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-        const bool likely = mine[e] && (q[e] >= kLikely || exp2(z[e] - lse2) >= kLikely);
+        const bool likely = mine[e] && (q[e] >= kLikely || exp2(z[e] - top - log_sum) >= kLikely);
         for (uint64_t those = __ballot(likely); those != 0; those &= those - 1) {
             const uint32_t i = __ffsll(static_cast<unsigned long long>(those)) - 1;
             const double s = product_of<E>(a, token, a.words[uint64_t(token) * a.k + e * 64 + i]);
             if (lane == i) z[e] = s * a.scale * kLog2ed;
         }
     }
-    top = others.s == 0.0f ? -__builtin_inf() : double(base(others.m));
+    top = top_others;
 #pragma unroll
     for (int e = 0; e < 2; ++e) top = fmax(top, z[e]);
     join();
     double lp[2], p[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) lp[e] = (z[e] - lse2) * kLn2d, p[e] = mine[e] ? exp(lp[e]) : 0.0;
+    for (int e = 0; e < 2; ++e) lp[e] = (z[e] - top - log_sum) * kLn2d, p[e] = mine[e] ? exp(lp[e]) : 0.0;
     const double p_rest = rest_sum / sum, lp_rest = log(rest_sum) - log(sum);
     // the teacher
     double named = wave_sum(q[0] + q[1]), q_rest = 0.0;
@@ -362,8 +366,9 @@ __global__ __launch_bounds__(kLossLanes) void distill_loss_kernel(const Loss a) 
         if (mine[e]) a.slopes[uint64_t(token) * a.k + e * 64 + lane] = float(v[e] * by);
     if (lane == 0) {
         r_out[0] = r32;
-        r_out[a.stats_row] = others.s == 0.0f ? 0.0f : base(others.m) + log2f(others.s);
-        r_out[2 * a.stats_row] = float(v_rest * by);
+        r_out[a.stats_row] = base(others.m);
+        r_out[2 * a.stats_row] = others.s == 0.0f ? 0.0f : log2f(others.s);
+        r_out[3 * a.stats_row] = float(v_rest * by);
     }
 }
 
@@ -458,7 +463,7 @@ __global__ __launch_bounds__(kGradThreads) void distill_keep_grad_kernel(uint16_
     }
     // the row's weight over c, of which kLift is taken out
     const float whole = a.grad[row] * scale * a.stats[row] / (norm != nullptr ? *norm : 1.0f);
-    const float l = a.stats[a.stats_row + row], by = a.stats[2 * a.stats_row + row] * whole;
+    const float m = a.stats[a.stats_row + row], l = a.stats[2 * a.stats_row + row], by = a.stats[3 * a.stats_row + row] * whole;
     const uint8_t* starts = a.starts + row * (a.spans + 1);
     const uint32_t from = starts[col0 / kSpan], to = starts[min(col0 / kSpan + kKeepColumns / kSpan, a.spans)];
 #pragma unroll
@@ -467,7 +472,7 @@ __global__ __launch_bounds__(kGradThreads) void distill_keep_grad_kernel(uint16_
         if (c >= ld) break;
         u32x4* p = reinterpret_cast<u32x4*>(k + c);
         const u32x4 v = *p;
-        const float more = base(parts[uint64_t(c / kSpan) * tokens + row].x) - l;
+        const float more = fmaf(base(parts[uint64_t(c / kSpan) * tokens + row].x) - m, scale * kLog2e, -l);
         u32x4 o;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -587,9 +592,9 @@ __global__ __launch_bounds__(kRowLanes) void distill_grad_kernel(float* logits, 
     const uint64_t row = blockIdx.x;
     float* x = logits + row * ld;
     const RowOf kind = row_of(a, row);
-    const float l = a.stats[a.stats_row + row], by = a.stats[2 * a.stats_row + row];
+    const float m = a.stats[a.stats_row + row], l = a.stats[2 * a.stats_row + row], by = a.stats[3 * a.stats_row + row];
     for (uint32_t j = threadIdx.x; j < vocab; j += kRowLanes)
-        x[j] = kind == kZero ? 0.0f : kind == kNan ? __builtin_nanf("") : by == 0.0f ? 0.0f : exp2f(fmaf(x[j], scale2, -l)) * by;
+        x[j] = kind == kZero ? 0.0f : kind == kNan ? __builtin_nanf("") : by == 0.0f ? 0.0f : exp2f(fmaf(x[j] - m, scale2, -l)) * by;
     if (kind != kComputed) return;
     __syncthreads();
     const uint32_t n = a.starts[row * (a.spans + 1) + a.spans];

@@ -586,7 +586,7 @@ DistillOut distill_forward(const Tensor& hidden_, const Tensor& weight_, const T
     o.status = at::empty({n}, bytes);
     const Tensor lists = like(hidden, {2, n, k});   // the teacher's, the products
     float *teacher = at_ptr<float>(lists), *picked = teacher + n * k;
-    if (grad) o.slopes = like(hidden, {n, k}), o.stats = like(hidden, {3, n});
+    if (grad) o.slopes = like(hidden, {n, k}), o.stats = like(hidden, {4, n});
     check(sf_distill_lists(at_ptr<int64_t>(ids), ld(ids), at_ptr<float>(logps), ld(logps), at_ptr<uint8_t>(mask), n, int(k), v,
                            whole, at_ptr<int32_t>(o.words), teacher, at_ptr<uint8_t>(o.starts), at_ptr<uint8_t>(o.status), st),
           "sf_distill_lists");
@@ -749,8 +749,8 @@ std::pair<Tensor, Tensor> distill_backward_torch(const Tensor& grad_, const Tens
     const Tensor n = o.starts.select(1, o.starts.size(1) - 1).to(at::kLong).unsqueeze(1);
     const Tensor there = at::arange(k, n.options()).unsqueeze(0) < n;
     const Tensor at = at::where(there, o.words.to(at::kLong), at::full_like(n, v));
-    const Tensor z = at::matmul(h, w.t()) * (a.scale / std::log(2.0));
-    Tensor d = at::exp2(z - stats.select(0, 1).unsqueeze(1)) * stats.select(0, 2).unsqueeze(1);
+    const Tensor z = (at::matmul(h, w.t()) - stats.select(0, 1).unsqueeze(1)) * (a.scale / std::log(2.0));
+    Tensor d = at::exp2(z - stats.select(0, 2).unsqueeze(1)) * stats.select(0, 3).unsqueeze(1);
     d = at::cat({d, at::zeros({d.size(0), 1}, d.options())}, 1);
     d = d.scatter(1, at, at::where(there, o.slopes.to(at::kFloat), at::zeros({}, d.options()))).narrow(1, 0, v);
     d = d * (grad * a.scale * stats.select(0, 0)).unsqueeze(1);

@@ -74,7 +74,7 @@ struct Tiles {
     const int64_t* labels;
     const int32_t* order;     // [tokens + 1] the rows with a label and their number, or null: all rows
     float scale2;             // scale * log2(e)
-    float2* parts;            // [tiles of words, parts_row] maximum in base 2 and sum
+    float2* parts;            // [tiles of words, parts_row] maximum in base 2 (kPick: as it is) and sum
     uint64_t parts_row;       // tokens of the whole call, of which these are some
     float* target;            // [tokens] the label's product, unscaled
     uint16_t* keep;           // [tokens, ld_keep] or null
@@ -153,7 +153,8 @@ __device__ __forceinline__ void interleave() {
 // but one are on their way while one is used.  kOrder: tokens in the order of
 // a.order, otherwise all of them.  kPick: a token's words leave the tile for
 // a.picked, before its maximum and its sum, which are then those of all others, and
-// kept are logarithms (pack_log2): with 64 words a token and a fifth of the tokens left
+// kept are logarithms (pack_log2).  Its maximum stays unscaled and is subtracted before the
+// scale: a low temperature's differences are exact however large the logits over it are.  With 64 words a token and a fifth of the tokens left
 // out 2810 us at 4092 x 4096 x 128256, 8,250 at 8190 x 5120 x 152064, 1.2 PFLOP/s of the
 // rows that count; with one label picked by its index 2,832 and 8,394.
 template <typename Fmt, int kWV, int kWT, int kFV, int kFT, int kDeep, bool kKeep, bool kOrder, bool kPick>
@@ -392,13 +393,14 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
         float m = shared[t];
 #pragma unroll
         for (int w = 1; w < kWV; ++w) m = fmaxf(m, shared[w * kBT + t]);
-        top[j] = m * a.scale2;
+        top[j] = kPick ? m : m * a.scale2;
     }
     __syncthreads();   // read by all before it is overwritten
     uint8_t* const turn = lds + wave * 16 * kTurnRow;
 #pragma unroll
     for (int j = 0; j < kFT; ++j) {
-        // exp2(scale2 x - base(top)): the product is not rounded before the difference
+        // exp2(scale2 x - base(top)): the product is not rounded before the difference, or (kPick)
+        // exp2(scale2 (x - base(top)))
         const float c = base(top[j]);
         sum[j] = 0.0f;
 #pragma unroll
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Ti
             f32x4 t, e;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                t[r] = fmaf(acc[i][j][r], a.scale2, -c);
+                t[r] = kPick ? (acc[i][j][r] - c) * a.scale2 : fmaf(acc[i][j][r], a.scale2, -c);
                 e[r] = __builtin_amdgcn_exp2f(t[r]);
                 sum[j] += e[r];
             }
