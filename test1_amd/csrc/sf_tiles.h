@@ -38,12 +38,12 @@ template <typename Fmt>
 __device__ __forceinline__ uint32_t pack_log2(float a, float b) {   // a, b <= 0
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(a * (-1.0f / kOctaves<Fmt>), b * (-1.0f / kOctaves<Fmt>)));
 }
-// 2^(more - what is kept).
+// 2^(more - what is kept); 0 of none, whatever more is: the columns that pad a last tile whose
+// words are all picked are relative to no maximum, and more is above 0 where the other words are far below.
 template <typename Fmt>
 __device__ __forceinline__ float exp2_kept(uint32_t u, float more) {
     const float e = __builtin_amdgcn_exp2f(fmaf(float(u), -kOctaves<Fmt> / 65535.0f, more));
-    // of 128 octaves the last one's exponential is 0 by itself: more is not above 0
-    return kOctaves<Fmt> < 127.0f && u == 65535 ? 0.0f : e;
+    return u == 65535 ? 0.0f : e;
 }
 
 // ---------------------------------------------------------------------

@@ -35,3 +35,29 @@ def check(shape, dtype, dev, temperature, kind, rest):
 def test_low_temperatures(dev, shape, temperature, kind, rest):
     for dtype in TYPES if shape[1] < 2048 else TYPES[:1]:
         check(shape, dtype, dev, temperature, kind, rest)
+
+
+# tokens, hidden, vocabulary, words, masked: few tokens; a product of the framework's own; one of close rows
+@pytest.mark.parametrize("shape", [(70, 64, 257, 1, False), (70, 64, 300, 44, False), (300, 128, 895, 127, True), (4200, 2048, 513, 1, False),
+                                   (4200, 2048, 4097, 1, True)])
+def test_a_last_span_whose_words_are_all_named(dev, shape):
+    """What pads the vocabulary to a whole span stays out of the hidden gradient, where all other words are far
+    below: there is no word of the last span that the padding could be relative to."""
+    n, h, v, k, masked = shape
+    for dtype in (torch.bfloat16, torch.float16):
+        for below in (2, 4):
+            g = torch.Generator(device=dev).manual_seed(v + below)
+            hidden = torch.randint(0, 3, (n, h), generator=g, device=dev).to(dtype)
+            hidden[:, 64:] = 0   # logits of the others around -128 and -256
+            weight = torch.randint(-1, 2, (v, h), generator=g, device=dev)
+            weight[:v // 256 * 256] -= below
+            weight = weight.to(dtype)
+            ids = torch.arange(v - k, v, device=dev).expand(n, k).contiguous()
+            logps = torch.log_softmax(torch.randn(n, k + 1, generator=g, device=dev), dim=1)[:, :k].contiguous()
+            mask = torch.rand(n, generator=g, device=dev) < (0.8 if masked else 2.0)
+            up = torch.randn(n, generator=g, device=dev) / n
+            want, bound = exact_logits.distill(hidden, weight, ids, logps, mask, 1.0, "forward", True, up)
+            hr, wr = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+            loss = linear_distill(hr, wr, ids, logps, mask if masked else None)
+            for got, w, b in zip((loss.detach(), *torch.autograd.grad(loss, (hr, wr), up)), want, bound):
+                near(got, w, b)
