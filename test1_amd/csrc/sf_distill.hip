@@ -320,7 +320,8 @@ __global__ __launch_bounds__(kLossLanes) void distill_loss_kernel(const Loss a) 
     double lp[2], p[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) lp[e] = (z[e] - top - log_sum) * kLn2d, p[e] = mine[e] ? exp(lp[e]) : 0.0;
-    const double p_rest = rest_sum / sum, lp_rest = log(rest_sum) - log(sum);
+    // of a rest far below the mass is 0, its logarithm and what it shares are not
+    const double p_rest = rest_sum / sum, lp_rest = (top_others - top + log2(double(others.s)) - log_sum) * kLn2d;
     // the teacher
     double named = wave_sum(q[0] + q[1]), q_rest = 0.0;
     if (!a.rest) {
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(kLossLanes) void distill_loss_kernel(const Loss a) 
     }
     if (lane == 0) a.loss[token] = float(loss);
     if (a.slopes == nullptr) return;
-    if (rest_sum == 0.0) v_rest = 0.0;   // there is nothing to share it
+    if (others.s == 0.0f) v_rest = 0.0;   // there is nothing to share it
     double r = fmax(wave_max(fmax(mine[0] ? fabs(v[0]) : 0.0, mine[1] ? fabs(v[1]) : 0.0)), fabs(v_rest));
     if (loss != loss) r = __builtin_nan("");
     const float r32 = float(r);

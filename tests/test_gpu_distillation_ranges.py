@@ -6,6 +6,7 @@ import torch
 
 import exact_logits
 from alignment_reference import near
+from distill_reference import distill
 from test1_amd.distillation import linear_distill
 
 pytestmark = pytest.mark.gpu
@@ -31,7 +32,7 @@ def check(shape, dtype, dev, temperature, kind, rest):
 
 @pytest.mark.parametrize("temperature", [1.0, 0.01, 1e-4, 1e-6, 1e-8, 1e-9, 1e-12, 1e-20, 1e-30])
 @pytest.mark.parametrize("shape", SHAPES)
-@pytest.mark.parametrize("kind,rest", [("forward", False), ("reverse", True)])
+@pytest.mark.parametrize("kind,rest", [("forward", False), ("reverse", True), ("forward", True)])
 def test_low_temperatures(dev, shape, temperature, kind, rest):
     for dtype in TYPES if shape[1] < 2048 else TYPES[:1]:
         check(shape, dtype, dev, temperature, kind, rest)
@@ -59,5 +60,30 @@ def test_a_last_span_whose_words_are_all_named(dev, shape):
             want, bound = exact_logits.distill(hidden, weight, ids, logps, mask, 1.0, "forward", True, up)
             hr, wr = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
             loss = linear_distill(hr, wr, ids, logps, mask if masked else None)
+            for got, w, b in zip((loss.detach(), *torch.autograd.grad(loss, (hr, wr), up)), want, bound):
+                near(got, w, b)
+
+
+@pytest.mark.parametrize("kind,rest", [("forward", True), ("forward", False), ("reverse", True)])
+@pytest.mark.parametrize("gap", [700.0, 1000.0, 5000.0])
+def test_a_rest_far_below_the_words(dev, gap, kind, rest):
+    """All words outside the teacher's `gap` nats or so below: their mass leaves the exponents of 64 bits, its
+    logarithm and the derivative they share do not.  By large hidden states, and by the temperature."""
+    n, h, v, k = 70, 64, 700, 5
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        for temperature in (1.0, 0.01):
+            g = torch.Generator(device=dev).manual_seed(3)
+            hidden = (torch.rand(n, h, generator=g, device=dev) + 0.5) * (gap * temperature / h)
+            weight = torch.rand(v, h, generator=g, device=dev) * 0.02 - 1.0
+            ids = torch.rand(n, v, generator=g, device=dev).argsort(dim=1)[:, :k].contiguous()
+            ids[:] = ids[0]
+            weight[ids[0]] += 1.0
+            hidden, weight = hidden.to(dtype), weight.to(dtype)
+            logps = torch.log_softmax(torch.randn(n, k + 1, generator=g, device=dev), dim=1)[:, :k].contiguous()
+            up = torch.randn(n, generator=g, device=dev) * temperature
+            want, bound = distill(hidden, weight, ids, logps, None, 1 / temperature, kind, rest, grad=up)
+            assert want[0].isfinite().all() and (kind == "reverse" or not rest or (want[0] > 50).any())
+            hr, wr = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+            loss = linear_distill(hr, wr, ids, logps, None, temperature, kind, rest)
             for got, w, b in zip((loss.detach(), *torch.autograd.grad(loss, (hr, wr), up)), want, bound):
                 near(got, w, b)
