@@ -62,7 +62,10 @@ def _torch_distill(hidden, weight, ids, logps, mask, scale, kind, rest, bias=Non
             some = ~inside.all(dim=-1)
             others = torch.where(inside | ~some.unsqueeze(-1), -math.inf, logp)
             others = torch.where(some.unsqueeze(-1), others, zero)
-            lp_rest = torch.where(some, torch.logsumexp(others, dim=-1), zero)
+            # relative to their largest, beside which the logarithm may be nothing: what they share comes of it
+            largest = others.detach().amax(dim=-1, keepdim=True)
+            largest = torch.where(largest.isfinite(), largest, zero)
+            lp_rest = torch.where(some, (others - largest).exp().sum(dim=-1).log() + largest.squeeze(-1), zero)
             q_rest = (1 - named.squeeze(-1)).clamp(min=_LEAST_REST if kind == "reverse" else 0.0)
             q_rest = torch.where(some, q_rest, zero)
         else:
