@@ -87,3 +87,45 @@ def test_a_rest_far_below_the_words(dev, gap, kind, rest):
             loss = linear_distill(hr, wr, ids, logps, None, temperature, kind, rest)
             for got, w, b in zip((loss.detach(), *torch.autograd.grad(loss, (hr, wr), up)), want, bound):
                 near(got, w, b)
+
+
+@pytest.mark.parametrize("temperature", [30.0, 1e6, 1e30])
+@pytest.mark.parametrize("kind,rest", [("forward", False), ("reverse", True), ("forward", True)])
+def test_high_temperatures(dev, temperature, kind, rest):
+    for shape in SHAPES[:3]:
+        for dtype in TYPES:
+            check(shape, dtype, dev, temperature, kind, rest)
+
+
+def test_calls_beside_each_other_and_in_other_modes(dev):
+    """Two steps on two streams at once; under inference mode and autocast; of one token, of more dimensions, of none."""
+    hidden, weight, ids, logps, mask, up = exact_logits.inputs((700, 512, 30_000, 20), torch.bfloat16, dev)
+
+    def step():
+        hr, wr = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+        loss = linear_distill(hr, wr, ids, logps, mask, 20.0)
+        return loss.detach(), *torch.autograd.grad(loss, (hr, wr), up)
+
+    want = step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams * 2:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
+    with torch.inference_mode():
+        assert torch.equal(linear_distill(hidden.clone(), weight, ids, logps, mask, 20.0), want[0])
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    each = linear_distill(hidden, weight, ids, logps, None, 20.0)
+    one = linear_distill(hidden[3], weight, ids[3], logps[3], torch.ones((), dtype=torch.bool, device=dev), 20.0)
+    # another tile's order of sums: 512 terms in a row of 8 U on each side, and the result's rounding
+    assert one.shape == () and (one - each[3]).abs() <= (1040 + 2 * each[3].abs()) * 2.0 ** -24
+    cube = linear_distill(hidden.view(7, 10, 10, 512), weight, ids.view(7, 10, 10, 20), logps.view(7, 10, 10, 20), None, 20.0)
+    assert torch.equal(cube.flatten(), each)
+    hr, wr = hidden[:0].clone().requires_grad_(True), weight.clone().requires_grad_(True)
+    loss = linear_distill(hr, wr, ids[:0], logps[:0], mask[:0])
+    gh, gw = torch.autograd.grad(loss.sum(), (hr, wr))
+    assert loss.shape == (0,) and gh.shape == (0, 512) and (gw == 0).all()

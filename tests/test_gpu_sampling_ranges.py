@@ -83,3 +83,35 @@ def test_all_kinds_of_rows_over_several_parts(dev, vocab, dtype):
             u = torch.rand(2, generator=g, device=dev)
             out = sample_tokens(x, u, s.get("t", 1.0), s.get("k", 0), s.get("p", 1.0), s.get("m", 0.0))
             against(x, u.cpu(), out, **s)
+
+
+@pytest.mark.parametrize("t", [20.0, 1e4, 1e30])
+@pytest.mark.parametrize("vocab", LENGTHS)
+def test_high_temperatures(dev, vocab, t):
+    t = float(torch.tensor(t))
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    for dtype in TYPES:
+        x = rows("plain", 2, vocab, dtype, dev, seed=2)
+        x[1, vocab // 4:] = float("-inf")
+        for k in (1, 128):
+            largest_are(x, k, t)
+        for s in (dict(t=t, k=50, p=0.95), dict(t=t, k=300), dict(t=t, p=0.93), dict(t=t, m=0.5), dict(t=t)):
+            draws_are(x, g, **s)
+
+
+def test_other_modes_and_settings(dev):
+    """Under inference mode and autocast, of logits with a gradient, settings beyond the vocabulary."""
+    x = rows("plain", 5, 40_003, torch.bfloat16, dev)
+    u = torch.rand(5, device=dev)
+    want, top = sample_tokens(x, u, top_p=0.9), top_logps(x, 30)
+    same = lambda a, b: all(torch.equal(p, q) for p, q in zip(a, b))  # noqa: E731
+    with torch.inference_mode():
+        assert same(sample_tokens(x.clone(), u, top_p=0.9), want) and same(top_logps(x, 30), top)
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert same(sample_tokens(x, u, top_p=0.9), want)
+    out = top_logps(torch.nn.Parameter(x), 30)
+    assert same(out, top) and not out.logps.requires_grad
+    assert same(sample_tokens(x, u, top_k=1 << 40), sample_tokens(x, u))
+    assert same(sample_tokens(x, u, top_k=torch.full((5,), 1 << 40, device=dev)), sample_tokens(x, u, top_k=torch.zeros(5, dtype=torch.int64, device=dev)))
+    for s in (dict(temperature=torch.tensor(0.7)), dict(temperature=torch.tensor(0.7, device=dev)), dict(top_k=torch.tensor(40))):
+        assert same(sample_tokens(x, u, **s), sample_tokens(x, u, **{n: v.item() for n, v in s.items()}))
