@@ -709,8 +709,6 @@ std::pair<Tensor, Tensor> distill_backward_close(const Tensor& grad, const Tenso
     return {gh, gw};
 }
 
-// The gradients by torch operations, where what was saved came back as something else.
-
 std::pair<Tensor, Tensor> distill_backward(const Tensor& grad, const Tensor& hidden, const Tensor& weight,
                                            const DistillOut& o, const DistillArgs& a, bool need_hidden, bool need_weight) {
     if (!in_tiles(hidden, weight)) return distill_backward_whole(grad, hidden, weight, o, a, need_hidden, need_weight);
@@ -738,6 +736,7 @@ std::pair<Tensor, Tensor> distill_backward(const Tensor& grad, const Tensor& hid
     });
 }
 
+// The gradients by torch operations, where what was saved came back as something else.
 std::pair<Tensor, Tensor> distill_backward_torch(const Tensor& grad_, const Tensor& hidden, const Tensor& weight,
                                                  const DistillOut& o, const DistillArgs& a, bool need_hidden,
                                                  bool need_weight) {

@@ -6,7 +6,9 @@
 // those the words with less than top_p of their mass before them; of those the
 // words with w_j >= min_p.  The word drawn is the first kept one, by its index,
 // whose running mass exceeds u times the kept mass: no sort of the vocabulary.
-// Which word that is hangs on sums of up to 2^30 terms, so masses are 64-bit.
+// Which word that is hangs on sums of up to 2^30 terms, so the masses that decide it are
+// 64-bit.  (The mass of all words of a row that goes by lists is for its log-probability
+// alone: a lane's 64 are summed in fp32.)
 //
 // Two launches.  rows_parts_kernel cuts rows into parts of up to 2048 16-byte
 // vectors, which a workgroup holds in registers, and leaves of each its maximum,

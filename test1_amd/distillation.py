@@ -8,7 +8,8 @@ The reference's output unit trains on labels alone (slide_fsdp.py:77-113).
 
 Numerics: logits and the softmax's sums are fp32, as ``linear_logps``', the logits of
 a token's likely words 64-bit; its few words, what lies outside them and the
-divergence itself, a small difference of large terms, are in 64 bits.  The
+divergence itself, a small difference of large terms, are in 64 bits.  Differences
+of logits are taken before the temperature, however low it is.  The
 gradient's products take 16-bit operands of 16-bit inputs: the derivatives by the
 logits, rounded once (the exponentials that they come from are kept to 2^-10.5 of
 themselves, in float16 2^-12.5), and the hidden rows as they are.
@@ -136,8 +137,8 @@ def linear_distill(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torc
 
     0, without gradient, where the mask is False or the teacher has no word; NaN
     where an id is outside the vocabulary or stands twice.  Differentiable once by
-    ``hidden`` and ``weight``; tokens whose upstream gradient is 0 leave the
-    gradients alone.  Under ``no_grad`` nothing is kept.  Autocast does not change
+    ``hidden`` and ``weight``; on a GPU, tokens whose upstream gradient is 0 leave the
+    gradients alone, whatever their hidden states hold.  Under ``no_grad`` nothing is kept.  Autocast does not change
     it.  It is not multiplied by temperature^2."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError("linear_distill: hidden [..., H] and weight [V, H] expected")

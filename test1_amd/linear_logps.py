@@ -263,7 +263,9 @@ def linear_logps(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tenso
     float16 or float32), ``labels`` [...] int64.  0, without gradient, where
     the label is ``ignore_index``; NaN where it is outside the vocabulary.
     Differentiable once by ``hidden`` and ``weight``; under ``no_grad`` nothing
-    is kept.  Autocast does not change it."""
+    is kept.  Autocast does not change it.  Logits over the temperature are
+    fp32: the results are off by 2^-24 of their magnitude, and NaN where that is 2^31
+    or more (a temperature of 1e-9 or so)."""
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError("linear_logps: hidden [..., H] and weight [V, H] expected")
     if labels.shape != hidden.shape[:-1]:

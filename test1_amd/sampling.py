@@ -7,8 +7,12 @@ that ``policy_loss`` takes, with their log-probabilities under the policy that
 sampled them, come from ``sample_tokens``.
 
 The kernels (``csrc/sf_sample.hip``) read the logits once, a sampled row's
-border again, and sort no vocabulary; masses are summed in 64 bits, so that a
-draw is decided as in exact arithmetic.  On a host, and for calls that the
+border again, and sort no vocabulary.  What a draw is decided by is summed in 64
+bits, as in exact arithmetic; the mass of all words, which log-probabilities
+take, too, but of calls whose words are listed (``top_logps``, draws of the
+largest or of up to 128): there each lane sums up to 64 words in fp32.
+Logits that are large over the temperature, masks of any finite value among
+them, cost no accuracy.  On a host, and for calls that the
 kernels cannot serve (traced, batched by vmap), the same runs as torch
 operations.  Neither is differentiable.
 """
@@ -67,7 +71,8 @@ def top_logps(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogp
     dimension and their words, by falling logit, the first of equals first.
 
     ``logits`` [..., V] bfloat16, float16 or float32; ``k`` from 1 to
-    ``TOP_MOST`` (128) and V; ``temperature`` above 0.  A row with a NaN or
+    ``TOP_MOST`` (128) and V; ``temperature`` above 0 (beyond 1e-30 and 1e30 as
+    those).  A row with a NaN or
     +infinity, or of -infinities alone, gives NaN and -1.  No gradient."""
     _check_logits("top_logps", logits)
     k = int(k)

@@ -138,7 +138,8 @@ class OutputLayer(nn.Module):
                     temperature: float = 1.0, kind: str = "forward", rest: bool = True) -> torch.Tensor:
         """Each next token's divergence from a teacher's, [B, S - 1] fp32, 0 where
         the mask is False; no logits are kept.  With a bias, which the kernels do
-        not add, by torch operations from all logits."""
+        not add, by torch operations from all logits, several [N, V] tensors in 64
+        bits."""
         hidden_states, bias = self.norm(hidden_states)[..., :-1, :], getattr(self.lm_head, "bias", None)
         if bias is None:
             return linear_distill(hidden_states, self.lm_head.weight, teacher.ids, teacher.logps, mask, temperature, kind, rest)
@@ -849,7 +850,7 @@ class SlideFSDP(nn.Module):
     def sample_tokens(self, input_ids: torch.Tensor, uniforms: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                       **settings) -> SampledTokens:
         """One token behind each row's last one (with ``attention_mask`` the last
-        whose mask is not 0) under the model as it is, drawn by ``uniforms`` [B],
+        whose mask is not 0, of a row without one the first) under the model as it is, drawn by ``uniforms`` [B],
         with its log-probability; ``settings`` as ``sampling.sample_tokens`` takes
         them.  Its log-probabilities are what ``policy_loss`` takes as
         ``old_logps``.  A token takes a whole forward: there is no cache of keys
