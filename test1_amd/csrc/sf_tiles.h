@@ -153,9 +153,10 @@ __device__ __forceinline__ void interleave() {
 // but one are on their way while one is used.  kOrder: tokens in the order of
 // a.order, otherwise all of them.  kPick: a token's words leave the tile for
 // a.picked, before its maximum and its sum, which are then those of all others, and
-// kept are logarithms (pack_log2).  Its maximum stays unscaled and is subtracted before the
-// scale: a low temperature's differences are exact however large the logits over it are.  With 64 words a token and a fifth of the tokens left
-// out 2,810-2,870 us at 4092 x 4096 x 128256, 8,250-8,580 at 8190 x 5120 x 152064 (by the box), 1.2 PFLOP/s of the
+// kept are logarithms (pack_log2).  Its maximum stays unscaled and is subtracted before
+// the scale: differences hold at low temperatures, however large the logits over them
+// are.  With 64 words a token and a fifth of the tokens left out 2,810-2,870 us at 4092 x
+// 4096 x 128256, 8,250-8,580 at 8190 x 5120 x 152064 (by the box), 1.2 PFLOP/s of the
 // rows that count; with one label picked by its index 2,832 and 8,394.
 template <typename Fmt, int kWV, int kWT, int kFV, int kFT, int kDeep, bool kKeep, bool kOrder, bool kPick>
 __global__ __launch_bounds__(kWV * kWT * 64, 2) void logps_tiles_kernel(const Tiles a) {
